@@ -444,6 +444,47 @@ int lq_wq_matmul(const float* x, const uint32_t* packed, const float* scales, co
  * (lucid/nn/quantized/mlx_linear.py forward). */
 int lq_bias_act_f32(float* y, const float* bias, size_t M, int N, int relu, lq_stream stream);
 
+/* ------------------------------------------------- quantized key / value cache
+ * No counterpart in Lucid.  Pages of page_size tokens; a page holds, per key / value head, page_size rows of head_dim codes,
+ * so that a head's rows of a page are contiguous: codes [num_pages, kv_heads, page_size, head_dim * bits / 8] bytes, scale and
+ * zero float32 [num_pages, kv_heads, page_size].  Slot s is row s % page_size of page s / page_size.  A row is quantized by
+ * itself, as a row of lq_quantize_rows_dynamic_i8 with eps = 1e-8 (lucid/quantization/_qparams.py:198-215,
+ * _functional.py:164-182), on the signed grid of its bits: [-128, 127] or [-8, 7].  Stored is code - qmin, two 4-bit codes in a
+ * byte, the first in the low half; a row stands for (code - zero) * scale.  Zero points are whole numbers of the grid;
+ * k_zero = v_zero = NULL: a symmetric cache, whose zero points are 0.  page_size: a multiple of 16; head_dim: a multiple of 16
+ * (8 bits) or 32 (4 bits), at most 256; buffers 16-byte aligned; at most 2^31 - 1 slots. */
+typedef struct lq_kv_cache {
+    uint8_t* k_codes;
+    uint8_t* v_codes;
+    float* k_scale;
+    float* v_scale;
+    float* k_zero;
+    float* v_zero;
+    int num_pages, page_size, kv_heads, head_dim, bits;
+} lq_kv_cache;
+/* Quantizes the keys and values of `tokens` tokens into their slots.  k, v: LQ_F32 or LQ_F16, kv_heads * head_dim values per
+ * token, tokens ldk / ldv values apart (slices of a packed qkv row are taken), rows 16-byte aligned.  A slot that is negative or
+ * beyond the cache is skipped; slots of one call are distinct otherwise (of tokens that share one, codes and scale may come from
+ * different ones). */
+int lq_kv_cache_write(const lq_kv_cache* cache, const void* k, const void* v, int dtype, size_t ldk, size_t ldv, const int32_t* slots,
+                      size_t tokens, lq_stream stream);
+/* The rows of `tokens` slots as LQ_F32 or LQ_F16 [tokens, kv_heads, head_dim]: (code - zero) * scale in float32, float16 rounded
+ * from that.  A slot that is negative or beyond the cache gives zeros. */
+int lq_kv_cache_read(const lq_kv_cache* cache, const int32_t* slots, size_t tokens, void* k, void* v, int dtype, lq_stream stream);
+/* Attention of new tokens over their sequences' pages.  q: LQ_F32 or LQ_F16 [tokens, heads, head_dim], tokens ldq values apart;
+ * out the same type, contiguous.  Query head i reads key / value head i / (heads / kv_heads).  Sequence b's queries are rows
+ * q_starts[b] .. q_starts[b + 1] (int32 [batch + 1], rising), its keys the first kv_lens[b] tokens of the pages page_table[b, :]
+ * (int32 [batch, table_width]), which hold the new tokens too; its last query sits at the last key.  A query at place p sees the
+ * keys j <= p (all when causal == 0), of those j > p - window when window > 0:
+ *     out = sum_j softmax_j(scale * q . k_j) v_j
+ * Queries that see no key, and rows of no sequence, give zeros.  Keys of a page that is negative or beyond the cache are not
+ * seen; lengths beyond the table are cut to it.  Scores, sums and products are float32: codes enter the matrix products as the
+ * whole numbers they are, scales after them; float16 queries and probabilities as one float16, float32 ones as two, of 22 bits together.  max_chunk: the
+ * most queries of a sequence, or 0; the work is divided by it, and results differ by rounding alone. */
+int lq_paged_attention(const lq_kv_cache* cache, const void* q, size_t ldq, void* out, int dtype, int tokens, int heads, int batch,
+                       const int32_t* page_table, int table_width, const int32_t* q_starts, const int32_t* kv_lens, float scale, int causal,
+                       int window, int max_chunk, lq_stream stream);
+
 /* ------------------------------------------------- ranges kept by the producer */
 /* Dynamic per-tensor quantization of a small tensor (n <= 262144) in one launch:
  * global min / max (MinMaxObserver, observer.py:363-375; x.min() / x.max() in

@@ -257,6 +257,18 @@ class LstmArgs(C.Structure):
     ]
 
 
+class KvCache(C.Structure):
+    """``lq_kv_cache`` of ``include/lucid_hip.h``."""
+
+    _fields_ = [
+        ("k_codes", _vp), ("v_codes", _vp), ("k_scale", _vp), ("v_scale", _vp), ("k_zero", _vp), ("v_zero", _vp),
+        ("num_pages", _i), ("page_size", _i), ("kv_heads", _i), ("head_dim", _i), ("bits", _i),
+    ]
+
+
+_SIGNATURES["lq_kv_cache_write"] = [C.POINTER(KvCache), _vp, _vp, _i, _sz, _sz, _vp, _sz, _vp]
+_SIGNATURES["lq_kv_cache_read"] = [C.POINTER(KvCache), _vp, _sz, _vp, _vp, _i, _vp]
+_SIGNATURES["lq_paged_attention"] = [C.POINTER(KvCache), _vp, _sz, _vp, _i, _i, _i, _i, _vp, _i, _vp, _vp, _f, _i, _i, _i, _vp]
 _SIGNATURES["lq_lstm_sequence_pays"] = [_i] * 3 + [C.POINTER(_i)]
 _SIGNATURES["lq_lstm_fused_layers"] = [_i] * 6 + [C.POINTER(_i)]
 _SIGNATURES["lq_lstm_sequence_f32"] = [C.POINTER(LstmArgs), _vp]

@@ -6,6 +6,7 @@ kernel; inputs and outputs are float32 tensors on the ``hip`` device.
 
 from __future__ import annotations
 
+import ctypes as C
 import math
 
 from .. import _C
@@ -108,6 +109,74 @@ def scaled_dot_product_attention_qkv(qkv: Tensor, num_heads: int, scale: float |
     out._range = _new_range() if track_range else None
     _C.call("lq_attention_f32", qkv.data_ptr, out.data_ptr, B, Tn, num_heads, D, s,
             out._range.data_ptr if track_range else None, None)
+    return out
+
+
+def _paged_attention(name, cache, q_ptr, ldq, dtype, tokens, heads, out, page_table, q_starts, kv_lens, scale, causal, window, max_chunk) -> None:
+    from ..quantization._kv_cache import _check_ids
+    if not isinstance(page_table, Tensor) or page_table.ndim != 2:
+        raise _C.ShapeMismatch(f"{name}: page_table is a (batch, pages) tensor")
+    batch, width = page_table.shape
+    _check_ids(name, "page_table", page_table, page_table.shape)
+    _check_ids(name, "q_starts", q_starts, (batch + 1,))
+    _check_ids(name, "kv_lens", kv_lens, (batch,))
+    if heads < 1 or heads % cache.kv_heads:
+        raise _C.ShapeMismatch(f"{name}: {heads} query heads for {cache.kv_heads} key / value heads")
+    if window is not None and window < 1:
+        raise ValueError(f"{name}: window {window}; at least 1, or None for all keys")
+    if max_chunk is not None and max_chunk < 1:
+        raise ValueError(f"{name}: max_chunk {max_chunk}; at least 1, or None")
+    _C.call("lq_paged_attention", C.byref(cache._struct), q_ptr, ldq, out.data_ptr, dtype.code, tokens, heads, batch, page_table.data_ptr, width,
+            q_starts.data_ptr, kv_lens.data_ptr, 1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale), 1 if causal else 0,
+            0 if window is None else window, 0 if max_chunk is None else max_chunk, None)
+
+
+def paged_attention(q: Tensor, cache, page_table: Tensor, q_starts: Tensor, kv_lens: Tensor, scale: float | None = None, causal: bool = True,
+                    window: int | None = None, max_chunk: int | None = None, out: Tensor | None = None) -> Tensor:
+    """Attention of new tokens over the pages of their sequences in a ``quantization.PagedKVCache``.
+
+    ``q`` is ``(tokens, heads, head_dim)``, float32 or float16, and so is the result; ``heads`` is a multiple of the cache's
+    ``kv_heads``, and query head ``i`` reads key / value head ``i // (heads // kv_heads)``.  The tokens of sequence ``b`` are rows
+    ``q_starts[b]`` to ``q_starts[b + 1]`` (int32 ``(batch + 1,)``, rising); its keys are the first ``kv_lens[b]`` (int32
+    ``(batch,)``) tokens of the pages ``page_table[b]`` (int32 ``(batch, pages)``), its own new tokens, already written, the last of them.
+    A token sees the keys up to its own (all with ``causal=False``), with ``window`` the last ``window`` of those up to its own place.
+    Tokens that see no key, and rows of ``q`` that belong to no sequence (a padded batch), give zeros.  Keys of a page
+    that is negative or beyond the cache are not seen; a length beyond ``page_table`` is cut to it.
+
+    ``max_chunk``: the most tokens of a sequence in this call, where the program knows it; the work is divided by
+    it, and results differ by rounding alone.  Default ``scale``: ``1 / sqrt(head_dim)``."""
+    from ..quantization._kv_cache import _check_cache, _check_rows
+    _check_cache("paged_attention", cache)
+    if not isinstance(q, Tensor) or q.ndim != 3:
+        raise _C.ShapeMismatch("paged_attention: q is a (tokens, heads, head_dim) tensor")
+    tokens, heads, _ = q.shape
+    _check_rows("paged_attention", "q", q, (tokens, heads, cache.head_dim))
+    if out is None:
+        out = Tensor.empty(q.shape, q.dtype, "hip")
+    else:
+        _check_rows("paged_attention", "out", out, q.shape)
+        if out.dtype != q.dtype:
+            raise _C.DtypeMismatch(f"paged_attention: q is {q.dtype}, out {out.dtype}")
+    _paged_attention("paged_attention", cache, q.data_ptr, heads * cache.head_dim, q.dtype, tokens, heads, out, page_table, q_starts, kv_lens, scale,
+                     causal, window, max_chunk)
+    return out
+
+
+def paged_attention_qkv(qkv: Tensor, num_heads: int, cache, page_table: Tensor, q_starts: Tensor, kv_lens: Tensor, scale: float | None = None,
+                        causal: bool = True, window: int | None = None, max_chunk: int | None = None) -> Tensor:
+    """``paged_attention`` of the queries in the packed output of a qkv Linear, ``(..., (num_heads + 2 * kv_heads) * head_dim)`` with the
+    queries first; the keys and values beside them are those that ``quantization.kv_cache_write_qkv`` has written.  Returns
+    ``(..., num_heads * head_dim)``."""
+    from ..quantization._kv_cache import _check_cache, _check_rows
+    _check_cache("paged_attention_qkv", cache)
+    num_heads = int(num_heads)
+    row = (num_heads + 2 * cache.kv_heads) * cache.head_dim
+    if not isinstance(qkv, Tensor) or qkv.ndim < 2 or qkv.shape[-1] != row:
+        raise _C.ShapeMismatch(f"paged_attention_qkv: qkv has rows of {num_heads} + 2 * {cache.kv_heads} heads of {cache.head_dim}, {row} values")
+    _check_rows("paged_attention_qkv", "qkv", qkv, qkv.shape)
+    out = Tensor.empty((*qkv.shape[:-1], num_heads * cache.head_dim), qkv.dtype, "hip")
+    _paged_attention("paged_attention_qkv", cache, qkv.data_ptr, row, qkv.dtype, qkv.numel // row, num_heads, out, page_table, q_starts, kv_lens,
+                     scale, causal, window, max_chunk)
     return out
 
 

@@ -1,0 +1,92 @@
+"""What the key / value cache and its attention refuse, without a device: Python's checks, and those of the C entry points (the
+pointers given are never followed)."""
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import lucid_amd as L
+import lucid_amd.nn.functional as F
+import lucid_amd.quantization as Q
+from lucid_amd import _C
+
+P = 4096  # an aligned address that nothing reads
+
+
+def struct(**kw):
+    d = dict(k_codes=P, v_codes=P, k_scale=P, v_scale=P, k_zero=None, v_zero=None, num_pages=4, page_size=16, kv_heads=2, head_dim=64, bits=8)
+    d.update(kw)
+    return _C.KvCache(*d.values())
+
+
+@pytest.mark.parametrize("kw,error", [
+    (dict(num_pages=0), L.ShapeMismatch), (dict(kv_heads=0), L.ShapeMismatch), (dict(page_size=0), L.ShapeMismatch),
+    (dict(page_size=24), L.ShapeMismatch), (dict(num_pages=1 << 27, page_size=16), L.ShapeMismatch), (dict(head_dim=8), NotImplementedError),
+    (dict(head_dim=272), NotImplementedError), (dict(head_dim=72), NotImplementedError), (dict(head_dim=48, bits=4), NotImplementedError),
+    (dict(bits=2), NotImplementedError), (dict(k_codes=None), ValueError), (dict(v_scale=None), ValueError), (dict(k_zero=P), ValueError),
+    (dict(v_codes=P + 8), ValueError), (dict(k_zero=P, v_zero=P + 4), ValueError)])
+def test_c_entries_refuse_a_bad_cache(kw, error):
+    c = C.byref(struct(**kw))
+    with pytest.raises(error):
+        _C.call("lq_kv_cache_write", c, P, P, _C.F32, 128, 128, P, 1, None)
+    with pytest.raises(error):
+        _C.call("lq_kv_cache_read", c, P, 1, P, P, _C.F32, None)
+    with pytest.raises(error):
+        _C.call("lq_paged_attention", c, P, 128, P, _C.F32, 1, 2, 1, P, 1, P, P, 1.0, 1, 0, 0, None)
+
+
+@pytest.mark.parametrize("at,value,error", [
+    (1, None, ValueError), (1, P + 4, ValueError), (2, None, ValueError), (3, _C.I8, L.DtypeMismatch), (3, _C.BF16, L.DtypeMismatch),
+    (4, 124, L.ShapeMismatch), (4, 130, ValueError), (5, 64, L.ShapeMismatch), (6, None, ValueError), (7, 1 << 40, L.ShapeMismatch)])
+def test_c_write_refuses(at, value, error):
+    args = [C.byref(struct()), P, P, _C.F32, 128, 128, P, 1, None]
+    args[at] = value
+    with pytest.raises(error, match="kv_cache_write"):
+        _C.call("lq_kv_cache_write", *args)
+
+
+@pytest.mark.parametrize("at,value,error", [
+    (1, None, ValueError), (2, 1 << 40, L.ShapeMismatch), (3, None, ValueError), (4, P + 8, ValueError), (5, _C.F64, L.DtypeMismatch)])
+def test_c_read_refuses(at, value, error):
+    args = [C.byref(struct()), P, 1, P, P, _C.F16, None]
+    args[at] = value
+    with pytest.raises(error, match="kv_cache_read"):
+        _C.call("lq_kv_cache_read", *args)
+
+
+@pytest.mark.parametrize("at,value,error", [
+    (1, None, ValueError), (1, P + 8, ValueError), (2, 192, L.ShapeMismatch), (2, 258, ValueError), (3, None, ValueError),
+    (4, _C.I32, L.DtypeMismatch), (5, -1, ValueError), (5, 1 << 24, L.ShapeMismatch), (6, 3, L.ShapeMismatch), (6, 0, L.ShapeMismatch),
+    (7, -1, ValueError), (8, None, ValueError), (9, -1, ValueError), (9, 1 << 27, L.ShapeMismatch), (10, None, ValueError),
+    (11, None, ValueError), (14, -1, ValueError), (15, -2, ValueError)])
+def test_c_attention_refuses(at, value, error):
+    args = [C.byref(struct()), P, 256, P, _C.F32, 1, 4, 1, P, 1, P, P, 1.0, 1, 0, 0, None]
+    args[at] = value
+    with pytest.raises(error, match="paged_attention"):
+        _C.call("lq_paged_attention", *args)
+
+
+def test_c_entries_without_tokens_do_nothing():
+    c = C.byref(struct())
+    _C.call("lq_kv_cache_write", c, None, None, _C.F32, 0, 0, None, 0, None)
+    _C.call("lq_kv_cache_read", c, None, 0, None, None, _C.F32, None)
+    _C.call("lq_paged_attention", c, None, 0, None, _C.F32, 0, 4, 1, P, 1, P, P, 1.0, 1, 0, 0, None)
+
+
+@pytest.mark.parametrize("args,error", [
+    ((0, 16, 2, 64), L.ShapeMismatch), ((4, 8, 2, 64), L.ShapeMismatch), ((4, 40, 2, 64), L.ShapeMismatch), ((4, 16, 0, 64), L.ShapeMismatch),
+    ((1 << 27, 16, 1, 16), L.ShapeMismatch), ((4, 16, 2, 20), NotImplementedError), ((4, 16, 2, 512), NotImplementedError),
+    ((4, 16, 2, 48, Q.per_channel_affine, Q.qint4), NotImplementedError), ((4, 16, 2, 64, Q.per_tensor_affine), ValueError),
+    ((4, 16, 2, 64, Q.per_channel_affine, Q.quint8), NotImplementedError), ((4, 16, 2, 64, "per_channel_affine"), ValueError)])
+def test_a_cache_refuses_what_no_kernel_takes(args, error):
+    with pytest.raises(error, match="PagedKVCache"):
+        Q.PagedKVCache(*args)
+
+
+def test_operators_want_a_cache():
+    x = L.tensor(np.zeros((1, 2, 64), np.float32))
+    for f in (lambda: Q.kv_cache_write(None, x, x, x), lambda: Q.kv_cache_write_qkv(x, x, 2, x), lambda: Q.kv_cache_read({}, x),
+              lambda: F.paged_attention(x, None, x, x, x), lambda: F.paged_attention_qkv(x, 2, "cache", x, x, x)):
+        with pytest.raises(TypeError, match="PagedKVCache"):
+            f()
