@@ -452,7 +452,7 @@ int lq_bias_act_f32(float* y, const float* bias, size_t M, int N, int relu, lq_s
  * _functional.py:164-182), on the signed grid of its bits: [-128, 127] or [-8, 7].  Stored is code - qmin, two 4-bit codes in a
  * byte, the first in the low half; a row stands for (code - zero) * scale.  Zero points are whole numbers of the grid;
  * k_zero = v_zero = NULL: a symmetric cache, whose zero points are 0.  page_size: a multiple of 16; head_dim: a multiple of 16
- * (8 bits) or 32 (4 bits), at most 256; buffers 16-byte aligned; at most 2^31 - 1 slots. */
+ * (8 bits) or 32 (4 bits), at most 256; buffers 16-byte aligned; at most 2^31 - 1 slots and 65535 heads. */
 typedef struct lq_kv_cache {
     uint8_t* k_codes;
     uint8_t* v_codes;

@@ -8,7 +8,7 @@ namespace lq {
 inline int check_kv_cache(const lq_kv_cache* c, const char* name) {
     LQ_REQUIRE(c, LQ_ERR_VALUE, "%s: cache is NULL", name);
     LQ_REQUIRE(c->bits == 8 || c->bits == 4, LQ_ERR_NOT_IMPLEMENTED, "%s: codes of %d bits; 8 and 4 are built", name, c->bits);
-    LQ_REQUIRE(c->num_pages >= 1 && c->kv_heads >= 1, LQ_ERR_SHAPE, "%s: a cache of %d pages and %d heads", name, c->num_pages, c->kv_heads);
+    LQ_REQUIRE(c->num_pages >= 1 && c->kv_heads >= 1 && c->kv_heads <= 65535, LQ_ERR_SHAPE, "%s: a cache of %d pages and %d heads", name, c->num_pages, c->kv_heads);
     LQ_REQUIRE(c->page_size >= 16 && c->page_size % 16 == 0, LQ_ERR_SHAPE, "%s: pages of %d tokens; a multiple of 16 is needed", name,
                c->page_size);
     const int step = 128 / c->bits;  // (16 bytes of codes)

@@ -1,97 +1,10 @@
 // Attention of new tokens over the pages of a quantized key / value cache (lq_paged_attention).
+#include <algorithm>
 #include <type_traits>
 
-#include "kv_cache.hpp"
+#include "paged_attention.hpp"
 
 using namespace lq;
-
-namespace {
-
-struct AttnArgs {
-    const uint8_t* k_codes;
-    const uint8_t* v_codes;
-    const float* k_scale;
-    const float* v_scale;
-    const float* k_zero;
-    const float* v_zero;
-    const int* table;
-    const int* q_starts;
-    const int* kv_lens;
-    size_t ldq;
-    int pages, page_size, kv_heads, dim, tokens, heads, batch, width, causal, window;
-    float scale;
-};
-
-// a wavefront per row and head: lane = key for the scores, then lane = column for the values
-template <class T, int BITS>
-__global__ __launch_bounds__(64) void paged_attention_simple_kernel(AttnArgs a, const T* __restrict__ q, T* __restrict__ out) {
-    __shared__ float sq[256], sp[64];
-    __shared__ int srow[64];
-    const int lane = threadIdx.x, head = blockIdx.x % a.heads, row = blockIdx.x / a.heads;
-    const int kv = head / (a.heads / a.kv_heads);
-    int b = -1;
-    for (int i = 0; i < a.batch; ++i)
-        if (row >= a.q_starts[i] && row < a.q_starts[i + 1]) b = i;
-    float acc[4] = {}, m = -__builtin_inff(), l = 0.f;
-    if (b >= 0) {
-        const int len = a.kv_lens[b] < a.width * a.page_size ? a.kv_lens[b] : a.width * a.page_size;
-        const int place = len - a.q_starts[b + 1] + row;
-        const int end = a.causal && place + 1 < len ? place + 1 : len;
-        const int begin = a.window > 0 && place - a.window + 1 > 0 ? place - a.window + 1 : 0;
-        for (int d = lane; d < a.dim; d += 64) sq[d] = float(q[size_t(row) * a.ldq + size_t(head) * a.dim + d]);
-        __syncthreads();
-        const float qmin = -float(1 << (BITS - 1));
-        for (int j0 = begin; j0 < end; j0 += 64) {
-            const int j = j0 + lane;
-            int r = -1;
-            float s = -__builtin_inff();
-            if (j < end) {
-                const int page = a.table[size_t(b) * a.width + j / a.page_size];
-                if (unsigned(page) < unsigned(a.pages)) {
-                    const size_t at = (size_t(page) * a.kv_heads + kv) * a.page_size + j % a.page_size;
-                    r = page * a.page_size + j % a.page_size;
-                    const float z = qmin - (a.k_zero ? a.k_zero[at] : 0.f);
-                    float dot = 0.f;
-                    for (int d = 0; d < a.dim; ++d) {
-                        const size_t e = at * a.dim + d;
-                        const unsigned u = BITS == 8 ? a.k_codes[e] : a.k_codes[e / 2] >> (e % 2 * 4) & 15;
-                        dot = __builtin_fmaf(sq[d], float(u) + z, dot);
-                    }
-                    s = dot * a.k_scale[at] * a.scale;
-                }
-            }
-            float top = s;
-            for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-            const float mn = fmaxf(m, top), use = mn == -__builtin_inff() ? 0.f : mn;
-            const float p = r < 0 ? 0.f : __expf(s - use), f = __expf(m - use);
-            float sum = p;
-            for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
-            l = l * f + sum, m = mn;
-            __syncthreads();
-            sp[lane] = p, srow[lane] = r;
-            __syncthreads();
-            for (int i = 0; i < 4; ++i) acc[i] *= f;
-            for (int t = 0; t < 64; ++t) {
-                if (srow[t] < 0) continue;
-                const size_t at = (size_t(srow[t] / a.page_size) * a.kv_heads + kv) * a.page_size + srow[t] % a.page_size;
-                const float z = qmin - (a.v_zero ? a.v_zero[at] : 0.f), w = sp[t] * a.v_scale[at];
-                for (int i = 0; i < 4; ++i) {
-                    const int d = lane + 64 * i;
-                    if (d >= a.dim) break;
-                    const size_t e = at * a.dim + d;
-                    const unsigned u = BITS == 8 ? a.v_codes[e] : a.v_codes[e / 2] >> (e % 2 * 4) & 15;
-                    acc[i] = __builtin_fmaf(w, float(u) + z, acc[i]);
-                }
-            }
-        }
-    }
-    for (int i = 0; i < 4; ++i) {
-        const int d = lane + 64 * i;
-        if (d < a.dim) out[(size_t(row) * a.heads + head) * a.dim + d] = T(l == 0.f ? 0.f : acc[i] / l);
-    }
-}
-
-}  // namespace
 
 extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ldq, void* out, int dtype, int tokens, int heads, int batch,
                                   const int32_t* page_table, int table_width, const int32_t* q_starts, const int32_t* kv_lens, float scale,
@@ -110,15 +23,31 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
     LQ_REQUIRE(int64_t(tokens) * heads <= 1 << 25, LQ_ERR_SHAPE, "paged_attention: %d tokens of %d heads (at most 2^25 rows)", tokens, heads);
     LQ_REQUIRE(int64_t(table_width) * c->page_size <= 0x40000000, LQ_ERR_SHAPE, "paged_attention: %d pages of %d tokens (at most 2^30 keys)",
                table_width, c->page_size);
-    AttnArgs a;
+    AttnArgs a{};
     a.k_codes = c->k_codes, a.v_codes = c->v_codes, a.k_scale = c->k_scale, a.v_scale = c->v_scale, a.k_zero = c->k_zero, a.v_zero = c->v_zero;
     a.table = page_table, a.q_starts = q_starts, a.kv_lens = kv_lens, a.ldq = ldq;
-    a.pages = c->num_pages, a.page_size = c->page_size, a.kv_heads = c->kv_heads, a.dim = c->head_dim;
-    a.tokens = tokens, a.heads = heads, a.batch = batch, a.width = table_width, a.causal = causal, a.window = window, a.scale = scale;
+    a.page_size = FastDiv(unsigned(c->page_size)), a.group = FastDiv(unsigned(heads / c->kv_heads));
+    a.pages = c->num_pages, a.kv_heads = c->kv_heads, a.dim = c->head_dim;
+    a.tokens = tokens, a.heads = heads, a.batch = batch, a.width = table_width, a.causal = causal != 0, a.window = window, a.scale = scale;
+    const int group = heads / c->kv_heads;
+    const int sequences = std::min(batch, tokens);
+    const int chunk = max_chunk ? std::min(max_chunk, tokens) : batch == 1 ? tokens : (tokens + batch - 1) / std::max(batch, 1);
+    const int qt = chunk * group <= 16 ? 1 : 2, rows = 16 * qt;
+    const int tiles = sequences + int(int64_t(tokens) * group / rows);
+    a.target = 512, a.max_rows = 0x7fffffff;
+    a.items = tiles + (a.target + a.kv_heads - 1) / a.kv_heads;
+    const bool join = int64_t(table_width) * c->page_size > attn::kMinKeys;
+    auto lock = scratch_lock(as_stream(stream));
+    if (join) {
+        const int dim = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
+        void* p = nullptr;
+        rc = call_buffer(9, size_t(a.items) * a.kv_heads * rows * (dim + 2) * sizeof(float), as_stream(stream), &p);
+        if (rc) return rc;
+        a.partial = static_cast<float*>(p);
+    }
     auto launch = [&](auto type, auto bits) {
         using T = decltype(type);
-        paged_attention_simple_kernel<T, decltype(bits)::value>
-            <<<unsigned(tokens * heads), 64, 0, as_stream(stream)>>>(a, static_cast<const T*>(q), static_cast<T*>(out));
+        attn::launch_rows_of<T, decltype(bits)::value>(a, static_cast<const T*>(q), static_cast<T*>(out), tiles, qt, join, as_stream(stream));
     };
     using B8 = std::integral_constant<int, 8>;
     using B4 = std::integral_constant<int, 4>;

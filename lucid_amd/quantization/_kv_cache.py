@@ -40,7 +40,7 @@ class PagedKVCache:
         self.num_pages, self.page_size, self.kv_heads, self.head_dim = int(num_pages), int(page_size), int(kv_heads), int(head_dim)
         self.qscheme, self.qdtype = qscheme, qdtype
         step = 128 // qdtype.bits
-        if self.num_pages < 1 or self.kv_heads < 1 or self.page_size < 16 or self.page_size % 16:
+        if self.num_pages < 1 or not 1 <= self.kv_heads <= 65535 or self.page_size < 16 or self.page_size % 16:
             raise _C.ShapeMismatch(f"PagedKVCache: {num_pages} pages of {page_size} tokens with {kv_heads} heads (pages are multiples of 16)")
         if self.num_pages * self.page_size > 0x7fffffff:
             raise _C.ShapeMismatch(f"PagedKVCache: {num_pages} pages of {page_size} tokens are more than 2^31 - 1 slots")
