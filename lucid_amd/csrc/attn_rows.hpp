@@ -10,7 +10,6 @@
 //                  either 16, eight slots of 32 keys.  A: the lane reads the same eight keys at DIM / 16 neighbouring columns, and a few
 //                  byte permutations turn them into column tiles: tile j is columns i * DIM / 16 + j, i = 0..15.
 //
-// The next 32 keys are requested before these are worked on, their page numbers before that.
 #pragma once
 #include <type_traits>
 
@@ -24,21 +23,17 @@ struct RowsKernel {
     static constexpr bool F32 = std::is_same_v<T, float>;
     static constexpr int PARTS = F32 ? 2 : 1;  // float16 parts of a float32
     static constexpr int R = 16 * QT, WAVES = 4, SLABS = DIM / 32, TILES = DIM / 16;
+    static constexpr int NT = rows_keys(BITS, DIM, QT) / 16, KEYS = 16 * NT, UNIT = KEYS * WAVES;
     static constexpr int KW = DIM * BITS / 128;      // dwords of a key per lane
     static constexpr int VB = DIM / 16 * BITS / 8;   // bytes of a key of V per lane
     static constexpr int VW = VB < 4 ? 1 : VB / 4;
     static constexpr int LDS_ROW = DIM + 4;          // floats
-    static constexpr int LDS_BYTES = 2 * 16 * LDS_ROW * 4;
-
-    // 32 keys
-    struct Step {
-        uint32_t k[2][KW];
-        uint32_t v[8][VW];
-        f32x4 ks[2], vs[2], vz[2];
-        float kz[2];
-        int at;       // the first key
-        int ok;       // bit t: the 16 keys of tile t lie on a page
-    };
+    static constexpr int ROWS = DIM <= 128 ? 16 : 8;  // rows that the wavefronts' results have room for at a time
+    // queries take registers of every wavefront, or, where they are many, LDS
+    static constexpr int FRAGS = QT * SLABS * PARTS;
+    static constexpr bool Q_LDS = FRAGS >= 16;
+    static constexpr int JOIN_BYTES = WAVES * ROWS * LDS_ROW * 4, Q_BYTES = Q_LDS ? FRAGS * 1024 : 0;
+    static constexpr int LDS_BYTES = JOIN_BYTES > Q_BYTES ? JOIN_BYTES : Q_BYTES;
 
     // first column of slab i's eight of lanes g
     static __device__ __forceinline__ int column(int i, int g) {
@@ -47,182 +42,261 @@ struct RowsKernel {
         else return 128 * (i / 4) + 32 * g + 8 * (i % 4);
     }
 
+    using Segs = Segments<R, UNIT>;
+
     static __device__ __forceinline__ void run(const AttnArgs& a, const T* __restrict__ q, T* __restrict__ out, float* lds) {
+        clear_other_rows(a, out, blockIdx.x, gridDim.x);
+        unsigned x = 0, end = 0, per_head = 0;
+        while (true) {
+            typename Segs::Segment seg;
+            unsigned head;
+            {  // (found anew for each segment: kept, what it takes would cost the registers of a wavefront)
+                Segs segs(a);
+                if (per_head == 0) {
+                    per_head = segs.total;
+                    const unsigned all = per_head * unsigned(a.kv_heads), share = a.each ? segs.share() : 1u;
+                    if (all == 0 || blockIdx.x > (all - 1) / share) return;
+                    x = blockIdx.x * share, end = min(all, x + share);
+                }
+                head = x / per_head;
+                seg = segs.at(x - head * per_head);
+            }
+            const unsigned n = min(seg.units - seg.unit, end - x);
+            float* piece = n == seg.units ? nullptr : a.partial + (2 * size_t(blockIdx.x) + (seg.unit ? 0 : 1)) * kPiece<R, DIM>;
+            segment(a, q, out, lds, seg, int(head), n, piece);
+            x += n;
+            if (x >= end) break;
+            __syncthreads();
+        }
+    }
+
+    // `n` units of a segment from its unit on; piece: where the sums go, or NULL for the result
+    static __device__ __forceinline__ void segment(const AttnArgs& a, const T* __restrict__ q, T* __restrict__ out, float* lds,
+                                                   const typename Segs::Segment& it, int head, unsigned n, float* piece) {
         const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
         const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
-        const int head = blockIdx.y, group = int(a.group.d);
-        clear_other_rows(a, out, blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y);
-        Item it;
-        if (!find_item<R>(a, blockIdx.x, false, it)) return;
+        const int group = int(a.group.d);
         const int rows = it.s.chunk * group, row0 = it.tile * R, at = it.s.len - it.s.chunk;
         const int last_row = min(rows, row0 + R) - 1;
         const int first_token = int(a.group(unsigned(row0))), last_token = int(a.group(unsigned(last_row)));
         const Keys seen = keys_of(a, it.s, first_token, last_token);
-        // this item's keys
-        const int base = seen.lo & ~31, share = ((seen.hi - base + it.parts - 1) / it.parts + kMinKeys - 1) / kMinKeys * kMinKeys;
-        const int from = min(seen.hi, base + it.part * share), to = min(seen.hi, from + share);
+        // these keys
+        const int from = min(seen.hi, (seen.lo & ~31) + int(it.unit) * UNIT);
+        const int to = a.each ? min(seen.hi, from + int(n) * UNIT) : seen.hi;
         // keys that all rows see: between them nothing is masked
         const int all_lo = a.window > 0 ? max(0, at + last_token - a.window + 1) : 0;
         const int all_hi = a.causal ? min(it.s.len, at + first_token + 1) : it.s.len;
 
-        // queries: column c of tile t is row row0 + 16 t + c
-        h8 qf[QT][SLABS][PARTS];
-        float factor[QT];
+        // queries: column c of tile t is row row0 + 16 t + c.  Requested ahead of the keys, turned into fragments behind those requests;
+        // what lies past the head's columns or the last row is read from where there is something, and dropped.
+        using Raw = std::conditional_t<F32, f32x4, h8>;
+        Raw raw[QT][SLABS][PARTS];
         int lo[QT], hi[QT];
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
-            const int row = row0 + 16 * t + c, used = min(row, last_row);
-            const int token = int(a.group(unsigned(used))), h = head * group + (used - token * group);
-            const T* src = q + size_t(it.s.q0 + token) * a.ldq + size_t(h) * a.dim;
+            const int used = min(row0 + 16 * t + c, last_row), token = int(a.group(unsigned(used)));
+            const T* src = q + size_t(it.s.q0 + token) * a.ldq + size_t(head * group + (used - token * group)) * a.dim;
             const Keys mine = keys_of(a, it.s, token, token);
             lo[t] = mine.lo, hi[t] = mine.hi;
-            factor[t] = a.scale * kLog2e;
-            float x[SLABS][8];
-            float top = 0.f;
 #pragma unroll
             for (int i = 0; i < SLABS; ++i) {
                 const int d = column(i, g);
-                const bool there = d < a.dim && row <= last_row;
-                if constexpr (F32) {
-                    const float4 u = there ? *reinterpret_cast<const float4*>(src + d) : float4{0, 0, 0, 0};
-                    const float4 w = there ? *reinterpret_cast<const float4*>(src + d + 4) : float4{0, 0, 0, 0};
-                    x[i][0] = u.x, x[i][1] = u.y, x[i][2] = u.z, x[i][3] = u.w, x[i][4] = w.x, x[i][5] = w.y, x[i][6] = w.z, x[i][7] = w.w;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[i][e]));
-                } else {
-                    h8 u = {};
-                    if (there) u = *reinterpret_cast<const h8*>(src + d);
-                    // 4-bit codes leave a dword in the order 0 4 1 5 2 6 3 7
-                    if constexpr (BITS == 4) u = __builtin_shufflevector(u, u, 0, 4, 1, 5, 2, 6, 3, 7);
-                    qf[t][i][0] = u;
+                for (int p = 0; p < PARTS; ++p) raw[t][i][p] = reinterpret_cast<const Raw*>(src + (d < a.dim ? d : 0))[p];
+            }
+        }
+
+        const int row_bytes = a.dim * BITS / 8;
+        const int* table = a.table + size_t(it.seq) * a.width;
+        // Page numbers a step ahead, by a vector load (the compiler moves scalar loads to where they are used): lanes 0 to NT - 1 have those
+        // of a step's tiles.  An index past the table reads 0, and its keys are past `to`.
+        const auto table_rows = rows_at(table, a.width * 4);
+        auto pages_of = [&](int key) {
+            return int(__builtin_amdgcn_raw_buffer_load_b32(table_rows, int(a.page_size(unsigned(key + 16 * (lane & (NT - 1))))) * 4, 0, 0));
+        };
+        // lane offsets: key c's codes, and four keys' columns; lanes past the head's columns read the first ones (and meet zeros of q,
+        // or make columns that nobody stores)
+        int k_off[(KW + 3) / 4];
+#pragma unroll
+        for (int i = 0; i < (KW + 3) / 4; ++i) {
+            const int d = column(i * (16 / BITS), g);
+            k_off[i] = c * row_bytes + (d < a.dim ? d * BITS / 8 : 0);
+        }
+        const int v_off = 4 * g * row_bytes + (c * TILES < a.dim ? c * VB : 0);
+        // 32 keys at a time.  One set of registers: each part is requested again as soon as its last reader has had it, codes of K
+        // behind the scores, scales behind the probabilities, V behind the products.
+        uint32_t kw[NT][KW], vw[4 * NT][VW];
+        f32x4 ks[NT], vs4[NT], vz[NT];
+        float kz[NT];
+        size_t place[NT];  // rows of the cache where the tiles begin
+        int ok = 0;       // bit t: tile t lies on a page
+        auto locate = [&](int key, int pages) {
+            ok = 0;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const unsigned page = unsigned(__builtin_amdgcn_readlane(pages, t));
+                const bool there = key + 16 * t < to && page < unsigned(a.pages);
+                ok |= int(there) << t;
+                const unsigned in_page = unsigned(key + 16 * t) - a.page_size(unsigned(key + 16 * t)) * a.page_size.d;
+                place[t] = there ? (size_t(page) * unsigned(a.kv_heads) + unsigned(head)) * a.page_size.d + in_page : 0;
+            }
+        };
+        constexpr int ONCE = 2;  // non-temporal: 4352 keys of 64 sequences 112 -> 104 us
+        auto request_k = [&] {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const auto rows = rows_at(a.k_codes + place[t] * unsigned(row_bytes), 16 * row_bytes);
+#pragma unroll
+                for (int i = 0; i < (KW + 3) / 4; ++i) {
+                    if constexpr (KW >= 4) {
+                        const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(rows, k_off[i], 0, ONCE);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) kw[t][4 * i + e] = w[e];
+                    } else {
+                        const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(rows, k_off[i], 0, ONCE);
+                        kw[t][0] = w[0], kw[t][1] = w[1];
+                    }
+                }
+                if constexpr (AFFINE) kz[t] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows_at(a.k_zero + place[t], 64), 4 * c, 0, 0));
+            }
+        };
+        auto four = [&](const float* p) {
+            return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rows_at(p, 64), 16 * g, 0, 0));
+        };
+        auto request_scales = [&] {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) ks[t] = four(a.k_scale + place[t]), vs4[t] = four(a.v_scale + place[t]);
+        };
+        auto request_v = [&] {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const auto rows = rows_at(a.v_codes + place[t] * unsigned(row_bytes), 16 * row_bytes);
+                if constexpr (AFFINE) vz[t] = four(a.v_zero + place[t]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t(&w)[VW] = vw[4 * t + e];
+                    const int skip = e * row_bytes;
+                    if constexpr (VB == 2) {
+                        w[0] = __builtin_amdgcn_raw_buffer_load_b16(rows, v_off, skip, ONCE);
+                    } else if constexpr (VB == 4) {
+                        w[0] = __builtin_amdgcn_raw_buffer_load_b32(rows, v_off, skip, ONCE);
+                    } else if constexpr (VB == 8) {
+                        const u32x2 u = __builtin_amdgcn_raw_buffer_load_b64(rows, v_off, skip, ONCE);
+                        w[0] = u[0], w[1] = u[1];
+                    } else {
+                        const u32x4 u = __builtin_amdgcn_raw_buffer_load_b128(rows, v_off, skip, ONCE);
+                        w[0] = u[0], w[1] = u[1], w[2] = u[2], w[3] = u[3];
+                    }
                 }
             }
+        };
+
+        int key = from + KEYS * wave, pages = pages_of(key);
+        if (key < to) {
+            locate(key, pages);
+            pages = pages_of(key + UNIT);
+            request_k(), request_scales(), request_v();
+        }
+        h8 qf[Q_LDS ? 1 : QT][SLABS][PARTS];
+        h8* const q_lds = reinterpret_cast<h8*>(lds) + lane;
+        float factor[QT];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            const bool used = row0 + 16 * t + c <= last_row;
+            factor[t] = a.scale * kLog2e;
+            int up = 0;
             if constexpr (F32) {
                 // times 2^up, so that the row's largest value is in [2^13, 2^14): low parts down to 2^-24 of it are normal numbers
+                float top = 0.f;
+#pragma unroll
+                for (int i = 0; i < SLABS; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        if (!(used && column(i, g) < a.dim)) raw[t][i][e / 4][e % 4] = 0.f;
+                        top = fmaxf(top, fabsf(raw[t][i][e / 4][e % 4]));
+                    }
                 top = rows4_max(top);
-                const int up = max(-126, min(126, 14 - __builtin_amdgcn_frexp_expf(top)));
+                up = max(-126, min(126, 14 - __builtin_amdgcn_frexp_expf(top)));
                 factor[t] = __builtin_ldexpf(factor[t], -up);
+            }
 #pragma unroll
-                for (int i = 0; i < SLABS; ++i) {
-                    constexpr int order[2][8] = {{0, 1, 2, 3, 4, 5, 6, 7}, {0, 4, 1, 5, 2, 6, 3, 7}};
-                    Frag f[2];
+            for (int i = 0; i < SLABS; ++i) {
+                Frag f[PARTS];
+                // 4-bit codes leave a dword in the order 0 4 1 5 2 6 3 7
+                constexpr int order[2][8] = {{0, 1, 2, 3, 4, 5, 6, 7}, {0, 4, 1, 5, 2, 6, 3, 7}};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float u = __builtin_ldexpf(x[i][order[BITS == 4][2 * e]], up), w = __builtin_ldexpf(x[i][order[BITS == 4][2 * e + 1]], up);
+                for (int e = 0; e < 4; ++e) {
+                    const int n0 = order[BITS == 4][2 * e], n1 = order[BITS == 4][2 * e + 1];
+                    if constexpr (F32) {
+                        const float u = __builtin_ldexpf(raw[t][i][n0 / 4][n0 % 4], up), w = __builtin_ldexpf(raw[t][i][n1 / 4][n1 % 4], up);
                         f[0].p[e] = to_h2(u, w);
                         f[1].p[e] = to_h2(u - float(f[0].p[e].x), w - float(f[0].p[e].y));
+                    } else {
+                        f[0].p[e] = h2{raw[t][i][0][n0], raw[t][i][0][n1]};
+                        if (!(used && column(i, g) < a.dim)) f[0].p[e] = h2{0, 0};
                     }
-                    qf[t][i][0] = f[0].v, qf[t][i][1] = f[1].v;
+                }
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    if constexpr (!Q_LDS) qf[t][i][p] = f[p].v;
+                    else if ((t * SLABS + i) % WAVES == wave) q_lds[((t * SLABS + i) * PARTS + p) * 64] = f[p].v;
                 }
             }
         }
+        if constexpr (Q_LDS) __syncthreads();
 
         f32x4 o[QT][TILES] = {};
         float m[QT], l[QT], unit = 0.f, per_unit = 0.f;
 #pragma unroll
         for (int t = 0; t < QT; ++t) m[t] = -__builtin_inff(), l[t] = 0.f;
 
-        const int row_bytes = a.dim * BITS / 8;
-        const int* table = a.table + size_t(it.seq) * a.width;
-        auto pages_of = [&](int key, int (&page)[2]) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) page[t] = key + 16 * t < to ? table[a.page_size(unsigned(key + 16 * t))] : -1;
-        };
-        // lane offsets: key c's codes, and four keys' columns; lanes past the head's columns read the first ones (and meet zeros of q,
-        // or make columns that nobody stores)
-        unsigned k_off[(KW + 3) / 4];
-#pragma unroll
-        for (int i = 0; i < (KW + 3) / 4; ++i) {
-            const int d = column(i * (16 / BITS), g);
-            k_off[i] = unsigned(c * row_bytes + (d < a.dim ? d * BITS / 8 : 0));
-        }
-        const unsigned v_off = unsigned(4 * g * row_bytes + (c * TILES < a.dim ? c * VB : 0));
-        auto request = [&](Step& s, int key, const int (&page)[2]) {
-            s.at = key, s.ok = 0;
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const bool ok = unsigned(page[t]) < unsigned(a.pages);
-                s.ok |= int(ok) << t;
-                const int in_page = key + 16 * t - int(a.page_size(unsigned(key + 16 * t)) * a.page_size.d);
-                const size_t row = ok ? (size_t(unsigned(page[t])) * unsigned(a.kv_heads) + unsigned(head)) * a.page_size.d + unsigned(in_page) : 0;
-                const uint8_t* kp = a.k_codes + row * unsigned(row_bytes);
-                const uint8_t* vp = a.v_codes + row * unsigned(row_bytes);
-                if constexpr (KW >= 4) {
-#pragma unroll
-                    for (int i = 0; i < KW / 4; ++i) {
-                        const uint4 w = *reinterpret_cast<const uint4*>(kp + k_off[i]);
-                        s.k[t][4 * i] = w.x, s.k[t][4 * i + 1] = w.y, s.k[t][4 * i + 2] = w.z, s.k[t][4 * i + 3] = w.w;
-                    }
-                } else {
-                    const uint2 w = *reinterpret_cast<const uint2*>(kp + k_off[0]);
-                    s.k[t][0] = w.x, s.k[t][1] = w.y;
-                }
-                s.ks[t] = *reinterpret_cast<const f32x4*>(a.k_scale + row + 4 * g);
-                s.vs[t] = *reinterpret_cast<const f32x4*>(a.v_scale + row + 4 * g);
-                if constexpr (AFFINE) {
-                    s.kz[t] = a.k_zero[row + c];
-                    s.vz[t] = *reinterpret_cast<const f32x4*>(a.v_zero + row + 4 * g);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint8_t* p = vp + v_off + unsigned(e * row_bytes);
-                    uint32_t(&w)[VW] = s.v[4 * t + e];
-                    if constexpr (VB == 2) {
-                        w[0] = *reinterpret_cast<const uint16_t*>(p);
-                    } else if constexpr (VB == 4) {
-                        w[0] = *reinterpret_cast<const uint32_t*>(p);
-                    } else if constexpr (VB == 8) {
-                        const uint2 u = *reinterpret_cast<const uint2*>(p);
-                        w[0] = u.x, w[1] = u.y;
-                    } else {
-                        const uint4 u = *reinterpret_cast<const uint4*>(p);
-                        w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-                    }
-                }
-            }
-        };
-
-        auto work = [&](Step& s) {
+        const uint32_t high = BITS == 4 ? magic() : 0;
+        for (; key < to; key += UNIT) {
+            const int ok_now = ok;
+            if constexpr (Q_LDS) asm volatile("" ::: "memory");  // (else all fragments of the queries are read ahead, into registers there are not)
             // scores
-            f32x4 sc[QT][2];
+            f32x4 sc[QT][NT];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                Offsets<BITS> off;
-                if constexpr (AFFINE) off.set(s.kz[t], s.kz[t]);
+            for (int t = 0; t < NT; ++t) {
+                const Offsets<BITS> off = AFFINE ? Offsets<BITS>(kz[t], kz[t]) : Offsets<BITS>();
 #pragma unroll
                 for (int x = 0; x < QT; ++x) sc[x][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int i = 0; i < SLABS; ++i) {
                     Frag f;
                     if constexpr (BITS == 8) {
-                        const uint32_t w0 = s.k[t][2 * i], w1 = s.k[t][2 * i + 1];
+                        const uint32_t w0 = kw[t][2 * i], w1 = kw[t][2 * i + 1];
                         f.p[0] = bytes01(w0, off.of1024), f.p[1] = bytes23(w0, off.of1024);
                         f.p[2] = bytes01(w1, off.of1024), f.p[3] = bytes23(w1, off.of1024);
                     } else {
-                        const uint32_t w = s.k[t][i], u = w >> 8;
-                        f.p[0] = nibbles0(w, off.of1024), f.p[1] = nibbles4(w, off.of64);
-                        f.p[2] = nibbles0(u, off.of1024), f.p[3] = nibbles4(u, off.of64);
+                        const uint32_t w = kw[t][i], u = w >> 8;
+                        f.p[0] = nibbles0(w, high, off.of1024), f.p[1] = nibbles4(w, high, off.of64);
+                        f.p[2] = nibbles0(u, high, off.of1024), f.p[3] = nibbles4(u, high, off.of64);
                     }
 #pragma unroll
                     for (int x = 0; x < QT; ++x)
 #pragma unroll
                         for (int p = PARTS - 1; p >= 0; --p)
-                            sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.v, qf[x][i][p], sc[x][t], 0, 0, 0);
+                            sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.v, Q_LDS ? q_lds[((x * SLABS + i) * PARTS + p) * 64] : qf[Q_LDS ? 0 : x][i][p],
+                                                                              sc[x][t], 0, 0, 0);
                 }
             }
-            const bool whole = s.at >= all_lo && s.at + 32 <= min(all_hi, to) && s.ok == 3;
-            float vs[2][4], vtop = 0.f;
+            locate(key + UNIT, pages);
+            pages = pages_of(key + 2 * UNIT);
+            request_k();
+            const bool whole = key >= all_lo && key + KEYS <= min(all_hi, to) && ok_now == (1 << NT) - 1;
+            float vs[NT][4], vtop = 0.f;
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int key = s.at + 16 * t + 4 * g + r;
-                    vs[t][r] = s.vs[t][r];
+                    const int j = key + 16 * t + 4 * g + r;
+                    vs[t][r] = vs4[t][r];
                     // (a zero point that is no number reaches every row through the matrix product: the scale has it for those that see it)
                     if constexpr (AFFINE)
-                        if (!(fabsf(s.vz[t][r]) <= 2048.f)) vs[t][r] = __builtin_nanf(""), s.vz[t][r] = 0.f;
+                        if (!whole && !(fabsf(vz[t][r]) <= 2048.f)) vs[t][r] = __builtin_nanf(""), vz[t][r] = 0.f;
                     // (what no row sees may be anything)
-                    if (!whole && !(key >= seen.lo && key < to && (s.ok >> t & 1))) vs[t][r] = 0.f;
+                    if (!whole && !(j >= seen.lo && j < to && (ok_now >> t & 1))) vs[t][r] = 0.f;
                     vtop = fmaxf(vtop, fabsf(vs[t][r]));
                 }
             // the unit of the outputs
@@ -237,19 +311,19 @@ struct RowsKernel {
                     for (int j = 0; j < TILES; ++j) o[x][j] *= f;
                 unit = top, per_unit = kProbability / top;
             }
-            Frag pf[QT][PARTS];
+            Frag pf[QT][NT / 2][PARTS];
 #pragma unroll
             for (int x = 0; x < QT; ++x) {
                 float top = -__builtin_inff();
-                float e[2][4];
+                float e[NT][4];
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        e[t][r] = sc[x][t][r] * (s.ks[t][r] * factor[x]);
+                        e[t][r] = sc[x][t][r] * (ks[t][r] * factor[x]);
                         if (!whole) {
-                            const int key = s.at + 16 * t + 4 * g + r;
-                            if (!(key >= lo[x] && key < min(hi[x], to) && (s.ok >> t & 1))) e[t][r] = -__builtin_inff();
+                            const int j = key + 16 * t + 4 * g + r;
+                            if (!(j >= lo[x] && j < min(hi[x], to) && (ok_now >> t & 1))) e[t][r] = -__builtin_inff();
                         }
                         top = fmaxf(top, e[t][r]);
                     }
@@ -264,7 +338,7 @@ struct RowsKernel {
                 const float mm = m[x] == -__builtin_inff() ? 0.f : m[x];
                 float sum = 0.f;
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const float p = __builtin_amdgcn_exp2f(e[t][r] - mm);
@@ -274,195 +348,195 @@ struct RowsKernel {
                     }
                 l[x] += sum;
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         const float u = e[t][2 * r], w = e[t][2 * r + 1];
                         const h2 h = to_h2(u, w);
-                        pf[x][0].p[2 * t + r] = h;
-                        if constexpr (F32) pf[x][1].p[2 * t + r] = to_h2(u - float(h.x), w - float(h.y));
+                        pf[x][t / 2][0].p[2 * (t % 2) + r] = h;
+                        if constexpr (F32) pf[x][t / 2][1].p[2 * (t % 2) + r] = to_h2(u - float(h.x), w - float(h.y));
                     }
             }
+            request_scales();
             // values: slots 2 i and 2 i + 1 are keys 2 i and 2 i + 1 of the lane's eight
-            Offsets<BITS> off[4];
-            if constexpr (AFFINE)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) off[i].set(s.vz[i / 2][2 * (i % 2)], s.vz[i / 2][2 * (i % 2) + 1]);
             constexpr int PER = BITS == 8 ? 4 : VB == 2 ? 4 : 8;  // column tiles of a dword
 #pragma unroll
-            for (int w = 0; w < VW; ++w) {
-                Frag f[PER];
+            for (int k = 0; k < NT / 2; ++k) {
+                Offsets<BITS> off[4];
+                if constexpr (AFFINE)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t x = s.v[2 * i][w], y = s.v[2 * i + 1][w];
-                    if constexpr (BITS == 8) {
-                        const uint32_t u0 = __builtin_amdgcn_perm(y, x, 0x05010400u), u1 = __builtin_amdgcn_perm(y, x, 0x07030602u);
-                        f[0].p[i] = bytes01(u0, off[i].of1024), f[1].p[i] = bytes23(u0, off[i].of1024);
-                        f[2].p[i] = bytes01(u1, off[i].of1024), f[3].p[i] = bytes23(u1, off[i].of1024);
-                    } else {
+                    for (int i = 0; i < 4; ++i) off[i] = Offsets<BITS>(vz[2 * k + i / 2][2 * (i % 2)], vz[2 * k + i / 2][2 * (i % 2) + 1]);
 #pragma unroll
-                        for (int h = 0; h < PER / 4; ++h) {
-                            const uint32_t u = __builtin_amdgcn_perm(y, x, h ? 0x07060302u : 0x05040100u), n = u >> 8;
-                            f[4 * h].p[i] = nibbles0(u, off[i].of1024), f[4 * h + 1].p[i] = nibbles4(u, off[i].of64);
-                            f[4 * h + 2].p[i] = nibbles0(n, off[i].of1024), f[4 * h + 3].p[i] = nibbles4(n, off[i].of64);
+                for (int w = 0; w < VW; ++w) {
+                    Frag f[PER];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t x = vw[8 * k + 2 * i][w], y = vw[8 * k + 2 * i + 1][w];
+                        if constexpr (BITS == 8) {
+                            const uint32_t u0 = __builtin_amdgcn_perm(y, x, 0x05010400u), u1 = __builtin_amdgcn_perm(y, x, 0x07030602u);
+                            f[0].p[i] = bytes01(u0, off[i].of1024), f[1].p[i] = bytes23(u0, off[i].of1024);
+                            f[2].p[i] = bytes01(u1, off[i].of1024), f[3].p[i] = bytes23(u1, off[i].of1024);
+                        } else {
+#pragma unroll
+                            for (int h = 0; h < PER / 4; ++h) {
+                                const uint32_t u = __builtin_amdgcn_perm(y, x, h ? 0x07060302u : 0x05040100u), n = u >> 8;
+                                f[4 * h].p[i] = nibbles0(u, high, off[i].of1024), f[4 * h + 1].p[i] = nibbles4(u, high, off[i].of64);
+                                f[4 * h + 2].p[i] = nibbles0(n, high, off[i].of1024), f[4 * h + 3].p[i] = nibbles4(n, high, off[i].of64);
+                            }
                         }
                     }
+#pragma unroll
+                    for (int j = 0; j < PER; ++j)
+#pragma unroll
+                        for (int x = 0; x < QT; ++x)
+#pragma unroll
+                            for (int p = PARTS - 1; p >= 0; --p)
+                                o[x][w * PER + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[j].v, pf[x][k][p].v, o[x][w * PER + j], 0, 0, 0);
                 }
-#pragma unroll
-                for (int j = 0; j < PER; ++j)
-#pragma unroll
-                    for (int x = 0; x < QT; ++x)
-#pragma unroll
-                        for (int p = PARTS - 1; p >= 0; --p)
-                            o[x][w * PER + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[j].v, pf[x][p].v, o[x][w * PER + j], 0, 0, 0);
             }
-        };
-
-        int key = from + 32 * wave;
-        if (key < to) {
-            Step s0, s1;
-            int page[2];
-            pages_of(key, page);
-            request(s0, key, page);
-            pages_of(key + 128, page);
-            while (true) {
-                request(s1, key + 128, page);
-                pages_of(key + 256, page);
-                work(s0);
-                key += 128;
-                if (key >= to) break;
-                request(s0, key + 128, page);
-                pages_of(key + 256, page);
-                work(s1);
-                key += 128;
-                if (key >= to) break;
-            }
+            request_v();
         }
 
-        // The four wavefronts' results: rows' maxima first, then sums in the order (0 + 2) + (1 + 3).
-        __shared__ float s_m[WAVES][R], s_l[WAVES][R];
+        // The wavefronts' results meet in LDS, ROWS rows at a time, and every thread adds up some columns of them.
+        __shared__ float s_m[WAVES][R], s_l[WAVES][R], s_unit[WAVES];
 #pragma unroll
         for (int x = 0; x < QT; ++x) {
             l[x] = rows4_sum(l[x]);
             if (g == 0) s_m[wave][16 * x + c] = m[x], s_l[wave][16 * x + c] = l[x];
         }
-        __syncthreads();
-        float top[QT], total[QT];
-#pragma unroll
-        for (int x = 0; x < QT; ++x) {
-            const int r = 16 * x + c;
-            top[x] = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-            const float mm = top[x] == -__builtin_inff() ? 0.f : top[x];
-            float f[WAVES];
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) f[w] = __builtin_amdgcn_exp2f(s_m[w][r] - mm);
-            total[x] = s_l[0][r] * f[0] + s_l[2][r] * f[2] + (s_l[1][r] * f[1] + s_l[3][r] * f[3]);
-            const float mine = __builtin_amdgcn_exp2f(m[x] - mm) * (unit * (1.f / kProbability));
-#pragma unroll
-            for (int j = 0; j < TILES; ++j) o[x][j] *= mine;
-        }
-        auto place = [&](int slot, int r, int j) { return lds + (slot * 16 + c) * LDS_ROW + (4 * g + r) * TILES + j; };
+        if (lane == 0) s_unit[wave] = unit * (1.f / kProbability);
 #pragma unroll
         for (int x = 0; x < QT; ++x)
 #pragma unroll
-            for (int round = 2; round >= 1; round >>= 1) {
-                if (wave >= round && wave < 2 * round) {
+            for (int part = 0; part < 16 / ROWS; ++part) {
+                if (Q_LDS || x + part) __syncthreads();  // (whoever reads what lies there is done)
+                if (c / ROWS == part) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
 #pragma unroll
                         for (int j = 0; j < TILES; j += 4)
-                            *reinterpret_cast<f32x4*>(place(wave - round, r, j)) = f32x4{o[x][j][r], o[x][j + 1][r], o[x][j + 2][r], o[x][j + 3][r]};
+                            *reinterpret_cast<f32x4*>(lds + (wave * ROWS + c % ROWS) * LDS_ROW + (4 * g + r) * TILES + j) =
+                                f32x4{o[x][j][r], o[x][j + 1][r], o[x][j + 2][r], o[x][j + 3][r]};
                 }
                 __syncthreads();
-                if (wave < round) {
+                for (int e = int(threadIdx.x) * 4; e < ROWS * DIM; e += 1024) {
+                    const int r = e / DIM, d = e % DIM, row = 16 * x + part * ROWS + r;
+                    if (row0 + row > last_row) break;
+                    const float top = fmaxf(fmaxf(s_m[0][row], s_m[1][row]), fmaxf(s_m[2][row], s_m[3][row]));
+                    const float mm = top == -__builtin_inff() ? 0.f : top;
+                    f32x4 v = {0, 0, 0, 0};
+                    float total = 0.f;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-#pragma unroll
-                        for (int j = 0; j < TILES; j += 4) {
-                            const f32x4 v = *reinterpret_cast<const f32x4*>(place(wave, r, j));
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[x][j + e][r] += v[e];
-                        }
-                }
-                __syncthreads();
-            }
-        if (wave) return;
-        float* part = a.partial + partial_at(a, int(blockIdx.x), head, R, DIM);
-#pragma unroll
-        for (int x = 0; x < QT; ++x) {
-            const int row = row0 + 16 * x + c;
-            if (row > last_row) continue;
-            if (it.parts > 1) {
-                if (g == 0) part[R * DIM + 16 * x + c] = top[x], part[R * DIM + R + 16 * x + c] = total[x];
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int j = 0; j < TILES; j += 4)
-                        *reinterpret_cast<f32x4*>(part + (16 * x + c) * DIM + (4 * g + r) * TILES + j) =
-                            f32x4{o[x][j][r], o[x][j + 1][r], o[x][j + 2][r], o[x][j + 3][r]};
-                continue;
-            }
-            const float f = total[x] == 0.f ? 0.f : 1.f / total[x];
-            const int token = int(a.group(unsigned(row)));
-            T* dst = out + (size_t(it.s.q0 + token) * a.heads + size_t(head * group + row - token * group)) * a.dim;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int d = (4 * g + r) * TILES;
-                if (d >= a.dim) continue;
-#pragma unroll
-                for (int j = 0; j < TILES; j += 4) {
-                    const f32x4 v = f32x4{o[x][j][r], o[x][j + 1][r], o[x][j + 2][r], o[x][j + 3][r]} * f;
-                    if constexpr (F32) *reinterpret_cast<f32x4*>(dst + d + j) = v;
-                    else *reinterpret_cast<uint2*>(dst + d + j) = uint2{as_u32(to_h2(v[0], v[1])), as_u32(to_h2(v[2], v[3]))};
+                    for (int w = 0; w < WAVES; ++w) {
+                        const float f = __builtin_amdgcn_exp2f(s_m[w][row] - mm);
+                        v += *reinterpret_cast<const f32x4*>(lds + (w * ROWS + r) * LDS_ROW + d) * (f * s_unit[w]);
+                        total += s_l[w][row] * f;
+                    }
+                    if (piece) {
+                        if (d == 0) piece[R * DIM + row] = top, piece[R * DIM + R + row] = total;
+                        *reinterpret_cast<f32x4*>(piece + row * DIM + d) = v;
+                    } else if (d < a.dim) {
+                        v *= total == 0.f ? 0.f : 1.f / total;
+                        const int token = int(a.group(unsigned(row0 + row)));
+                        T* dst = out + (size_t(it.s.q0 + token) * a.heads + size_t(head * group + row0 + row - token * group)) * a.dim + d;
+                        if constexpr (F32) *reinterpret_cast<f32x4*>(dst) = v;
+                        else *reinterpret_cast<uint2*>(dst) = uint2{as_u32(to_h2(v[0], v[1])), as_u32(to_h2(v[2], v[3]))};
+                    }
                 }
             }
-        }
     }
 };
 
 template <class T, int BITS, bool AFFINE, int DIM, int QT>
-__global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void attn_rows_kernel(AttnArgs a, const T* __restrict__ q, T* __restrict__ out) {
+__global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void attn_rows_kernel(AttnArgs a, const T* __restrict__ q, T* __restrict__ out) {
     using K = RowsKernel<T, BITS, AFFINE, DIM, QT>;
     __shared__ __attribute__((aligned(16))) float lds[K::LDS_BYTES / 4];
     K::run(a, q, out, lds);
 }
 
-// Joins the parts of the tiles that have several.
-template <class T, int DIM, int R>
+// Joins the pieces of the segments that several blocks have one of: a wavefront per row, whose lanes have four columns each and, where
+// that leaves lanes, the pieces in turn.
+template <class T, int DIM, int R, int UNIT>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, T* __restrict__ out) {
-    Item it;
-    if (!find_item<R>(a, blockIdx.x, true, it) || it.parts == 1 || it.first + it.parts > a.items) return;
-    const int head = blockIdx.y, group = int(a.group.d), rows = min(R, it.s.chunk * group - it.tile * R);
-    const size_t step = partial_at(a, 1, 0, R, DIM);
-    const float* part = a.partial + partial_at(a, it.first, head, R, DIM);
-    for (int e = int(threadIdx.x) * 4; e < rows * DIM; e += 1024) {
-        const int r = e / DIM, d = e % DIM;
-        if (d >= a.dim) continue;
-        float top = -__builtin_inff();
-        for (int i = 0; i < it.parts; ++i) top = fmaxf(top, part[i * step + R * DIM + r]);
-        const float mm = top == -__builtin_inff() ? 0.f : top;
-        float total = 0.f;
-        f32x4 v = {0, 0, 0, 0};
-        for (int i = 0; i < it.parts; ++i) {
-            const float* p = part + i * step;
-            const float f = __builtin_amdgcn_exp2f(p[R * DIM + r] - mm);
-            total += p[R * DIM + R + r] * f;
-            v += *reinterpret_cast<const f32x4*>(p + e) * f;
+    Segments<R, UNIT> segs(a);
+    const unsigned share = segs.share(), head = blockIdx.y;
+    // block.x counts tiles; the segment begins at unit `x` of its head
+    int tile = int(blockIdx.x), seq = -1;
+    unsigned x = 0, units = 0;
+    Sequence s{0, 0, 0};
+    for (unsigned before = 0;; segs.first += 64, segs.load()) {
+        if (segs.first >= a.batch) return;
+        unsigned upto = segs.tiles;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const unsigned o = __shfl_up(upto, d, 64);
+            if (segs.lane >= d) upto += o;
         }
-        v *= total == 0.f ? 0.f : 1.f / total;
-        const int row = it.tile * R + r, token = int(a.group(unsigned(row)));
-        T* dst = out + (size_t(it.s.q0 + token) * a.heads + size_t(head * group + row - token * group)) * a.dim + d;
-        if constexpr (std::is_same_v<T, float>) *reinterpret_cast<f32x4*>(dst) = v;
-        else *reinterpret_cast<uint2*>(dst) = uint2{as_u32(to_h2(v[0], v[1])), as_u32(to_h2(v[2], v[3]))};
+        const unsigned long long past = __ballot(upto > unsigned(tile));
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            auto get = [&](unsigned v) { return unsigned(__builtin_amdgcn_readlane(int(v), l)); };
+            seq = segs.first + l, units = get(segs.units);
+            tile -= int(get(upto) - get(segs.tiles));
+            x = before + get(segs.upto) - get(segs.tiles) * units + unsigned(tile) * units;
+            s = Sequence{int(get(unsigned(segs.s.q0))), int(get(unsigned(segs.s.chunk))), int(get(unsigned(segs.s.len)))};
+            break;
+        }
+        tile -= int(unsigned(__builtin_amdgcn_readlane(int(upto), 63)));
+        before += unsigned(__builtin_amdgcn_readlane(int(segs.upto), 63));
     }
+    x += head * segs.total;
+    const unsigned b0 = x / share, b1 = (x + units - 1) / share;
+    if (b0 == b1 || b1 >= unsigned(a.blocks)) return;
+    const int parts = int(b1 - b0) + 1;
+    constexpr int QUADS = DIM / 4, EVERY = 64 / QUADS;
+    const int lane = threadIdx.x & 63, d = lane % QUADS * 4, mine = lane / QUADS;
+    const int group = int(a.group.d), r = blockIdx.z * 4 + (threadIdx.x >> 6);
+    if (r >= s.chunk * group - tile * R) return;
+    // the first piece is the second of its block's two, the others are the first of theirs
+    auto piece = [&](int i) { return a.partial + (2 * size_t(b0 + i) + (i == 0)) * kPiece<R, DIM>; };
+    float top = -__builtin_inff();
+    for (int i = lane; i < parts; i += 64) top = fmaxf(top, piece(i)[R * DIM + r]);
+#pragma unroll
+    for (int e = 1; e < 64; e *= 2) top = fmaxf(top, __shfl_xor(top, e, 64));
+    const float mm = top == -__builtin_inff() ? 0.f : top;
+    float total = 0.f;
+    f32x4 v = {0, 0, 0, 0};
+    for (int i0 = 0; i0 < parts; i0 += 4 * EVERY) {
+        f32x4 y[4];
+        float m[4], l[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float* p = piece(min(i0 + u * EVERY + mine, parts - 1));
+            y[u] = *reinterpret_cast<const f32x4*>(p + r * DIM + d);
+            m[u] = p[R * DIM + r], l[u] = p[R * DIM + R + r];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (i0 + u * EVERY + mine >= parts) continue;
+            const float f = __builtin_amdgcn_exp2f(m[u] - mm);
+            total += l[u] * f, v += y[u] * f;
+        }
+    }
+#pragma unroll
+    for (int e = QUADS; e < 64; e *= 2) {
+        total += __shfl_xor(total, e, 64);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += __shfl_xor(v[k], e, 64);
+    }
+    if (d >= a.dim || mine) return;
+    v *= total == 0.f ? 0.f : 1.f / total;
+    const int row = tile * R + r, token = int(a.group(unsigned(row)));
+    T* dst = out + (size_t(s.q0 + token) * a.heads + size_t(int(head) * group + row - token * group)) * a.dim + d;
+    if constexpr (std::is_same_v<T, float>) *reinterpret_cast<f32x4*>(dst) = v;
+    else *reinterpret_cast<uint2*>(dst) = uint2{as_u32(to_h2(v[0], v[1])), as_u32(to_h2(v[2], v[3]))};
 }
 
-// grid: items (tiles for the join), heads
 template <class T, int BITS, int DIM, int QT>
 void launch_rows(const AttnArgs& a, const T* q, T* out, int tiles, bool join, hipStream_t st) {
-    if (a.k_zero) attn_rows_kernel<T, BITS, true, DIM, QT><<<dim3(a.items, a.kv_heads), 256, 0, st>>>(a, q, out);
-    else attn_rows_kernel<T, BITS, false, DIM, QT><<<dim3(a.items, a.kv_heads), 256, 0, st>>>(a, q, out);
-    if (join) attn_join_kernel<T, DIM, 16 * QT><<<dim3(tiles, a.kv_heads), 256, 0, st>>>(a, out);
+    if (a.k_zero) attn_rows_kernel<T, BITS, true, DIM, QT><<<a.blocks, 256, 0, st>>>(a, q, out);
+    else attn_rows_kernel<T, BITS, false, DIM, QT><<<a.blocks, 256, 0, st>>>(a, q, out);
+    if (join) attn_join_kernel<T, DIM, 16 * QT, 4 * rows_keys(BITS, DIM, QT)><<<dim3(tiles, a.kv_heads, 4 * QT), 256, 0, st>>>(a, out);
 }
 
 template <class T, int BITS>

@@ -34,14 +34,21 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
     const int chunk = max_chunk ? std::min(max_chunk, tokens) : batch == 1 ? tokens : (tokens + batch - 1) / std::max(batch, 1);
     const int qt = chunk * group <= 16 ? 1 : 2, rows = 16 * qt;
     const int tiles = sequences + int(int64_t(tokens) * group / rows);
-    a.target = 512, a.max_rows = 0x7fffffff;
-    a.items = tiles + (a.target + a.kv_heads - 1) / a.kv_heads;
-    const bool join = int64_t(table_width) * c->page_size > attn::kMinKeys;
+    const int dim = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
+    const int64_t most = int64_t(table_width) * c->page_size;  // keys of a sequence
+    LQ_REQUIRE(int64_t(tiles) * c->kv_heads * (most / 128 + 1) < 0x7fffffff, LQ_ERR_NOT_IMPLEMENTED,
+               "paged_attention: %d tiles of queries for %lld keys of %d heads are more than one call takes", tiles, (long long)most, c->kv_heads);
+    a.max_rows = 0x7fffffff;
+    // Up to 512 keys a block has a whole segment: four steps of each wavefront, where joining pieces takes another launch (one token of 197
+    // keys 10.3 -> 7.6 us).  Beyond, as many shares as blocks are resident.
+    const bool join = most > 512;
+    const int resident = (dim > 128 ? 1 : 2) * 256;
+    a.each = join ? resident : 0, a.least = 1;
+    a.blocks = join ? resident : tiles * a.kv_heads;
     auto lock = scratch_lock(as_stream(stream));
     if (join) {
-        const int dim = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
         void* p = nullptr;
-        rc = call_buffer(9, size_t(a.items) * a.kv_heads * rows * (dim + 2) * sizeof(float), as_stream(stream), &p);
+        rc = call_buffer(9, size_t(2) * a.blocks * rows * (dim + 2) * sizeof(float), as_stream(stream), &p);
         if (rc) return rc;
         a.partial = static_cast<float*>(p);
     }

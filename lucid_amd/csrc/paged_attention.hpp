@@ -31,11 +31,12 @@ struct AttnArgs {
     size_t ldq;
     FastDiv page_size{1}, group{1};
     int pages, kv_heads, dim, tokens, heads, batch, width, causal, window;
-    int items;     // blocks there are for the items of a head
-    int target;    // blocks that the keys of a launch are shared out to
+    int blocks;
+    int each;      // of so many blocks each has a share of the units, at least `least`; 0: a segment
+    int least;
     int max_rows;  // sequences of more rows are another launch's
     float scale;
-    float* partial;  // results of items that share a tile
+    float* partial;  // pieces of segments
 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -45,7 +46,6 @@ namespace attn {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLazy = 8.f;        // a row's maximum is renewed when it has grown by this (powers of two)
 constexpr float kProbability = 0x1p7f;  // probabilities are kept times this
-constexpr int kMinKeys = 128;       // of an item's share of keys: a step of 32 for each of four wavefronts
 
 // f over the four lanes of one number in the four rows of 16 lanes; every lane gets it
 template <class F>
@@ -85,81 +85,81 @@ __device__ __forceinline__ Keys keys_of(const AttnArgs& a, const Sequence& s, in
     return k;
 }
 
-// What the blocks of a launch do is found by each of them from the lengths, which only the device knows: tiles of R rows, the
-// keys of a sequence's tiles shared out to `chunks` items each, so that all items of a launch are about equally long.
-struct Item {
-    int seq, tile, part, parts;  // part of its parts
-    int first;                   // number of the tile's first item
+// What the blocks of a launch do is found by each of them from the lengths, which only the device knows.  A segment is a tile of
+// R rows of a sequence with one key head; it is `units` units of UNIT keys long, and all segments of a launch, head by head, make one line of
+// units, which the blocks share out evenly: where a sequence ends, a block goes on with the next one.  A segment that several
+// blocks have a piece of is joined by another launch.  `each` = 0: a block per segment, for short sequences.
+template <int R, int UNIT>
+struct Segments {
+    const AttnArgs& a;
+    const int lane;
+    unsigned total;     // units of a head
+    // 64 sequences, one a lane: units of their segments, tiles, units of one
+    int first;          // the first of them
+    unsigned before;    // units of the sequences before it
+    unsigned upto, tiles, units;
     Sequence s;
-};
 
-// the sums over the lanes before this one and itself
-__device__ __forceinline__ unsigned scan(unsigned v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const unsigned o = __shfl_up(v, d, 64);
-        if (lane >= d) v += o;
+    __device__ __forceinline__ explicit Segments(const AttnArgs& args) : a(args), lane(threadIdx.x & 63), total(0) {
+        for (first = 0; first < a.batch; first += 64) {
+            load();
+            total += unsigned(__builtin_amdgcn_readlane(int(upto), 63));
+        }
+        if (a.batch > 64) first = 0, load();
+        first = 0, before = 0;
     }
-    return v;
-}
-
-// Item number `id` of a launch with tiles of R rows (tiles instead of items with `whole`: id counts tiles).  False: there is none.
-// Every wavefront finds it for itself, 64 sequences at a time.
-template <int R>
-__device__ __forceinline__ bool find_item(const AttnArgs& a, unsigned id, bool whole, Item& item) {
-    const int lane = threadIdx.x & 63;
-    auto tiles_of = [&](const Sequence& s) {
-        const int rows = s.chunk * int(a.group.d);
-        return rows > a.max_rows ? 0u : unsigned(rows + R - 1) / R;
-    };
-    auto extent_of = [&](const Sequence& s) {
-        const Keys k = keys_of(a, s, 0, s.chunk - 1);
-        return unsigned(k.hi - (k.lo & ~31));
-    };
-    unsigned long long sum = 0;
-    for (int b = lane; b < a.batch; b += 64) {
-        const Sequence s = sequence_of(a, b);
-        sum += (unsigned long long)(tiles_of(s)) * extent_of(s);
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d, 64);
-    const unsigned long long share = (sum * unsigned(a.kv_heads) + a.target - 1) / unsigned(a.target);
-    const unsigned long long keys = (share + kMinKeys - 1) / kMinKeys * kMinKeys;
-    const unsigned each = keys < kMinKeys ? kMinKeys : keys > 0x40000000ull ? 0x40000000u : unsigned(keys);
-    unsigned items = 0, tiles = 0;  // of the sequences before these
-    for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        const int b = b0 + lane;
-        Sequence s{0, 0, 0};
-        unsigned t = 0, parts = 1;
+    __device__ __forceinline__ void load() {
+        const int b = first + lane;
+        s = Sequence{0, 0, 0}, tiles = 0, units = 1;
         if (b < a.batch) {
             s = sequence_of(a, b);
-            t = tiles_of(s);
-            parts = max(1u, (extent_of(s) + each - 1) / each);
+            const int rows = s.chunk * int(a.group.d);
+            tiles = rows > a.max_rows ? 0u : unsigned(rows + R - 1) / R;
+            const Keys k = keys_of(a, s, 0, s.chunk - 1);
+            units = a.each ? max(1u, unsigned(k.hi - (k.lo & ~31) + UNIT - 1) / UNIT) : 1u;
         }
-        const unsigned items_to = items + scan(t * parts, lane), tiles_to = tiles + scan(t, lane);
-        const unsigned long long past = __ballot((whole ? tiles_to : items_to) > id);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            auto get = [&](unsigned v) { return __builtin_amdgcn_readlane(int(v), at); };
-            item.seq = b0 + at, item.parts = get(parts);
-            item.s = Sequence{get(s.q0), get(s.chunk), get(s.len)};
-            const int n = get(t), first = get(items_to) - n * item.parts;
-            const int k = int(id) - (whole ? get(tiles_to) - n : first);
-            item.tile = whole ? k : k / item.parts;
-            item.part = whole ? 0 : k - item.tile * item.parts;
-            item.first = first + item.tile * item.parts;
-            return true;
+        upto = tiles * units;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const unsigned o = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += o;
         }
-        items = __builtin_amdgcn_readlane(int(items_to), 63), tiles = __builtin_amdgcn_readlane(int(tiles_to), 63);
     }
-    return false;
-}
+    struct Segment {
+        int seq, tile;
+        unsigned unit, units;  // the unit asked for, and how many there are
+        Sequence s;
+    };
+    // the segment of unit `x` < total of a head
+    __device__ __forceinline__ Segment at(unsigned x) {
+        if (x < before) first = 0, before = 0, load();
+        while (true) {
+            const unsigned long long past = __ballot(upto > x - before);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                auto get = [&](unsigned v) { return unsigned(__builtin_amdgcn_readlane(int(v), l)); };
+                Segment g;
+                g.seq = first + l, g.units = get(units);
+                const unsigned k = x - before - (get(upto) - get(tiles) * g.units);
+                g.tile = int(k / g.units), g.unit = k - unsigned(g.tile) * g.units;
+                g.s = Sequence{int(get(unsigned(s.q0))), int(get(unsigned(s.chunk))), int(get(unsigned(s.len)))};
+                return g;
+            }
+            before += unsigned(__builtin_amdgcn_readlane(int(upto), 63));
+            first += 64;
+            load();
+        }
+    }
+    // units that each of a.each blocks takes
+    __device__ __forceinline__ unsigned share() const {
+        return max(unsigned(a.least), (total * unsigned(a.kv_heads) + unsigned(a.each) - 1) / unsigned(a.each));
+    }
+};
 
-// Partial results of an item and head: R rows of `stride` floats, each the sums over its keys, then the rows' maximum and sum of
-// probabilities.
-__device__ __forceinline__ size_t partial_at(const AttnArgs& a, int item, int head, int rows, int stride) {
-    return (size_t(item) * a.kv_heads + head) * rows * (stride + 2);
-}
+// A piece of a segment: R rows of DIM sums over its keys, then the rows' maxima and sums of probabilities.  A block has room for two, the
+// first for a segment that begins in a block before it, the second for one that goes on in the next.
+template <int R, int DIM>
+constexpr size_t kPiece = size_t(R) * (DIM + 2);
 
 // Zeros for the rows of q that belong to no sequence, dealt to the blocks.
 template <class T>
@@ -174,26 +174,30 @@ __device__ __forceinline__ void clear_other_rows(const AttnArgs& a, T* out, unsi
 }
 
 // ---- codes to float16: 1024 + u is the float16 0x6400 | u for u < 1024
-constexpr uint32_t kMagic = 0x64006400u;
 __device__ __forceinline__ h2 as_h2(uint32_t v) { return __builtin_bit_cast(h2, v); }
 __device__ __forceinline__ uint32_t as_u32(h2 v) { return __builtin_bit_cast(uint32_t, v); }
+// 0x64006400 in a vector register: beside a mask in a scalar one it makes "and, or" one instruction
+__device__ __forceinline__ uint32_t magic() {
+    uint32_t m = 0x64006400u;
+    asm volatile("" : "+v"(m));
+    return m;
+}
 
 // What turns 1024 + u (and 64 + u) into c - z: c = u + qmin.
 template <int BITS>
 struct Offsets {
     h2 of1024, of64;
-    __device__ __forceinline__ Offsets() { set(0.f, 0.f); }
-    __device__ __forceinline__ void set(float za, float zb) {
-        constexpr float half = float(1 << (BITS - 1));
-        of1024 = to_h2(-1024.f - half - za, -1024.f - half - zb);
-        of64 = to_h2(-64.f - half - za, -64.f - half - zb);
+    __device__ __forceinline__ Offsets() : of1024(h2{base, base}), of64(h2{base + 960, base + 960}) {}
+    __device__ __forceinline__ Offsets(float za, float zb) {
+        of1024 = to_h2(float(base) - za, float(base) - zb), of64 = of1024 + h2{960, 960};
     }
+    static constexpr _Float16 base = -1024 - (1 << (BITS - 1));
 };
 // both halves' low bits: 4-bit codes at bits 0 and 16, or at 4 and 20
-__device__ __forceinline__ h2 nibbles0(uint32_t w, h2 of1024) { return as_h2((w & 0x000f000fu) | kMagic) + of1024; }
-__device__ __forceinline__ h2 nibbles4(uint32_t w, h2 of64) {
+__device__ __forceinline__ h2 nibbles0(uint32_t w, uint32_t magic, h2 of1024) { return as_h2((w & 0x000f000fu) | magic) + of1024; }
+__device__ __forceinline__ h2 nibbles4(uint32_t w, uint32_t magic, h2 of64) {
     const _Float16 s = _Float16(0.0625f);
-    return __builtin_elementwise_fma(as_h2((w & 0x00f000f0u) | kMagic), h2{s, s}, of64);
+    return __builtin_elementwise_fma(as_h2((w & 0x00f000f0u) | magic), h2{s, s}, of64);
 }
 // bytes 0 and 1, or 2 and 3
 __device__ __forceinline__ h2 bytes01(uint32_t w, h2 of1024) {
@@ -203,11 +207,24 @@ __device__ __forceinline__ h2 bytes23(uint32_t w, h2 of1024) {
     return as_h2(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) + of1024;
 }
 
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// `bytes` of the cache as a buffer: the address stays in scalar registers, and what lies behind is not read
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const void* p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00027000);
+}
+
 union Frag {
     h2 p[4];
     h8 v;
 };
 
+// Keys of a unit of attn_rows_kernel: 16 * NT for each of four wavefronts.  Where a row of codes is short, a wavefront takes 64 keys at a time
+// and not 32, with as many registers for them.
+constexpr int rows_keys(int bits, int dim, int qt) { return bits * dim <= 512 && qt == 1 ? 64 : 32; }
+
+// One token, or a few, of each sequence: tiles of 16 * qt rows.  `tiles`: a bound for those of all sequences; join: segments may be in pieces.
 template <class T, int BITS>
 void launch_rows_of(const AttnArgs& a, const T* q, T* out, int tiles, int qt, bool join, hipStream_t st);
 
