@@ -454,8 +454,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void attn_rows_kernel(AttnA
     K::run(a, q, out, lds);
 }
 
-// Joins the pieces of the segments that several blocks have one of: a wavefront per row, whose lanes have four columns each and, where
-// that leaves lanes, the pieces in turn.
+// Joins the pieces of the segments that several blocks have one of.
 template <class T, int DIM, int R, int UNIT>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, T* __restrict__ out) {
     Segments<R, UNIT> segs(a);
@@ -488,48 +487,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, T* __restric
     x += head * segs.total;
     const unsigned b0 = x / share, b1 = (x + units - 1) / share;
     if (b0 == b1 || b1 >= unsigned(a.blocks)) return;
-    const int parts = int(b1 - b0) + 1;
-    constexpr int QUADS = DIM / 4, EVERY = 64 / QUADS;
-    const int lane = threadIdx.x & 63, d = lane % QUADS * 4, mine = lane / QUADS;
-    const int group = int(a.group.d), r = blockIdx.z * 4 + (threadIdx.x >> 6);
-    if (r >= s.chunk * group - tile * R) return;
     // the first piece is the second of its block's two, the others are the first of theirs
-    auto piece = [&](int i) { return a.partial + (2 * size_t(b0 + i) + (i == 0)) * kPiece<R, DIM>; };
-    float top = -__builtin_inff();
-    for (int i = lane; i < parts; i += 64) top = fmaxf(top, piece(i)[R * DIM + r]);
-#pragma unroll
-    for (int e = 1; e < 64; e *= 2) top = fmaxf(top, __shfl_xor(top, e, 64));
-    const float mm = top == -__builtin_inff() ? 0.f : top;
-    float total = 0.f;
-    f32x4 v = {0, 0, 0, 0};
-    for (int i0 = 0; i0 < parts; i0 += 4 * EVERY) {
-        f32x4 y[4];
-        float m[4], l[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const float* p = piece(min(i0 + u * EVERY + mine, parts - 1));
-            y[u] = *reinterpret_cast<const f32x4*>(p + r * DIM + d);
-            m[u] = p[R * DIM + r], l[u] = p[R * DIM + R + r];
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            if (i0 + u * EVERY + mine >= parts) continue;
-            const float f = __builtin_amdgcn_exp2f(m[u] - mm);
-            total += l[u] * f, v += y[u] * f;
-        }
-    }
-#pragma unroll
-    for (int e = QUADS; e < 64; e *= 2) {
-        total += __shfl_xor(total, e, 64);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] += __shfl_xor(v[k], e, 64);
-    }
-    if (d >= a.dim || mine) return;
-    v *= total == 0.f ? 0.f : 1.f / total;
-    const int row = tile * R + r, token = int(a.group(unsigned(row)));
-    T* dst = out + (size_t(s.q0 + token) * a.heads + size_t(int(head) * group + row - token * group)) * a.dim + d;
-    if constexpr (std::is_same_v<T, float>) *reinterpret_cast<f32x4*>(dst) = v;
-    else *reinterpret_cast<uint2*>(dst) = uint2{as_u32(to_h2(v[0], v[1])), as_u32(to_h2(v[2], v[3]))};
+    join_row<T, DIM, R>(a, out, s, tile, int(head), blockIdx.z * 4 + (threadIdx.x >> 6), int(b1 - b0) + 1,
+                        [&](int i) { return a.partial + (2 * size_t(b0 + i) + (i == 0)) * kPiece<R, DIM>; });
 }
 
 template <class T, int BITS, int DIM, int QT>

@@ -189,15 +189,6 @@ CacheView view_of(const lq_kv_cache* c) {
     return v;
 }
 
-// f with a type, a number of bits and a constant
-template <class F>
-void by_type(int dtype, int bits, F&& f) {
-    using B8 = std::integral_constant<int, 8>;
-    using B4 = std::integral_constant<int, 4>;
-    if (dtype == LQ_F32) bits == 8 ? f(float{}, B8{}) : f(float{}, B4{});
-    else bits == 8 ? f(_Float16{}, B8{}) : f(_Float16{}, B4{});
-}
-
 }  // namespace
 
 extern "C" {

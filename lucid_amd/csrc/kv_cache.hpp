@@ -1,5 +1,7 @@
 // The quantized key / value cache as its kernels see it (layout: lq_kv_cache in lucid_hip.h).
 #pragma once
+#include <type_traits>
+
 #include "common.hpp"
 
 namespace lq {
@@ -36,5 +38,14 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // two float32 as two float16, each rounded to nearest even (v_cvt_pk_f16_f32)
 __device__ __forceinline__ h2 to_h2(float a, float b) { return __builtin_convertvector(f32x2{a, b}, h2); }
+
+// f with a value of the type and the number of bits as constants
+template <class F>
+void by_type(int dtype, int bits, F&& f) {
+    using B8 = std::integral_constant<int, 8>;
+    using B4 = std::integral_constant<int, 4>;
+    if (dtype == LQ_F32) bits == 8 ? f(float{}, B8{}) : f(float{}, B4{});
+    else bits == 8 ? f(_Float16{}, B8{}) : f(_Float16{}, B4{});
+}
 
 }  // namespace lq

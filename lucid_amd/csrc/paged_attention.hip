@@ -29,37 +29,65 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
     a.page_size = FastDiv(unsigned(c->page_size)), a.group = FastDiv(unsigned(heads / c->kv_heads));
     a.pages = c->num_pages, a.kv_heads = c->kv_heads, a.dim = c->head_dim;
     a.tokens = tokens, a.heads = heads, a.batch = batch, a.width = table_width, a.causal = causal != 0, a.window = window, a.scale = scale;
-    const int group = heads / c->kv_heads;
-    const int sequences = std::min(batch, tokens);
-    const int chunk = max_chunk ? std::min(max_chunk, tokens) : batch == 1 ? tokens : (tokens + batch - 1) / std::max(batch, 1);
-    const int qt = chunk * group <= 16 ? 1 : 2, rows = 16 * qt;
-    const int tiles = sequences + int(int64_t(tokens) * group / rows);
+    const int group = heads / c->kv_heads, sequences = std::min(batch, tokens);
+    const int64_t all_rows = int64_t(tokens) * group, most = int64_t(table_width) * c->page_size;  // keys of a sequence
     const int dim = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
-    const int64_t most = int64_t(table_width) * c->page_size;  // keys of a sequence
-    LQ_REQUIRE(int64_t(tiles) * c->kv_heads * (most / 128 + 1) < 0x7fffffff, LQ_ERR_NOT_IMPLEMENTED,
-               "paged_attention: %d tiles of queries for %lld keys of %d heads are more than one call takes", tiles, (long long)most, c->kv_heads);
-    a.max_rows = 0x7fffffff;
-    // Up to 512 keys a block has a whole segment: four steps of each wavefront, where joining pieces takes another launch (one token of 197
-    // keys 10.3 -> 7.6 us).  Beyond, as many shares as blocks are resident.
-    const bool join = most > 512;
-    const int resident = (dim > 128 ? 1 : 2) * 256;
-    a.each = join ? resident : 0, a.least = 1;
-    a.blocks = join ? resident : tiles * a.kv_heads;
-    auto lock = scratch_lock(as_stream(stream));
-    if (join) {
+    // The longest chunk, or a guess at it: a single sequence has all tokens; equally many each otherwise.
+    const int chunk = max_chunk ? std::min(max_chunk, tokens) : batch == 1 ? tokens : (tokens + batch - 1) / std::max(batch, 1);
+    // Sequences of more than kFewRows rows go to attn_chunk_kernel, the others to attn_rows_kernel.  Where there can be both, and the longest
+    // chunk says that there are, both are launched and each takes its own; otherwise either takes all.
+    constexpr int kFewRows = 32;
+    const bool chunks = int64_t(chunk) * group > kFewRows, few = !chunks || sequences > 1;
+    hipStream_t st = as_stream(stream);
+    auto lock = scratch_lock(st);
+    auto room = [&](size_t floats) {
         void* p = nullptr;
-        rc = call_buffer(9, size_t(2) * a.blocks * rows * (dim + 2) * sizeof(float), as_stream(stream), &p);
-        if (rc) return rc;
+        const int rc = call_buffer(9, floats * sizeof(float), st, &p);
         a.partial = static_cast<float*>(p);
-    }
-    auto launch = [&](auto type, auto bits) {
-        using T = decltype(type);
-        attn::launch_rows_of<T, decltype(bits)::value>(a, static_cast<const T*>(q), static_cast<T*>(out), tiles, qt, join, as_stream(stream));
+        return rc;
     };
-    using B8 = std::integral_constant<int, 8>;
-    using B4 = std::integral_constant<int, 4>;
-    if (dtype == LQ_F32) c->bits == 8 ? launch(float{}, B8{}) : launch(float{}, B4{});
-    else c->bits == 8 ? launch(_Float16{}, B8{}) : launch(_Float16{}, B4{});
-    LQ_CHECK_LAUNCH("paged_attention");
+    if (chunks) {
+        constexpr int R = 128;
+        const int tiles = sequences + int(all_rows / R);
+        a.min_rows = few ? kFewRows + 1 : 1, a.max_rows = 0x7fffffff;
+        // Few tiles: each one's keys in parts, a block for each.
+        a.parts = int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(most / 1024, 16), 1024 / (int64_t(tiles) * c->kv_heads))));
+        LQ_REQUIRE(int64_t(tiles) * a.parts * c->kv_heads <= 0xffffff, LQ_ERR_NOT_IMPLEMENTED, "paged_attention: %d tiles of queries for %d heads",
+                   tiles, c->kv_heads);
+        if (a.parts > 1) {
+            rc = room(size_t(tiles) * a.parts * c->kv_heads * R * (dim + 2));
+            if (rc) return rc;
+        }
+        auto launch = [&](auto type, auto bits) {
+            using T = decltype(type);
+            rc = attn::launch_chunk_of<T, decltype(bits)::value>(a, static_cast<const T*>(q), static_cast<T*>(out), tiles, st);
+        };
+        by_type(dtype, c->bits, launch);
+        if (rc) return rc;
+        LQ_CHECK_LAUNCH("paged_attention");
+    }
+    if (few) {
+        const int qt = int64_t(chunk) * group <= 16 ? 1 : 2, rows = 16 * qt;
+        a.min_rows = 1, a.max_rows = chunks ? kFewRows : 0x7fffffff;
+        const int tiles = sequences + int((chunks ? std::min<int64_t>(all_rows, int64_t(sequences) * kFewRows) : all_rows) / rows);
+        LQ_REQUIRE(int64_t(tiles) * c->kv_heads * (most / 128 + 1) < 0x7fffffff, LQ_ERR_NOT_IMPLEMENTED,
+                   "paged_attention: %d tiles of queries for %lld keys of %d heads are more than one call takes", tiles, (long long)most, c->kv_heads);
+        // Up to 512 keys a block has a whole segment: four steps of each wavefront, where joining pieces takes another launch (one token
+        // of 197 keys 10.3 -> 7.6 us).  Beyond, as many shares as blocks are resident.
+        const bool join = most > 512;
+        const int resident = (dim > 128 ? 1 : 2) * 256;
+        a.each = join ? resident : 0, a.least = 1;
+        a.blocks = join ? resident : tiles * a.kv_heads;
+        if (join) {
+            rc = room(size_t(2) * a.blocks * rows * (dim + 2));
+            if (rc) return rc;
+        }
+        auto launch = [&](auto type, auto bits) {
+            using T = decltype(type);
+            attn::launch_rows_of<T, decltype(bits)::value>(a, static_cast<const T*>(q), static_cast<T*>(out), tiles, qt, join, st);
+        };
+        by_type(dtype, c->bits, launch);
+        LQ_CHECK_LAUNCH("paged_attention");
+    }
     return LQ_OK;
 }

@@ -34,7 +34,8 @@ struct AttnArgs {
     int blocks;
     int each;      // of so many blocks each has a share of the units, at least `least`; 0: a segment
     int least;
-    int max_rows;  // sequences of more rows are another launch's
+    int min_rows, max_rows;  // sequences of fewer or more rows are another launch's
+    int parts;     // of a tile's keys, a block each
     float scale;
     float* partial;  // pieces of segments
 };
@@ -46,6 +47,9 @@ namespace attn {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLazy = 8.f;        // a row's maximum is renewed when it has grown by this (powers of two)
 constexpr float kProbability = 0x1p7f;  // probabilities are kept times this
+
+__device__ __forceinline__ h2 as_h2(uint32_t v) { return __builtin_bit_cast(h2, v); }
+__device__ __forceinline__ uint32_t as_u32(h2 v) { return __builtin_bit_cast(uint32_t, v); }
 
 // f over the four lanes of one number in the four rows of 16 lanes; every lane gets it
 template <class F>
@@ -114,7 +118,7 @@ struct Segments {
         if (b < a.batch) {
             s = sequence_of(a, b);
             const int rows = s.chunk * int(a.group.d);
-            tiles = rows > a.max_rows ? 0u : unsigned(rows + R - 1) / R;
+            tiles = rows < a.min_rows || rows > a.max_rows ? 0u : unsigned(rows + R - 1) / R;
             const Keys k = keys_of(a, s, 0, s.chunk - 1);
             units = a.each ? max(1u, unsigned(k.hi - (k.lo & ~31) + UNIT - 1) / UNIT) : 1u;
         }
@@ -156,10 +160,87 @@ struct Segments {
     }
 };
 
+// Tile number `id` of R rows of the sequences of a launch; of each sequence's the last one first.  False: there is none.
+struct Tile {
+    int seq, tile;
+    Sequence s;
+};
+template <int R>
+__device__ __forceinline__ bool find_tile(const AttnArgs& a, unsigned id, Tile& it) {
+    const int lane = threadIdx.x & 63;
+    unsigned before = 0;
+    for (int first = 0; first < a.batch; first += 64) {
+        Sequence s{0, 0, 0};
+        if (first + lane < a.batch) s = sequence_of(a, first + lane);
+        const int rows = s.chunk * int(a.group.d);
+        const unsigned tiles = rows < a.min_rows || rows > a.max_rows ? 0u : unsigned(rows + R - 1) / R;
+        unsigned upto = tiles;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const unsigned o = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += o;
+        }
+        const unsigned long long past = __ballot(upto > id - before);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            auto get = [&](unsigned v) { return unsigned(__builtin_amdgcn_readlane(int(v), l)); };
+            it.seq = first + l, it.tile = int(get(upto) - 1 - (id - before));
+            it.s = Sequence{int(get(unsigned(s.q0))), int(get(unsigned(s.chunk))), int(get(unsigned(s.len)))};
+            return true;
+        }
+        before += unsigned(__builtin_amdgcn_readlane(int(upto), 63));
+    }
+    return false;
+}
+
 // A piece of a segment: R rows of DIM sums over its keys, then the rows' maxima and sums of probabilities.  A block has room for two, the
 // first for a segment that begins in a block before it, the second for one that goes on in the next.
 template <int R, int DIM>
 constexpr size_t kPiece = size_t(R) * (DIM + 2);
+
+// Row r of a tile from its pieces, by a wavefront: a lane has four columns and, where that leaves lanes, the pieces in turn.
+template <class T, int DIM, int R, class Piece>
+__device__ __forceinline__ void join_row(const AttnArgs& a, T* out, const Sequence& s, int tile, int head, int r, int parts, Piece piece) {
+    constexpr int QUADS = DIM / 4, EVERY = 64 / QUADS;
+    const int lane = threadIdx.x & 63, d = lane % QUADS * 4, mine = lane / QUADS;
+    const int group = int(a.group.d);
+    if (r >= s.chunk * group - tile * R) return;
+    float top = -__builtin_inff();
+    for (int i = lane; i < parts; i += 64) top = fmaxf(top, piece(i)[R * DIM + r]);
+#pragma unroll
+    for (int e = 1; e < 64; e *= 2) top = fmaxf(top, __shfl_xor(top, e, 64));
+    const float mm = top == -__builtin_inff() ? 0.f : top;
+    float total = 0.f;
+    f32x4 v = {0, 0, 0, 0};
+    for (int i0 = 0; i0 < parts; i0 += 4 * EVERY) {
+        f32x4 y[4];
+        float m[4], l[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float* p = piece(min(i0 + u * EVERY + mine, parts - 1));
+            y[u] = *reinterpret_cast<const f32x4*>(p + r * DIM + d);
+            m[u] = p[R * DIM + r], l[u] = p[R * DIM + R + r];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (i0 + u * EVERY + mine >= parts) continue;
+            const float f = __builtin_amdgcn_exp2f(m[u] - mm);
+            total += l[u] * f, v += y[u] * f;
+        }
+    }
+#pragma unroll
+    for (int e = QUADS; e < 64; e *= 2) {
+        total += __shfl_xor(total, e, 64);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += __shfl_xor(v[k], e, 64);
+    }
+    if (d >= a.dim || mine) return;
+    v *= total == 0.f ? 0.f : 1.f / total;
+    const int row = tile * R + r, token = int(a.group(unsigned(row)));
+    T* dst = out + (size_t(s.q0 + token) * a.heads + size_t(head * group + row - token * group)) * a.dim + d;
+    if constexpr (std::is_same_v<T, float>) *reinterpret_cast<f32x4*>(dst) = v;
+    else *reinterpret_cast<uint2*>(dst) = uint2{as_u32(to_h2(v[0], v[1])), as_u32(to_h2(v[2], v[3]))};
+}
 
 // Zeros for the rows of q that belong to no sequence, dealt to the blocks.
 template <class T>
@@ -174,8 +255,6 @@ __device__ __forceinline__ void clear_other_rows(const AttnArgs& a, T* out, unsi
 }
 
 // ---- codes to float16: 1024 + u is the float16 0x6400 | u for u < 1024
-__device__ __forceinline__ h2 as_h2(uint32_t v) { return __builtin_bit_cast(h2, v); }
-__device__ __forceinline__ uint32_t as_u32(h2 v) { return __builtin_bit_cast(uint32_t, v); }
 // 0x64006400 in a vector register: beside a mask in a scalar one it makes "and, or" one instruction
 __device__ __forceinline__ uint32_t magic() {
     uint32_t m = 0x64006400u;
@@ -227,6 +306,10 @@ constexpr int rows_keys(int bits, int dim, int qt) { return bits * dim <= 512 &&
 // One token, or a few, of each sequence: tiles of 16 * qt rows.  `tiles`: a bound for those of all sequences; join: segments may be in pieces.
 template <class T, int BITS>
 void launch_rows_of(const AttnArgs& a, const T* q, T* out, int tiles, int qt, bool join, hipStream_t st);
+
+// A chunk of a sequence: tiles of 128 rows.
+template <class T, int BITS>
+int launch_chunk_of(const AttnArgs& a, const T* q, T* out, int tiles, hipStream_t st);
 
 }  // namespace attn
 }  // namespace lq
