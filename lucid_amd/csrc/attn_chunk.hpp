@@ -61,9 +61,7 @@ struct ChunkKernel {
         const int from = min(seen.hi, base + part * share), to = min(seen.hi, from + share);
         // this wavefront's rows, and the keys that all of them see
         const int w0 = min(row0 + 32 * wave, last_row), w1 = min(row0 + 32 * wave + 31, last_row);
-        const bool any = row0 + 32 * wave <= last_row;
         const int token0 = int(a.group(unsigned(w0))), token1 = int(a.group(unsigned(w1)));
-        const Keys wave_seen = keys_of(a, it.s, token0, token1);
         const int all_lo = a.window > 0 ? max(0, at + token1 - a.window + 1) : 0;
         const int all_hi = min(to, a.causal ? min(it.s.len, at + token0 + 1) : it.s.len);
 
@@ -96,35 +94,64 @@ struct ChunkKernel {
         float kz[KP];
         f32x4 vz[VP][2];
         float ks_reg, vs_reg, vzero = 0.f;  // of key `lane`
+        // Lanes of a wavefront whose pieces lie in one tile of 16 keys share a scalar base, and their offsets do not change.
+        constexpr bool K_ONE = PIECES >= 4, V_ONE = DIM >= 128;
         auto request = [&] {
 #pragma unroll
             for (int i = 0; i < KP; ++i) {
                 const int u = tid + i * THREADS, key = u / PIECES, piece = u % PIECES;
                 if (KEYS * PIECES % THREADS && u >= KEYS * PIECES) break;
-                const size_t row = place_of(key >> 4) + (key & 15);
-                kreg[i] = *reinterpret_cast<const uint4*>(a.k_codes + row * unsigned(row_bytes) + (piece * 16 < row_bytes ? piece * 16 : 0));
-                if constexpr (AFFINE) kz[i] = a.k_zero[row];
+                const int byte = piece * 16 < row_bytes ? piece * 16 : 0;
+                if constexpr (K_ONE) {
+                    const size_t row = place_of(__builtin_amdgcn_readfirstlane(key >> 4));
+                    const auto rows = rows_at(a.k_codes + row * unsigned(row_bytes), 16 * row_bytes);
+                    kreg[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rows, (key & 15) * row_bytes + byte, 0, 0));
+                    if constexpr (AFFINE) kz[i] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rows_at(a.k_zero + row, 64), (key & 15) * 4, 0, 0));
+                } else {
+                    const size_t row = place_of(key >> 4) + (key & 15);
+                    kreg[i] = *reinterpret_cast<const uint4*>(a.k_codes + row * unsigned(row_bytes) + byte);
+                    if constexpr (AFFINE) kz[i] = a.k_zero[row];
+                }
             }
 #pragma unroll
             for (int i = 0; i < VP; ++i) {
                 const int u = tid + i * THREADS, chunk = u / (DIM / 4), d = u % (DIM / 4) * 4;
                 if (VUNITS % THREADS && u >= VUNITS) break;
-                const size_t row = place_of(chunk >> 1) + 4 * (chunk & 1);
-                const uint8_t* p = a.v_codes + row * unsigned(row_bytes) + (d < a.dim ? d * BITS / 8 : 0);
+                const int byte = d < a.dim ? d * BITS / 8 : 0;
+                if constexpr (V_ONE) {
+                    const size_t row = place_of(__builtin_amdgcn_readfirstlane(chunk >> 1));
+                    const auto rows = rows_at(a.v_codes + row * unsigned(row_bytes), 16 * row_bytes);
+                    const int off = 4 * (chunk & 1) * row_bytes + byte;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint8_t* pe = p + ((e & 3) + 2 * (e & 4)) * row_bytes;  // keys 0..3 and 8..11 from here
-                    if constexpr (BITS == 8) vreg[i][e] = *reinterpret_cast<const uint32_t*>(pe);
-                    else vreg[i][e] = *reinterpret_cast<const uint16_t*>(pe);
+                    for (int e = 0; e < 8; ++e) {
+                        const int skip = ((e & 3) + 2 * (e & 4)) * row_bytes;  // keys 0..3 and 8..11 from here
+                        if constexpr (BITS == 8) vreg[i][e] = __builtin_amdgcn_raw_buffer_load_b32(rows, off, skip, 0);
+                        else vreg[i][e] = __builtin_amdgcn_raw_buffer_load_b16(rows, off, skip, 0);
+                    }
+                    if constexpr (AFFINE)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            vz[i][e] = __builtin_bit_cast(
+                                f32x4, __builtin_amdgcn_raw_buffer_load_b128(rows_at(a.v_zero + row, 64), 16 * (chunk & 1) + 32 * e, 0, 0));
+                } else {
+                    const size_t row = place_of(chunk >> 1) + 4 * (chunk & 1);
+                    const uint8_t* p = a.v_codes + row * unsigned(row_bytes) + byte;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint8_t* pe = p + ((e & 3) + 2 * (e & 4)) * row_bytes;
+                        if constexpr (BITS == 8) vreg[i][e] = *reinterpret_cast<const uint32_t*>(pe);
+                        else vreg[i][e] = *reinterpret_cast<const uint16_t*>(pe);
+                    }
+                    if constexpr (AFFINE)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) vz[i][e] = *reinterpret_cast<const f32x4*>(a.v_zero + row + 8 * e);
                 }
-                if constexpr (AFFINE)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) vz[i][e] = *reinterpret_cast<const f32x4*>(a.v_zero + row + 8 * e);
             }
             const size_t row = place_of(lane >> 4) + (lane & 15);
             ks_reg = a.k_scale[row], vs_reg = a.v_scale[row];
             if constexpr (AFFINE) vzero = a.v_zero[row];
         };
+        bool not_finite = false;  // among the scales of the keys that were settled last
         float unit = 0.f, per_unit = 0.f, regrow = 1.f;  // regrow: what the outputs so far are to be multiplied by
         const uint32_t high = BITS == 4 ? magic() : 0;
         auto settle = [&](int key, char* stage) {
@@ -184,6 +211,7 @@ struct ChunkKernel {
             float vs = vs_reg;
             if (AFFINE && !(fabsf(vzero) <= 2048.f)) vs = __builtin_nanf("");
             if (!(key + lane >= seen.lo && key + lane < to && (ok >> (lane >> 4) & 1))) vs = 0.f;
+            not_finite = __ballot(!(fabsf(vs) < __builtin_inff())) != 0;
             float top = fmaxf(0.f, fabsf(vs));
             top = rows4_max(top);
 #pragma unroll
@@ -217,7 +245,7 @@ struct ChunkKernel {
                 for (int p = 0; p < PARTS; ++p) {
                     const int d = 16 * i + 8 * h;
                     raw[i][p] = reinterpret_cast<const Raw*>(src + (d < a.dim ? d : 0))[p];
-                    if (d >= a.dim) raw[i][p] = Raw{};
+                    if (d >= a.dim || a.scale == 0.f) raw[i][p] = Raw{};
                 }
             if (from < to) {
                 locate(from, pages);
@@ -225,8 +253,9 @@ struct ChunkKernel {
                 request();
             }
             // a negative scale changes the queries' signs: the largest score is the largest product then too
+            // (and of a scale of 0 all scores are 0, the masked ones still none)
             const bool minus = factor < 0.f;
-            factor = fabsf(factor);
+            factor = factor == 0.f ? 1.f : fabsf(factor);
             int up = 0;
             if constexpr (F32) {
                 float top = 0.f;
@@ -262,7 +291,7 @@ struct ChunkKernel {
         f32x16 o[TILES] = {};
         float m = -__builtin_inff(), l = 0.f;  // m: of scores without the row's factor
 
-        auto work = [&](const char* stage, int ok_now, float grown) {
+        auto work = [&](const char* stage, int ok_now, float grown, bool odd) {
             const float* scales = reinterpret_cast<const float*>(stage + K_BYTES + V_BYTES);
             f32x16 s[2];
 #pragma unroll
@@ -275,7 +304,6 @@ struct ChunkKernel {
                     for (int p = PARTS - 1; p >= 0; --p) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[i][p], s[t], 0, 0, 0);
                 }
             }
-            const bool whole = key >= all_lo && key + KEYS <= all_hi && ok_now == 15;
             float top = -__builtin_inff();
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -283,23 +311,27 @@ struct ChunkKernel {
                 for (int b = 0; b < 4; ++b) {
                     const f32x4 ks = *reinterpret_cast<const f32x4*>(scales + 32 * t + 8 * b + 4 * h);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float x = s[t][4 * b + r] * ks[r];
-                        if (!whole) {
-                            const int j = key + 32 * t + 8 * b + 4 * h + r;
-                            if (!(j >= lo && j < hi && (ok_now >> (2 * t + b / 2) & 1))) x = -__builtin_inff();
-                        }
-                        s[t][4 * b + r] = x;
-                        top = fmaxf(top, x);
-                    }
+                    for (int r = 0; r < 4; ++r) s[t][4 * b + r] *= ks[r];
                 }
+            // keys that some rows do not see: the exponential makes them zeros
+            if (!(key >= all_lo && key + KEYS <= all_hi && ok_now == 15)) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int j = key + 32 * t + 8 * (i / 4) + 4 * h + i % 4;
+                        if (!(j >= lo && j < hi && (ok_now >> (2 * t + i / 8) & 1))) s[t][i] = -__builtin_inff();
+                    }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
             top = halves(top, [](float x, float y) { return fmaxf(x, y); });
-            const float risen = (top - m) * factor;
             float f = grown;
-            if (__ballot(risen > kLazy || (m == -__builtin_inff() && top > m))) {
+            if (__ballot((top - m) * factor > kLazy || (m == -__builtin_inff() && top > m))) {
                 const float now = fmaxf(m, top), e = now == m ? 1.f : m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((m - now) * factor);
-                l *= e, f *= e;
-                m = now;
+                l *= e, m = now, f *= e;
             }
             if (__ballot(f != 1.f)) {
 #pragma unroll
@@ -308,32 +340,40 @@ struct ChunkKernel {
                     for (int i = 0; i < 16; ++i) o[d][i] *= f;
             }
             const float mm = m == -__builtin_inff() ? 0.f : -m * factor;
-            Frag pf[4][PARTS];
             float sum = 0.f;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     const f32x4 vs = *reinterpret_cast<const f32x4*>(scales + KEYS + 32 * t + 8 * b + 4 * h);
-                    float p[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float x = s[t][4 * b + r];
-                        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, factor, mm));
-                        if (!whole && x == -__builtin_inff()) p[r] = 0.f;
-                        sum += p[r];
-                        p[r] *= vs[r];
-                        if (!whole && x == -__builtin_inff()) p[r] = 0.f;
-                    }
-                    Frag* to_frag = pf[2 * t + b / 2];
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const h2 x = to_h2(p[2 * r], p[2 * r + 1]);
-                        to_frag[0].p[2 * (b % 2) + r] = x;
-                        if constexpr (F32) to_frag[1].p[2 * (b % 2) + r] = to_h2(p[2 * r] - float(x.x), p[2 * r + 1] - float(x.y));
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][4 * b + r], factor, mm));
+                        sum += p;
+                        s[t][4 * b + r] = p * vs[r];
                     }
                 }
             l += sum;
+            // a scale that is no finite number shows in the rows that see its key, not in the others
+            if (odd) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int j = key + 32 * t + 8 * (i / 4) + 4 * h + i % 4;
+                        if (!(j >= lo && j < hi && (ok_now >> (2 * t + i / 8) & 1))) s[t][i] = 0.f;
+                    }
+            }
+            Frag pf[4][PARTS];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const h2 x = to_h2(s[t][i], s[t][i + 1]);
+                    Frag* to_frag = pf[2 * t + i / 8];
+                    to_frag[0].p[i % 8 / 2] = x;
+                    if constexpr (F32) to_frag[1].p[i % 8 / 2] = to_h2(s[t][i] - float(x.x), s[t][i + 1] - float(x.y));
+                }
 #pragma unroll
             for (int d = 0; d < TILES; ++d)
 #pragma unroll
@@ -353,6 +393,7 @@ struct ChunkKernel {
                 const int ok_now = ok;
                 own_unit = unit;
                 const float grown = regrow;
+                const bool odd = not_finite;
                 const bool more = key + KEYS < to;
                 if (more) {
                     locate(key + KEYS, pages);
@@ -360,15 +401,7 @@ struct ChunkKernel {
                     request();
                 }
                 char* stage = lds + side * STAGE;
-                // (a tile that none of a wavefront's rows sees: its outputs still go to the new unit)
-                if (any && key < wave_seen.hi && key + KEYS > wave_seen.lo) {
-                    work(stage, ok_now, grown);
-                } else if (grown != 1.f) {
-#pragma unroll
-                    for (int d = 0; d < TILES; ++d)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[d][i] *= grown;
-                }
+                work(stage, ok_now, grown, odd);
                 side ^= 1;
                 if (more) {
                     settle(key + KEYS, lds + side * STAGE);
