@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "paged_attention.hpp"
+#include "wave_reduce.hpp"
 
 namespace lq {
 namespace attn {
@@ -153,6 +154,9 @@ struct ChunkKernel {
         };
         bool not_finite = false;  // among the scales of the keys that were settled last
         float unit = 0.f, per_unit = 0.f, regrow = 1.f;  // regrow: what the outputs so far are to be multiplied by
+        // a negative scale changes the queries' signs, and of a scale of 0 all scores are 0, the masked ones still none.  What is left
+        // goes with the keys' scales, with float32 queries, which have a factor for each row, with the scores
+        const float key_factor = a.scale == 0.f ? 1.f : fabsf(a.scale * kLog2e);
         const uint32_t high = BITS == 4 ? magic() : 0;
         auto settle = [&](int key, char* stage) {
 #pragma unroll
@@ -213,9 +217,7 @@ struct ChunkKernel {
             if (!(key + lane >= seen.lo && key + lane < to && (ok >> (lane >> 4) & 1))) vs = 0.f;
             not_finite = __ballot(!(fabsf(vs) < __builtin_inff())) != 0;
             float top = fmaxf(0.f, fabsf(vs));
-            top = rows4_max(top);
-#pragma unroll
-            for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
+            top = wave_max(top);
             regrow = 1.f;
             if (__builtin_amdgcn_readfirstlane(int(!(top <= unit) || unit == 0.f))) {
                 const float next = fminf(fmaxf(__uint_as_float(__float_as_uint(top) & 0x7f800000u), 0x1p-100f), 0x1p124f) * 4.f;
@@ -223,14 +225,14 @@ struct ChunkKernel {
             }
             if (wave == 0) {
                 float* to_lds = reinterpret_cast<float*>(stage + K_BYTES + V_BYTES);
-                to_lds[lane] = ks_reg, to_lds[KEYS + lane] = vs * per_unit;
+                to_lds[lane] = F32 ? ks_reg : ks_reg * key_factor, to_lds[KEYS + lane] = vs * per_unit;
             }
         };
 
         int key = from, pages = pages_of(from);
         // ---- queries: column n is row row0 + 32 wave + n
         h8 qf[SLABS][PARTS];
-        float factor = a.scale * kLog2e;
+        float factor = key_factor;
         int lo, hi;
         {
             const int used = min(row0 + 32 * wave + n, last_row), token = int(a.group(unsigned(used)));
@@ -252,10 +254,7 @@ struct ChunkKernel {
                 pages = pages_of(from + KEYS);
                 request();
             }
-            // a negative scale changes the queries' signs: the largest score is the largest product then too
-            // (and of a scale of 0 all scores are 0, the masked ones still none)
-            const bool minus = factor < 0.f;
-            factor = factor == 0.f ? 1.f : fabsf(factor);
+            const bool minus = a.scale < 0.f;
             int up = 0;
             if constexpr (F32) {
                 float top = 0.f;
@@ -265,7 +264,7 @@ struct ChunkKernel {
                     for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(raw[i][e / 4][e % 4]));
                 top = halves(top, [](float x, float y) { return fmaxf(x, y); });
                 up = max(-126, min(126, 14 - __builtin_amdgcn_frexp_expf(top)));
-                factor = __builtin_ldexpf(factor, -up);
+                factor = __builtin_ldexpf(key_factor, -up);
             }
             constexpr int order[2][8] = {{0, 1, 2, 3, 4, 5, 6, 7}, {0, 4, 1, 5, 2, 6, 3, 7}};
 #pragma unroll
@@ -289,29 +288,41 @@ struct ChunkKernel {
             }
         }
         f32x16 o[TILES] = {};
-        float m = -__builtin_inff(), l = 0.f;  // m: of scores without the row's factor
+        float m = -__builtin_inff(), l = 0.f;
 
         auto work = [&](const char* stage, int ok_now, float grown, bool odd) {
             const float* scales = reinterpret_cast<const float*>(stage + K_BYTES + V_BYTES);
-            f32x16 s[2];
+            // (neighbouring products go to different accumulators; the next fragments are read ahead of them)
+            f32x16 s[2] = {};
+            {
+                h8 k[2][2];
+                auto read = [&](int i) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                s[t] = f32x16{};
+                    for (int t = 0; t < 2; ++t) k[i & 1][t] = *reinterpret_cast<const h8*>(stage + k_at(32 * t + n, 2 * i + h));
+                };
+                read(0);
 #pragma unroll
                 for (int i = 0; i < SLABS; ++i) {
-                    const h8 k = *reinterpret_cast<const h8*>(stage + k_at(32 * t + n, 2 * i + h));
+                    if (i + 1 < SLABS) read(i + 1);
 #pragma unroll
-                    for (int p = PARTS - 1; p >= 0; --p) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[i][p], s[t], 0, 0, 0);
+                    for (int p = PARTS - 1; p >= 0; --p)
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i & 1][t], qf[i][p], s[t], 0, 0, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, 2 * PARTS, 0);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            float top = -__builtin_inff();
+            // s becomes the exponent: the score less the row's maximum so far
+            const float mm = m == -__builtin_inff() ? 0.f : -m;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     const f32x4 ks = *reinterpret_cast<const f32x4*>(scales + 32 * t + 8 * b + 4 * h);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[t][4 * b + r] *= ks[r];
+                    for (int r = 0; r < 4; ++r)
+                        s[t][4 * b + r] = __builtin_fmaf(F32 ? s[t][4 * b + r] * factor : s[t][4 * b + r], ks[r], mm);
                 }
             // keys that some rows do not see: the exponential makes them zeros
             if (!(key >= all_lo && key + KEYS <= all_hi && ok_now == 15)) {
@@ -323,15 +334,25 @@ struct ChunkKernel {
                         if (!(j >= lo && j < hi && (ok_now >> (2 * t + i / 8) & 1))) s[t][i] = -__builtin_inff();
                     }
             }
+            float top = -__builtin_inff();
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
             top = halves(top, [](float x, float y) { return fmaxf(x, y); });
             float f = grown;
-            if (__ballot((top - m) * factor > kLazy || (m == -__builtin_inff() && top > m))) {
-                const float now = fmaxf(m, top), e = now == m ? 1.f : m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((m - now) * factor);
-                l *= e, m = now, f *= e;
+            const bool first = m == -__builtin_inff();
+            if (__ballot(top > kLazy || (first && top > m))) {
+                const float by = first ? top : fmaxf(top, 0.f);  // (-inf: no key seen yet)
+                const float e = first ? 0.f : __builtin_amdgcn_exp2f(-by);
+                if (by != -__builtin_inff()) {
+                    m = first ? by : m + by;
+                    l *= e, f *= e;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[t][i] -= by;
+                }
             }
             if (__ballot(f != 1.f)) {
 #pragma unroll
@@ -339,7 +360,6 @@ struct ChunkKernel {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[d][i] *= f;
             }
-            const float mm = m == -__builtin_inff() ? 0.f : -m * factor;
             float sum = 0.f;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -348,7 +368,7 @@ struct ChunkKernel {
                     const f32x4 vs = *reinterpret_cast<const f32x4*>(scales + KEYS + 32 * t + 8 * b + 4 * h);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][4 * b + r], factor, mm));
+                        const float p = __builtin_amdgcn_exp2f(s[t][4 * b + r]);
                         sum += p;
                         s[t][4 * b + r] = p * vs[r];
                     }
@@ -374,14 +394,21 @@ struct ChunkKernel {
                     to_frag[0].p[i % 8 / 2] = x;
                     if constexpr (F32) to_frag[1].p[i % 8 / 2] = to_h2(s[t][i] - float(x.x), s[t][i + 1] - float(x.y));
                 }
+            h8 v[4];
+            auto read = [&](int x) { v[x % 4] = *reinterpret_cast<const h8*>(stage + v_at(32 * (x % TILES) + n, 2 * (x / TILES) + h)); };
+            read(0), read(1);
 #pragma unroll
-            for (int d = 0; d < TILES; ++d)
+            for (int x = 0; x < 4 * TILES; x += 2) {
+                if (x + 2 < 4 * TILES) read(x + 2), read(x + 3);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const h8 v = *reinterpret_cast<const h8*>(stage + v_at(32 * d + n, 2 * i + h));
+                for (int p = PARTS - 1; p >= 0; --p)
 #pragma unroll
-                    for (int p = PARTS - 1; p >= 0; --p) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pf[i][p].v, o[d], 0, 0, 0);
-                }
+                    for (int y = x; y < x + 2; ++y)
+                        o[y % TILES] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[y % 4], pf[y / TILES][p].v, o[y % TILES], 0, 0, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 2 * PARTS, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         };
 
         float own_unit = 0.f;
@@ -415,7 +442,7 @@ struct ChunkKernel {
         const float scale = own_unit * (1.f / kProbability) * (a.parts == 1 ? (l == 0.f ? 0.f : 1.f / l) : 1.f);
         if (a.parts > 1) {
             float* piece = a.partial + (size_t(item) * a.kv_heads + head) * kPiece<R, DIM>;
-            if (h == 0) piece[R * DIM + 32 * wave + n] = m == -__builtin_inff() ? m : m * factor, piece[R * DIM + R + 32 * wave + n] = l;
+            if (h == 0) piece[R * DIM + 32 * wave + n] = m, piece[R * DIM + R + 32 * wave + n] = l;
 #pragma unroll
             for (int d = 0; d < TILES; ++d)
 #pragma unroll
