@@ -21,6 +21,9 @@ namespace attn {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+// v_mul_legacy_f32: a product in which 0 times anything is 0
+__device__ float mul_legacy(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
+
 // the value of the lane 32 further on (or back) with this one's
 template <class F>
 __device__ __forceinline__ float halves(float v, F f) {
@@ -75,6 +78,16 @@ struct ChunkKernel {
         size_t place[4];
         int ok = 0;
         auto locate = [&](int key, int pages) {
+            if (a.page_size.d % KEYS == 0) {  // (all on one page)
+                const unsigned page = unsigned(__builtin_amdgcn_readlane(pages, 0));
+                const bool there = key < to && page < unsigned(a.pages);
+                ok = there ? (1 << min(4, (to - key + 15) / 16)) - 1 : 0;
+                const unsigned in_page = unsigned(key) - a.page_size(unsigned(key)) * a.page_size.d;
+                place[0] = there ? (size_t(page) * unsigned(a.kv_heads) + unsigned(head)) * a.page_size.d + in_page : 0;
+                const size_t step = there ? 16 : 0;
+                place[1] = place[0] + step, place[2] = place[1] + step, place[3] = place[2] + step;
+                return;
+            }
             ok = 0;
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -97,7 +110,7 @@ struct ChunkKernel {
         float ks_reg, vs_reg, vzero = 0.f;  // of key `lane`
         // Lanes of a wavefront whose pieces lie in one tile of 16 keys share a scalar base, and their offsets do not change.
         constexpr bool K_ONE = PIECES >= 4, V_ONE = DIM >= 128;
-        auto request = [&] {
+        auto request_k = [&] {
 #pragma unroll
             for (int i = 0; i < KP; ++i) {
                 const int u = tid + i * THREADS, key = u / PIECES, piece = u % PIECES;
@@ -114,6 +127,11 @@ struct ChunkKernel {
                     if constexpr (AFFINE) kz[i] = a.k_zero[row];
                 }
             }
+            const size_t row = place_of(lane >> 4) + (lane & 15);
+            ks_reg = a.k_scale[row], vs_reg = a.v_scale[row];
+            if constexpr (AFFINE) vzero = a.v_zero[row];
+        };
+        auto request_v = [&] {
 #pragma unroll
             for (int i = 0; i < VP; ++i) {
                 const int u = tid + i * THREADS, chunk = u / (DIM / 4), d = u % (DIM / 4) * 4;
@@ -148,88 +166,78 @@ struct ChunkKernel {
                         for (int e = 0; e < 2; ++e) vz[i][e] = *reinterpret_cast<const f32x4*>(a.v_zero + row + 8 * e);
                 }
             }
-            const size_t row = place_of(lane >> 4) + (lane & 15);
-            ks_reg = a.k_scale[row], vs_reg = a.v_scale[row];
-            if constexpr (AFFINE) vzero = a.v_zero[row];
         };
-        bool not_finite = false;  // among the scales of the keys that were settled last
-        float unit = 0.f, per_unit = 0.f, regrow = 1.f;  // regrow: what the outputs so far are to be multiplied by
+        // outputs are kept in units of 2^unit, see the top of paged_attention.hpp; regrow: what those so far are to be multiplied by
+        int unit = -98;
+        float regrow = 1.f;
         // a negative scale changes the queries' signs, and of a scale of 0 all scores are 0, the masked ones still none.  What is left
         // goes with the keys' scales, with float32 queries, which have a factor for each row, with the scores
         const float key_factor = a.scale == 0.f ? 1.f : fabsf(a.scale * kLog2e);
         const uint32_t high = BITS == 4 ? magic() : 0;
-        auto settle = [&](int key, char* stage) {
-#pragma unroll
-            for (int i = 0; i < KP; ++i) {
+        // what is requested becomes float16 in LDS, a part at a time: eight columns of a key, and at last the scales
+        constexpr int K_EIGHTS = BITS == 8 ? 2 : 4, K_STEPS = KP * K_EIGHTS + 1;
+        auto settle_k = [&](int part, int key, char* stage) {
+            if (part < KP * K_EIGHTS) {
+                const int i = part / K_EIGHTS, e = part % K_EIGHTS;
                 const int u = tid + i * THREADS, k = u / PIECES, piece = u % PIECES;
-                if (KEYS * PIECES % THREADS && u >= KEYS * PIECES) break;
+                if (KEYS * PIECES % THREADS && u >= KEYS * PIECES) return;
                 const Offsets<BITS> off = AFFINE ? Offsets<BITS>(kz[i], kz[i]) : Offsets<BITS>();
                 const uint32_t w[4] = {kreg[i].x, kreg[i].y, kreg[i].z, kreg[i].w};
+                Frag f;
                 if constexpr (BITS == 8) {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        Frag f;
-                        f.p[0] = bytes01(w[2 * e], off.of1024), f.p[1] = bytes23(w[2 * e], off.of1024);
-                        f.p[2] = bytes01(w[2 * e + 1], off.of1024), f.p[3] = bytes23(w[2 * e + 1], off.of1024);
-                        *reinterpret_cast<h8*>(stage + k_at(k, 2 * piece + e)) = f.v;
-                    }
+                    f.p[0] = bytes01(w[2 * e], off.of1024), f.p[1] = bytes23(w[2 * e], off.of1024);
+                    f.p[2] = bytes01(w[2 * e + 1], off.of1024), f.p[3] = bytes23(w[2 * e + 1], off.of1024);
                 } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        Frag f;
-                        const uint32_t u1 = w[e] >> 8;
-                        f.p[0] = nibbles0(w[e], high, off.of1024), f.p[1] = nibbles4(w[e], high, off.of64);
-                        f.p[2] = nibbles0(u1, high, off.of1024), f.p[3] = nibbles4(u1, high, off.of64);
-                        *reinterpret_cast<h8*>(stage + k_at(k, 4 * piece + e)) = f.v;
-                    }
+                    const uint32_t u1 = w[e] >> 8;
+                    f.p[0] = nibbles0(w[e], high, off.of1024), f.p[1] = nibbles4(w[e], high, off.of64);
+                    f.p[2] = nibbles0(u1, high, off.of1024), f.p[3] = nibbles4(u1, high, off.of64);
                 }
+                *reinterpret_cast<h8*>(stage + k_at(k, K_EIGHTS * piece + e)) = f.v;
+                return;
             }
-#pragma unroll
-            for (int i = 0; i < VP; ++i) {
-                const int u = tid + i * THREADS, chunk = u / (DIM / 4), d = u % (DIM / 4) * 4;
-                if (VUNITS % THREADS && u >= VUNITS) break;
-                Frag f[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    Offsets<BITS> off;
-                    if constexpr (AFFINE) {
-                        // (a zero point that is no number reaches every row through the matrix product: the scale has it instead)
-                        const float z0 = vz[i][e / 2][2 * (e % 2)], z1 = vz[i][e / 2][2 * (e % 2) + 1];
-                        off = Offsets<BITS>(fabsf(z0) <= 2048.f ? z0 : 0.f, fabsf(z1) <= 2048.f ? z1 : 0.f);
-                    }
-                    const uint32_t x = vreg[i][2 * e], y = vreg[i][2 * e + 1];
-                    if constexpr (BITS == 8) {
-                        const uint32_t u0 = __builtin_amdgcn_perm(y, x, 0x05010400u), u1 = __builtin_amdgcn_perm(y, x, 0x07030602u);
-                        f[0].p[e] = bytes01(u0, off.of1024), f[1].p[e] = bytes23(u0, off.of1024);
-                        f[2].p[e] = bytes01(u1, off.of1024), f[3].p[e] = bytes23(u1, off.of1024);
-                    } else {
-                        const uint32_t u0 = __builtin_amdgcn_perm(y, x, 0x05040100u), u1 = u0 >> 8;
-                        f[0].p[e] = nibbles0(u0, high, off.of1024), f[1].p[e] = nibbles4(u0, high, off.of64);
-                        f[2].p[e] = nibbles0(u1, high, off.of1024), f[3].p[e] = nibbles4(u1, high, off.of64);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) *reinterpret_cast<h8*>(stage + v_at(d + j, chunk)) = f[j].v;
-            }
-            // scales; the unit of the outputs (all wavefronts come to the same)
+            // scales, and the unit (all wavefronts come to the same): above the largest of them by up to four times, and seldom renewed
             float vs = vs_reg;
             if (AFFINE && !(fabsf(vzero) <= 2048.f)) vs = __builtin_nanf("");
-            if (!(key + lane >= seen.lo && key + lane < to && (ok >> (lane >> 4) & 1))) vs = 0.f;
-            not_finite = __ballot(!(fabsf(vs) < __builtin_inff())) != 0;
-            float top = fmaxf(0.f, fabsf(vs));
-            top = wave_max(top);
-            regrow = 1.f;
-            if (__builtin_amdgcn_readfirstlane(int(!(top <= unit) || unit == 0.f))) {
-                const float next = fminf(fmaxf(__uint_as_float(__float_as_uint(top) & 0x7f800000u), 0x1p-100f), 0x1p124f) * 4.f;
-                regrow = unit / next, unit = next, per_unit = kProbability / next;
+            if (!((key + lane >= seen.lo) & (key + lane < to) & (ok >> (lane >> 4) & 1))) vs = 0.f;
+            const float top = fminf(wave_max(fmaxf(0.f, fabsf(vs))), 0x1p124f);
+            const int needed = __builtin_amdgcn_readfirstlane(top > 0.f ? __builtin_amdgcn_frexp_expf(top) : -126);
+            const int next = needed > unit ? needed + 1 : unit;
+            regrow = __builtin_ldexpf(1.f, unit - next);
+            unit = next;
+            // (every wavefront writes them: the same)
+            float* to_lds = reinterpret_cast<float*>(stage + K_BYTES + V_BYTES);
+            to_lds[lane] = F32 ? ks_reg : ks_reg * key_factor;
+            to_lds[KEYS + lane] = vs * __builtin_ldexpf(kProbability, -unit);
+        };
+        constexpr int V_STEPS = VP * 8;
+        Frag vf[4];
+        auto settle_v = [&](int part, char* stage) {
+            const int i = part / 8, e = part % 8;
+            const int u = tid + i * THREADS, chunk = u / (DIM / 4), d = u % (DIM / 4) * 4;
+            if (e >= 4) {
+                if (VUNITS % THREADS && u >= VUNITS) return;
+                *reinterpret_cast<h8*>(stage + v_at(d + e - 4, chunk)) = vf[e - 4].v;
+                return;
             }
-            if (wave == 0) {
-                float* to_lds = reinterpret_cast<float*>(stage + K_BYTES + V_BYTES);
-                to_lds[lane] = F32 ? ks_reg : ks_reg * key_factor, to_lds[KEYS + lane] = vs * per_unit;
+            Offsets<BITS> off;
+            if constexpr (AFFINE) {
+                // (a zero point that is no number reaches every row through the matrix product: the scale has it instead)
+                const float z0 = vz[i][e / 2][2 * (e % 2)], z1 = vz[i][e / 2][2 * (e % 2) + 1];
+                off = Offsets<BITS>(fabsf(z0) <= 2048.f ? z0 : 0.f, fabsf(z1) <= 2048.f ? z1 : 0.f);
+            }
+            const uint32_t x = vreg[i][2 * e], y = vreg[i][2 * e + 1];
+            if constexpr (BITS == 8) {
+                const uint32_t u0 = __builtin_amdgcn_perm(y, x, 0x05010400u), u1 = __builtin_amdgcn_perm(y, x, 0x07030602u);
+                vf[0].p[e] = bytes01(u0, off.of1024), vf[1].p[e] = bytes23(u0, off.of1024);
+                vf[2].p[e] = bytes01(u1, off.of1024), vf[3].p[e] = bytes23(u1, off.of1024);
+            } else {
+                const uint32_t u0 = __builtin_amdgcn_perm(y, x, 0x05040100u), u1 = u0 >> 8;
+                vf[0].p[e] = nibbles0(u0, high, off.of1024), vf[1].p[e] = nibbles4(u0, high, off.of64);
+                vf[2].p[e] = nibbles0(u1, high, off.of1024), vf[3].p[e] = nibbles4(u1, high, off.of64);
             }
         };
 
-        int key = from, pages = pages_of(from);
+        int pages = pages_of(from);
         // ---- queries: column n is row row0 + 32 wave + n
         h8 qf[SLABS][PARTS];
         float factor = key_factor;
@@ -252,7 +260,7 @@ struct ChunkKernel {
             if (from < to) {
                 locate(from, pages);
                 pages = pages_of(from + KEYS);
-                request();
+                request_k(), request_v();
             }
             const bool minus = a.scale < 0.f;
             int up = 0;
@@ -288,70 +296,96 @@ struct ChunkKernel {
             }
         }
         f32x16 o[TILES] = {};
-        float m = -__builtin_inff(), l = 0.f;
+        float m = -__builtin_inff(), l = 0.f, l1 = 0.f;
+        const unsigned span = unsigned(max(0, hi - lo));
 
-        auto work = [&](const char* stage, int ok_now, float grown, bool odd) {
-            const float* scales = reinterpret_cast<const float*>(stage + K_BYTES + V_BYTES);
-            // (neighbouring products go to different accumulators; the next fragments are read ahead of them)
-            f32x16 s[2] = {};
-            {
-                h8 k[2][2];
-                auto read = [&](int i) {
+        // 32 keys after 32 keys: while the matrix pipe has the next ones' scores the vector unit has these ones' exponentials, and while it has
+        // these ones' values, the next ones' exponents and the codes of those behind them.  One wavefront's instructions alternate: two
+        // wavefronts of a SIMD, each with one after the other, took turns at both units (8192 tokens of 16 384 2112 us).
+        f32x16 x;  // exponents: scores less the row's maximum so far
+        f32x16 s;  // the next scores
+        Frag pf[2][PARTS];
+        const auto scales_of = [&](const char* stage) { return reinterpret_cast<const float*>(stage + K_BYTES + V_BYTES); };
+        // two keys' probabilities
+        auto probabilities = [&](const char* stage, int half, int pair) {
+            const int b = pair / 2, r = pair % 2;
+            const f32x2 vs = *reinterpret_cast<const f32x2*>(scales_of(stage) + KEYS + 32 * half + 8 * b + 4 * h + 2 * r);
+            const float e0 = __builtin_amdgcn_exp2f(x[2 * pair]), e1 = __builtin_amdgcn_exp2f(x[2 * pair + 1]);
+            l += e0, l1 += e1;
+            // (0 times anything is 0: a scale that is no number shows in the rows that see its key only)
+            const float p0 = mul_legacy(e0, vs.x), p1 = mul_legacy(e1, vs.y);
+            const h2 y = to_h2(p0, p1);
+            pf[b / 2][0].p[2 * (b % 2) + r] = y;
+            if constexpr (F32) pf[b / 2][1].p[2 * (b % 2) + r] = to_h2(p0 - float(y.x), p1 - float(y.y));
+        };
+        // two keys' exponents
+        auto exponents = [&](const char* stage, int half, int pair, float mm) {
+            const f32x2 ks = *reinterpret_cast<const f32x2*>(scales_of(stage) + 32 * half + 8 * (pair / 2) + 4 * h + 2 * (pair % 2));
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) k[i & 1][t] = *reinterpret_cast<const h8*>(stage + k_at(32 * t + n, 2 * i + h));
-                };
-                read(0);
+            for (int r = 0; r < 2; ++r) x[2 * pair + r] = __builtin_fmaf(F32 ? s[2 * pair + r] * factor : s[2 * pair + r], ks[r], mm);
+        };
+        // Matrix products one by one, the next fragment read ahead of each, and behind it the vector unit's share of what is to be done
+        // meanwhile: f of the parts [n step / steps, n (step + 1) / steps) of n.  A step is kept together.
+        auto deal = [](int n, int step, int steps, auto f) {
 #pragma unroll
-                for (int i = 0; i < SLABS; ++i) {
-                    if (i + 1 < SLABS) read(i + 1);
+            for (int i = n * step / steps; i < n * (step + 1) / steps; ++i) f(i);
+        };
+        constexpr int AHEAD = F32 ? 1 : 3;  // fragments: about as long as LDS takes
+        auto scores = [&](const char* stage, int half, auto meanwhile) {
+            constexpr int STEPS = SLABS * PARTS;
+            s = f32x16{};
+            h8 k[AHEAD + 1];
+            auto read = [&](int i) { k[i % (AHEAD + 1)] = *reinterpret_cast<const h8*>(stage + k_at(32 * half + n, 2 * i + h)); };
 #pragma unroll
-                    for (int p = PARTS - 1; p >= 0; --p)
+            for (int i = 0; i < AHEAD; ++i) read(i);
 #pragma unroll
-                        for (int t = 0; t < 2; ++t) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i & 1][t], qf[i][p], s[t], 0, 0, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x008, 2 * PARTS, 0);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+            for (int x = 0; x < STEPS; ++x) {
+                const int i = x / PARTS, p = PARTS - 1 - x % PARTS;
+                if (p == PARTS - 1 && i + AHEAD < SLABS) read(i + AHEAD);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i % (AHEAD + 1)], qf[i][p], s, 0, 0, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                meanwhile(x, STEPS);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            // s becomes the exponent: the score less the row's maximum so far
-            const float mm = m == -__builtin_inff() ? 0.f : -m;
+        };
+        auto products = [&](const char* stage, int half, auto meanwhile) {
+            constexpr int STEPS = 2 * TILES * PARTS;
+            h8 v[AHEAD + 1];
+            auto read = [&](int i) { v[i % (AHEAD + 1)] = *reinterpret_cast<const h8*>(stage + v_at(32 * (i % TILES) + n, 2 * (2 * half + i / TILES) + h)); };
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int i = 0; i < AHEAD; ++i) read(i);
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const f32x4 ks = *reinterpret_cast<const f32x4*>(scales + 32 * t + 8 * b + 4 * h);
+            for (int x = 0; x < STEPS; ++x) {
+                const int i = x / PARTS, p = PARTS - 1 - x % PARTS;
+                if (p == PARTS - 1 && i + AHEAD < 2 * TILES) read(i + AHEAD);
+                o[i % TILES] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i % (AHEAD + 1)], pf[i / TILES][p].v, o[i % TILES], 0, 0, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                meanwhile(x, STEPS);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        // masks keys `at` .. `at` + 31, renews the maximum where it has grown by enough, and the outputs' unit
+        auto raise = [&](int at, int ok_at, float f) {
+            if (!(at >= all_lo && at + 32 <= all_hi && ok_at == 3)) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        s[t][4 * b + r] = __builtin_fmaf(F32 ? s[t][4 * b + r] * factor : s[t][4 * b + r], ks[r], mm);
+                for (int i = 0; i < 16; ++i) {
+                    const int j = at + 8 * (i / 4) + 4 * h + i % 4;
+                    if (!((unsigned(j - lo) < span) & (ok_at >> (i / 8) & 1))) x[i] = -__builtin_inff();
                 }
-            // keys that some rows do not see: the exponential makes them zeros
-            if (!(key >= all_lo && key + KEYS <= all_hi && ok_now == 15)) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int j = key + 32 * t + 8 * (i / 4) + 4 * h + i % 4;
-                        if (!(j >= lo && j < hi && (ok_now >> (2 * t + i / 8) & 1))) s[t][i] = -__builtin_inff();
-                    }
             }
             float top = -__builtin_inff();
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
-            top = halves(top, [](float x, float y) { return fmaxf(x, y); });
-            float f = grown;
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]);
+            top = halves(top, [](float u, float w) { return fmaxf(u, w); });
             const bool first = m == -__builtin_inff();
             if (__ballot(top > kLazy || (first && top > m))) {
                 const float by = first ? top : fmaxf(top, 0.f);  // (-inf: no key seen yet)
-                const float e = first ? 0.f : __builtin_amdgcn_exp2f(-by);
                 if (by != -__builtin_inff()) {
+                    const float e = first ? 0.f : __builtin_amdgcn_exp2f(-by);
                     m = first ? by : m + by;
-                    l *= e, f *= e;
+                    l *= e, l1 *= e, f *= e;
 #pragma unroll
-                    for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) s[t][i] -= by;
+                    for (int i = 0; i < 16; ++i) x[i] -= by;
                 }
             }
             if (__ballot(f != 1.f)) {
@@ -360,86 +394,59 @@ struct ChunkKernel {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[d][i] *= f;
             }
-            float sum = 0.f;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const f32x4 vs = *reinterpret_cast<const f32x4*>(scales + KEYS + 32 * t + 8 * b + 4 * h);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float p = __builtin_amdgcn_exp2f(s[t][4 * b + r]);
-                        sum += p;
-                        s[t][4 * b + r] = p * vs[r];
-                    }
-                }
-            l += sum;
-            // a scale that is no finite number shows in the rows that see its key, not in the others
-            if (odd) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int j = key + 32 * t + 8 * (i / 4) + 4 * h + i % 4;
-                        if (!(j >= lo && j < hi && (ok_now >> (2 * t + i / 8) & 1))) s[t][i] = 0.f;
-                    }
-            }
-            Frag pf[4][PARTS];
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const h2 x = to_h2(s[t][i], s[t][i + 1]);
-                    Frag* to_frag = pf[2 * t + i / 8];
-                    to_frag[0].p[i % 8 / 2] = x;
-                    if constexpr (F32) to_frag[1].p[i % 8 / 2] = to_h2(s[t][i] - float(x.x), s[t][i + 1] - float(x.y));
-                }
-            h8 v[4];
-            auto read = [&](int x) { v[x % 4] = *reinterpret_cast<const h8*>(stage + v_at(32 * (x % TILES) + n, 2 * (x / TILES) + h)); };
-            read(0), read(1);
-#pragma unroll
-            for (int x = 0; x < 4 * TILES; x += 2) {
-                if (x + 2 < 4 * TILES) read(x + 2), read(x + 3);
-#pragma unroll
-                for (int p = PARTS - 1; p >= 0; --p)
-#pragma unroll
-                    for (int y = x; y < x + 2; ++y)
-                        o[y % TILES] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[y % 4], pf[y / TILES][p].v, o[y % TILES], 0, 0, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-                __builtin_amdgcn_sched_group_barrier(0x008, 2 * PARTS, 0);
-                __builtin_amdgcn_sched_barrier(0);
-            }
         };
+        auto exponent_offset = [&] { return m == -__builtin_inff() ? 0.f : -m; };
 
-        float own_unit = 0.f;
         if (from < to) {
-            settle(from, lds);
+#pragma unroll
+            for (int i = 0; i < K_STEPS; ++i) settle_k(i, from, lds);
+#pragma unroll
+            for (int i = 0; i < V_STEPS; ++i) settle_v(i, lds);
+            int ok_now = ok;
+            locate(from + KEYS, pages);
+            pages = pages_of(from + 2 * KEYS);
+            request_k(), request_v();
             __syncthreads();
+            scores(lds, 0, [](int, int) {});
+#pragma unroll
+            for (int i = 0; i < 8; ++i) exponents(lds, 0, i, 0.f);
+            raise(from, ok_now & 3, regrow);
             int side = 0;
-            for (; key < to; key += KEYS) {
-                const int ok_now = ok;
-                own_unit = unit;
-                const float grown = regrow;
-                const bool odd = not_finite;
-                const bool more = key + KEYS < to;
-                if (more) {
-                    locate(key + KEYS, pages);
-                    pages = pages_of(key + 2 * KEYS);
-                    request();
-                }
-                char* stage = lds + side * STAGE;
-                work(stage, ok_now, grown, odd);
+            for (int key = from;; key += KEYS) {
+                char* const now = lds + side * STAGE;
+                char* const next = lds + (side ^ 1) * STAGE;
+                scores(now, 1, [&](int step, int steps) { deal(8, step, steps, [&](int i) { probabilities(now, 0, i); }); });
+                float mm = exponent_offset();
+                products(now, 0, [&](int step, int steps) {
+                    deal(8, step, steps, [&](int i) { exponents(now, 1, i, mm); });
+                    deal(K_STEPS, step, steps, [&](int i) { settle_k(i, key + KEYS, next); });
+                });
+                const int ok_next = ok;
+                locate(key + 2 * KEYS, pages);
+                pages = pages_of(key + 3 * KEYS);
+                request_k();
+                raise(key + 32, ok_now >> 2, 1.f);
+                __syncthreads();
+                // (behind the last keys: the scores of what lies there, which nobody takes)
+                scores(next, 0, [&](int step, int steps) { deal(8, step, steps, [&](int i) { probabilities(now, 1, i); }); });
+                mm = exponent_offset();
+                products(now, 1, [&](int step, int steps) {
+                    deal(8, step, steps, [&](int i) { exponents(next, 0, i, mm); });
+                    deal(V_STEPS, step, steps, [&](int i) { settle_v(i, next); });
+                });
+                if (key + KEYS >= to) break;
+                request_v();
+                raise(key + KEYS, ok_next & 3, regrow);
+                __syncthreads();
+                ok_now = ok_next;
                 side ^= 1;
-                if (more) {
-                    settle(key + KEYS, lds + side * STAGE);
-                    __syncthreads();
-                }
             }
+            l += l1;
         }
         l = halves(l, [](float x, float y) { return x + y; });
         const int row = row0 + 32 * wave + n;
         if (row > last_row) return;
-        const float scale = own_unit * (1.f / kProbability) * (a.parts == 1 ? (l == 0.f ? 0.f : 1.f / l) : 1.f);
+        const float scale = __builtin_ldexpf(1.f / kProbability, unit) * (a.parts == 1 ? (l == 0.f ? 0.f : 1.f / l) : 1.f);
         if (a.parts > 1) {
             float* piece = a.partial + (size_t(item) * a.kv_heads + head) * kPiece<R, DIM>;
             if (h == 0) piece[R * DIM + 32 * wave + n] = m, piece[R * DIM + R + 32 * wave + n] = l;
