@@ -56,13 +56,12 @@ struct ChunkKernel {
         const unsigned item = blockIdx.x / unsigned(a.kv_heads);
         const int head = int(blockIdx.x - item * unsigned(a.kv_heads));
         Tile it;
-        if (!find_tile<R>(a, item / unsigned(a.parts), it)) return;
-        const int part = int(item % unsigned(a.parts));
+        if (!find_tile<R>(a, item, false, it)) return;
         const int rows = it.s.chunk * group, row0 = it.tile * R, at = it.s.len - it.s.chunk;
         const int last_row = min(rows, row0 + R) - 1;
         const Keys seen = keys_of(a, it.s, int(a.group(unsigned(row0))), int(a.group(unsigned(last_row))));
-        const int base = seen.lo & ~(KEYS - 1), share = ((seen.hi - base + a.parts - 1) / a.parts + KEYS - 1) / KEYS * KEYS;
-        const int from = min(seen.hi, base + part * share), to = min(seen.hi, from + share);
+        const int base = seen.lo & ~(KEYS - 1), share = ((seen.hi - base + it.parts - 1) / it.parts + KEYS - 1) / KEYS * KEYS;
+        const int from = min(seen.hi, base + it.part * share), to = min(seen.hi, from + share);
         // this wavefront's rows, and the keys that all of them see
         const int w0 = min(row0 + 32 * wave, last_row), w1 = min(row0 + 32 * wave + 31, last_row);
         const int token0 = int(a.group(unsigned(w0))), token1 = int(a.group(unsigned(w1)));
@@ -446,8 +445,8 @@ struct ChunkKernel {
         l = halves(l, [](float x, float y) { return x + y; });
         const int row = row0 + 32 * wave + n;
         if (row > last_row) return;
-        const float scale = __builtin_ldexpf(1.f / kProbability, unit) * (a.parts == 1 ? (l == 0.f ? 0.f : 1.f / l) : 1.f);
-        if (a.parts > 1) {
+        const float scale = __builtin_ldexpf(1.f / kProbability, unit) * (it.parts == 1 ? (l == 0.f ? 0.f : 1.f / l) : 1.f);
+        if (it.parts > 1) {
             float* piece = a.partial + (size_t(item) * a.kv_heads + head) * kPiece<R, DIM>;
             if (h == 0) piece[R * DIM + 32 * wave + n] = m, piece[R * DIM + R + 32 * wave + n] = l;
 #pragma unroll
@@ -483,32 +482,32 @@ __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void attn_chunk_kernel(Att
 template <class T, int DIM, int R>
 __global__ __launch_bounds__(256) void attn_parts_kernel(AttnArgs a, T* __restrict__ out) {
     Tile it;
-    if (!find_tile<R>(a, blockIdx.x, it)) return;
-    const float* first = a.partial + (size_t(blockIdx.x) * a.parts * a.kv_heads + blockIdx.y) * kPiece<R, DIM>;
-    join_row<T, DIM, R>(a, out, it.s, it.tile, int(blockIdx.y), blockIdx.z * 4 + (threadIdx.x >> 6), a.parts,
+    if (!find_tile<R>(a, blockIdx.x, true, it) || it.parts == 1 || it.first + it.parts > a.blocks) return;
+    const float* first = a.partial + (size_t(it.first) * a.kv_heads + blockIdx.y) * kPiece<R, DIM>;
+    join_row<T, DIM, R>(a, out, it.s, it.tile, int(blockIdx.y), blockIdx.z * 4 + (threadIdx.x >> 6), it.parts,
                         [&](int i) { return first + size_t(i) * a.kv_heads * kPiece<R, DIM>; });
 }
 
 template <class T, int BITS, int DIM>
-int launch_chunk(const AttnArgs& a, const T* q, T* out, int tiles, hipStream_t st) {
+int launch_chunk(const AttnArgs& a, const T* q, T* out, int tiles, bool join, hipStream_t st) {
     auto go = [&](auto affine) {
         using K = ChunkKernel<T, BITS, decltype(affine)::value, DIM>;
         auto kernel = attn_chunk_kernel<T, BITS, decltype(affine)::value, DIM>;
         static DeviceOnce once;
         const int rc = allow_dynamic_lds(once, reinterpret_cast<const void*>(kernel), K::LDS_BYTES);
         if (rc) return rc;
-        kernel<<<unsigned(tiles) * a.parts * a.kv_heads, K::THREADS, K::LDS_BYTES, st>>>(a, q, out);
-        if (a.parts > 1) attn_parts_kernel<T, DIM, K::R><<<dim3(tiles, a.kv_heads, K::R / 4), 256, 0, st>>>(a, out);
+        kernel<<<unsigned(a.blocks) * a.kv_heads, K::THREADS, K::LDS_BYTES, st>>>(a, q, out);
+        if (join) attn_parts_kernel<T, DIM, K::R><<<dim3(tiles, a.kv_heads, K::R / 4), 256, 0, st>>>(a, out);
         return int(LQ_OK);
     };
     return a.k_zero ? go(std::true_type{}) : go(std::false_type{});
 }
 
 template <class T, int BITS>
-int launch_chunk_of(const AttnArgs& a, const T* q, T* out, int tiles, hipStream_t st) {
-    if (a.dim <= 64) return launch_chunk<T, BITS, 64>(a, q, out, tiles, st);
-    if (a.dim <= 128) return launch_chunk<T, BITS, 128>(a, q, out, tiles, st);
-    return launch_chunk<T, BITS, 256>(a, q, out, tiles, st);
+int launch_chunk_of(const AttnArgs& a, const T* q, T* out, int tiles, bool join, hipStream_t st) {
+    if (a.dim <= 64) return launch_chunk<T, BITS, 64>(a, q, out, tiles, join, st);
+    if (a.dim <= 128) return launch_chunk<T, BITS, 128>(a, q, out, tiles, join, st);
+    return launch_chunk<T, BITS, 256>(a, q, out, tiles, join, st);
 }
 
 }  // namespace attn

@@ -36,8 +36,8 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
     const int chunk = max_chunk ? std::min(max_chunk, tokens) : batch == 1 ? tokens : (tokens + batch - 1) / std::max(batch, 1);
     // Sequences of more than kFewRows rows go to attn_chunk_kernel, the others to attn_rows_kernel.  Where there can be both, and the longest
     // chunk says that there are, both are launched and each takes its own; otherwise either takes all.
-    constexpr int kFewRows = 32;
-    const bool chunks = int64_t(chunk) * group > kFewRows, few = !chunks || sequences > 1;
+    constexpr int kFewRows = 96;
+    const bool chunks = int64_t(chunk) * group > kFewRows, few = !chunks || (sequences > 1 && all_rows < int64_t(sequences) * 512);
     hipStream_t st = as_stream(stream);
     auto lock = scratch_lock(st);
     auto room = [&](size_t floats) {
@@ -50,17 +50,18 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
         constexpr int R = 128;
         const int tiles = sequences + int(all_rows / R);
         a.min_rows = few ? kFewRows + 1 : 1, a.max_rows = 0x7fffffff;
-        // Few tiles: each one's keys in parts, a block for each.
-        a.parts = int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(most / 1024, 16), 1024 / (int64_t(tiles) * c->kv_heads))));
-        LQ_REQUIRE(int64_t(tiles) * a.parts * c->kv_heads <= 0xffffff, LQ_ERR_NOT_IMPLEMENTED, "paged_attention: %d tiles of queries for %d heads",
-                   tiles, c->kv_heads);
-        if (a.parts > 1) {
-            rc = room(size_t(tiles) * a.parts * c->kv_heads * R * (dim + 2));
+        a.each = 1024, a.least = 256;
+        const bool join = most > a.least;
+        a.blocks = tiles + (join ? (a.each + c->kv_heads - 1) / c->kv_heads : 0);
+        LQ_REQUIRE(int64_t(a.blocks) * c->kv_heads <= 0xffffff, LQ_ERR_NOT_IMPLEMENTED, "paged_attention: %d tiles of queries for %d heads", tiles,
+                   c->kv_heads);
+        if (join) {
+            rc = room(size_t(a.blocks) * c->kv_heads * R * (dim + 2));
             if (rc) return rc;
         }
         auto launch = [&](auto type, auto bits) {
             using T = decltype(type);
-            rc = attn::launch_chunk_of<T, decltype(bits)::value>(a, static_cast<const T*>(q), static_cast<T*>(out), tiles, st);
+            rc = attn::launch_chunk_of<T, decltype(bits)::value>(a, static_cast<const T*>(q), static_cast<T*>(out), tiles, join, st);
         };
         by_type(dtype, c->bits, launch);
         if (rc) return rc;

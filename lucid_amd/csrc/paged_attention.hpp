@@ -35,7 +35,6 @@ struct AttnArgs {
     int each;      // of so many blocks each has a share of the units, at least `least`; 0: a segment
     int least;
     int min_rows, max_rows;  // sequences of fewer or more rows are another launch's
-    int parts;     // of a tile's keys, a block each
     float scale;
     float* partial;  // pieces of segments
 };
@@ -160,35 +159,59 @@ struct Segments {
     }
 };
 
-// Tile number `id` of R rows of the sequences of a launch; of each sequence's the last one first.  False: there is none.
+// Tiles of R rows of a launch, of each sequence's the last one first (it sees the most keys), their keys in parts, a block each: of about as many
+// keys that there are a.each parts in all, and at least a.least.
 struct Tile {
-    int seq, tile;
+    int seq, tile, part, parts;
+    int first;  // number of the tile's first part
     Sequence s;
 };
+// Part number `id`, or with `whole` tile number `id`.  False: there is none.
 template <int R>
-__device__ __forceinline__ bool find_tile(const AttnArgs& a, unsigned id, Tile& it) {
+__device__ __forceinline__ bool find_tile(const AttnArgs& a, unsigned id, bool whole, Tile& it) {
     const int lane = threadIdx.x & 63;
-    unsigned before = 0;
-    for (int first = 0; first < a.batch; first += 64) {
-        Sequence s{0, 0, 0};
-        if (first + lane < a.batch) s = sequence_of(a, first + lane);
+    Sequence s{0, 0, 0};
+    unsigned tiles = 0, extent = 0;
+    auto load = [&](int b) {
+        s = Sequence{0, 0, 0};
+        if (b < a.batch) s = sequence_of(a, b);
         const int rows = s.chunk * int(a.group.d);
-        const unsigned tiles = rows < a.min_rows || rows > a.max_rows ? 0u : unsigned(rows + R - 1) / R;
-        unsigned upto = tiles;
+        tiles = rows < a.min_rows || rows > a.max_rows ? 0u : unsigned(rows + R - 1) / R;
+        const Keys k = keys_of(a, s, 0, s.chunk - 1);
+        extent = unsigned(k.hi - (k.lo & ~63));
+    };
+    unsigned long long sum = 0;
+    for (int first = 0; first < a.batch; first += 64) {
+        load(first + lane);
+        sum += (unsigned long long)(tiles) * extent;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d, 64);
+    const unsigned long long share = (sum * unsigned(a.kv_heads) + unsigned(a.each) - 1) / unsigned(a.each);
+    const unsigned most = share < unsigned(a.least) ? unsigned(a.least) : share > 0x40000000ull ? 0x40000000u : unsigned(share);
+    unsigned before = 0, tiles_before = 0;
+    for (int first = 0; first < a.batch; first += 64) {
+        if (a.batch > 64) load(first + lane);
+        const unsigned parts = max(1u, (extent + most - 1) / most);
+        unsigned upto = tiles * parts, tiles_to = tiles;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
-            const unsigned o = __shfl_up(upto, d, 64);
-            if (lane >= d) upto += o;
+            const unsigned o = __shfl_up(upto, d, 64), p = __shfl_up(tiles_to, d, 64);
+            if (lane >= d) upto += o, tiles_to += p;
         }
-        const unsigned long long past = __ballot(upto > id - before);
+        const unsigned long long past = __ballot((whole ? tiles_before + tiles_to : before + upto) > id);
         if (past) {
             const int l = __builtin_ctzll(past);
             auto get = [&](unsigned v) { return unsigned(__builtin_amdgcn_readlane(int(v), l)); };
-            it.seq = first + l, it.tile = int(get(upto) - 1 - (id - before));
+            const unsigned n = get(tiles), p = get(parts), begin = before + get(upto) - n * p;
+            const unsigned k = whole ? id - (tiles_before + get(tiles_to) - n) : (id - begin) / p;
+            it.seq = first + l, it.tile = int(n - 1 - k), it.parts = int(p), it.part = whole ? 0 : int(id - begin - k * p);
+            it.first = int(begin + k * p);
             it.s = Sequence{int(get(unsigned(s.q0))), int(get(unsigned(s.chunk))), int(get(unsigned(s.len)))};
             return true;
         }
         before += unsigned(__builtin_amdgcn_readlane(int(upto), 63));
+        tiles_before += unsigned(__builtin_amdgcn_readlane(int(tiles_to), 63));
     }
     return false;
 }
@@ -309,7 +332,7 @@ void launch_rows_of(const AttnArgs& a, const T* q, T* out, int tiles, int qt, bo
 
 // A chunk of a sequence: tiles of 128 rows.
 template <class T, int BITS>
-int launch_chunk_of(const AttnArgs& a, const T* q, T* out, int tiles, hipStream_t st);
+int launch_chunk_of(const AttnArgs& a, const T* q, T* out, int tiles, bool join, hipStream_t st);
 
 }  // namespace attn
 }  // namespace lq
