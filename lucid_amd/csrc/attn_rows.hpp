@@ -22,6 +22,9 @@ template <class T, int BITS, bool AFFINE, int DIM, int QT>
 struct RowsKernel {
     static constexpr bool F32 = std::is_same_v<T, float>;
     static constexpr int PARTS = F32 ? 2 : 1;  // float16 parts of a float32
+    // Probabilities are two float16 for float16 results as well: one alone makes the error 1.5 times that of the result's own rounding, and
+    // the matrix pipe has the time.
+    static constexpr int P_PARTS = 2;
     static constexpr int R = 16 * QT, WAVES = 4, SLABS = DIM / 32, TILES = DIM / 16;
     static constexpr int NT = rows_keys(BITS, DIM, QT) / 16, KEYS = 16 * NT, UNIT = KEYS * WAVES;
     static constexpr int KW = DIM * BITS / 128;      // dwords of a key per lane
@@ -311,7 +314,7 @@ struct RowsKernel {
                     for (int j = 0; j < TILES; ++j) o[x][j] *= f;
                 unit = top, per_unit = kProbability / top;
             }
-            Frag pf[QT][NT / 2][PARTS];
+            Frag pf[QT][NT / 2][P_PARTS];
 #pragma unroll
             for (int x = 0; x < QT; ++x) {
                 float top = -__builtin_inff();
@@ -354,7 +357,7 @@ struct RowsKernel {
                         const float u = e[t][2 * r], w = e[t][2 * r + 1];
                         const h2 h = to_h2(u, w);
                         pf[x][t / 2][0].p[2 * (t % 2) + r] = h;
-                        if constexpr (F32) pf[x][t / 2][1].p[2 * (t % 2) + r] = to_h2(u - float(h.x), w - float(h.y));
+                        pf[x][t / 2][1].p[2 * (t % 2) + r] = to_h2(u - float(h.x), w - float(h.y));
                     }
             }
             request_scales();
@@ -390,7 +393,7 @@ struct RowsKernel {
 #pragma unroll
                         for (int x = 0; x < QT; ++x)
 #pragma unroll
-                            for (int p = PARTS - 1; p >= 0; --p)
+                            for (int p = P_PARTS - 1; p >= 0; --p)
                                 o[x][w * PER + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[j].v, pf[x][k][p].v, o[x][w * PER + j], 0, 0, 0);
                 }
             }
