@@ -21,9 +21,6 @@ namespace attn {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-// v_mul_legacy_f32: a product in which 0 times anything is 0
-__device__ float mul_legacy(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
-
 // the value of the lane 32 further on (or back) with this one's
 template <class F>
 __device__ __forceinline__ float halves(float v, F f) {
@@ -168,7 +165,7 @@ struct ChunkKernel {
         };
         // outputs are kept in units of 2^unit, see the top of paged_attention.hpp; regrow: what those so far are to be multiplied by
         int unit = -98;
-        float regrow = 1.f;
+        float unit_value = 0x1p-98f, per_unit = 0x1p105f, regrow = 1.f;
         // a negative scale changes the queries' signs, and of a scale of 0 all scores are 0, the masked ones still none.  What is left
         // goes with the keys' scales, with float32 queries, which have a factor for each row, with the scores
         const float key_factor = a.scale == 0.f ? 1.f : fabsf(a.scale * kLog2e);
@@ -198,15 +195,17 @@ struct ChunkKernel {
             float vs = vs_reg;
             if (AFFINE && !(fabsf(vzero) <= 2048.f)) vs = __builtin_nanf("");
             if (!((key + lane >= seen.lo) & (key + lane < to) & (ok >> (lane >> 4) & 1))) vs = 0.f;
-            const float top = fminf(wave_max(fmaxf(0.f, fabsf(vs))), 0x1p124f);
-            const int needed = __builtin_amdgcn_readfirstlane(top > 0.f ? __builtin_amdgcn_frexp_expf(top) : -126);
-            const int next = needed > unit ? needed + 1 : unit;
-            regrow = __builtin_ldexpf(1.f, unit - next);
-            unit = next;
+            regrow = 1.f;
+            if (__ballot(fabsf(vs) > unit_value && unit < 126)) {
+                const float top = fminf(wave_max(fmaxf(0.f, fabsf(vs))), 0x1p124f);
+                const int next = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(top)) + 1;
+                regrow = __builtin_ldexpf(1.f, unit - next);
+                unit = next, unit_value = __builtin_ldexpf(1.f, next), per_unit = __builtin_ldexpf(kProbability, -next);
+            }
             // (every wavefront writes them: the same)
             float* to_lds = reinterpret_cast<float*>(stage + K_BYTES + V_BYTES);
             to_lds[lane] = F32 ? ks_reg : ks_reg * key_factor;
-            to_lds[KEYS + lane] = vs * __builtin_ldexpf(kProbability, -unit);
+            to_lds[KEYS + lane] = vs * per_unit;
         };
         constexpr int V_STEPS = VP * 8;
         Frag vf[4];
@@ -375,9 +374,10 @@ struct ChunkKernel {
             float top = -__builtin_inff();
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]);
-            top = halves(top, [](float u, float w) { return fmaxf(u, w); });
+            // (a lane has half of the keys: only where one of the two has grown by enough do they ask each other)
             const bool first = m == -__builtin_inff();
             if (__ballot(top > kLazy || (first && top > m))) {
+                top = halves(top, [](float u, float w) { return fmaxf(u, w); });
                 const float by = first ? top : fmaxf(top, 0.f);  // (-inf: no key seen yet)
                 if (by != -__builtin_inff()) {
                     const float e = first ? 0.f : __builtin_amdgcn_exp2f(-by);

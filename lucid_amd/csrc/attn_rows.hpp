@@ -249,7 +249,8 @@ struct RowsKernel {
         if constexpr (Q_LDS) __syncthreads();
 
         f32x4 o[QT][TILES] = {};
-        float m[QT], l[QT], unit = 0.f, per_unit = 0.f;
+        float m[QT], l[QT], unit_value = 0x1p-98f, per_unit = 0x1p105f;
+        int unit = -98;
 #pragma unroll
         for (int t = 0; t < QT; ++t) m[t] = -__builtin_inff(), l[t] = 0.f;
 
@@ -288,66 +289,94 @@ struct RowsKernel {
             pages = pages_of(key + 2 * UNIT);
             request_k();
             const bool whole = key >= all_lo && key + KEYS <= min(all_hi, to) && ok_now == (1 << NT) - 1;
-            float vs[NT][4], vtop = 0.f;
+            float vs[NT][4];
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int j = key + 16 * t + 4 * g + r;
-                    vs[t][r] = vs4[t][r];
-                    // (a zero point that is no number reaches every row through the matrix product: the scale has it for those that see it)
-                    if constexpr (AFFINE)
-                        if (!whole && !(fabsf(vz[t][r]) <= 2048.f)) vs[t][r] = __builtin_nanf(""), vz[t][r] = 0.f;
-                    // (what no row sees may be anything)
-                    if (!whole && !(j >= seen.lo && j < to && (ok_now >> t & 1))) vs[t][r] = 0.f;
-                    vtop = fmaxf(vtop, fabsf(vs[t][r]));
-                }
-            // the unit of the outputs
-            vtop = rows4_max(vtop);
-            if (__builtin_amdgcn_readfirstlane(int(!(vtop <= unit) || unit == 0.f))) {
-                // the next power of two and another one, so that it is seldom renewed; powers that have a reciprocal
-                const float top = fminf(fmaxf(__uint_as_float(__float_as_uint(vtop) & 0x7f800000u), 0x1p-100f), 0x1p124f) * 4.f;
-                const float f = unit / top;
-#pragma unroll
-                for (int x = 0; x < QT; ++x)
-#pragma unroll
-                    for (int j = 0; j < TILES; ++j) o[x][j] *= f;
-                unit = top, per_unit = kProbability / top;
-            }
-            Frag pf[QT][NT / 2][P_PARTS];
-#pragma unroll
-            for (int x = 0; x < QT; ++x) {
-                float top = -__builtin_inff();
-                float e[NT][4];
+                for (int r = 0; r < 4; ++r) vs[t][r] = vs4[t][r];
+            // what no row sees may be anything; and a zero point that is no number reaches every row through the matrix product: the scale
+            // has it for those that see it
+            if (!whole) {
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        e[t][r] = sc[x][t][r] * (ks[t][r] * factor[x]);
-                        if (!whole) {
-                            const int j = key + 16 * t + 4 * g + r;
-                            if (!(j >= lo[x] && j < min(hi[x], to) && (ok_now >> t & 1))) e[t][r] = -__builtin_inff();
-                        }
-                        top = fmaxf(top, e[t][r]);
+                        const int j = key + 16 * t + 4 * g + r;
+                        if constexpr (AFFINE)
+                            if (!(fabsf(vz[t][r]) <= 2048.f)) vs[t][r] = __builtin_nanf(""), vz[t][r] = 0.f;
+                        if (!((j >= seen.lo) & (j < to) & (ok_now >> t & 1))) vs[t][r] = 0.f;
                     }
-                top = rows4_max(top);
-                if (__ballot(top > m[x] + kLazy)) {
-                    const float now = fmaxf(m[x], top), f = now == m[x] ? 1.f : __builtin_amdgcn_exp2f(m[x] - now);
-                    l[x] *= f;
+            }
+            // the unit of the outputs: a power of two, renewed to up to four times the largest scale, and seldom
+            float vtop = 0.f;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) vtop = fmaxf(vtop, fabsf(vs[t][r]));
+            if (__ballot(vtop > unit_value && unit < 126)) {
+                const int next = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(fminf(rows4_max(vtop), 0x1p124f))) + 1;
+                const float f = __builtin_ldexpf(1.f, unit - next);
+#pragma unroll
+                for (int x = 0; x < QT; ++x)
 #pragma unroll
                     for (int j = 0; j < TILES; ++j) o[x][j] *= f;
-                    m[x] = now;
+                unit = next, unit_value = __builtin_ldexpf(1.f, next), per_unit = __builtin_ldexpf(kProbability, -next);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) vs[t][r] *= per_unit;
+            Frag pf[QT][NT / 2][P_PARTS];
+#pragma unroll
+            for (int x = 0; x < QT; ++x) {
+                // exponents: scores less the row's maximum so far
+                const float mm = m[x] == -__builtin_inff() ? 0.f : -m[x];
+                float e[NT][4];
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) e[t][r] = __builtin_fmaf(sc[x][t][r], ks[t][r] * factor[x], mm);
+                if (!whole) {
+                    const int first = lo[x], count = max(0, min(hi[x], to) - first);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int j = key + 16 * t + 4 * g + r;
+                            if (!((unsigned(j - first) < unsigned(count)) & (ok_now >> t & 1))) e[t][r] = -__builtin_inff();
+                        }
                 }
-                const float mm = m[x] == -__builtin_inff() ? 0.f : m[x];
+                float top = -__builtin_inff();
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) top = fmaxf(top, e[t][r]);
+                // (a lane has a quarter of the keys: only where one of them has grown by enough do the four ask each other)
+                const bool first = m[x] == -__builtin_inff();
+                if (__ballot(top > kLazy || (first && top > m[x]))) {
+                    top = rows4_max(top);
+                    const float by = first ? top : fmaxf(top, 0.f);  // (-inf: no key seen yet)
+                    if (by != -__builtin_inff()) {
+                        const float f = first ? 0.f : __builtin_amdgcn_exp2f(-by);
+                        m[x] = first ? by : m[x] + by;
+                        l[x] *= f;
+#pragma unroll
+                        for (int j = 0; j < TILES; ++j) o[x][j] *= f;
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) e[t][r] -= by;
+                    }
+                }
                 float sum = 0.f;
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float p = __builtin_amdgcn_exp2f(e[t][r] - mm);
+                        const float p = __builtin_amdgcn_exp2f(e[t][r]);
                         sum += p;
-                        e[t][r] = p * (vs[t][r] * per_unit);
-                        if (!whole && p == 0.f) e[t][r] = 0.f;
+                        // (0 times anything is 0: a scale that is no number shows in the rows that see its key only)
+                        e[t][r] = mul_legacy(p, vs[t][r]);
                     }
                 l[x] += sum;
 #pragma unroll
@@ -407,7 +436,7 @@ struct RowsKernel {
             l[x] = rows4_sum(l[x]);
             if (g == 0) s_m[wave][16 * x + c] = m[x], s_l[wave][16 * x + c] = l[x];
         }
-        if (lane == 0) s_unit[wave] = unit * (1.f / kProbability);
+        if (lane == 0) s_unit[wave] = __builtin_ldexpf(1.f / kProbability, unit);
 #pragma unroll
         for (int x = 0; x < QT; ++x)
 #pragma unroll

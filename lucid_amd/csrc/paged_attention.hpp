@@ -50,6 +50,9 @@ constexpr float kProbability = 0x1p7f;  // probabilities are kept times this
 __device__ __forceinline__ h2 as_h2(uint32_t v) { return __builtin_bit_cast(h2, v); }
 __device__ __forceinline__ uint32_t as_u32(h2 v) { return __builtin_bit_cast(uint32_t, v); }
 
+// v_mul_legacy_f32: a product in which 0 times anything is 0
+__device__ float mul_legacy(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
+
 // f over the four lanes of one number in the four rows of 16 lanes; every lane gets it
 template <class F>
 __device__ __forceinline__ float rows4(float v, F f) {
