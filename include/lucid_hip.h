@@ -465,7 +465,7 @@ typedef struct lq_kv_cache {
 /* Quantizes the keys and values of `tokens` tokens into their slots.  k, v: LQ_F32 or LQ_F16, kv_heads * head_dim values per
  * token, tokens ldk / ldv values apart (slices of a packed qkv row are taken), rows 16-byte aligned.  A slot that is negative or
  * beyond the cache is skipped; slots of one call are distinct otherwise (of tokens that share one, codes and scale may come from
- * different ones). */
+ * different ones).  tokens * kv_heads < 2^26 here and in lq_kv_cache_read. */
 int lq_kv_cache_write(const lq_kv_cache* cache, const void* k, const void* v, int dtype, size_t ldk, size_t ldv, const int32_t* slots,
                       size_t tokens, lq_stream stream);
 /* The rows of `tokens` slots as LQ_F32 or LQ_F16 [tokens, kv_heads, head_dim]: (code - zero) * scale in float32, float16 rounded
@@ -479,7 +479,8 @@ int lq_kv_cache_read(const lq_kv_cache* cache, const int32_t* slots, size_t toke
  *     out = sum_j softmax_j(scale * q . k_j) v_j
  * Queries that see no key, and rows of no sequence, give zeros.  Keys of a page that is negative or beyond the cache are not
  * seen; lengths beyond the table are cut to it.  Scores, sums and products are float32: codes enter the matrix products as the
- * whole numbers they are, scales after them; float16 queries and probabilities as one float16, float32 ones as two, of 22 bits together.  max_chunk: the
+ * whole numbers they are, scales after them; float16 queries as they are, float32 ones as two float16 of 22 bits together; probabilities as
+ * two as well, of a float16 result's long chunks as one (half a step 2^-11, as the result's own rounding).  max_chunk: the
  * most queries of a sequence, or 0; the work is divided by it, and results differ by rounding alone. */
 int lq_paged_attention(const lq_kv_cache* cache, const void* q, size_t ldq, void* out, int dtype, int tokens, int heads, int batch,
                        const int32_t* page_table, int table_width, const int32_t* q_starts, const int32_t* kv_lens, float scale, int causal,
