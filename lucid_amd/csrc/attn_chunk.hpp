@@ -47,7 +47,7 @@ struct ChunkKernel {
         const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, n = lane & 31;
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int group = int(a.group.d);
-        clear_other_rows(a, out, blockIdx.x, gridDim.x);
+        clear_other_rows(a, out, a.q_starts[0], a.q_starts[a.batch], blockIdx.x, gridDim.x);
         // heads vary fastest: blocks are dealt to the 8 XCDs in turn, and those of one head find its keys in the same L2.  Of a
         // sequence's tiles the last ones, which see the most keys, come first.
         const unsigned item = blockIdx.x / unsigned(a.kv_heads);

@@ -48,7 +48,7 @@ struct RowsKernel {
     using Segs = Segments<R, UNIT>;
 
     static __device__ __forceinline__ void run(const AttnArgs& a, const T* __restrict__ q, T* __restrict__ out, float* lds) {
-        clear_other_rows(a, out, blockIdx.x, gridDim.x);
+        const int first_row = a.q_starts[0], end_row = a.q_starts[a.batch];
         unsigned x = 0, end = 0, per_head = 0;
         while (true) {
             typename Segs::Segment seg;
@@ -56,6 +56,7 @@ struct RowsKernel {
             {  // (found anew for each segment: kept, what it takes would cost the registers of a wavefront)
                 Segs segs(a);
                 if (per_head == 0) {
+                    clear_other_rows(a, out, first_row, end_row, blockIdx.x, gridDim.x);
                     per_head = segs.total;
                     const unsigned all = per_head * unsigned(a.kv_heads), share = a.each ? segs.share() : 1u;
                     if (all == 0 || blockIdx.x > (all - 1) / share) return;
@@ -441,6 +442,7 @@ struct RowsKernel {
         for (int x = 0; x < QT; ++x)
 #pragma unroll
             for (int part = 0; part < 16 / ROWS; ++part) {
+                if (x + part && row0 + 16 * x + part * ROWS > last_row) break;
                 if (Q_LDS || x + part) __syncthreads();  // (whoever reads what lies there is done)
                 if (c / ROWS == part) {
 #pragma unroll
@@ -497,12 +499,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, T* __restric
     Sequence s{0, 0, 0};
     for (unsigned before = 0;; segs.first += 64, segs.load()) {
         if (segs.first >= a.batch) return;
-        unsigned upto = segs.tiles;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const unsigned o = __shfl_up(upto, d, 64);
-            if (segs.lane >= d) upto += o;
-        }
+        const unsigned upto = sum_upto(segs.tiles);
         const unsigned long long past = __ballot(upto > unsigned(tile));
         if (past) {
             const int l = __builtin_ctzll(past);

@@ -53,6 +53,17 @@ __device__ __forceinline__ uint32_t as_u32(h2 v) { return __builtin_bit_cast(uin
 // v_mul_legacy_f32: a product in which 0 times anything is 0
 __device__ float mul_legacy(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
 
+// The sum over the lanes up to this one, within 16 of them and then across, by the operand's own lane patterns: six of them cost what
+// one exchange through shared memory's network does, and this stands in every block's way to its first load.
+template <int PATTERN, int ROWS = 0xf>
+__device__ __forceinline__ unsigned add_lanes(unsigned v) {
+    return v + unsigned(__builtin_amdgcn_update_dpp(0, int(v), PATTERN, ROWS, 0xf, false));
+}
+__device__ __forceinline__ unsigned sum_upto(unsigned v) {
+    v = add_lanes<0x111>(v), v = add_lanes<0x112>(v), v = add_lanes<0x114>(v), v = add_lanes<0x118>(v);  // 1, 2, 4, 8 lanes before
+    return add_lanes<0x143, 0xc>(add_lanes<0x142, 0xa>(v));  // the last lane of the row of 16, of the half
+}
+
 // f over the four lanes of one number in the four rows of 16 lanes; every lane gets it
 template <class F>
 __device__ __forceinline__ float rows4(float v, F f) {
@@ -124,12 +135,7 @@ struct Segments {
             const Keys k = keys_of(a, s, 0, s.chunk - 1);
             units = a.each ? max(1u, unsigned(k.hi - (k.lo & ~31) + UNIT - 1) / UNIT) : 1u;
         }
-        upto = tiles * units;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const unsigned o = __shfl_up(upto, d, 64);
-            if (lane >= d) upto += o;
-        }
+        upto = sum_upto(tiles * units);
     }
     struct Segment {
         int seq, tile;
@@ -147,7 +153,7 @@ struct Segments {
                 Segment g;
                 g.seq = first + l, g.units = get(units);
                 const unsigned k = x - before - (get(upto) - get(tiles) * g.units);
-                g.tile = int(k / g.units), g.unit = k - unsigned(g.tile) * g.units;
+                g.tile = int(g.units == 1 ? k : k / g.units), g.unit = k - unsigned(g.tile) * g.units;
                 g.s = Sequence{int(get(unsigned(s.q0))), int(get(unsigned(s.chunk))), int(get(unsigned(s.len)))};
                 return g;
             }
@@ -196,12 +202,7 @@ __device__ __forceinline__ bool find_tile(const AttnArgs& a, unsigned id, bool w
     for (int first = 0; first < a.batch; first += 64) {
         if (a.batch > 64) load(first + lane);
         const unsigned parts = max(1u, (extent + most - 1) / most);
-        unsigned upto = tiles * parts, tiles_to = tiles;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const unsigned o = __shfl_up(upto, d, 64), p = __shfl_up(tiles_to, d, 64);
-            if (lane >= d) upto += o, tiles_to += p;
-        }
+        const unsigned upto = sum_upto(tiles * parts), tiles_to = sum_upto(tiles);
         const unsigned long long past = __ballot((whole ? tiles_before + tiles_to : before + upto) > id);
         if (past) {
             const int l = __builtin_ctzll(past);
@@ -231,6 +232,20 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, T* out, const Sequen
     const int lane = threadIdx.x & 63, d = lane % QUADS * 4, mine = lane / QUADS;
     const int group = int(a.group.d);
     if (r >= s.chunk * group - tile * R) return;
+    // eight pieces of a lane at a time, the first while the maximum is looked for (64 pieces of 16 rows: FIXME us, four and after it 8.6)
+    constexpr int DEEP = 8;
+    f32x4 y[DEEP];
+    float m[DEEP], l[DEEP];
+    auto request = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < DEEP; ++u) {
+            if (u == DEEP / 2 && i0 + u * EVERY >= parts) break;
+            const float* p = piece(min(i0 + u * EVERY + mine, parts - 1));
+            y[u] = *reinterpret_cast<const f32x4*>(p + r * DIM + d);
+            m[u] = p[R * DIM + r], l[u] = p[R * DIM + R + r];
+        }
+    };
+    request(0);
     float top = -__builtin_inff();
     for (int i = lane; i < parts; i += 64) top = fmaxf(top, piece(i)[R * DIM + r]);
 #pragma unroll
@@ -238,21 +253,16 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, T* out, const Sequen
     const float mm = top == -__builtin_inff() ? 0.f : top;
     float total = 0.f;
     f32x4 v = {0, 0, 0, 0};
-    for (int i0 = 0; i0 < parts; i0 += 4 * EVERY) {
-        f32x4 y[4];
-        float m[4], l[4];
+    for (int i0 = 0;;) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const float* p = piece(min(i0 + u * EVERY + mine, parts - 1));
-            y[u] = *reinterpret_cast<const f32x4*>(p + r * DIM + d);
-            m[u] = p[R * DIM + r], l[u] = p[R * DIM + R + r];
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < DEEP; ++u) {
             if (i0 + u * EVERY + mine >= parts) continue;
             const float f = __builtin_amdgcn_exp2f(m[u] - mm);
             total += l[u] * f, v += y[u] * f;
         }
+        i0 += DEEP * EVERY;
+        if (i0 >= parts) break;
+        request(i0);
     }
 #pragma unroll
     for (int e = QUADS; e < 64; e *= 2) {
@@ -268,10 +278,10 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, T* out, const Sequen
     else *reinterpret_cast<uint2*>(dst) = uint2{as_u32(to_h2(v[0], v[1])), as_u32(to_h2(v[2], v[3]))};
 }
 
-// Zeros for the rows of q that belong to no sequence, dealt to the blocks.
+// Zeros for the rows of q that belong to no sequence, those before row `first` and from row `end`, dealt to the blocks.
 template <class T>
-__device__ __forceinline__ void clear_other_rows(const AttnArgs& a, T* out, unsigned block, unsigned blocks) {
-    const int before = max(0, min(a.q_starts[0], a.tokens)), after = max(before, min(a.q_starts[a.batch], a.tokens));
+__device__ __forceinline__ void clear_other_rows(const AttnArgs& a, T* out, int first, int end, unsigned block, unsigned blocks) {
+    const int before = max(0, min(first, a.tokens)), after = max(before, min(end, a.tokens));
     const int rows = before + a.tokens - after;
     const size_t width = size_t(a.heads) * a.dim * sizeof(T) / 16;
     for (unsigned i = block; i < unsigned(rows); i += blocks) {
