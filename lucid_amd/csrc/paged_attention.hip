@@ -29,7 +29,7 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
     a.page_size = FastDiv(unsigned(c->page_size)), a.group = FastDiv(unsigned(heads / c->kv_heads));
     a.pages = c->num_pages, a.kv_heads = c->kv_heads, a.dim = c->head_dim;
     a.tokens = tokens, a.heads = heads, a.batch = batch, a.width = table_width, a.causal = causal != 0, a.window = window, a.scale = scale;
-    const int group = heads / c->kv_heads, sequences = std::min(batch, tokens);
+    const int group = heads / c->kv_heads, sequences = std::max(1, std::min(batch, tokens));  // (of no sequence: the rows' zeros)
     const int64_t all_rows = int64_t(tokens) * group, most = int64_t(table_width) * c->page_size;  // keys of a sequence
     const int dim = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
     // The longest chunk, or a guess at it: a single sequence has all tokens; equally many each otherwise.
@@ -50,7 +50,7 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
         constexpr int R = 128;
         const int tiles = sequences + int(all_rows / R);
         a.min_rows = few ? kFewRows + 1 : 1, a.max_rows = 0x7fffffff;
-        a.each = 1024, a.least = 256;
+        a.each = getenv("LQ_T") ? atoi(getenv("LQ_T")) : 1024, a.least = 256;
         const bool join = most > a.least;
         a.blocks = tiles + (join ? (a.each + c->kv_heads - 1) / c->kv_heads : 0);
         LQ_REQUIRE(int64_t(a.blocks) * c->kv_heads <= 0xffffff, LQ_ERR_NOT_IMPLEMENTED, "paged_attention: %d tiles of queries for %d heads", tiles,

@@ -142,6 +142,15 @@ def test_rows_of_no_sequence_are_zeros_whatever_the_memory_held(chunks, lengths)
     assert not none.numpy().any()
 
 
+@pytest.mark.parametrize("tokens,width,max_chunk", [(1, 4, None), (3, 4, 1), (3, 100, None), (60, 4, 60), (200, 100, 200), (700, 0, None)])
+def test_a_batch_of_no_sequences_gives_zeros(tokens, width, max_chunk):
+    b = Batch([1], [20], 4, 2, 64, seed=4)
+    out = hip(np.full((tokens, 4, 64), np.nan, np.float16))
+    F.paged_attention(hip(np.ones((tokens, 4, 64), np.float16)), b.cache, L.Tensor.empty((0, width), L.int32), ids([0]),
+                      L.Tensor.empty((0,), L.int32), max_chunk=max_chunk, out=out)
+    assert not out.numpy().any()
+
+
 @pytest.mark.parametrize("chunks,lengths", [([1, 1], [500, 100]), ([6, 3], [400, 90]), ([130, 70], [600, 200])])
 def test_what_nobody_sees_may_be_anything(chunks, lengths):
     """NaN scales behind the lengths, before the window and in pages of others; pages that are not there."""
