@@ -1,8 +1,10 @@
 // Attention of many rows (a chunk of a prompt) over paged quantized keys and values.
 //
-// Bound by the matrix pipe and, more, by what the vector unit does for each score (a scale, a maximum, an exponential, a sum, a scale, a
-// rounding: some ten instructions per four cycles of a matrix product) and for each code.  So a code is turned into float16 once for a
-// block's 128 rows, on its way into LDS, and a wavefront has 32 rows, whose accumulators, maxima and sums stay in its registers:
+// Bound by the vector unit, by what it does for each score (an exponent, a maximum, an exponential, a sum, a scale, a rounding: some ten issue
+// slots beside four cycles of a matrix product) and for each code, and then by the matrix pipe: of 8192 tokens of 16 384 (32 heads
+// of 128 on 8, float16, 8 bits, 1949 us: 0.85 PFLOP/s of the 1.16 that a large library product reaches) the one is busy 57 % of
+// the time, the other 33 %.  So a code is turned into float16 once for a block's 128 or 256 rows, on its way into LDS, and a wavefront has 32 rows, whose
+// accumulators, maxima and sums stay in its registers:
 //
 //   S^T = K Q^T    v_mfma_f32_32x32x16_f16, A: K from LDS, lane (h, n) key n of 32, columns 8h..8h+7 of 16; B: Q in registers.
 //   O^T = V^T P^T  lane (h, n) has row n's probabilities of keys 4h..4h+3 and 8+4h..8+4h+3 of 16: B as they are.  A: V^T from LDS, where
@@ -28,11 +30,11 @@ __device__ __forceinline__ float halves(float v, F f) {
     return f(__uint_as_float(x[0]), __uint_as_float(x[1]));
 }
 
-template <class T, int BITS, bool AFFINE, int DIM>
+template <class T, int BITS, bool AFFINE, int DIM, int WAVES>
 struct ChunkKernel {
     static constexpr bool F32 = std::is_same_v<T, float>;
     static constexpr int PARTS = F32 ? 2 : 1;
-    static constexpr int WAVES = 4, THREADS = 64 * WAVES, R = 32 * WAVES, KEYS = 64;
+    static constexpr int THREADS = 64 * WAVES, R = 32 * WAVES, KEYS = 64;
     static constexpr int SLABS = DIM / 16, TILES = DIM / 32;
     static constexpr int PIECES = DIM * BITS / 128;                                 // 16-byte pieces of a key's codes
     static constexpr int KP = (KEYS * PIECES + THREADS - 1) / THREADS;               // of a thread
@@ -298,8 +300,9 @@ struct ChunkKernel {
         const unsigned span = unsigned(max(0, hi - lo));
 
         // 32 keys after 32 keys: while the matrix pipe has the next ones' scores the vector unit has these ones' exponentials, and while it has
-        // these ones' values, the next ones' exponents and the codes of those behind them.  One wavefront's instructions alternate: two
-        // wavefronts of a SIMD, each with one after the other, took turns at both units (8192 tokens of 16 384 2112 us).
+        // these ones' values, the next ones' exponents and the codes of those behind them.  One wavefront's instructions alternate: with
+        // float32 rows, three wavefronts' worth of products in one, 83 -> 70 us (3 x 333 of 2048); float16 ones, of which a SIMD's two wavefronts
+        // filled each other's gaps, within 1 %.
         f32x16 x;  // exponents: scores less the row's maximum so far
         f32x16 s;  // the next scores
         Frag pf[2][PARTS];
@@ -472,42 +475,45 @@ struct ChunkKernel {
     }
 };
 
-template <class T, int BITS, bool AFFINE, int DIM>
-__global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void attn_chunk_kernel(AttnArgs a, const T* __restrict__ q, T* __restrict__ out) {
+template <class T, int BITS, bool AFFINE, int DIM, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, DIM <= 128 ? 2 : 1) void attn_chunk_kernel(AttnArgs a, const T* __restrict__ q, T* __restrict__ out) {
     extern __shared__ __attribute__((aligned(16))) char chunk_lds[];
-    ChunkKernel<T, BITS, AFFINE, DIM>::run(a, q, out, chunk_lds);
+    ChunkKernel<T, BITS, AFFINE, DIM, WAVES>::run(a, q, out, chunk_lds);
 }
 
-// Joins the parts of a tile's keys.
+// Joins the parts of a tile's keys, kJoined rows a block.
+constexpr int kJoined = 16;
 template <class T, int DIM, int R>
 __global__ __launch_bounds__(256) void attn_parts_kernel(AttnArgs a, T* __restrict__ out) {
     Tile it;
     if (!find_tile<R>(a, blockIdx.x, true, it) || it.parts == 1 || it.first + it.parts > a.blocks) return;
     const float* first = a.partial + (size_t(it.first) * a.kv_heads + blockIdx.y) * kPiece<R, DIM>;
-    join_row<T, DIM, R>(a, out, it.s, it.tile, int(blockIdx.y), blockIdx.z * 4 + (threadIdx.x >> 6), it.parts,
-                        [&](int i) { return first + size_t(i) * a.kv_heads * kPiece<R, DIM>; });
+    // (several rows a wavefront: what finding the tile takes is worth more than one)
+    for (int r = blockIdx.z * kJoined + (threadIdx.x >> 6); r < int(blockIdx.z + 1) * kJoined; r += 4)
+        join_row<T, DIM, R>(a, out, it.s, it.tile, int(blockIdx.y), r, it.parts,
+                            [&](int i) { return first + size_t(i) * a.kv_heads * kPiece<R, DIM>; });
 }
 
-template <class T, int BITS, int DIM>
+template <class T, int BITS, int DIM, int WAVES>
 int launch_chunk(const AttnArgs& a, const T* q, T* out, int tiles, bool join, hipStream_t st) {
     auto go = [&](auto affine) {
-        using K = ChunkKernel<T, BITS, decltype(affine)::value, DIM>;
-        auto kernel = attn_chunk_kernel<T, BITS, decltype(affine)::value, DIM>;
+        using K = ChunkKernel<T, BITS, decltype(affine)::value, DIM, WAVES>;
+        auto kernel = attn_chunk_kernel<T, BITS, decltype(affine)::value, DIM, WAVES>;
         static DeviceOnce once;
         const int rc = allow_dynamic_lds(once, reinterpret_cast<const void*>(kernel), K::LDS_BYTES);
         if (rc) return rc;
         kernel<<<unsigned(a.blocks) * a.kv_heads, K::THREADS, K::LDS_BYTES, st>>>(a, q, out);
-        if (join) attn_parts_kernel<T, DIM, K::R><<<dim3(tiles, a.kv_heads, K::R / 4), 256, 0, st>>>(a, out);
+        if (join) attn_parts_kernel<T, DIM, K::R><<<dim3(tiles, a.kv_heads, K::R / kJoined), 256, 0, st>>>(a, out);
         return int(LQ_OK);
     };
     return a.k_zero ? go(std::true_type{}) : go(std::false_type{});
 }
 
 template <class T, int BITS>
-int launch_chunk_of(const AttnArgs& a, const T* q, T* out, int tiles, bool join, hipStream_t st) {
-    if (a.dim <= 64) return launch_chunk<T, BITS, 64>(a, q, out, tiles, join, st);
-    if (a.dim <= 128) return launch_chunk<T, BITS, 128>(a, q, out, tiles, join, st);
-    return launch_chunk<T, BITS, 256>(a, q, out, tiles, join, st);
+int launch_chunk_of(const AttnArgs& a, const T* q, T* out, bool wide, int tiles, bool join, hipStream_t st) {
+    if (a.dim <= 64) return launch_chunk<T, BITS, 64, 4>(a, q, out, tiles, join, st);
+    if (a.dim > 128) return launch_chunk<T, BITS, 256, 4>(a, q, out, tiles, join, st);
+    return wide ? launch_chunk<T, BITS, 128, 8>(a, q, out, tiles, join, st) : launch_chunk<T, BITS, 128, 4>(a, q, out, tiles, join, st);
 }
 
 }  // namespace attn

@@ -510,8 +510,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, T* __restric
             s = Sequence{int(get(unsigned(segs.s.q0))), int(get(unsigned(segs.s.chunk))), int(get(unsigned(segs.s.len)))};
             break;
         }
-        tile -= int(unsigned(__builtin_amdgcn_readlane(int(upto), 63)));
-        before += unsigned(__builtin_amdgcn_readlane(int(segs.upto), 63));
+        tile -= int(of_last(upto));
+        before += of_last(segs.upto);
     }
     x += head * segs.total;
     const unsigned b0 = x / share, b1 = (x + units - 1) / share;

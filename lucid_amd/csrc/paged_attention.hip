@@ -47,12 +47,22 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
         return rc;
     };
     if (chunks) {
-        constexpr int R = 128;
+        // Tiles of 128 rows, two blocks a CU, one of which has the CU to itself when the other has ended; or of 256, one block a CU, in
+        // which a code is turned into float16 for twice as many rows.  The latter where blocks are alike and fill the places: one
+        // sequence of 1024 rows or more, in two rounds of blocks or more or behind three times as many keys.  us, 128 / 256 rows, 32 heads of 128 on
+        // 8, float16: 8192 tokens of 16 384 2070 / 1949, 8192 of 8192 742 / 701, 1000 of 16 000 362 / 334, 2048 of 8192 331 / 327; but 2048 of 4096
+        // 164 / 172, 1000 of 1000 52.5 / 55.9, and of four sequences of 1934 to 8192 keys 274 / 311 (of four of 8192 372 / 342: their lengths are
+        // on the device).
+        const int64_t rows = int64_t(chunk) * group;
+        const bool wide = dim == 128 && batch == 1 && rows >= 1024 && (rows * c->kv_heads >= 512 * 256 || most >= 4 * int64_t(chunk));
+        const int R = wide ? 256 : 128;
         const int tiles = sequences + int(all_rows / R);
         a.min_rows = few ? kFewRows + 1 : 1, a.max_rows = 0x7fffffff;
-        a.each = getenv("LQ_T") ? atoi(getenv("LQ_T")) : 1024, a.least = 256;
-        const bool join = most > a.least;
-        a.blocks = tiles + (join ? (a.each + c->kv_heads - 1) / c->kv_heads : 0);
+        a.each = (dim > 128 || wide ? 1 : 2) * 256, a.least = 384;
+        // (four rounds of blocks of one sequence are left whole: joining none of 129 tiles of 8 heads takes 25 us)
+        const bool join = most > a.least && !(batch == 1 && rows * c->kv_heads >= int64_t(4) * a.each * R);
+        if (!join) a.least = 0x40000000;
+        a.blocks = tiles + (join ? (2 * a.each + c->kv_heads - 1) / c->kv_heads : 0);
         LQ_REQUIRE(int64_t(a.blocks) * c->kv_heads <= 0xffffff, LQ_ERR_NOT_IMPLEMENTED, "paged_attention: %d tiles of queries for %d heads", tiles,
                    c->kv_heads);
         if (join) {
@@ -61,7 +71,7 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
         }
         auto launch = [&](auto type, auto bits) {
             using T = decltype(type);
-            rc = attn::launch_chunk_of<T, decltype(bits)::value>(a, static_cast<const T*>(q), static_cast<T*>(out), tiles, join, st);
+            rc = attn::launch_chunk_of<T, decltype(bits)::value>(a, static_cast<const T*>(q), static_cast<T*>(out), wide, tiles, join, st);
         };
         by_type(dtype, c->bits, launch);
         if (rc) return rc;

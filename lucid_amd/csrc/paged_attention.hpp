@@ -15,6 +15,7 @@
 // far: 2^7 v_scale / unit times a probability of at most 2^8 fits float16, and outputs are kept in units of unit / 2^7.
 #pragma once
 #include "kv_cache.hpp"
+#include "wave_reduce.hpp"
 
 namespace lq {
 
@@ -55,14 +56,18 @@ __device__ float mul_legacy(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
 
 // The sum over the lanes up to this one, within 16 of them and then across, by the operand's own lane patterns: six of them cost what
 // one exchange through shared memory's network does, and this stands in every block's way to its first load.
-template <int PATTERN, int ROWS = 0xf>
-__device__ __forceinline__ unsigned add_lanes(unsigned v) {
-    return v + unsigned(__builtin_amdgcn_update_dpp(0, int(v), PATTERN, ROWS, 0xf, false));
+template <int PATTERN, int ROWS = 0xf, class N>
+__device__ __forceinline__ N add_lanes(N v) {
+    return v + __builtin_bit_cast(N, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), PATTERN, ROWS, 0xf, false));
 }
-__device__ __forceinline__ unsigned sum_upto(unsigned v) {
+template <class N>
+__device__ __forceinline__ N sum_upto(N v) {
     v = add_lanes<0x111>(v), v = add_lanes<0x112>(v), v = add_lanes<0x114>(v), v = add_lanes<0x118>(v);  // 1, 2, 4, 8 lanes before
     return add_lanes<0x143, 0xc>(add_lanes<0x142, 0xa>(v));  // the last lane of the row of 16, of the half
 }
+// the last lane's number
+template <class N>
+__device__ __forceinline__ N of_last(N v) { return __builtin_bit_cast(N, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63)); }
 
 // f over the four lanes of one number in the four rows of 16 lanes; every lane gets it
 template <class F>
@@ -120,7 +125,7 @@ struct Segments {
     __device__ __forceinline__ explicit Segments(const AttnArgs& args) : a(args), lane(threadIdx.x & 63), total(0) {
         for (first = 0; first < a.batch; first += 64) {
             load();
-            total += unsigned(__builtin_amdgcn_readlane(int(upto), 63));
+            total += of_last(upto);
         }
         if (a.batch > 64) first = 0, load();
         first = 0, before = 0;
@@ -157,7 +162,7 @@ struct Segments {
                 g.s = Sequence{int(get(unsigned(s.q0))), int(get(unsigned(s.chunk))), int(get(unsigned(s.len)))};
                 return g;
             }
-            before += unsigned(__builtin_amdgcn_readlane(int(upto), 63));
+            before += of_last(upto);
             first += 64;
             load();
         }
@@ -168,13 +173,36 @@ struct Segments {
     }
 };
 
-// Tiles of R rows of a launch, of each sequence's the last one first (it sees the most keys), their keys in parts, a block each: of about as many
-// keys that there are a.each parts in all, and at least a.least.
+// Tiles of R rows of a launch, of each sequence's the last one first (it sees the most keys), their keys in parts, a block each.
 struct Tile {
     int seq, tile, part, parts;
     int first;  // number of the tile's first part
     Sequence s;
 };
+// Parts of `extent` keys where none shall have more than `most`, or hardly more: whoever counts them counts alike, and up to `most` it is 1.
+__device__ __forceinline__ unsigned parts_of(unsigned extent, unsigned most) {
+    return max(1u, unsigned(__builtin_ceilf(float(extent) * __builtin_amdgcn_rcpf(float(most)) * (1.f - 0x1p-20f))));
+}
+// The most keys of a part: so many that there are about twice as many parts of all tiles as places for blocks (a.each), where lengths differ
+// the blocks that end early then take another.  Up to 64 sequences of about the same length (one a lane; 0 tiles: not this launch's)
+// have equal parts, which come in whole rounds: a lane each tries the longest in 1, 2, 3, ... parts, and the shortest sum of the rounds'
+// lengths counts, in keys, of which a block costs kBlock besides its own and one whose part is joined kPart more.
+constexpr float kBlock = 128.f, kPart = 320.f, kAlike = 0.8f;
+__device__ __forceinline__ unsigned part_keys(const AttnArgs& a, float keys, unsigned tiles, unsigned extent, int lane) {
+    const float heads = float(a.kv_heads), places = float(a.each);
+    const unsigned share = max(unsigned(a.least), unsigned(fminf(keys * heads / (2.f * places), 0x1p30f)) + 1u);
+    const unsigned longest = unsigned(wave_max(tiles ? float(extent) : 0.f)), all = of_last(sum_upto(tiles));
+    if (a.batch > 64 || keys < kAlike * float(all) * float(longest)) return share;
+    const int in = lane < 32 ? lane + 1 : 16 * (lane - 30);
+    const unsigned most = max(unsigned(a.least), (longest / unsigned(in) + 64u) & ~63u);
+    unsigned n = 0;
+    for (int i = 0; i < a.batch; ++i)
+        n += unsigned(__builtin_amdgcn_readlane(int(tiles), i)) * parts_of(unsigned(__builtin_amdgcn_readlane(int(extent), i)), most);
+    const float rounds = __builtin_ceilf(float(n) * heads / places) * (float(most) + kBlock + (n > all ? kPart : 0.f));
+    const float cost = n > unsigned(a.blocks) ? __builtin_inff() : rounds;
+    const unsigned long long best = __ballot(cost == wave_min(cost));
+    return unsigned(__builtin_amdgcn_readlane(int(most), __builtin_ctzll(best)));
+}
 // Part number `id`, or with `whole` tile number `id`.  False: there is none.
 template <int R>
 __device__ __forceinline__ bool find_tile(const AttnArgs& a, unsigned id, bool whole, Tile& it) {
@@ -189,19 +217,17 @@ __device__ __forceinline__ bool find_tile(const AttnArgs& a, unsigned id, bool w
         const Keys k = keys_of(a, s, 0, s.chunk - 1);
         extent = unsigned(k.hi - (k.lo & ~63));
     };
-    unsigned long long sum = 0;
+    float keys = 0.f;
     for (int first = 0; first < a.batch; first += 64) {
         load(first + lane);
-        sum += (unsigned long long)(tiles) * extent;
+        keys += float(tiles) * float(extent);
     }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d, 64);
-    const unsigned long long share = (sum * unsigned(a.kv_heads) + unsigned(a.each) - 1) / unsigned(a.each);
-    const unsigned most = share < unsigned(a.least) ? unsigned(a.least) : share > 0x40000000ull ? 0x40000000u : unsigned(share);
+    keys = of_last(sum_upto(keys));
+    const unsigned most = part_keys(a, keys, tiles, extent, lane);
     unsigned before = 0, tiles_before = 0;
     for (int first = 0; first < a.batch; first += 64) {
         if (a.batch > 64) load(first + lane);
-        const unsigned parts = max(1u, (extent + most - 1) / most);
+        const unsigned parts = parts_of(extent, most);
         const unsigned upto = sum_upto(tiles * parts), tiles_to = sum_upto(tiles);
         const unsigned long long past = __ballot((whole ? tiles_before + tiles_to : before + upto) > id);
         if (past) {
@@ -214,8 +240,8 @@ __device__ __forceinline__ bool find_tile(const AttnArgs& a, unsigned id, bool w
             it.s = Sequence{int(get(unsigned(s.q0))), int(get(unsigned(s.chunk))), int(get(unsigned(s.len)))};
             return true;
         }
-        before += unsigned(__builtin_amdgcn_readlane(int(upto), 63));
-        tiles_before += unsigned(__builtin_amdgcn_readlane(int(tiles_to), 63));
+        before += of_last(upto);
+        tiles_before += of_last(tiles_to);
     }
     return false;
 }
@@ -232,7 +258,7 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, T* out, const Sequen
     const int lane = threadIdx.x & 63, d = lane % QUADS * 4, mine = lane / QUADS;
     const int group = int(a.group.d);
     if (r >= s.chunk * group - tile * R) return;
-    // eight pieces of a lane at a time, the first while the maximum is looked for (64 pieces of 16 rows: FIXME us, four and after it 8.6)
+    // eight pieces of a lane at a time, the first while the maximum is looked for (64 pieces of 16 rows: 6.1 us, four and after it 8.6)
     constexpr int DEEP = 8;
     f32x4 y[DEEP];
     float m[DEEP], l[DEEP];
@@ -248,8 +274,7 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, T* out, const Sequen
     request(0);
     float top = -__builtin_inff();
     for (int i = lane; i < parts; i += 64) top = fmaxf(top, piece(i)[R * DIM + r]);
-#pragma unroll
-    for (int e = 1; e < 64; e *= 2) top = fmaxf(top, __shfl_xor(top, e, 64));
+    top = wave_max(top);
     const float mm = top == -__builtin_inff() ? 0.f : top;
     float total = 0.f;
     f32x4 v = {0, 0, 0, 0};
@@ -345,7 +370,7 @@ void launch_rows_of(const AttnArgs& a, const T* q, T* out, int tiles, int qt, bo
 
 // A chunk of a sequence: tiles of 128 rows.
 template <class T, int BITS>
-int launch_chunk_of(const AttnArgs& a, const T* q, T* out, int tiles, bool join, hipStream_t st);
+int launch_chunk_of(const AttnArgs& a, const T* q, T* out, bool wide, int tiles, bool join, hipStream_t st);
 
 }  // namespace attn
 }  // namespace lq
