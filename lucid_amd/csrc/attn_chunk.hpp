@@ -2,8 +2,8 @@
 //
 // Bound by the vector unit, by what it does for each score (an exponent, a maximum, an exponential, a sum, a scale, a rounding: some ten issue
 // slots beside four cycles of a matrix product) and for each code, and then by the matrix pipe: of 8192 tokens of 16 384 (32 heads
-// of 128 on 8, float16, 8 bits, 1949 us: 0.85 PFLOP/s of the 1.16 that a large library product reaches) the one is busy 57 % of
-// the time, the other 33 %.  So a code is turned into float16 once for a block's 128 or 256 rows, on its way into LDS, and a wavefront has 32 rows, whose
+// of 128 on 8, float16, 8 bits, 1910 us: 0.86 PFLOP/s of the 1.16 that a large library product reaches) the one is busy 50 % of
+// the time, the other 37 %.  So a code is turned into float16 once for a block's 128 or 256 rows, on its way into LDS, and a wavefront has 32 rows, whose
 // accumulators, maxima and sums stay in its registers:
 //
 //   S^T = K Q^T    v_mfma_f32_32x32x16_f16, A: K from LDS, lane (h, n) key n of 32, columns 8h..8h+7 of 16; B: Q in registers.
@@ -11,7 +11,8 @@
 //                  a column's keys lie in that order, so that a fragment is 16 consecutive bytes.
 //
 // 64 keys at a time, in two sets of LDS: while one is worked on, the next keys' codes are on their way to registers, and go
-// into the other one after that.  Rows of LDS are swizzled by 16 bytes, so that neither the fragments nor the writes meet in a bank.
+// into the other one after that.  Rows of LDS are swizzled by 16 bytes over all 64 banks, so that fragments do not meet in one (keys'
+// rows swizzled over half of the banks cost 2 %); the writes of values, four columns apart, meet in pairs.
 #pragma once
 #include <type_traits>
 
@@ -42,7 +43,7 @@ struct ChunkKernel {
     static constexpr int K_BYTES = KEYS * DIM * 2, V_BYTES = DIM * KEYS * 2, STAGE = K_BYTES + V_BYTES + 2 * KEYS * 4;
     static constexpr int LDS_BYTES = 2 * STAGE;
 
-    static __device__ __forceinline__ int k_at(int key, int chunk) { return key * DIM * 2 + ((chunk ^ (key & 7)) << 4); }
+    static __device__ __forceinline__ int k_at(int key, int chunk) { return key * DIM * 2 + ((chunk ^ (key & (DIM >= 128 ? 15 : 7))) << 4); }
     static __device__ __forceinline__ int v_at(int d, int chunk) { return K_BYTES + d * KEYS * 2 + ((chunk ^ ((d ^ (d >> 2)) & 7)) << 4); }
 
     static __device__ __forceinline__ void run(const AttnArgs& a, const T* __restrict__ q, T* __restrict__ out, char* lds) {
