@@ -144,7 +144,7 @@ def paged_attention(q: Tensor, cache, page_table: Tensor, q_starts: Tensor, kv_l
     that is negative or beyond the cache are not seen; a length beyond ``page_table`` is cut to it.
 
     ``max_chunk``: the most tokens of a sequence in this call, where the program knows it; the work is divided by
-    it, and results differ by rounding alone.  Default ``scale``: ``1 / sqrt(head_dim)``."""
+    it, and results differ by rounding alone.  Default ``scale``: ``1 / sqrt(head_dim)``.  ``out`` may be ``q``."""
     from ..quantization._kv_cache import _check_cache, _check_rows
     _check_cache("paged_attention", cache)
     if not isinstance(q, Tensor) or q.ndim != 3:

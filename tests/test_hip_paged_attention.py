@@ -224,6 +224,41 @@ def test_a_length_beyond_the_table_is_cut():
         b.check(b.run())
 
 
+LONG = [  # one long sequence before many keys, as blocks of twice as many rows; equal lengths; more sequences than lanes
+    ([300], [1300], 4, 1, 128, 64, 8, True, np.float16), ([260], [1100], 8, 2, 96, 16, 4, False, np.float32),
+    ([512], [2100], 2, 1, 128, 32, 4, True, np.float16), ([300], [2000], 4, 1, 80, 48, 8, False, np.float32),
+    ([130] * 5, [900] * 5, 2, 1, 64, 16, 8, True, np.float16), ([120, 130, 110], [1500, 1499, 1450], 1, 1, 128, 16, 4, False, np.float16),
+    ([100] * 70, [100 + 13 * i for i in range(70)], 1, 1, 32, 16, 8, True, np.float32)]
+
+
+@pytest.mark.parametrize("case", range(len(LONG)))
+def test_long_chunks(case):
+    b = Batch(*LONG[case], seed=case, tail=3)
+    b.check(b.run())
+    b.check(b.run(window=333), window=333)
+    b.check(b.run(causal=False, scale=-0.05), causal=False, scale=-0.05)
+
+
+def test_a_prompt_whose_tiles_fill_the_device_is_its_halves():
+    b = Batch([4096], [4096], 64, 16, 16, seed=7)
+    whole = b.run().astype(np.float64)
+    q, n = b.q, 2048
+    for at in (0, n):
+        b.q, b.q_starts, b.kv_lens = q[at:at + n], np.array([0, n], np.int32), np.array([at + n], np.int32)
+        half = b.run().astype(np.float64)
+        # both are off by half a step of the result and half a step of each probability at most, and by a float32 score's few units
+        tol = 2 * 2.0 ** -11 * (np.abs(half) + np.abs(b.pages["v"]).max()) + 1e-5
+        assert np.all(np.abs(whole[at:at + n] - half) <= tol)
+
+
+@pytest.mark.parametrize("chunks,lengths", [([1, 1, 1], [300, 900, 20]), ([5, 30], [50, 1400]), ([150, 1], [700, 900]), ([300], [1300])])
+def test_the_result_may_take_the_queries_place(chunks, lengths):
+    b = Batch(chunks, lengths, 4, 1, 128, seed=9, tail=2)
+    q = hip(b.q)
+    F.paged_attention(q, b.cache, ids(b.table), ids(b.q_starts), ids(b.kv_lens), out=q)
+    assert np.array_equal(q.numpy(), b.run())
+
+
 def test_packed_queries():
     b = Batch([5, 60], [80, 90], 6, 2, 64, seed=1)
     packed = np.concatenate([b.q, b.rng.standard_normal((65, 4, 64)).astype(np.float16)], 1).reshape(5, 13, 640)
