@@ -451,7 +451,8 @@ struct ChunkKernel {
         if (row > last_row) return;
         const float scale = __builtin_ldexpf(1.f / kProbability, unit) * (it.parts == 1 ? (l == 0.f ? 0.f : 1.f / l) : 1.f);
         if (it.parts > 1) {
-            float* piece = a.partial + (size_t(item) * a.kv_heads + head) * kPiece<R, DIM>;
+            if (it.first + it.parts > a.pieces) return;
+            float* piece = a.partial + (size_t(it.first + it.part) * a.kv_heads + head) * kPiece<R, DIM>;
             if (h == 0) piece[R * DIM + 32 * wave + n] = m, piece[R * DIM + R + 32 * wave + n] = l;
 #pragma unroll
             for (int d = 0; d < TILES; ++d)
@@ -487,7 +488,7 @@ constexpr int kJoined = 16;
 template <class T, int DIM, int R>
 __global__ __launch_bounds__(256) void attn_parts_kernel(AttnArgs a, T* __restrict__ out) {
     Tile it;
-    if (!find_tile<R>(a, blockIdx.x, true, it) || it.parts == 1 || it.first + it.parts > a.blocks) return;
+    if (!find_tile<R>(a, blockIdx.x, true, it) || it.parts == 1 || it.first + it.parts > a.pieces) return;
     const float* first = a.partial + (size_t(it.first) * a.kv_heads + blockIdx.y) * kPiece<R, DIM>;
     // (several rows a wavefront: what finding the tile takes is worth more than one)
     for (int r = blockIdx.z * kJoined + (threadIdx.x >> 6); r < int(blockIdx.z + 1) * kJoined; r += 4)

@@ -66,7 +66,8 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
         LQ_REQUIRE(int64_t(a.blocks) * c->kv_heads <= 0xffffff, LQ_ERR_NOT_IMPLEMENTED, "paged_attention: %d tiles of queries for %d heads", tiles,
                    c->kv_heads);
         if (join) {
-            rc = room(size_t(a.blocks) * c->kv_heads * R * (dim + 2));
+            a.pieces = std::min(a.blocks, (4 * a.each + c->kv_heads - 1) / c->kv_heads + 64);  // (64: rounding)
+            rc = room(size_t(a.pieces) * c->kv_heads * R * (dim + 2));
             if (rc) return rc;
         }
         auto launch = [&](auto type, auto bits) {

@@ -35,6 +35,7 @@ struct AttnArgs {
     int blocks;
     int each;      // of so many blocks each has a share of the units, at least `least`; 0: a segment
     int least;
+    int pieces;    // parts of tiles of several that there is room for
     int min_rows, max_rows;  // sequences of fewer or more rows are another launch's
     float scale;
     float* partial;  // pieces of segments
@@ -176,7 +177,7 @@ struct Segments {
 // Tiles of R rows of a launch, of each sequence's the last one first (it sees the most keys), their keys in parts, a block each.
 struct Tile {
     int seq, tile, part, parts;
-    int first;  // number of the tile's first part
+    int first;  // number of its first part among those of tiles of several
     Sequence s;
 };
 // Parts of `extent` keys where none shall have more than `most`, or hardly more: whoever counts them counts alike, and up to `most` it is 1.
@@ -184,7 +185,7 @@ __device__ __forceinline__ unsigned parts_of(unsigned extent, unsigned most) {
     return max(1u, unsigned(__builtin_ceilf(float(extent) * __builtin_amdgcn_rcpf(float(most)) * (1.f - 0x1p-20f))));
 }
 // The most keys of a part: so many that there are about twice as many parts of all tiles as places for blocks (a.each), where lengths differ
-// the blocks that end early then take another.  Up to 64 sequences of about the same length (one a lane; 0 tiles: not this launch's)
+// the blocks that end early then take another.  (Tiles of several parts, each longer than one, then have 4 a.each parts at most, for all heads.)  Up to 64 sequences of about the same length (one a lane; 0 tiles: not this launch's)
 // have equal parts, which come in whole rounds: a lane each tries the longest in 1, 2, 3, ... parts, and the shortest sum of the rounds'
 // lengths counts, in keys, of which a block costs kBlock besides its own and one whose part is joined kPart more.
 constexpr float kBlock = 128.f, kPart = 320.f, kAlike = 0.8f;
@@ -199,7 +200,7 @@ __device__ __forceinline__ unsigned part_keys(const AttnArgs& a, float keys, uns
     for (int i = 0; i < a.batch; ++i)
         n += unsigned(__builtin_amdgcn_readlane(int(tiles), i)) * parts_of(unsigned(__builtin_amdgcn_readlane(int(extent), i)), most);
     const float rounds = __builtin_ceilf(float(n) * heads / places) * (float(most) + kBlock + (n > all ? kPart : 0.f));
-    const float cost = n > unsigned(a.blocks) ? __builtin_inff() : rounds;
+    const float cost = n > unsigned(a.blocks) || (n > all && n > unsigned(a.pieces)) ? __builtin_inff() : rounds;
     const unsigned long long best = __ballot(cost == wave_min(cost));
     return unsigned(__builtin_amdgcn_readlane(int(most), __builtin_ctzll(best)));
 }
@@ -224,11 +225,11 @@ __device__ __forceinline__ bool find_tile(const AttnArgs& a, unsigned id, bool w
     }
     keys = of_last(sum_upto(keys));
     const unsigned most = part_keys(a, keys, tiles, extent, lane);
-    unsigned before = 0, tiles_before = 0;
+    unsigned before = 0, tiles_before = 0, split_before = 0;
     for (int first = 0; first < a.batch; first += 64) {
         if (a.batch > 64) load(first + lane);
-        const unsigned parts = parts_of(extent, most);
-        const unsigned upto = sum_upto(tiles * parts), tiles_to = sum_upto(tiles);
+        const unsigned parts = parts_of(extent, most), split = parts > 1 ? tiles * parts : 0u;
+        const unsigned upto = sum_upto(tiles * parts), tiles_to = sum_upto(tiles), split_to = sum_upto(split);
         const unsigned long long past = __ballot((whole ? tiles_before + tiles_to : before + upto) > id);
         if (past) {
             const int l = __builtin_ctzll(past);
@@ -236,12 +237,13 @@ __device__ __forceinline__ bool find_tile(const AttnArgs& a, unsigned id, bool w
             const unsigned n = get(tiles), p = get(parts), begin = before + get(upto) - n * p;
             const unsigned k = whole ? id - (tiles_before + get(tiles_to) - n) : (id - begin) / p;
             it.seq = first + l, it.tile = int(n - 1 - k), it.parts = int(p), it.part = whole ? 0 : int(id - begin - k * p);
-            it.first = int(begin + k * p);
+            it.first = int(split_before + get(split_to) - get(split) + k * p);
             it.s = Sequence{int(get(unsigned(s.q0))), int(get(unsigned(s.chunk))), int(get(unsigned(s.len)))};
             return true;
         }
         before += of_last(upto);
         tiles_before += of_last(tiles_to);
+        split_before += of_last(split_to);
     }
     return false;
 }

@@ -38,7 +38,8 @@ def test_c_entries_refuse_a_bad_cache(kw, error):
 
 @pytest.mark.parametrize("at,value,error", [
     (1, None, ValueError), (1, P + 4, ValueError), (2, None, ValueError), (3, _C.I8, L.DtypeMismatch), (3, _C.BF16, L.DtypeMismatch),
-    (4, 124, L.ShapeMismatch), (4, 130, ValueError), (5, 64, L.ShapeMismatch), (6, None, ValueError), (7, 1 << 40, L.ShapeMismatch)])
+    (4, 124, L.ShapeMismatch), (4, 130, ValueError), (5, 64, L.ShapeMismatch), (6, None, ValueError), (7, 1 << 40, L.ShapeMismatch),
+    (7, 1 << 25, L.ShapeMismatch)])
 def test_c_write_refuses(at, value, error):
     args = [C.byref(struct()), P, P, _C.F32, 128, 128, P, 1, None]
     args[at] = value
@@ -47,7 +48,7 @@ def test_c_write_refuses(at, value, error):
 
 
 @pytest.mark.parametrize("at,value,error", [
-    (1, None, ValueError), (2, 1 << 40, L.ShapeMismatch), (3, None, ValueError), (4, P + 8, ValueError), (5, _C.F64, L.DtypeMismatch)])
+    (1, None, ValueError), (2, 1 << 40, L.ShapeMismatch), (2, 1 << 25, L.ShapeMismatch), (3, None, ValueError), (4, P + 8, ValueError), (5, _C.F64, L.DtypeMismatch)])
 def test_c_read_refuses(at, value, error):
     args = [C.byref(struct()), P, 1, P, P, _C.F16, None]
     args[at] = value
