@@ -492,7 +492,7 @@ __global__ __launch_bounds__(256) void attn_parts_kernel(AttnArgs a, T* __restri
     const float* first = a.partial + (size_t(it.first) * a.kv_heads + blockIdx.y) * kPiece<R, DIM>;
     // (several rows a wavefront: what finding the tile takes is worth more than one)
     for (int r = blockIdx.z * kJoined + (threadIdx.x >> 6); r < int(blockIdx.z + 1) * kJoined; r += 4)
-        join_row<T, DIM, R>(a, out, it.s, it.tile, int(blockIdx.y), r, it.parts,
+        join_row<T, DIM, R, false>(a, out, it.s, it.tile, int(blockIdx.y), r, it.parts,
                             [&](int i) { return first + size_t(i) * a.kv_heads * kPiece<R, DIM>; });
 }
 

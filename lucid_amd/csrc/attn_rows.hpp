@@ -489,7 +489,7 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void attn_rows_kernel(AttnA
 }
 
 // Joins the pieces of the segments that several blocks have one of.
-template <class T, int DIM, int R, int UNIT>
+template <class T, int DIM, int R, int UNIT, bool APART>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, T* __restrict__ out) {
     Segments<R, UNIT> segs(a);
     const unsigned share = segs.share(), head = blockIdx.y;
@@ -517,15 +517,21 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, T* __restric
     const unsigned b0 = x / share, b1 = (x + units - 1) / share;
     if (b0 == b1 || b1 >= unsigned(a.blocks)) return;
     // the first piece is the second of its block's two, the others are the first of theirs
-    join_row<T, DIM, R>(a, out, s, tile, int(head), blockIdx.z * 4 + (threadIdx.x >> 6), int(b1 - b0) + 1,
-                        [&](int i) { return a.partial + (2 * size_t(b0 + i) + (i == 0)) * kPiece<R, DIM>; });
+    const auto piece = [&](int i) { return a.partial + (2 * size_t(b0 + i) + (i == 0)) * kPiece<R, DIM>; };
+    const int parts = int(b1 - b0) + 1;
+    if constexpr (APART) join_row<T, DIM, R, true>(a, out, s, tile, int(head), blockIdx.z, parts, piece);
+    else join_row<T, DIM, R, false>(a, out, s, tile, int(head), blockIdx.z * 4 + (threadIdx.x >> 6), parts, piece);
 }
 
 template <class T, int BITS, int DIM, int QT>
 void launch_rows(const AttnArgs& a, const T* q, T* out, int tiles, bool join, hipStream_t st) {
     if (a.k_zero) attn_rows_kernel<T, BITS, true, DIM, QT><<<a.blocks, 256, 0, st>>>(a, q, out);
     else attn_rows_kernel<T, BITS, false, DIM, QT><<<a.blocks, 256, 0, st>>>(a, q, out);
-    if (join) attn_join_kernel<T, DIM, 16 * QT, 4 * rows_keys(BITS, DIM, QT)><<<dim3(tiles, a.kv_heads, 4 * QT), 256, 0, st>>>(a, out);
+    if (!join) return;
+    // few segments are in many pieces (one token of 131 072 keys, 64 pieces: 4.5 us, 6.3 as four rows a block), many in few
+    constexpr int UNIT = 4 * rows_keys(BITS, DIM, QT);
+    if (tiles * a.kv_heads <= 32) attn_join_kernel<T, DIM, 16 * QT, UNIT, true><<<dim3(tiles, a.kv_heads, 16 * QT), 256, 0, st>>>(a, out);
+    else attn_join_kernel<T, DIM, 16 * QT, UNIT, false><<<dim3(tiles, a.kv_heads, 4 * QT), 256, 0, st>>>(a, out);
 }
 
 template <class T, int BITS>

@@ -187,7 +187,8 @@ __device__ __forceinline__ unsigned parts_of(unsigned extent, unsigned most) {
 // The most keys of a part: so many that there are about twice as many parts of all tiles as places for blocks (a.each), where lengths differ
 // the blocks that end early then take another.  (Tiles of several parts, each longer than one, then have 4 a.each parts at most, for all heads.)  Up to 64 sequences of about the same length (one a lane; 0 tiles: not this launch's)
 // have equal parts, which come in whole rounds: a lane each tries the longest in 1, 2, 3, ... parts, and the shortest sum of the rounds'
-// lengths counts, in keys, of which a block costs kBlock besides its own and one whose part is joined kPart more.
+// lengths counts, in keys, of which a block costs kBlock besides its own and one whose part is joined kPart more (us, parts of the share / in
+// rounds: 4 chunks of 512 over 8192 keys 400 / 387, one of 300 101 / 85; but 4 over 1934 to 8192 keys 281 / 292).
 constexpr float kBlock = 128.f, kPart = 320.f, kAlike = 0.8f;
 __device__ __forceinline__ unsigned part_keys(const AttnArgs& a, float keys, unsigned tiles, unsigned extent, int lane) {
     const float heads = float(a.kv_heads), places = float(a.each);
@@ -253,13 +254,16 @@ __device__ __forceinline__ bool find_tile(const AttnArgs& a, unsigned id, bool w
 template <int R, int DIM>
 constexpr size_t kPiece = size_t(R) * (DIM + 2);
 
-// Row r of a tile from its pieces, by a wavefront: a lane has four columns and, where that leaves lanes, the pieces in turn.
-template <class T, int DIM, int R, class Piece>
+// Row r of a tile from its pieces: a lane has four columns and, where that leaves lanes, the pieces in turn.  APART: the pieces are dealt to the
+// four wavefronts of a block, whose sums meet in LDS; otherwise each wavefront has a row.
+template <class T, int DIM, int R, bool APART, class Piece>
 __device__ __forceinline__ void join_row(const AttnArgs& a, T* out, const Sequence& s, int tile, int head, int r, int parts, Piece piece) {
     constexpr int QUADS = DIM / 4, EVERY = 64 / QUADS;
     const int lane = threadIdx.x & 63, d = lane % QUADS * 4, mine = lane / QUADS;
     const int group = int(a.group.d);
     if (r >= s.chunk * group - tile * R) return;
+    const int wave = APART ? __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6) : 0, step = APART ? 4 : 1;
+    const int n = (parts - wave + step - 1) / step;  // of this wavefront's
     // eight pieces of a lane at a time, the first while the maximum is looked for (64 pieces of 16 rows: 6.1 us, four and after it 8.6)
     constexpr int DEEP = 8;
     f32x4 y[DEEP];
@@ -267,8 +271,8 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, T* out, const Sequen
     auto request = [&](int i0) {
 #pragma unroll
         for (int u = 0; u < DEEP; ++u) {
-            if (u == DEEP / 2 && i0 + u * EVERY >= parts) break;
-            const float* p = piece(min(i0 + u * EVERY + mine, parts - 1));
+            if (u == DEEP / 2 && i0 + u * EVERY >= n) break;
+            const float* p = piece(min(wave + step * (i0 + u * EVERY + mine), parts - 1));
             y[u] = *reinterpret_cast<const f32x4*>(p + r * DIM + d);
             m[u] = p[R * DIM + r], l[u] = p[R * DIM + R + r];
         }
@@ -283,12 +287,12 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, T* out, const Sequen
     for (int i0 = 0;;) {
 #pragma unroll
         for (int u = 0; u < DEEP; ++u) {
-            if (i0 + u * EVERY + mine >= parts) continue;
+            if (i0 + u * EVERY + mine >= n) continue;
             const float f = __builtin_amdgcn_exp2f(m[u] - mm);
             total += l[u] * f, v += y[u] * f;
         }
         i0 += DEEP * EVERY;
-        if (i0 >= parts) break;
+        if (i0 >= n) break;
         request(i0);
     }
 #pragma unroll
@@ -296,6 +300,16 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, T* out, const Sequen
         total += __shfl_xor(total, e, 64);
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] += __shfl_xor(v[k], e, 64);
+    }
+    if constexpr (APART) {
+        __shared__ f32x4 sums[3][QUADS];
+        __shared__ float totals[3];
+        if (wave && !mine) sums[wave - 1][d / 4] = v;
+        if (wave && lane == 0) totals[wave - 1] = total;
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int w = 0; w < 3; ++w) total += totals[w], v += sums[w][d / 4];
     }
     if (d >= a.dim || mine) return;
     v *= total == 0.f ? 0.f : 1.f / total;
@@ -370,7 +384,7 @@ constexpr int rows_keys(int bits, int dim, int qt) { return bits * dim <= 512 &&
 template <class T, int BITS>
 void launch_rows_of(const AttnArgs& a, const T* q, T* out, int tiles, int qt, bool join, hipStream_t st);
 
-// A chunk of a sequence: tiles of 128 rows.
+// A chunk of a sequence: tiles of 128 rows, or 256 (wide).
 template <class T, int BITS>
 int launch_chunk_of(const AttnArgs& a, const T* q, T* out, bool wide, int tiles, bool join, hipStream_t st);
 
