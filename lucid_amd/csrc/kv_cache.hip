@@ -94,7 +94,8 @@ __device__ __forceinline__ RowGrid grid_of(const float (&x)[8], int bits) {
 // correctly rounded quotient (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990),
 // which takes 1 / s and the remainders neither underflowing nor infinite: lanes of other rows divide.  (A row's largest value of a
 // symmetric grid lies on the border of two codes, so that a test whether the estimate will do fails in nearly every wavefront.)
-template <int BITS>
+// ONE: of a float16 value and the symmetric scale of a float16 maximum the first step gives it already, for each of the 10^9 pairs.
+template <int BITS, bool ONE>
 __device__ __forceinline__ void codes_of(const float (&x)[8], RowGrid g, uint32_t (&w)[BITS / 4]) {
     constexpr int QMIN = -(1 << (BITS - 1)), STEPS = (1 << BITS) - 1;
     const float r = 1.0f / g.s, z = g.z - float(QMIN);
@@ -103,7 +104,7 @@ __device__ __forceinline__ void codes_of(const float (&x)[8], RowGrid g, uint32_
     for (int i = 0; i < 8; ++i) {
         float q = x[i] * r;
         q = __builtin_fmaf(__builtin_fmaf(-q, g.s, x[i]), r, q);
-        q = __builtin_fmaf(__builtin_fmaf(-q, g.s, x[i]), r, q);
+        if constexpr (!ONE) q = __builtin_fmaf(__builtin_fmaf(-q, g.s, x[i]), r, q);
         c[i] = __builtin_rintf(q) + z;
     }
     if (__builtin_expect(!(g.s < 0x1p120f), 0)) {  // infinite and NaN grids among them
@@ -137,8 +138,8 @@ struct CacheView {
 // tokens of 128 values: 2 KB of codes, 64 bytes of scales), in k and v a row is one piece.  Heads vary fastest over the blocks: those
 // that run together then cover whole lines of k and v of neighbouring tokens (writing 65 536 tokens of 8 heads of 128, float16 to 8
 // bits: 85 us, 96 with tokens fastest).  What streams past once (k and v, and the codes that are read back) leaves the caches to
-// others: non-temporal (75 us; reading the same back 59 us instead of 74, 131 072 tokens in 4 bits 139 instead of 149).  Bound by memory:
-// 403 MB at 5.4 and 6.8 TB/s, 671 MB, four fifths of them written, at 4.8; a large copy reaches 5.1.  Two tokens a lane read back
+// others: non-temporal (75 us, 73 with the shorter quotient; reading the same back 59 us instead of 74, 131 072 tokens in 4 bits 139 instead of 149).  Bound by memory:
+// 403 MB at 5.5 and 6.8 TB/s, 671 MB, four fifths of them written, at 4.8; a large copy reaches 5.1.  Two tokens a lane read back
 // 2 % faster at the largest size and need not be.
 template <class T, int BITS, int LPR, bool SYMMETRIC>
 __global__ __launch_bounds__(256) void kv_cache_write_kernel(CacheView c, const T* __restrict__ k, const T* __restrict__ v, size_t ldk,
@@ -157,8 +158,9 @@ __global__ __launch_bounds__(256) void kv_cache_write_kernel(CacheView c, const 
     const size_t to = c.row(slot, head);
     const RowGrid grids[2] = {grid_of<LPR, SYMMETRIC>(x[0], BITS), grid_of<LPR, SYMMETRIC>(x[1], BITS)};
     uint32_t words[2][BITS / 4];
-    codes_of<BITS>(x[0], grids[0], words[0]);
-    codes_of<BITS>(x[1], grids[1], words[1]);
+    constexpr bool ONE = SYMMETRIC && std::is_same_v<T, _Float16>;
+    codes_of<BITS, ONE>(x[0], grids[0], words[0]);
+    codes_of<BITS, ONE>(x[1], grids[1], words[1]);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         const RowGrid g = grids[which];

@@ -145,6 +145,25 @@ def test_all_quotients_of_a_row_are_rounded_as_the_division():
     assert np.array_equal(c.k_scale.numpy().ravel(), scale.ravel()) and np.array_equal(c.k_zero.numpy().ravel(), zero.ravel())
 
 
+@pytest.mark.parametrize("bits", [8, 4])
+def test_float16_rows_of_every_maximum(bits):
+    """Symmetric rows, one for each positive finite float16 as the largest value: the shorter way to the quotient gives the division's result."""
+    rng = np.random.default_rng(bits)
+    top = np.arange(1, 0x7c00, dtype=np.uint16)
+    x = (rng.integers(0, 1 << 16, (len(top), 1, 128)) % (top[:, None, None].astype(np.int64) + 1)).astype(np.uint16)  # (by their bits: all sizes alike)
+    near = rng.random(x.shape) < 0.5
+    x = np.where(near, top[:, None, None] - np.minimum(top[:, None, None], rng.integers(0, 4096, x.shape)), x).astype(np.uint16)
+    x[:, 0, 0] = top
+    x = (x | (rng.integers(0, 2, x.shape) << 15).astype(np.uint16)).view(np.float16)
+    c = make(1984, 16, 1, 128, True, bits)
+    Q.kv_cache_write(c, hip(x), hip(x[::-1]), ids(np.arange(len(top))))
+    for name, y in (("k", x), ("v", x[::-1])):
+        u, scale, _ = K.quantize(y.astype(np.float32), bits, True)
+        got = getattr(c, name + "_codes").numpy().view(np.uint8).reshape(-1, 128 * bits // 8)[:len(top)]
+        assert np.array_equal(got, K.pack(u, bits).reshape(got.shape))
+        assert np.array_equal(getattr(c, name + "_scale").numpy().ravel()[:len(top)], scale.ravel())
+
+
 def test_packed_rows_and_an_empty_call():
     rng = np.random.default_rng(5)
     for dtype in (np.float32, np.float16):
