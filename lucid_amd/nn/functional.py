@@ -6,12 +6,12 @@ kernel; inputs and outputs are float32 tensors on the ``hip`` device.
 
 from __future__ import annotations
 
-import ctypes as C
 import math
 
 from .. import _C
 from .. import _tensor as T
 from .._tensor import Tensor
+from ..quantization._kv_cache import _check_cache, _check_ids, _check_rows
 
 
 def _require_f32_hip(name: str, *ts: Tensor) -> None:
@@ -113,7 +113,6 @@ def scaled_dot_product_attention_qkv(qkv: Tensor, num_heads: int, scale: float |
 
 
 def _paged_attention(name, cache, q_ptr, ldq, dtype, tokens, heads, out, page_table, q_starts, kv_lens, scale, causal, window, max_chunk) -> None:
-    from ..quantization._kv_cache import _check_ids
     if not isinstance(page_table, Tensor) or page_table.ndim != 2:
         raise _C.ShapeMismatch(f"{name}: page_table is a (batch, pages) tensor")
     batch, width = page_table.shape
@@ -126,7 +125,7 @@ def _paged_attention(name, cache, q_ptr, ldq, dtype, tokens, heads, out, page_ta
         raise ValueError(f"{name}: window {window}; at least 1, or None for all keys")
     if max_chunk is not None and max_chunk < 1:
         raise ValueError(f"{name}: max_chunk {max_chunk}; at least 1, or None")
-    _C.call("lq_paged_attention", C.byref(cache._struct), q_ptr, ldq, out.data_ptr, dtype.code, tokens, heads, batch, page_table.data_ptr, width,
+    _C.call("lq_paged_attention", cache._ref, q_ptr, ldq, out.data_ptr, dtype.code, tokens, heads, batch, page_table.data_ptr, width,
             q_starts.data_ptr, kv_lens.data_ptr, 1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale), 1 if causal else 0,
             0 if window is None else window, 0 if max_chunk is None else max_chunk, None)
 
@@ -145,7 +144,6 @@ def paged_attention(q: Tensor, cache, page_table: Tensor, q_starts: Tensor, kv_l
 
     ``max_chunk``: the most tokens of a sequence in this call, where the program knows it; the work is divided by
     it, and results differ by rounding alone.  Default ``scale``: ``1 / sqrt(head_dim)``.  ``out`` may be ``q``."""
-    from ..quantization._kv_cache import _check_cache, _check_rows
     _check_cache("paged_attention", cache)
     if not isinstance(q, Tensor) or q.ndim != 3:
         raise _C.ShapeMismatch("paged_attention: q is a (tokens, heads, head_dim) tensor")
@@ -167,7 +165,6 @@ def paged_attention_qkv(qkv: Tensor, num_heads: int, cache, page_table: Tensor, 
     """``paged_attention`` of the queries in the packed output of a qkv Linear, ``(..., (num_heads + 2 * kv_heads) * head_dim)`` with the
     queries first; the keys and values beside them are those that ``quantization.kv_cache_write_qkv`` has written.  Returns
     ``(..., num_heads * head_dim)``."""
-    from ..quantization._kv_cache import _check_cache, _check_rows
     _check_cache("paged_attention_qkv", cache)
     num_heads = int(num_heads)
     row = (num_heads + 2 * cache.kv_heads) * cache.head_dim

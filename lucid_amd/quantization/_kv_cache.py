@@ -29,7 +29,7 @@ class PagedKVCache:
     ``(code - zero) * scale``.  All buffers begin as zeros: a slot that was never written stands for zeros."""
 
     __slots__ = ("num_pages", "page_size", "kv_heads", "head_dim", "qscheme", "qdtype", "k_codes", "v_codes", "k_scale", "v_scale",
-                 "k_zero", "v_zero", "_struct")
+                 "k_zero", "v_zero", "_struct", "_ref")
 
     def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, qscheme: QScheme = per_channel_symmetric,
                  qdtype: QDtype = qint8) -> None:
@@ -59,6 +59,7 @@ class PagedKVCache:
         pointers = [t.data_ptr if t is not None else None
                     for t in (self.k_codes, self.v_codes, self.k_scale, self.v_scale, self.k_zero, self.v_zero)]
         self._struct = _C.KvCache(*pointers, self.num_pages, self.page_size, self.kv_heads, self.head_dim, qdtype.bits)
+        self._ref = C.byref(self._struct)
 
     @property
     def num_slots(self) -> int:
@@ -84,7 +85,10 @@ def _check_cache(name: str, cache) -> None:
         raise TypeError(f"{name} expects a PagedKVCache, got {type(cache).__name__}")
 
 
+# (what a call checks of its tensors is a good part of what a small call takes: the usual case in one line)
 def _check_ids(name: str, what: str, t, shape) -> None:
+    if t.__class__ is Tensor and t.device == "hip" and t.dtype is T.int32 and t.shape == shape:
+        return
     if not isinstance(t, Tensor) or t.device != "hip":
         raise _C.DeviceMismatch(f"{name}: {what} must be a tensor on the 'hip' device")
     if t.dtype != T.int32:
@@ -94,6 +98,8 @@ def _check_ids(name: str, what: str, t, shape) -> None:
 
 
 def _check_rows(name: str, what: str, t, shape) -> None:
+    if t.__class__ is Tensor and t.device == "hip" and (t.dtype is T.float16 or t.dtype is T.float32) and t.shape == shape:
+        return
     if not isinstance(t, Tensor) or t.device != "hip":
         raise _C.DeviceMismatch(f"{name}: {what} must be a tensor on the 'hip' device")
     if t.dtype not in _FLOATS:
@@ -116,7 +122,7 @@ def kv_cache_write(cache: PagedKVCache, k: Tensor, v: Tensor, slots: Tensor) -> 
         raise _C.DtypeMismatch(f"kv_cache_write: k is {k.dtype}, v {v.dtype}")
     _check_ids("kv_cache_write", "slots", slots, shape[:1])
     width = cache.kv_heads * cache.head_dim
-    _C.call("lq_kv_cache_write", C.byref(cache._struct), k.data_ptr, v.data_ptr, k.dtype.code, width, width, slots.data_ptr, shape[0], None)
+    _C.call("lq_kv_cache_write", cache._ref, k.data_ptr, v.data_ptr, k.dtype.code, width, width, slots.data_ptr, shape[0], None)
 
 
 def kv_cache_write_qkv(cache: PagedKVCache, qkv: Tensor, num_heads: int, slots: Tensor) -> None:
@@ -131,7 +137,7 @@ def kv_cache_write_qkv(cache: PagedKVCache, qkv: Tensor, num_heads: int, slots: 
     _check_ids("kv_cache_write_qkv", "slots", slots, (tokens,))
     k = qkv.data_ptr + int(num_heads) * cache.head_dim * qkv.dtype.itemsize
     v = k + cache.kv_heads * cache.head_dim * qkv.dtype.itemsize
-    _C.call("lq_kv_cache_write", C.byref(cache._struct), k, v, qkv.dtype.code, row, row, slots.data_ptr, tokens, None)
+    _C.call("lq_kv_cache_write", cache._ref, k, v, qkv.dtype.code, row, row, slots.data_ptr, tokens, None)
 
 
 def kv_cache_read(cache: PagedKVCache, slots: Tensor, dtype=T.float32, out: tuple[Tensor, Tensor] | None = None) -> tuple[Tensor, Tensor]:
@@ -153,5 +159,5 @@ def kv_cache_read(cache: PagedKVCache, slots: Tensor, dtype=T.float32, out: tupl
         _check_rows("kv_cache_read", "out[1]", v, shape)
         if v.dtype != k.dtype:
             raise _C.DtypeMismatch(f"kv_cache_read: out is {k.dtype} and {v.dtype}")
-    _C.call("lq_kv_cache_read", C.byref(cache._struct), slots.data_ptr, shape[0], k.data_ptr, v.data_ptr, k.dtype.code, None)
+    _C.call("lq_kv_cache_read", cache._ref, slots.data_ptr, shape[0], k.data_ptr, v.data_ptr, k.dtype.code, None)
     return k, v
