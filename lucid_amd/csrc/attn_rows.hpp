@@ -49,27 +49,37 @@ struct RowsKernel {
 
     static __device__ __forceinline__ void run(const AttnArgs& a, const T* __restrict__ q, T* __restrict__ out, float* lds) {
         const int first_row = a.q_starts[0], end_row = a.q_starts[a.batch];
-        unsigned x = 0, end = 0, per_head = 0;
+        unsigned x, end;
+        int head;
+        typename Segs::Segment seg;
+        {
+            Segs segs(a);
+            clear_other_rows(a, out, first_row, end_row, blockIdx.x, gridDim.x);
+            const unsigned all = segs.total * unsigned(a.kv_heads), share = a.each ? segs.share() : 1u;
+            if (all == 0 || blockIdx.x > (all - 1) / share) return;
+            x = blockIdx.x * share, end = min(all, x + share);
+            head = int(x / segs.total);
+            seg = segs.at(x - unsigned(head) * segs.total);
+            if (seg.tiles == 0) return;
+        }
         while (true) {
-            typename Segs::Segment seg;
-            unsigned head;
-            {  // (found anew for each segment: kept, what it takes would cost the registers of a wavefront)
-                Segs segs(a);
-                if (per_head == 0) {
-                    clear_other_rows(a, out, first_row, end_row, blockIdx.x, gridDim.x);
-                    per_head = segs.total;
-                    const unsigned all = per_head * unsigned(a.kv_heads), share = a.each ? segs.share() : 1u;
-                    if (all == 0 || blockIdx.x > (all - 1) / share) return;
-                    x = blockIdx.x * share, end = min(all, x + share);
-                }
-                head = x / per_head;
-                seg = segs.at(x - head * per_head);
-            }
             const unsigned n = min(seg.units - seg.unit, end - x);
             float* piece = n == seg.units ? nullptr : a.partial + (2 * size_t(blockIdx.x) + (seg.unit ? 0 : 1)) * kPiece<R, DIM>;
-            segment(a, q, out, lds, seg, int(head), n, piece);
+            segment(a, q, out, lds, seg, head, n, piece);
             x += n;
             if (x >= end) break;
+            // on to the next tile, sequence (one that has tiles: there are units left) or head
+            seg.unit = 0;
+            if (++seg.tile == int(seg.tiles)) {
+                seg.tile = 0;
+                do {
+                    if (++seg.seq == a.batch) {
+                        if (++head == a.kv_heads) return;
+                        seg.seq = 0;
+                    }
+                    Segs::look(a, seg.seq, seg.s, seg.tiles, seg.units);
+                } while (seg.tiles == 0);
+            }
             __syncthreads();
         }
     }
@@ -489,38 +499,51 @@ __global__ __launch_bounds__(256, DIM > 128 ? 1 : 2) void attn_rows_kernel(AttnA
 }
 
 // Joins the pieces of the segments that several blocks have one of.
+// APART: a block for each row of each segment, of which there are few; otherwise the blocks find the segments by the places where one
+// share ends and the next begins, the first such place of a segment has it, four rows a block.
 template <class T, int DIM, int R, int UNIT, bool APART>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, T* __restrict__ out) {
     Segments<R, UNIT> segs(a);
-    const unsigned share = segs.share(), head = blockIdx.y;
-    // block.x counts tiles; the segment begins at unit `x` of its head
-    int tile = int(blockIdx.x), seq = -1;
-    unsigned x = 0, units = 0;
-    Sequence s{0, 0, 0};
-    for (unsigned before = 0;; segs.first += 64, segs.load()) {
-        if (segs.first >= a.batch) return;
-        const unsigned upto = sum_upto(segs.tiles);
-        const unsigned long long past = __ballot(upto > unsigned(tile));
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            auto get = [&](unsigned v) { return unsigned(__builtin_amdgcn_readlane(int(v), l)); };
-            seq = segs.first + l, units = get(segs.units);
-            tile -= int(get(upto) - get(segs.tiles));
-            x = before + get(segs.upto) - get(segs.tiles) * units + unsigned(tile) * units;
-            s = Sequence{int(get(unsigned(segs.s.q0))), int(get(unsigned(segs.s.chunk))), int(get(unsigned(segs.s.len)))};
-            break;
+    if (segs.total == 0) return;
+    const unsigned share = segs.share();
+    unsigned x, head;  // first unit of the segment in the line of all
+    typename Segments<R, UNIT>::Segment seg;
+    if constexpr (APART) {
+        head = blockIdx.y;
+        unsigned tile = blockIdx.x;
+        x = head * segs.total;
+        for (segs.first = 0;; segs.first += 64) {
+            if (segs.first >= a.batch) return;
+            segs.load(a.batch);
+            const unsigned upto = sum_upto(segs.tiles);
+            const unsigned long long past = __ballot(upto > tile);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                auto get = [&](unsigned v) { return unsigned(__builtin_amdgcn_readlane(int(v), l)); };
+                seg.units = get(segs.units);
+                tile -= get(upto) - get(segs.tiles);
+                x += get(segs.upto) - get(segs.tiles) * seg.units + tile * seg.units;
+                seg.tile = int(tile);
+                seg.s = Sequence{int(get(unsigned(segs.s.q0))), int(get(unsigned(segs.s.chunk))), int(get(unsigned(segs.s.len)))};
+                break;
+            }
+            tile -= of_last(upto), x += of_last(segs.upto);
         }
-        tile -= int(of_last(upto));
-        before += of_last(segs.upto);
+    } else {
+        x = (blockIdx.x + 1) * share;
+        if (x >= segs.total * unsigned(a.kv_heads)) return;
+        head = x / segs.total;
+        seg = segs.at(x - head * segs.total);
+        if (seg.unit == 0 || seg.tiles == 0) return;
+        x -= seg.unit;
     }
-    x += head * segs.total;
-    const unsigned b0 = x / share, b1 = (x + units - 1) / share;
-    if (b0 == b1 || b1 >= unsigned(a.blocks)) return;
+    const unsigned b0 = x / share, b1 = (x + seg.units - 1) / share;
+    if (b0 == b1 || b1 >= unsigned(a.blocks) || (!APART && b0 != blockIdx.x)) return;
     // the first piece is the second of its block's two, the others are the first of theirs
     const auto piece = [&](int i) { return a.partial + (2 * size_t(b0 + i) + (i == 0)) * kPiece<R, DIM>; };
     const int parts = int(b1 - b0) + 1;
-    if constexpr (APART) join_row<T, DIM, R, true>(a, out, s, tile, int(head), blockIdx.z, parts, piece);
-    else join_row<T, DIM, R, false>(a, out, s, tile, int(head), blockIdx.z * 4 + (threadIdx.x >> 6), parts, piece);
+    if constexpr (APART) join_row<T, DIM, R, true>(a, out, seg.s, seg.tile, int(head), blockIdx.z, parts, piece);
+    else join_row<T, DIM, R, false>(a, out, seg.s, seg.tile, int(head), blockIdx.z * 4 + (threadIdx.x >> 6), parts, piece);
 }
 
 template <class T, int BITS, int DIM, int QT>
@@ -531,7 +554,7 @@ void launch_rows(const AttnArgs& a, const T* q, T* out, int tiles, bool join, hi
     // few segments are in many pieces (one token of 131 072 keys, 64 pieces: 4.5 us, 6.3 as four rows a block), many in few
     constexpr int UNIT = 4 * rows_keys(BITS, DIM, QT);
     if (tiles * a.kv_heads <= 32) attn_join_kernel<T, DIM, 16 * QT, UNIT, true><<<dim3(tiles, a.kv_heads, 16 * QT), 256, 0, st>>>(a, out);
-    else attn_join_kernel<T, DIM, 16 * QT, UNIT, false><<<dim3(tiles, a.kv_heads, 4 * QT), 256, 0, st>>>(a, out);
+    else attn_join_kernel<T, DIM, 16 * QT, UNIT, false><<<dim3(a.blocks - 1, 1, 4 * QT), 256, 0, st>>>(a, out);
 }
 
 template <class T, int BITS>

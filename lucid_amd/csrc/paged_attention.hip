@@ -90,9 +90,10 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
         LQ_REQUIRE(int64_t(tiles) * c->kv_heads * (most / 128 + 1) < 0x7fffffff, LQ_ERR_NOT_IMPLEMENTED,
                    "paged_attention: %d tiles of queries for %lld keys of %d heads are more than one call takes", tiles, (long long)most, c->kv_heads);
         // Up to 512 keys a block has a whole segment: four steps of each wavefront, where joining pieces takes another launch (one token
-        // of 197 keys 10.3 -> 7.6 us).  Beyond, as many shares as blocks are resident.
-        const bool join = most > 512;
+        // of 197 keys 10.3 -> 7.6 us; 256 sequences of up to 500 keys, 2048 segments, 56 -> 47), unless segments are so many that each block's way to its
+        // own counts (2048 sequences, 16 384 segments, 801 -> 395 as shares).  Beyond, as many shares as blocks are resident.
         const int resident = (dim > 128 ? 1 : 2) * 256;
+        const bool join = most > 512 || int64_t(tiles) * c->kv_heads > 8 * resident;
         a.each = join ? resident : 0, a.least = 1;
         a.blocks = join ? resident : tiles * a.kv_heads;
         if (join) {

@@ -119,53 +119,75 @@ struct Segments {
     unsigned total;     // units of a head
     // 64 sequences, one a lane: units of their segments, tiles, units of one
     int first;          // the first of them
-    unsigned before;    // units of the sequences before it
     unsigned upto, tiles, units;
     Sequence s;
 
-    __device__ __forceinline__ explicit Segments(const AttnArgs& args) : a(args), lane(threadIdx.x & 63), total(0) {
-        for (first = 0; first < a.batch; first += 64) {
-            load();
-            total += of_last(upto);
+    // units up to the end of a lane's run of `run` sequences
+    int run;
+    unsigned run_upto;
+
+    __device__ __forceinline__ explicit Segments(const AttnArgs& args) : a(args), lane(threadIdx.x & 63) {
+        run = max(1, (a.batch + 63) / 64);
+        if (run == 1) {
+            first = 0, load(a.batch);
+            run_upto = upto;
+        } else {
+            unsigned sum = 0;
+#pragma unroll 4
+            for (int i = 0; i < run; ++i) {
+                const int b = lane * run + i;
+                Sequence x;
+                unsigned n, u;
+                look(a, min(b, a.batch - 1), x, n, u);
+                sum += b < a.batch ? n * u : 0u;
+            }
+            run_upto = sum_upto(sum);
         }
-        if (a.batch > 64) first = 0, load();
-        first = 0, before = 0;
+        total = of_last(run_upto);
     }
-    __device__ __forceinline__ void load() {
-        const int b = first + lane;
+    // a sequence of the batch, its tiles, and the units of each
+    static __device__ __forceinline__ void look(const AttnArgs& a, int b, Sequence& x, unsigned& n, unsigned& u) {
+        x = sequence_of(a, b);
+        const int rows = x.chunk * int(a.group.d);
+        n = rows < a.min_rows || rows > a.max_rows ? 0u : unsigned(rows + R - 1) / R;
+        const Keys k = keys_of(a, x, 0, x.chunk - 1);
+        u = a.each ? max(1u, unsigned(k.hi - (k.lo & ~31) + UNIT - 1) / UNIT) : 1u;
+    }
+    // 64 sequences from `first` on, those before `end`
+    __device__ __forceinline__ void load(int end) {
         s = Sequence{0, 0, 0}, tiles = 0, units = 1;
-        if (b < a.batch) {
-            s = sequence_of(a, b);
-            const int rows = s.chunk * int(a.group.d);
-            tiles = rows < a.min_rows || rows > a.max_rows ? 0u : unsigned(rows + R - 1) / R;
-            const Keys k = keys_of(a, s, 0, s.chunk - 1);
-            units = a.each ? max(1u, unsigned(k.hi - (k.lo & ~31) + UNIT - 1) / UNIT) : 1u;
-        }
+        if (first + lane < end) look(a, first + lane, s, tiles, units);
         upto = sum_upto(tiles * units);
     }
     struct Segment {
         int seq, tile;
         unsigned unit, units;  // the unit asked for, and how many there are
+        unsigned tiles;        // of the sequence
         Sequence s;
     };
-    // the segment of unit `x` < total of a head
+    // the segment of unit `x` < total of a head; no tiles: there is none (lengths that change meanwhile)
     __device__ __forceinline__ Segment at(unsigned x) {
-        if (x < before) first = 0, before = 0, load();
+        if (run > 1) {
+            const int l = __builtin_ctzll(__ballot(run_upto > x));
+            if (l) x -= unsigned(__builtin_amdgcn_readlane(int(run_upto), l - 1));
+            first = l * run, load(a.batch);
+        }
         while (true) {
-            const unsigned long long past = __ballot(upto > x - before);
+            const unsigned long long past = __ballot(upto > x);
             if (past) {
                 const int l = __builtin_ctzll(past);
                 auto get = [&](unsigned v) { return unsigned(__builtin_amdgcn_readlane(int(v), l)); };
                 Segment g;
-                g.seq = first + l, g.units = get(units);
-                const unsigned k = x - before - (get(upto) - get(tiles) * g.units);
+                g.seq = first + l, g.units = get(units), g.tiles = get(tiles);
+                const unsigned k = x - (get(upto) - g.tiles * g.units);
                 g.tile = int(g.units == 1 ? k : k / g.units), g.unit = k - unsigned(g.tile) * g.units;
                 g.s = Sequence{int(get(unsigned(s.q0))), int(get(unsigned(s.chunk))), int(get(unsigned(s.len)))};
                 return g;
             }
-            before += of_last(upto);
+            x -= of_last(upto);
             first += 64;
-            load();
+            if (first >= a.batch) return Segment{0, 0, 0, 1, 0, {0, 0, 0}};
+            load(a.batch);
         }
     }
     // units that each of a.each blocks takes

@@ -239,6 +239,16 @@ def test_long_chunks(case):
     b.check(b.run(causal=False, scale=-0.05), causal=False, scale=-0.05)
 
 
+@pytest.mark.parametrize("batch,longest,kv_heads,dtype", [(65, 40, 1, np.float32), (200, 900, 2, np.float16), (1100, 60, 4, np.float16),
+                                                          (1500, 700, 1, np.float32), (4300, 30, 1, np.float16)])
+def test_many_sequences_a_few_without_new_tokens(batch, longest, kv_heads, dtype):
+    rng = np.random.default_rng(batch)
+    chunks = rng.choice([0, 1, 1, 1, 3], batch)
+    b = Batch(list(chunks), list(rng.integers(1, longest + 1, batch)), kv_heads, kv_heads, 32, dtype=dtype, seed=1, tail=2)
+    b.check(b.run())
+    b.check(b.run(max_chunk=3, window=25), window=25)
+
+
 def test_a_prompt_whose_tiles_fill_the_device_is_its_halves():
     b = Batch([4096], [4096], 64, 16, 16, seed=7)
     whole = b.run().astype(np.float64)
