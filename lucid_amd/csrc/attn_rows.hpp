@@ -68,17 +68,26 @@ struct RowsKernel {
             segment(a, q, out, lds, seg, head, n, piece);
             x += n;
             if (x >= end) break;
-            // on to the next tile, sequence (one that has tiles: there are units left) or head
+            // on to the next tile, sequence (one that has tiles: there are units left) or head; behind eight sequences without, by a search
             seg.unit = 0;
             if (++seg.tile == int(seg.tiles)) {
                 seg.tile = 0;
-                do {
+                for (int empty = 0;; ++empty) {
+                    if (empty == 8) {
+                        Segs segs(a);
+                        if (segs.total == 0) return;
+                        head = int(x / segs.total);
+                        seg = segs.at(x - unsigned(head) * segs.total);
+                        if (seg.tiles == 0) return;
+                        break;
+                    }
                     if (++seg.seq == a.batch) {
                         if (++head == a.kv_heads) return;
                         seg.seq = 0;
                     }
                     Segs::look(a, seg.seq, seg.s, seg.tiles, seg.units);
-                } while (seg.tiles == 0);
+                    if (seg.tiles) break;
+                }
             }
             __syncthreads();
         }

@@ -247,6 +247,11 @@ def test_many_sequences_a_few_without_new_tokens(batch, longest, kv_heads, dtype
     b = Batch(list(chunks), list(rng.integers(1, longest + 1, batch)), kv_heads, kv_heads, 32, dtype=dtype, seed=1, tail=2)
     b.check(b.run())
     b.check(b.run(max_chunk=3, window=25), window=25)
+    # most of them idle
+    keep = (rng.random(batch) < 0.03).astype(int)
+    keep[batch // 2] = 2
+    b.q_starts = np.concatenate([[0], np.cumsum(keep)]).astype(np.int32)
+    b.check(b.run())
 
 
 def test_a_prompt_whose_tiles_fill_the_device_is_its_halves():
