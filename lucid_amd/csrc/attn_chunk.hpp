@@ -2,7 +2,7 @@
 //
 // Bound by the vector unit, by what it does for each score (an exponent, a maximum, an exponential, a sum, a scale, a rounding: some ten issue
 // slots beside four cycles of a matrix product) and for each code, and then by the matrix pipe: of 8192 tokens of 16 384 (32 heads
-// of 128 on 8, float16, 8 bits, 1910 us: 0.86 PFLOP/s of the 1.16 that a large library product reaches) the one is busy 50 % of
+// of 128 on 8, float16, 8 bits, 1885 to 2000 us: up to 0.87 PFLOP/s of the 1.16 that a large library product reaches) the one is busy 50 % of
 // the time, the other 37 %.  So a code is turned into float16 once for a block's 128 or 256 rows, on its way into LDS, and a wavefront has 32 rows, whose
 // accumulators, maxima and sums stay in its registers:
 //
