@@ -480,7 +480,7 @@ int lq_kv_cache_read(const lq_kv_cache* cache, const int32_t* slots, size_t toke
  * Queries that see no key, and rows of no sequence, give zeros.  Keys of a page that is negative or beyond the cache are not
  * seen; lengths beyond the table are cut to it.  Scores, sums and products are float32: codes enter the matrix products as the
  * whole numbers they are, scales after them; float16 queries as they are, float32 ones as two float16 of 22 bits together; probabilities as
- * two as well, of a float16 result's long chunks as one (half a step 2^-11, as the result's own rounding).  max_chunk: the
+ * two as well.  max_chunk: the
  * most queries of a sequence, or 0; the work is divided by it, and results differ by rounding alone. */
 int lq_paged_attention(const lq_kv_cache* cache, const void* q, size_t ldq, void* out, int dtype, int tokens, int heads, int batch,
                        const int32_t* page_table, int table_width, const int32_t* q_starts, const int32_t* kv_lens, float scale, int causal,

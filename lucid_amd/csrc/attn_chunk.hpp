@@ -34,7 +34,10 @@ __device__ __forceinline__ float halves(float v, F f) {
 template <class T, int BITS, bool AFFINE, int DIM, int WAVES>
 struct ChunkKernel {
     static constexpr bool F32 = std::is_same_v<T, float>;
-    static constexpr int PARTS = F32 ? 2 : 1;
+    static constexpr int PARTS = F32 ? 2 : 1;  // float16 parts of a query
+    // Probabilities are two float16 for float16 results as well: with one alone the error is 1.4 times that of the result's own rounding, and
+    // would depend on which kernel has a row.  (8192 of 16 384, float16, 1893 us with one, 2450 so: half as many products again.)
+    static constexpr int P_PARTS = 2;
     static constexpr int THREADS = 64 * WAVES, R = 32 * WAVES, KEYS = 64;
     static constexpr int SLABS = DIM / 16, TILES = DIM / 32;
     static constexpr int PIECES = DIM * BITS / 128;                                 // 16-byte pieces of a key's codes
@@ -306,7 +309,7 @@ struct ChunkKernel {
         // filled each other's gaps, within 1 %.
         f32x16 x;  // exponents: scores less the row's maximum so far
         f32x16 s;  // the next scores
-        Frag pf[2][PARTS];
+        Frag pf[2][P_PARTS];
         const auto scales_of = [&](const char* stage) { return reinterpret_cast<const float*>(stage + K_BYTES + V_BYTES); };
         // two keys' probabilities
         auto probabilities = [&](const char* stage, int half, int pair) {
@@ -318,7 +321,7 @@ struct ChunkKernel {
             const float p0 = mul_legacy(e0, vs.x), p1 = mul_legacy(e1, vs.y);
             const h2 y = to_h2(p0, p1);
             pf[b / 2][0].p[2 * (b % 2) + r] = y;
-            if constexpr (F32) pf[b / 2][1].p[2 * (b % 2) + r] = to_h2(p0 - float(y.x), p1 - float(y.y));
+            pf[b / 2][1].p[2 * (b % 2) + r] = to_h2(p0 - float(y.x), p1 - float(y.y));
         };
         // two keys' exponents
         auto exponents = [&](const char* stage, int half, int pair, float mm) {
@@ -351,15 +354,15 @@ struct ChunkKernel {
             }
         };
         auto products = [&](const char* stage, int half, auto meanwhile) {
-            constexpr int STEPS = 2 * TILES * PARTS;
+            constexpr int STEPS = 2 * TILES * P_PARTS;
             h8 v[AHEAD + 1];
             auto read = [&](int i) { v[i % (AHEAD + 1)] = *reinterpret_cast<const h8*>(stage + v_at(32 * (i % TILES) + n, 2 * (2 * half + i / TILES) + h)); };
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) read(i);
 #pragma unroll
             for (int x = 0; x < STEPS; ++x) {
-                const int i = x / PARTS, p = PARTS - 1 - x % PARTS;
-                if (p == PARTS - 1 && i + AHEAD < 2 * TILES) read(i + AHEAD);
+                const int i = x / P_PARTS, p = P_PARTS - 1 - x % P_PARTS;
+                if (p == P_PARTS - 1 && i + AHEAD < 2 * TILES) read(i + AHEAD);
                 o[i % TILES] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i % (AHEAD + 1)], pf[i / TILES][p].v, o[i % TILES], 0, 0, 0);
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 meanwhile(x, STEPS);

@@ -10,8 +10,7 @@
 //     o_d = sum_j (2^(S_j - m) v_scale_j) (c'_jd - z'_j) / sum_j 2^(S_j - m)
 // A product of a float16 and a code is exact in float32, and so is c - z.  float16 queries enter as they are, float32 ones as two float16
 // of 22 bits together (times a power of two for each row, so that neither part is subnormal where it counts).  Probabilities
-// times v_scale become two float16 as well, but one (half a step, 2^-11, as the result's own rounding) where a chunk of many rows has a
-// float16 result: its products would be half as many again.  Their sum is not rounded.  What makes that work whatever the scales is a power of two, `unit`, above the largest v_scale so
+// times v_scale become two float16 as well, for float16 results too (one alone makes the error 1.4 times that of the result's own rounding).  Their sum is not rounded.  What makes that work whatever the scales is a power of two, `unit`, above the largest v_scale so
 // far: 2^7 v_scale / unit times a probability of at most 2^8 fits float16, and outputs are kept in units of unit / 2^7.
 #pragma once
 #include "kv_cache.hpp"
