@@ -479,9 +479,9 @@ int lq_kv_cache_read(const lq_kv_cache* cache, const int32_t* slots, size_t toke
  *     out = sum_j softmax_j(scale * q . k_j) v_j
  * Queries that see no key, and rows of no sequence, give zeros.  Keys of a page that is negative or beyond the cache are not
  * seen; lengths beyond the table are cut to it.  Scores, sums and products are float32: codes enter the matrix products as the
- * whole numbers they are, scales after them; float16 queries as they are, float32 ones as two float16 of 22 bits together; probabilities as
- * two as well.  max_chunk: the
- * most queries of a sequence, or 0; the work is divided by it, and results differ by rounding alone. */
+ * whole numbers they are, scales after them; float16 queries as they are, float32 ones as two float16 of 22 bits together; probabilities times
+ * v_scale as two as well, against the largest that the row itself sees: keys that it does not see, or gives no weight, take none of
+ * its bits.  max_chunk: the most queries of a sequence, or 0; the work is divided by it, and results differ by rounding alone. */
 int lq_paged_attention(const lq_kv_cache* cache, const void* q, size_t ldq, void* out, int dtype, int tokens, int heads, int batch,
                        const int32_t* page_table, int table_width, const int32_t* q_starts, const int32_t* kv_lens, float scale, int causal,
                        int window, int max_chunk, lq_stream stream);

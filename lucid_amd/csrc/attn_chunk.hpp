@@ -169,9 +169,7 @@ struct ChunkKernel {
                 }
             }
         };
-        // outputs are kept in units of 2^unit, see the top of paged_attention.hpp; regrow: what those so far are to be multiplied by
-        int unit = -98;
-        float unit_value = 0x1p-98f, per_unit = 0x1p105f, regrow = 1.f;
+        Level level;  // of the keys that are settled
         // a negative scale changes the queries' signs, and of a scale of 0 all scores are 0, the masked ones still none.  What is left
         // goes with the keys' scales, with float32 queries, which have a factor for each row, with the scores
         const float key_factor = a.scale == 0.f ? 1.f : fabsf(a.scale * kLog2e);
@@ -197,21 +195,15 @@ struct ChunkKernel {
                 *reinterpret_cast<h8*>(stage + k_at(k, K_EIGHTS * piece + e)) = f.v;
                 return;
             }
-            // scales, and the unit (all wavefronts come to the same): above the largest of them by up to four times, and seldom renewed
-            float vs = vs_reg;
+            // scales (all wavefronts come to the same level)
+            float vs = vs_reg * (1.f / kValueUnit);
             if (AFFINE && !(fabsf(vzero) <= 2048.f)) vs = __builtin_nanf("");
-            if (!((key + lane >= seen.lo) & (key + lane < to) & (ok >> (lane >> 4) & 1))) vs = 0.f;
-            regrow = 1.f;
-            if (__ballot(fabsf(vs) > unit_value && unit < 126)) {
-                const float top = fminf(wave_max(fmaxf(0.f, fabsf(vs))), 0x1p124f);
-                const int next = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(top)) + 1;
-                regrow = __builtin_ldexpf(1.f, unit - next);
-                unit = next, unit_value = __builtin_ldexpf(1.f, next), per_unit = __builtin_ldexpf(kProbability, -next);
-            }
+            if (!((key + lane >= seen.lo) & (key + lane < to) & (ok >> (lane >> 4) & 1))) vs = level.hi;  // (its p is 0)
+            level.follow(fabsf(vs), fabsf(vs));
             // (every wavefront writes them: the same)
             float* to_lds = reinterpret_cast<float*>(stage + K_BYTES + V_BYTES);
             to_lds[lane] = F32 ? ks_reg : ks_reg * key_factor;
-            to_lds[KEYS + lane] = vs * per_unit;
+            to_lds[KEYS + lane] = vs;
         };
         constexpr int V_STEPS = VP * 8;
         Frag vf[4];
@@ -369,8 +361,8 @@ struct ChunkKernel {
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        // masks keys `at` .. `at` + 31, renews the maximum where it has grown by enough, and the outputs' unit
-        auto raise = [&](int at, int ok_at, float f) {
+        // masks keys `at` .. `at` + 31, renews the row's m where a w has grown by enough
+        auto raise = [&](const char* stage, int half, int at, int ok_at, Level level) {
             if (!(at >= all_lo && at + 32 <= all_hi && ok_at == 3)) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -383,22 +375,27 @@ struct ChunkKernel {
             for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]);
             // (a lane has half of the keys: only where one of the two has grown by enough do they ask each other)
             const bool first = m == -__builtin_inff();
-            if (__ballot(top > kLazy || (first && top > m))) {
-                top = halves(top, [](float u, float w) { return fmaxf(u, w); });
+            if (__ballot(top > kMost - level.at || (first && top > m)) || !level.even) {
+                top += level.at;  // a bound of log2 of the largest w
+                if (!level.even) {
+                    const float* vs = scales_of(stage) + KEYS + 32 * half + 4 * h;
+                    top = -__builtin_inff();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i] + float(level_of(vs[8 * (i / 4) + i % 4])));
+                }
+                top = halves(top, [](float u, float w) { return fmaxf(u, w); }) - kRenewed;
                 const float by = first ? top : fmaxf(top, 0.f);  // (-inf: no key seen yet)
                 if (by != -__builtin_inff()) {
-                    const float e = first ? 0.f : __builtin_amdgcn_exp2f(-by);
+                    const float f = first ? 0.f : __builtin_amdgcn_exp2f(-0.5f * by);  // (its square may be too small where l is large)
                     m = first ? by : m + by;
-                    l *= e, l1 *= e, f *= e;
+                    l = l * f * f, l1 = l1 * f * f;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) x[i] -= by;
+#pragma unroll
+                    for (int d = 0; d < TILES; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[d][i] *= f * f;
                 }
-            }
-            if (__ballot(f != 1.f)) {
-#pragma unroll
-                for (int d = 0; d < TILES; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[d][i] *= f;
             }
         };
         auto exponent_offset = [&] { return m == -__builtin_inff() ? 0.f : -m; };
@@ -409,6 +406,7 @@ struct ChunkKernel {
 #pragma unroll
             for (int i = 0; i < V_STEPS; ++i) settle_v(i, lds);
             int ok_now = ok;
+            Level level_now = level;
             locate(from + KEYS, pages);
             pages = pages_of(from + 2 * KEYS);
             request_k(), request_v();
@@ -416,7 +414,7 @@ struct ChunkKernel {
             scores(lds, 0, [](int, int) {});
 #pragma unroll
             for (int i = 0; i < 8; ++i) exponents(lds, 0, i, 0.f);
-            raise(from, ok_now & 3, regrow);
+            raise(lds, 0, from, ok_now & 3, level_now);
             int side = 0;
             for (int key = from;; key += KEYS) {
                 char* const now = lds + side * STAGE;
@@ -431,7 +429,7 @@ struct ChunkKernel {
                 locate(key + 2 * KEYS, pages);
                 pages = pages_of(key + 3 * KEYS);
                 request_k();
-                raise(key + 32, ok_now >> 2, 1.f);
+                raise(now, 1, key + 32, ok_now >> 2, level_now);
                 __syncthreads();
                 // (behind the last keys: the scores of what lies there, which nobody takes)
                 scores(next, 0, [&](int step, int steps) { deal(8, step, steps, [&](int i) { probabilities(now, 1, i); }); });
@@ -442,9 +440,9 @@ struct ChunkKernel {
                 });
                 if (key + KEYS >= to) break;
                 request_v();
-                raise(key + KEYS, ok_next & 3, regrow);
+                raise(next, 0, key + KEYS, ok_next & 3, level);
                 __syncthreads();
-                ok_now = ok_next;
+                ok_now = ok_next, level_now = level;
                 side ^= 1;
             }
             l += l1;
@@ -452,7 +450,7 @@ struct ChunkKernel {
         l = halves(l, [](float x, float y) { return x + y; });
         const int row = row0 + 32 * wave + n;
         if (row > last_row) return;
-        const float scale = __builtin_ldexpf(1.f / kProbability, unit) * (it.parts == 1 ? (l == 0.f ? 0.f : 1.f / l) : 1.f);
+        const float scale = kValueUnit * (it.parts == 1 ? (l == 0.f ? 0.f : 1.f / l) : 1.f);
         if (it.parts > 1) {
             if (it.first + it.parts > a.pieces) return;
             float* piece = a.partial + (size_t(it.first + it.part) * a.kv_heads + head) * kPiece<R, DIM>;

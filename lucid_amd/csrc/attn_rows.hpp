@@ -269,8 +269,8 @@ struct RowsKernel {
         if constexpr (Q_LDS) __syncthreads();
 
         f32x4 o[QT][TILES] = {};
-        float m[QT], l[QT], unit_value = 0x1p-98f, per_unit = 0x1p105f;
-        int unit = -98;
+        float m[QT], l[QT];
+        Level level;
 #pragma unroll
         for (int t = 0; t < QT; ++t) m[t] = -__builtin_inff(), l[t] = 0.f;
 
@@ -313,7 +313,7 @@ struct RowsKernel {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) vs[t][r] = vs4[t][r];
+                for (int r = 0; r < 4; ++r) vs[t][r] = vs4[t][r] * (1.f / kValueUnit);
             // what no row sees may be anything; and a zero point that is no number reaches every row through the matrix product: the scale
             // has it for those that see it
             if (!whole) {
@@ -324,28 +324,15 @@ struct RowsKernel {
                         const int j = key + 16 * t + 4 * g + r;
                         if constexpr (AFFINE)
                             if (!(fabsf(vz[t][r]) <= 2048.f)) vs[t][r] = __builtin_nanf(""), vz[t][r] = 0.f;
-                        if (!((j >= seen.lo) & (j < to) & (ok_now >> t & 1))) vs[t][r] = 0.f;
+                        if (!((j >= seen.lo) & (j < to) & (ok_now >> t & 1))) vs[t][r] = level.hi;  // (its p is 0)
                     }
             }
-            // the unit of the outputs: a power of two, renewed to up to four times the largest scale, and seldom
-            float vtop = 0.f;
+            float least = __builtin_inff(), most = 0.f;
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) vtop = fmaxf(vtop, fabsf(vs[t][r]));
-            if (__ballot(vtop > unit_value && unit < 126)) {
-                const int next = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(fminf(rows4_max(vtop), 0x1p124f))) + 1;
-                const float f = __builtin_ldexpf(1.f, unit - next);
-#pragma unroll
-                for (int x = 0; x < QT; ++x)
-#pragma unroll
-                    for (int j = 0; j < TILES; ++j) o[x][j] *= f;
-                unit = next, unit_value = __builtin_ldexpf(1.f, next), per_unit = __builtin_ldexpf(kProbability, -next);
-            }
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) vs[t][r] *= per_unit;
+                for (int r = 0; r < 4; ++r) least = fminf(least, fabsf(vs[t][r])), most = fmaxf(most, fabsf(vs[t][r]));
+            level.follow(least, most);
             Frag pf[QT][NT / 2][P_PARTS];
 #pragma unroll
             for (int x = 0; x < QT; ++x) {
@@ -373,15 +360,23 @@ struct RowsKernel {
                     for (int r = 0; r < 4; ++r) top = fmaxf(top, e[t][r]);
                 // (a lane has a quarter of the keys: only where one of them has grown by enough do the four ask each other)
                 const bool first = m[x] == -__builtin_inff();
-                if (__ballot(top > kLazy || (first && top > m[x]))) {
-                    top = rows4_max(top);
+                if (__ballot(top > kMost - level.at || (first && top > m[x])) || !level.even) {
+                    top += level.at;  // a bound of log2 of the largest w
+                    if (!level.even) {
+                        top = -__builtin_inff();
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) top = fmaxf(top, e[t][r] + float(level_of(vs[t][r])));
+                    }
+                    top = rows4_max(top) - kRenewed;
                     const float by = first ? top : fmaxf(top, 0.f);  // (-inf: no key seen yet)
                     if (by != -__builtin_inff()) {
-                        const float f = first ? 0.f : __builtin_amdgcn_exp2f(-by);
+                        const float f = first ? 0.f : __builtin_amdgcn_exp2f(-0.5f * by);  // (its square may be too small where l is large)
                         m[x] = first ? by : m[x] + by;
-                        l[x] *= f;
+                        l[x] = l[x] * f * f;
 #pragma unroll
-                        for (int j = 0; j < TILES; ++j) o[x][j] *= f;
+                        for (int j = 0; j < TILES; ++j) o[x][j] *= f * f;
 #pragma unroll
                         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -450,13 +445,12 @@ struct RowsKernel {
         }
 
         // The wavefronts' results meet in LDS, ROWS rows at a time, and every thread adds up some columns of them.
-        __shared__ float s_m[WAVES][R], s_l[WAVES][R], s_unit[WAVES];
+        __shared__ float s_m[WAVES][R], s_l[WAVES][R];
 #pragma unroll
         for (int x = 0; x < QT; ++x) {
             l[x] = rows4_sum(l[x]);
             if (g == 0) s_m[wave][16 * x + c] = m[x], s_l[wave][16 * x + c] = l[x];
         }
-        if (lane == 0) s_unit[wave] = __builtin_ldexpf(1.f / kProbability, unit);
 #pragma unroll
         for (int x = 0; x < QT; ++x)
 #pragma unroll
@@ -481,10 +475,11 @@ struct RowsKernel {
                     float total = 0.f;
 #pragma unroll
                     for (int w = 0; w < WAVES; ++w) {
-                        const float f = __builtin_amdgcn_exp2f(s_m[w][row] - mm);
-                        v += *reinterpret_cast<const f32x4*>(lds + (w * ROWS + r) * LDS_ROW + d) * (f * s_unit[w]);
-                        total += s_l[w][row] * f;
+                        const float f = __builtin_amdgcn_exp2f(0.5f * (s_m[w][row] - mm));  // (as above)
+                        v += *reinterpret_cast<const f32x4*>(lds + (w * ROWS + r) * LDS_ROW + d) * (f * f);
+                        total += s_l[w][row] * f * f;
                     }
+                    v *= kValueUnit;
                     if (piece) {
                         if (d == 0) piece[R * DIM + row] = top, piece[R * DIM + R + row] = total;
                         *reinterpret_cast<f32x4*>(piece + row * DIM + d) = v;

@@ -7,11 +7,13 @@
 // The mathematics.  Codes are whole numbers below 2^8, which float16 holds exactly, so that the matrix instruction gets them as they
 // are and the scales follow in float32:
 //     S_j = (scale log2 e) k_scale_j sum_d q_d (c_jd - z_j)
-//     o_d = sum_j (2^(S_j - m) v_scale_j) (c'_jd - z'_j) / sum_j 2^(S_j - m)
+//     o_d = sum_j w_j (c'_jd - z'_j) / sum_j p_j,   p_j = 2^(S_j - m), w_j = p_j v_scale_j
 // A product of a float16 and a code is exact in float32, and so is c - z.  float16 queries enter as they are, float32 ones as two float16
-// of 22 bits together (times a power of two for each row, so that neither part is subnormal where it counts).  Probabilities
-// times v_scale become two float16 as well, for float16 results too (one alone makes the error 1.4 times that of the result's own rounding).  Their sum is not rounded.  What makes that work whatever the scales is a power of two, `unit`, above the largest v_scale so
-// far: 2^7 v_scale / unit times a probability of at most 2^8 fits float16, and outputs are kept in units of unit / 2^7.
+// of 22 bits together (times a power of two for each row, so that neither part is subnormal where it counts).  So do the w_j, for float16
+// results too (one float16 alone makes the error 1.4 times that of the result's own rounding).  The sums of the p_j are not rounded.
+// What keeps a w_j's 22 bits whatever the scales is that a row's m goes by the keys that the row itself has seen, and by their w_j: it is
+// renewed where one may pass 2^15, so that it is 2^7 then, and two float16 hold a number to 2^-25 of 1.  Mostly the scales of the keys of a step
+// are within 2^8 of each other; then the exponents' maximum and one `Level` for all of them bound the w_j.  In other steps each key's scale counts.
 #pragma once
 #include "kv_cache.hpp"
 #include "wave_reduce.hpp"
@@ -45,8 +47,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 namespace attn {
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kLazy = 8.f;        // a row's maximum is renewed when it has grown by this (powers of two)
-constexpr float kProbability = 0x1p7f;  // probabilities are kept times this
+constexpr float kMost = 15.f, kRenewed = 7.f;  // log2 of the largest p v_scale of a row that is let be, and of what it becomes otherwise
+constexpr float kValueUnit = 0x1p16f;          // v_scale is kept in this, so that p is no subnormal beside the largest ones
 
 __device__ __forceinline__ h2 as_h2(uint32_t v) { return __builtin_bit_cast(h2, v); }
 __device__ __forceinline__ uint32_t as_u32(h2 v) { return __builtin_bit_cast(uint32_t, v); }
@@ -83,6 +85,23 @@ __device__ __forceinline__ float rows4_max(float v) {
 __device__ __forceinline__ float rows4_sum(float v) {
     return rows4(v, [](float a, float b) { return a + b; });
 }
+
+// |scale| is below 2^level_of(scale) and at least half of it (but for infinity; NaN and what is too small to bound p by count as 2^-84)
+__device__ __forceinline__ int level_of(float scale) { return __builtin_amdgcn_frexp_expf(fminf(fmaxf(fabsf(scale), 0x1p-84f), 0x1p112f)); }
+// What bounds the values' scales of a step's keys.
+struct Level {
+    float at = -16.f;    // all of them are at most 2^at = hi
+    bool even = true;    // and above lo = 2^(at - 8); if not, each key's own counts
+    float hi = 0x1p-16f, lo = 0x1p-24f;
+    // a lane has some of them, from `least` to `most`
+    __device__ __forceinline__ void follow(float least, float most) {
+        even = true;
+        if (!__ballot(!(most <= hi && least > lo))) return;
+        const int level = __builtin_amdgcn_readfirstlane(level_of(wave_max(fmaxf(most, 0.f)))) + 1;  // (room for what grows a little)
+        at = float(level), hi = __builtin_ldexpf(1.f, level), lo = __builtin_ldexpf(1.f, level - 8);
+        even = !__ballot(!(most <= hi && least > lo));
+    }
+};
 
 struct Sequence {
     int q0, chunk, len;  // first row of q, new tokens, keys
@@ -309,8 +328,8 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, T* out, const Sequen
 #pragma unroll
         for (int u = 0; u < DEEP; ++u) {
             if (i0 + u * EVERY + mine >= n) continue;
-            const float f = __builtin_amdgcn_exp2f(m[u] - mm);
-            total += l[u] * f, v += y[u] * f;
+            const float f = __builtin_amdgcn_exp2f(0.5f * (m[u] - mm));  // (its square may be too small where l is large)
+            total += l[u] * f * f, v += y[u] * f * f;
         }
         i0 += DEEP * EVERY;
         if (i0 >= n) break;

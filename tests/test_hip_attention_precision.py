@@ -3,7 +3,8 @@
 import numpy as np
 import pytest
 
-from test_hip_paged_attention import Batch
+import oracle.kv_cache as K
+from test_hip_paged_attention import GRID, LONG, Batch
 
 pytestmark = pytest.mark.gpu
 
@@ -23,3 +24,119 @@ def test_a_float16_result_is_off_by_its_own_rounding(bits, symmetric, dim, chunk
     want, got = b.want(), b.run(max_chunk=max_chunk)
     rounding = rms(want.astype(np.float16).astype(np.float64) - want)
     assert rms(got - want) <= 1.05 * rounding + 2.0 ** -18 * rms(want), (rms(got - want), rounding)
+
+
+def bounds(b, scale=None, causal=True, window=None):
+    """The float64 result and how far each element may be off, from what its own row sees.
+
+    u = 2^-24.  A row's scores: sums of dim products whose partial sums stay below a = scale sum |q k| (the largest of the seen keys), as
+    independent errors 4 sqrt(dim) u a at four deviations; float32 queries are two float16 of 22 bits, 2 u a; scale, maximum and exponential
+    round 8 units of 1 + a.  With e for all of that, probabilities off by a factor 1 + e move column d by e (sum_j p_j |v_jd| + |o_d|).  A
+    weight p_j v_scale_j is held to u of the row's largest one, its product with a code (of which a row has one of half the range at least)
+    adds u times twice that to each of n terms, as does their sum: 4 sqrt(n) + 8 units of 2 max_j p_j max_d |v_jd|.  A float16 result is rounded
+    by 2^-11 of itself, or 2^-25."""
+    scale, u = 1 / np.sqrt(b.dim) if scale is None else scale, 2.0 ** -24
+    q, group, page = b.q.astype(np.float64), b.heads // b.kv_heads, b.cache.page_size
+    want, tol = np.zeros(q.shape), np.zeros(q.shape)
+    for s in range(len(b.kv_lens)):
+        lo, hi, length = int(b.q_starts[s]), int(b.q_starts[s + 1]), int(b.kv_lens[s])
+        j = np.arange(length)
+        k, v = (b.pages[n][b.table[s][j // page], :, j % page].astype(np.float64) for n in "kv")
+        place = length - (hi - lo) + np.arange(hi - lo)[:, None]
+        seen = (j <= place) if causal else np.ones((hi - lo, length), bool)
+        if window is not None:
+            seen = seen & (j > place - window)
+        some = seen.any(1)
+        for h in range(b.heads if length and hi > lo else 0):
+            kh, vh = k[:, h // group], v[:, h // group]
+            with np.errstate(all="ignore"):
+                sc = np.where(seen, q[lo:hi, h] @ kh.T * scale, -np.inf)
+                a = np.where(seen, np.abs(q[lo:hi, h]) @ np.abs(kh).T * abs(scale), 0).max(1, keepdims=True)
+                p = np.exp(sc - sc.max(1, keepdims=True))
+                p = np.where(some[:, None], p / p.sum(1, keepdims=True), 0)
+            held = seen.any(0)  # (what nobody sees may be anything)
+            p, vh = p[:, held], vh[held]
+            o = p @ vh
+            e = u * (4 * np.sqrt(b.dim) * a + 2 * a + 8 * (1 + a))
+            n = seen.sum(1, keepdims=True)
+            t = e * (p @ np.abs(vh) + np.abs(o)) + u * (4 * np.sqrt(n) + 8) * 2 * (p * np.abs(vh).max(1)).max(1, keepdims=True, initial=0)
+            if b.dtype == np.float16:
+                t = t + 2.0 ** -11 * np.abs(o) + 2.0 ** -25
+            want[lo:hi, h], tol[lo:hi, h] = o, t
+    return want, tol
+
+
+def held(b, got, **kw):
+    want, tol = bounds(b, **kw)
+    assert got.shape == want.shape and got.dtype == b.dtype and np.isfinite(got).all()
+    off = np.abs(got - want)
+    worst = np.unravel_index(np.argmax(off - tol), off.shape)
+    assert (off <= tol).all(), (worst, got[worst], want[worst], tol[worst])
+
+
+def scaled(b, factor):
+    """The batch's values, those of token j of sequence s times factor(s, j, head), a power of two."""
+    u = K.unpack(b.cache.v_codes.numpy(), b.bits)
+    scale = b.cache.v_scale.numpy().copy()
+    zero = None if b.symmetric else b.cache.v_zero.numpy()
+    for s, length in enumerate(b.kv_lens):
+        for j in range(length):
+            at = (b.table[s, j // b.cache.page_size], slice(None), j % b.cache.page_size)
+            scale[at] *= factor(s, j)
+    b.put("v", u, scale.astype(np.float32), zero)
+
+
+SIZES = [([1, 3], [300, 700]), ([16, 5], [333, 40]), ([90], [700]), ([150, 100], [200, 900]), ([300], [1300])]
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("chunks,lengths", SIZES)
+def test_a_row_does_not_feel_values_that_it_does_not_see(chunks, lengths, dtype):
+    """The last token of each chunk has values 2^12 to 2^30 times the others': causality keeps them from the rows before it.  A key that has
+    left the window of all but the first row, likewise."""
+    for r in (12, 16) if dtype == np.float16 else (12, 17, 22, 30):
+        for bits, symmetric in ((8, True), (4, False)):
+            b = Batch(chunks, lengths, 4, 2, 64, bits=bits, symmetric=symmetric, dtype=dtype, seed=r)
+            scaled(b, lambda s, j: 2.0 ** (r * (j == lengths[s] - 1) - 4))
+            held(b, b.run())
+            b = Batch(chunks, lengths, 4, 2, 64, bits=bits, symmetric=symmetric, dtype=dtype, seed=r)
+            scaled(b, lambda s, j: 2.0 ** (r * (j == lengths[s] - chunks[s] - 19) - 4))  # the first key of the first row's window of 20
+            held(b, b.run(window=20), window=20)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("chunks,lengths", SIZES)
+def test_an_infinite_scale_is_felt_by_those_that_see_it_alone(chunks, lengths, dtype):
+    b = Batch(chunks, lengths, 4, 2, 64, dtype=dtype, seed=3)
+    scale = b.cache.v_scale.numpy().copy()
+    for s, n in enumerate(lengths):
+        scale[b.table[s, (n - 1) // 16], :, (n - 1) % 16] = np.inf
+    want, tol = bounds(b)
+    b.cache.v_scale.copy_from(scale)
+    got = b.run()
+    last = b.q_starts[1:] - 1
+    assert not np.isfinite(got[last]).all(-1).any()
+    others = np.setdiff1d(np.arange(len(got)), last)
+    assert (np.abs(got - want) <= tol)[others].all()
+
+
+@pytest.mark.parametrize("chunks,lengths", SIZES)
+def test_weights_of_all_sizes_keep_their_bits(chunks, lengths):
+    """Scales that differ from key to key, from page to page, grow, fall, or are zero here and there; so far apart that their ratio is beyond
+    a float32's exponents."""
+    rng = np.random.default_rng(len(chunks) + chunks[0])
+    jumble = rng.integers(-30, 31, (2, 2000))
+    for factor in (lambda s, j: 2.0 ** jumble[s, j], lambda s, j: 2.0 ** jumble[s, j // 16], lambda s, j: 2.0 ** (j // 16 % 60 - 30), lambda s, j: 2.0 ** (30 - j // 16 % 60),
+                   lambda s, j: 2.0 ** (j % 64 // 8), lambda s, j: float(jumble[s, j] % 3 > 0), lambda s, j: 2.0 ** (-40 if j % 300 else 85),
+                   lambda s, j: 2.0 ** (85 if j < 40 else -40), lambda s, j: 2.0 ** (100 if j == 7 else -12)):
+        b = Batch(chunks, lengths, 4, 2, 64, dtype=np.float32, seed=5)
+        scaled(b, factor)
+        held(b, b.run())
+        held(b, b.run(scale=1.0, window=100), scale=1.0, window=100)
+
+
+@pytest.mark.parametrize("case", range(len(GRID + LONG)))
+def test_each_row_against_what_it_sees(case):
+    b = Batch(*(GRID + LONG)[case], seed=case, tail=2)
+    held(b, b.run())
+    held(b, b.run(causal=False, window=70), causal=False, window=70)
