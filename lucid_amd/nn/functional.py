@@ -167,6 +167,8 @@ def paged_attention_qkv(qkv: Tensor, num_heads: int, cache, page_table: Tensor, 
     ``(..., num_heads * head_dim)``."""
     _check_cache("paged_attention_qkv", cache)
     num_heads = int(num_heads)
+    if num_heads < 1 or num_heads % cache.kv_heads:
+        raise _C.ShapeMismatch(f"paged_attention_qkv: {num_heads} query heads for {cache.kv_heads} key / value heads")
     row = (num_heads + 2 * cache.kv_heads) * cache.head_dim
     if not isinstance(qkv, Tensor) or qkv.ndim < 2 or qkv.shape[-1] != row:
         raise _C.ShapeMismatch(f"paged_attention_qkv: qkv has rows of {num_heads} + 2 * {cache.kv_heads} heads of {cache.head_dim}, {row} values")

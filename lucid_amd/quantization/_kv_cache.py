@@ -129,13 +129,16 @@ def kv_cache_write_qkv(cache: PagedKVCache, qkv: Tensor, num_heads: int, slots: 
     """``kv_cache_write`` of the keys and values in the packed output of a qkv Linear: ``qkv`` is
     ``(..., (num_heads + 2 * kv_heads) * head_dim)``, queries first, then keys, then values; ``slots`` has an entry per row."""
     _check_cache("kv_cache_write_qkv", cache)
-    row = (int(num_heads) + 2 * cache.kv_heads) * cache.head_dim
+    num_heads = int(num_heads)
+    if num_heads < 0:  # (the keys would begin before the row)
+        raise _C.ShapeMismatch(f"kv_cache_write_qkv: {num_heads} query heads")
+    row = (num_heads + 2 * cache.kv_heads) * cache.head_dim
     if not isinstance(qkv, Tensor) or qkv.ndim < 2 or qkv.shape[-1] != row:
         raise _C.ShapeMismatch(f"kv_cache_write_qkv: qkv has rows of {num_heads} + 2 * {cache.kv_heads} heads of {cache.head_dim}, {row} values")
     _check_rows("kv_cache_write_qkv", "qkv", qkv, qkv.shape)
     tokens = qkv.numel // row
     _check_ids("kv_cache_write_qkv", "slots", slots, (tokens,))
-    k = qkv.data_ptr + int(num_heads) * cache.head_dim * qkv.dtype.itemsize
+    k = qkv.data_ptr + num_heads * cache.head_dim * qkv.dtype.itemsize
     v = k + cache.kv_heads * cache.head_dim * qkv.dtype.itemsize
     _C.call("lq_kv_cache_write", cache._ref, k, v, qkv.dtype.code, row, row, slots.data_ptr, tokens, None)
 

@@ -91,3 +91,29 @@ def test_operators_want_a_cache():
               lambda: F.paged_attention(x, None, x, x, x), lambda: F.paged_attention_qkv(x, 2, "cache", x, x, x)):
         with pytest.raises(TypeError, match="PagedKVCache"):
             f()
+
+
+def bare_cache(kv_heads=2, head_dim=64):
+    """A cache whose buffers do not exist: for checks that come before anything is read."""
+    c = object.__new__(Q.PagedKVCache)
+    s = struct(kv_heads=kv_heads, head_dim=head_dim)
+    values = dict(num_pages=4, page_size=16, kv_heads=kv_heads, head_dim=head_dim, qscheme=Q.per_channel_symmetric, qdtype=Q.qint8, _struct=s, _ref=C.byref(s))
+    for n, v in values.items():
+        object.__setattr__(c, n, v)
+    return c
+
+
+@pytest.mark.parametrize("num_heads,width", [(-1, 3 * 64), (-3, 64), (-4, 0), (-(1 << 40), 64)])
+def test_packed_rows_of_fewer_than_no_queries_are_refused(num_heads, width):
+    """Keys of (num_heads + 2 kv_heads) heads a row lie num_heads heads from its start: with num_heads = -1, before the buffer."""
+    x, s = L.tensor(np.zeros((2, width), np.float32)), L.tensor(np.zeros(2, np.int32))
+    with pytest.raises(L.ShapeMismatch, match="kv_cache_write_qkv.*query heads"):
+        Q.kv_cache_write_qkv(bare_cache(), x, num_heads, s)
+    with pytest.raises(L.ShapeMismatch, match="paged_attention_qkv.*query heads"):
+        F.paged_attention_qkv(x, num_heads, bare_cache(), s, s, s)
+
+
+def test_packed_attention_without_queries_is_refused_before_it_asks_for_memory():
+    x, s = L.tensor(np.zeros((2, 256), np.float32)), L.tensor(np.zeros(2, np.int32))
+    with pytest.raises(L.ShapeMismatch, match="paged_attention_qkv.*query heads"):
+        F.paged_attention_qkv(x, 0, bare_cache(), s, s, s)
