@@ -26,7 +26,8 @@ class PagedKVCache:
     ``k_codes`` / ``v_codes`` are bytes (int8-tagged) ``(num_pages, kv_heads, page_size, head_dim * bits // 8)`` that hold
     code - quant_min, two 4-bit codes in a byte, the first in the low half; ``k_scale``, ``v_scale``, ``k_zero``, ``v_zero`` are
     float32 ``(num_pages, kv_heads, page_size)``, the last two ``None`` for a symmetric cache.  A row stands for
-    ``(code - zero) * scale``.  All buffers begin as zeros: a slot that was never written stands for zeros."""
+    ``(code - zero) * scale``.  All buffers begin as zeros: a slot that was never written stands for zeros.  They belong to
+    the cache: their contents may be written, the attributes are read-only."""
 
     __slots__ = ("num_pages", "page_size", "kv_heads", "head_dim", "qscheme", "qdtype", "k_codes", "v_codes", "k_scale", "v_scale",
                  "k_zero", "v_zero", "_struct", "_ref")
@@ -37,8 +38,8 @@ class PagedKVCache:
             raise NotImplementedError(f"PagedKVCache: qint8 and qint4 are built, got {qdtype!r}")
         if not isinstance(qscheme, QScheme) or not qscheme.is_per_channel:
             raise ValueError(f"PagedKVCache: every row has its own scale; qscheme is per_channel_symmetric or per_channel_affine, got {qscheme}")
-        self.num_pages, self.page_size, self.kv_heads, self.head_dim = int(num_pages), int(page_size), int(kv_heads), int(head_dim)
-        self.qscheme, self.qdtype = qscheme, qdtype
+        keep = lambda **kw: [object.__setattr__(self, n, v) for n, v in kw.items()]
+        keep(num_pages=int(num_pages), page_size=int(page_size), kv_heads=int(kv_heads), head_dim=int(head_dim), qscheme=qscheme, qdtype=qdtype)
         step = 128 // qdtype.bits
         if self.num_pages < 1 or not 1 <= self.kv_heads <= 65535 or self.page_size < 16 or self.page_size % 16:
             raise _C.ShapeMismatch(f"PagedKVCache: {num_pages} pages of {page_size} tokens with {kv_heads} heads (pages are multiples of 16)")
@@ -53,13 +54,20 @@ class PagedKVCache:
             _C.call("lq_fill_bytes", t.data_ptr, 0, t.nbytes, None)
             return t
 
-        self.k_codes, self.v_codes = (zeros((*rows, self.head_dim * qdtype.bits // 8), T.int8) for _ in range(2))
-        self.k_scale, self.v_scale = (zeros(rows, T.float32) for _ in range(2))
-        self.k_zero, self.v_zero = (None, None) if qscheme.is_symmetric else (zeros(rows, T.float32) for _ in range(2))
-        pointers = [t.data_ptr if t is not None else None
-                    for t in (self.k_codes, self.v_codes, self.k_scale, self.v_scale, self.k_zero, self.v_zero)]
-        self._struct = _C.KvCache(*pointers, self.num_pages, self.page_size, self.kv_heads, self.head_dim, qdtype.bits)
-        self._ref = C.byref(self._struct)
+        codes = [zeros((*rows, self.head_dim * qdtype.bits // 8), T.int8) for _ in range(2)]
+        scales = [zeros(rows, T.float32) for _ in range(2)]
+        zero_points = [None, None] if qscheme.is_symmetric else [zeros(rows, T.float32) for _ in range(2)]
+        pointers = [t.data_ptr if t is not None else None for t in codes + scales + zero_points]
+        struct = _C.KvCache(*pointers, self.num_pages, self.page_size, self.kv_heads, self.head_dim, qdtype.bits)
+        keep(k_codes=codes[0], v_codes=codes[1], k_scale=scales[0], v_scale=scales[1], k_zero=zero_points[0], v_zero=zero_points[1], _struct=struct,
+             _ref=C.byref(struct))
+
+    # The calls go by the addresses and sizes in _struct, for as long as the cache lives.
+    def __setattr__(self, name, value):
+        raise AttributeError(f"PagedKVCache: {name} is read-only (write into the buffers, or make another cache)")
+
+    def __delattr__(self, name):
+        raise AttributeError(f"PagedKVCache: {name} is read-only")
 
     @property
     def num_slots(self) -> int:

@@ -117,3 +117,14 @@ def test_packed_attention_without_queries_is_refused_before_it_asks_for_memory()
     x, s = L.tensor(np.zeros((2, 256), np.float32)), L.tensor(np.zeros(2, np.int32))
     with pytest.raises(L.ShapeMismatch, match="paged_attention_qkv.*query heads"):
         F.paged_attention_qkv(x, 0, bare_cache(), s, s, s)
+
+
+@pytest.mark.parametrize("name", ["num_pages", "page_size", "kv_heads", "head_dim", "qscheme", "qdtype", "k_codes", "v_scale", "k_zero", "_struct"])
+def test_a_cache_keeps_the_buffers_that_its_calls_write_to(name):
+    """The calls go by the addresses and sizes of the construction: another buffer in a buffer's place would free memory that they still write to."""
+    c = bare_cache()
+    with pytest.raises(AttributeError, match=name):
+        setattr(c, name, None)
+    with pytest.raises(AttributeError, match=name):
+        delattr(c, name)
+    assert c.num_slots == 64 and c.kv_heads == 2
