@@ -11,7 +11,7 @@ import math
 from .. import _C
 from .. import _tensor as T
 from .._tensor import Tensor
-from ..quantization._kv_cache import _check_cache, _check_ids, _check_rows
+from ..quantization._kv_cache import _check_cache, _check_ids, _check_rows, _written
 
 
 def _require_f32_hip(name: str, *ts: Tensor) -> None:
@@ -157,6 +157,7 @@ def paged_attention(q: Tensor, cache, page_table: Tensor, q_starts: Tensor, kv_l
             raise _C.DtypeMismatch(f"paged_attention: q is {q.dtype}, out {out.dtype}")
     _paged_attention("paged_attention", cache, q.data_ptr, heads * cache.head_dim, q.dtype, tokens, heads, out, page_table, q_starts, kv_lens, scale,
                      causal, window, max_chunk)
+    _written(out)
     return out
 
 

@@ -116,6 +116,11 @@ def _check_rows(name: str, what: str, t, shape) -> None:
         raise _C.ShapeMismatch(f"{name}: {what} has shape {t.shape}, expected {shape}")
 
 
+def _written(t: Tensor) -> None:
+    """A call has written `t`: what told of the values before (codes on a grid, a kept range) goes."""
+    t._grid = t._range = None
+
+
 def kv_cache_write(cache: PagedKVCache, k: Tensor, v: Tensor, slots: Tensor) -> None:
     """Quantizes keys and values ``(tokens, kv_heads, head_dim)`` (float32 or float16) into the slots ``slots`` (int32
     ``(tokens,)``).  A slot that is negative or beyond the cache is skipped: what pads a batch.  The others are distinct; of
@@ -171,4 +176,5 @@ def kv_cache_read(cache: PagedKVCache, slots: Tensor, dtype=T.float32, out: tupl
         if v.dtype != k.dtype:
             raise _C.DtypeMismatch(f"kv_cache_read: out is {k.dtype} and {v.dtype}")
     _C.call("lq_kv_cache_read", cache._ref, slots.data_ptr, shape[0], k.data_ptr, v.data_ptr, k.dtype.code, None)
+    _written(k), _written(v)
     return k, v

@@ -89,3 +89,34 @@ def test_prompts_in_chunks_then_token_by_token(heads, kv_heads, dim, page, bits,
         # the Linear: a sum of `width` products in float32 of rows that are off by the bound
         lin = want @ weight.T + bias
         assert np.abs(out - lin).max() <= (bound + 2.0 ** -24 * (np.sqrt(block.width) + 2) * 4 * np.abs(want).max()) * np.abs(weight).sum(1).max() + 2.0 ** -23
+
+
+def test_results_in_a_tensors_place_leave_nothing_of_what_it_was():
+    """A tensor that kept the range of what it held, or its codes on a grid, is the new result alone afterwards: what quantizes it next goes by the new
+    values."""
+    from lucid_amd._tensor import Grid
+
+    rng = np.random.default_rng(1)
+    cache = Q.PagedKVCache(2, 16, 2, 64)
+    k, v, q = (hip(rng.standard_normal((20, h, 64)).astype(np.float32)) for h in (2, 2, 4))
+    slots, table, starts, lens = ids(np.arange(20)), ids([[0, 1]]), ids([0, 20]), ids([20])
+    Q.kv_cache_write(cache, k, v, slots)
+    lin = nn.quantized.dynamic.Linear.from_float(nn.Linear(64, 64))
+
+    def small(*shape):  # values of 1e-3 with their range
+        return F.gelu(hip(np.full(shape, 1e-3, np.float32)), track_range=True)
+
+    def on_grid(*shape):
+        one = lambda a: hip(np.asarray(a))
+        return L.Tensor.on_grid(shape, Grid(one(np.ones(shape, np.int8)), one(np.float32(1e-3)), one(np.float32(0)), Q.qint8, 0))
+
+    for make in (small, on_grid):
+        out = make(20, 4, 64)
+        F.paged_attention(q, cache, table, starts, lens, out=out)
+        pair = make(20, 2, 64), make(20, 2, 64)
+        Q.kv_cache_read(cache, slots, out=pair)
+        for y in (out, *pair):
+            assert y._range is None and y._grid is None
+            assert np.array_equal(lin(y).numpy(), lin(hip(y.numpy())).numpy())
+        assert np.array_equal(out.numpy(), F.paged_attention(q, cache, table, starts, lens).numpy())
+        assert all(np.array_equal(a.numpy(), b.numpy()) for a, b in zip(pair, Q.kv_cache_read(cache, slots)))
