@@ -28,9 +28,11 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
     a.table = page_table, a.q_starts = q_starts, a.kv_lens = kv_lens, a.ldq = ldq;
     a.page_size = FastDiv(unsigned(c->page_size)), a.group = FastDiv(unsigned(heads / c->kv_heads));
     a.pages = c->num_pages, a.kv_heads = c->kv_heads, a.dim = c->head_dim;
-    a.tokens = tokens, a.heads = heads, a.batch = batch, a.width = table_width, a.causal = causal != 0, a.window = window, a.scale = scale;
+    a.tokens = tokens, a.heads = heads, a.batch = batch, a.width = table_width, a.causal = causal != 0, a.scale = scale;
     const int group = heads / c->kv_heads, sequences = std::max(1, std::min(batch, tokens));  // (of no sequence: the rows' zeros)
     const int64_t all_rows = int64_t(tokens) * group, most = int64_t(table_width) * c->page_size;  // keys of a sequence
+    // A place is at least -tokens and below `most`: a window of both together reaches every key, and kernels count places in 32 bits.
+    a.window = window < most + tokens ? window : 0;
     const int dim = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
     // The longest chunk, or a guess at it: a single sequence has all tokens; equally many each otherwise.
     const int chunk = max_chunk ? std::min(max_chunk, tokens) : batch == 1 ? tokens : (tokens + batch - 1) / std::max(batch, 1);

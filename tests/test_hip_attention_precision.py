@@ -140,3 +140,15 @@ def test_each_row_against_what_it_sees(case):
     b = Batch(*(GRID + LONG)[case], seed=case, tail=2)
     held(b, b.run())
     held(b, b.run(causal=False, window=70), causal=False, window=70)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("chunks,lengths", [([200], [100]), ([20, 3], [7, 40]), ([300, 150], [40, 600]), ([5], [0])])
+def test_windows_beyond_all_keys(chunks, lengths, dtype):
+    """As no window at all, also where a chunk is longer than its sequence."""
+    b = Batch(chunks, lengths, 4, 2, 64, dtype=dtype, seed=1)
+    for causal in (True, False):
+        want = b.run(causal=causal)
+        held(b, want, causal=causal)
+        for window in (max(lengths) + max(chunks), (1 << 30) + 1, (1 << 31) - 1):
+            assert np.array_equal(b.run(causal=causal, window=window), want), window
