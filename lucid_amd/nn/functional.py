@@ -112,6 +112,9 @@ def scaled_dot_product_attention_qkv(qkv: Tensor, num_heads: int, scale: float |
     return out
 
 
+_INT_MAX = 0x7fffffff
+
+
 def _paged_attention(name, cache, q_ptr, ldq, dtype, tokens, heads, out, page_table, q_starts, kv_lens, scale, causal, window, max_chunk) -> None:
     if not isinstance(page_table, Tensor) or page_table.ndim != 2:
         raise _C.ShapeMismatch(f"{name}: page_table is a (batch, pages) tensor")
@@ -125,9 +128,12 @@ def _paged_attention(name, cache, q_ptr, ldq, dtype, tokens, heads, out, page_ta
         raise ValueError(f"{name}: window {window}; at least 1, or None for all keys")
     if max_chunk is not None and max_chunk < 1:
         raise ValueError(f"{name}: max_chunk {max_chunk}; at least 1, or None")
+    if max(tokens, heads, batch, width) > _INT_MAX:
+        raise _C.ShapeMismatch(f"{name}: {tokens} tokens, {heads} heads, {batch} sequences of {width} pages")
+    # (ctypes takes the low 32 bits of a longer int)
     _C.call("lq_paged_attention", cache._ref, q_ptr, ldq, out.data_ptr, dtype.code, tokens, heads, batch, page_table.data_ptr, width,
             q_starts.data_ptr, kv_lens.data_ptr, 1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale), 1 if causal else 0,
-            0 if window is None else window, 0 if max_chunk is None else max_chunk, None)
+            0 if window is None else min(window, _INT_MAX), 0 if max_chunk is None else min(max_chunk, _INT_MAX), None)
 
 
 def paged_attention(q: Tensor, cache, page_table: Tensor, q_starts: Tensor, kv_lens: Tensor, scale: float | None = None, causal: bool = True,

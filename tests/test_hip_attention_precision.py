@@ -152,3 +152,23 @@ def test_windows_beyond_all_keys(chunks, lengths, dtype):
         held(b, want, causal=causal)
         for window in (max(lengths) + max(chunks), (1 << 30) + 1, (1 << 31) - 1):
             assert np.array_equal(b.run(causal=causal, window=window), want), window
+
+
+def test_a_longest_chunk_of_more_than_32_bits_is_one_beyond_all_tokens():
+    b = Batch([40, 40], [700, 600], 8, 2, 128, seed=1)
+    want = b.run(max_chunk=(1 << 31) - 1)
+    assert not np.array_equal(want, b.run(max_chunk=1))  # (the other kernel: results differ by rounding)
+    for n in (1 << 31, (1 << 32) + 1, 1 << 70):
+        assert np.array_equal(b.run(max_chunk=n), want)
+
+
+def test_a_window_of_more_than_32_bits_is_one_beyond_all_keys():
+    b = Batch([40, 3], [100, 60], 4, 2, 64, seed=1)
+    want = b.run()
+    for n in (1 << 31, (1 << 32) - 1, (1 << 32) + 1, (1 << 32) + 5, 1 << 70):
+        assert np.array_equal(b.run(window=n), want), n
+    for bad in (-1, -(1 << 32) + 5):
+        with pytest.raises(ValueError):
+            b.run(window=bad)
+        with pytest.raises(ValueError):
+            b.run(max_chunk=bad)
