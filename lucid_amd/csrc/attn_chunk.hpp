@@ -171,7 +171,7 @@ struct ChunkKernel {
         };
         Level level;  // of the keys that are settled
         // a negative scale changes the queries' signs, and of a scale of 0 all scores are 0, the masked ones still none.  What is left
-        // goes with the keys' scales, with float32 queries, which have a factor for each row, with the scores
+        // goes with the keys' scales (the sum of a row's products with codes, times it, may be infinite where the score is not)
         const float key_factor = a.scale == 0.f ? 1.f : fabsf(a.scale * kLog2e);
         const uint32_t high = BITS == 4 ? magic() : 0;
         // what is requested becomes float16 in LDS, a part at a time: eight columns of a key, and at last the scales
@@ -319,7 +319,7 @@ struct ChunkKernel {
         auto exponents = [&](const char* stage, int half, int pair, float mm) {
             const f32x2 ks = *reinterpret_cast<const f32x2*>(scales_of(stage) + 32 * half + 8 * (pair / 2) + 4 * h + 2 * (pair % 2));
 #pragma unroll
-            for (int r = 0; r < 2; ++r) x[2 * pair + r] = __builtin_fmaf(F32 ? s[2 * pair + r] * factor : s[2 * pair + r], ks[r], mm);
+            for (int r = 0; r < 2; ++r) x[2 * pair + r] = __builtin_fmaf(s[2 * pair + r], F32 ? ks[r] * factor : ks[r], mm);
         };
         // Matrix products one by one, the next fragment read ahead of each, and behind it the vector unit's share of what is to be done
         // meanwhile: f of the parts [n step / steps, n (step + 1) / steps) of n.  A step is kept together.

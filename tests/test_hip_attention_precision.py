@@ -172,3 +172,17 @@ def test_a_window_of_more_than_32_bits_is_one_beyond_all_keys():
             b.run(window=bad)
         with pytest.raises(ValueError):
             b.run(max_chunk=bad)
+
+
+@pytest.mark.parametrize("chunks,lengths", SIZES)
+def test_queries_near_the_largest_float_of_keys_near_the_smallest(chunks, lengths):
+    """Queries 2^118 times as large, the scale twice, keys 2^-119 times (their scales, 2^-7 and more here, stay normal numbers): every score is what it was,
+    to the bit, though the scaled sum of a query's products with codes passes 2^128."""
+    for bits, symmetric in ((8, True), (8, False), (4, False)):
+        b = Batch(chunks, lengths, 4, 2, 64, bits=bits, symmetric=symmetric, dtype=np.float32, seed=2)
+        want = b.run(scale=1.0)
+        held(b, want, scale=1.0)
+        b.q = b.q * np.float32(2.0 ** 118)
+        assert b.cache.k_scale.numpy().min() >= 2.0 ** -7
+        b.cache.k_scale.copy_from(b.cache.k_scale.numpy() * np.float32(2.0 ** -119))
+        assert np.array_equal(b.run(scale=2.0), want)
