@@ -48,7 +48,8 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
     auto lock = scratch_lock(st);
     auto room = [&](size_t floats) {
         void* p = nullptr;
-        const int rc = call_buffer(9, floats * sizeof(float), st, &p);
+        // (in a recording one buffer for all calls on the stream, which run one after another)
+        const int rc = kept_buffer(9, floats * sizeof(float), 0, st, &p, nullptr);
         a.partial = static_cast<float*>(p);
         return rc;
     };

@@ -393,3 +393,35 @@ def test_refusals():
         F.paged_attention_qkv(hip(np.zeros((5, 7 * 64), np.float16)), 4, b.cache, table, starts, lens)
     empty = F.paged_attention(L.Tensor.empty((0, 4, 64), L.float16), b.cache, table, starts, lens)
     assert empty.shape == (0, 4, 64)
+
+
+def held_by_a_graph(calls):
+    """Bytes of the pool that a graph of these calls holds."""
+    used = C.c_size_t()
+    L.synchronize()
+    _C.call("lq_memory_stats", C.byref(used), None)
+    before = used.value
+    with L.graph.capture() as g:
+        for call in calls:
+            call()
+    _C.call("lq_memory_stats", C.byref(used), None)
+    return g, used.value - before
+
+
+@pytest.mark.parametrize("chunks,lengths", [([1] * 4, [3000, 100, 1500, 9]), ([180, 6], [900, 2500])])
+def test_a_captured_step_of_many_layers_holds_one_set_of_pieces(chunks, lengths):
+    b = Batch(chunks, lengths, 8, 2, 128, seed=3)
+    t = [hip(b.q), ids(b.table), ids(b.q_starts), ids(b.kv_lens)]
+    outs = [hip(np.zeros_like(b.q)) for _ in range(12)]
+    call = lambda y: lambda: F.paged_attention(t[0], b.cache, *t[1:], out=y)
+    want = b.run()
+    one, alone = held_by_a_graph([call(outs[0])])
+    all_, together = held_by_a_graph([call(y) for y in outs])
+    assert alone and together == alone
+    for g in (one, all_, all_):
+        for y in outs:
+            y.copy_from(np.zeros_like(b.q))
+        g.replay()
+        L.synchronize()
+        for y in outs[:1 if g is one else 12]:
+            assert np.array_equal(y.numpy(), want)
