@@ -74,7 +74,8 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
         LQ_REQUIRE(int64_t(a.blocks) * c->kv_heads <= 0xffffff, LQ_ERR_NOT_IMPLEMENTED, "paged_attention: %d tiles of queries for %d heads", tiles,
                    c->kv_heads);
         if (join) {
-            a.pieces = std::min(a.blocks, (4 * a.each + c->kv_heads - 1) / c->kv_heads + 64);  // (64: rounding)
+            // (parts of tiles of several, see part_keys; its sums' rounding, 2^-24 of them for every 64 sequences, is worth less than 64 parts of all heads)
+            a.pieces = std::min(a.blocks, (4 * a.each + 64) / c->kv_heads + 1);
             rc = room(size_t(a.pieces) * c->kv_heads * R * (dim + 2));
             if (rc) return rc;
         }

@@ -425,3 +425,16 @@ def test_a_captured_step_of_many_layers_holds_one_set_of_pieces(chunks, lengths)
         L.synchronize()
         for y in outs[:1 if g is one else 12]:
             assert np.array_equal(y.numpy(), want)
+
+
+def test_room_for_pieces_does_not_grow_with_the_heads():
+    """Tiles of several parts have at most 4 parts for each of the 512 places of blocks, over all heads; a part is 128 rows of 64 columns, a maximum and a
+    sum each, in float32.  Beside them some rounding."""
+    b = Batch([70] * 100, [420] * 100, 64, 64, 16, dtype=np.float16, seed=3)
+    t = [hip(b.q), ids(b.table), ids(b.q_starts), ids(b.kv_lens)]
+    out = hip(np.zeros_like(b.q))
+    g, nbytes = held_by_a_graph([lambda: F.paged_attention(t[0], b.cache, *t[1:], out=out)])
+    assert nbytes <= (4 * 512 + 256) * 128 * (64 + 2) * 4
+    g.replay()
+    L.synchronize()
+    assert np.array_equal(out.numpy(), b.run())
