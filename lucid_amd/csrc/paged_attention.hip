@@ -34,16 +34,20 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
     // A place is at least -tokens and below `most`: a window of both together reaches every key, and kernels count places in 32 bits.
     a.window = window < most + tokens ? window : 0;
     const int dim = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
-    // The longest chunk, or a guess at it: a single sequence has all tokens; equally many each otherwise.
-    const int chunk = max_chunk ? std::min(max_chunk, tokens) : batch == 1 ? tokens : (tokens + batch - 1) / std::max(batch, 1);
+    // The longest chunk, or a guess at it: equally many tokens each, but for what one sequence can have if each of the others has one where that is 8192
+    // rows and more (a prompt of 3700 tokens among 255 single ones, four query heads a key head, 765 -> 508 us; of 2000 367 either way).
+    const int one = tokens - (sequences - 1);
+    const int chunk = max_chunk ? std::min(max_chunk, tokens) : int64_t(one) * group >= 8192 ? one : (tokens + sequences - 1) / sequences;
     // Sequences of more than few_rows rows go to attn_chunk_kernel, the others to attn_rows_kernel, which reads the keys once for every 32
     // rows.  us, rows / chunk kernel, 8 heads of 128, 8 bits: 16 float16 sequences of up to 4096 keys 64 rows 53.6 / 67, 80 rows 62 / 57, 128 rows
     // 86 / 64; 64 of up to 1024 64 rows 70 / 78, 80 rows 84 / 70; 16 float32 ones of up to 4096 96 rows 74 / 90, 128 rows 96 / 95, 192 rows 126 / 135
     // but 240 rows 152 / 145; one float16 sequence of 16 384 80 rows 39 / 42, 128 rows 36 / 46, 192 rows 51 / 48.
-    // Where there can be both, and the longest chunk says that there are, both are launched and each takes its own; otherwise
-    // (chunks of 512 rows in the mean: an idle launch is lost there for little) either takes all.
+    // Where there can be both, both are launched and each takes its own; otherwise either takes all (one prompt of 8192 among 31 single tokens: the chunk
+    // kernel alone 1245 us, both 1000).  There are chunks alone where the longest leaves no room for a sequence without tokens, and
+    // 512 rows in the mean: an idle launch is lost for little otherwise.
     const int few_rows = batch == 1 ? 128 : dtype == LQ_F32 ? 96 : 64;
-    const bool chunks = int64_t(chunk) * group > few_rows, few = !chunks || (sequences > 1 && all_rows < int64_t(sequences) * 512);
+    const bool chunks = int64_t(chunk) * group > few_rows, alike = int64_t(sequences) * chunk - tokens < chunk && all_rows >= int64_t(sequences) * 512;
+    const bool few = !chunks || (sequences > 1 && !alike);
     hipStream_t st = as_stream(stream);
     auto lock = scratch_lock(st);
     auto room = [&](size_t floats) {
@@ -63,8 +67,9 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
         const int64_t rows = int64_t(chunk) * group;
         const bool wide = dim == 128 && batch == 1 && rows >= 1024 && (rows * c->kv_heads >= 512 * 256 || most >= 4 * int64_t(chunk));
         const int R = wide ? 256 : 128;
-        const int tiles = sequences + int(all_rows / R);
         a.min_rows = few ? few_rows + 1 : 1, a.max_rows = 0x7fffffff;
+        // (a block at least: of no sequence it clears the rows)
+        const int tiles = std::max(1, int(std::min<int64_t>(sequences, all_rows / a.min_rows) + all_rows / R));
         // (parts of 256 / 384 / 512 keys at least: 3 chunks of 333, float32, 52 / 50.5 / 61 us; 8 of 300 over up to 700 keys 69 / 63 / 64)
         a.each = (dim > 128 || wide ? 1 : 2) * 256, a.least = 384;
         // (four rounds of blocks of one sequence are left whole: joining none of 129 tiles of 8 heads takes 25 us)
@@ -88,7 +93,9 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
         LQ_CHECK_LAUNCH("paged_attention");
     }
     if (few) {
-        const int qt = int64_t(chunk) * group <= 16 ? 1 : 2, rows = 16 * qt;
+        // (the mean of those that the longest one leaves, or of all)
+        const int others = !chunks ? chunk : max_chunk ? (tokens - chunk) / (sequences - 1) : tokens / sequences;
+        const int qt = int64_t(others) * group <= 16 ? 1 : 2, rows = 16 * qt;
         a.min_rows = 1, a.max_rows = chunks ? few_rows : 0x7fffffff;
         const int tiles = sequences + int((chunks ? std::min<int64_t>(all_rows, int64_t(sequences) * few_rows) : all_rows) / rows);
         LQ_REQUIRE(int64_t(tiles) * c->kv_heads * (most / 128 + 1) < 0x7fffffff, LQ_ERR_NOT_IMPLEMENTED,

@@ -186,3 +186,15 @@ def test_queries_near_the_largest_float_of_keys_near_the_smallest(chunks, length
         assert b.cache.k_scale.numpy().min() >= 2.0 ** -7
         b.cache.k_scale.copy_from(b.cache.k_scale.numpy() * np.float32(2.0 ** -119))
         assert np.array_equal(b.run(scale=2.0), want)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("chunks,lengths,max_chunk", [
+    ([300, 1, 300], [310, 400, 700], 300), ([300, 280, 299], [300, 280, 900], 300),  # alike: long chunks alone, one of them a token
+    ([1200, 1, 0, 900], [1300, 700, 20, 900], 1200), ([1200, 1, 0, 900], [1300, 700, 20, 900], None), ([700] + [1] * 9, [900] + [300] * 9, 700),
+    ([0, 0, 600, 3], [5, 0, 600, 64], 600), ([2100] + [1] * 4, [2100] + [90] * 4, None), ([2] * 70 + [260], [40] * 70 + [300], 260), ([60, 1] * 3, [99, 98] * 3, 7)])
+def test_prompts_beside_single_tokens(chunks, lengths, max_chunk, dtype):
+    """Batches whose sequences go to either kernel, or all to one, with rows of none behind them."""
+    for kw in ({}, dict(window=130)):
+        b = Batch(chunks, lengths, 4, 1, 64, bits=4 if len(kw) else 8, dtype=dtype, seed=len(chunks), tail=3)
+        held(b, b.run(max_chunk=max_chunk, **kw), **kw)
