@@ -39,9 +39,10 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
     const int one = tokens - (sequences - 1);
     const int chunk = max_chunk ? std::min(max_chunk, tokens) : int64_t(one) * group >= 8192 ? one : (tokens + sequences - 1) / sequences;
     // Sequences of more than few_rows rows go to attn_chunk_kernel, the others to attn_rows_kernel, which reads the keys once for every 32
-    // rows.  us, rows / chunk kernel, 8 heads of 128, 8 bits: 16 float16 sequences of up to 4096 keys 64 rows 53.6 / 67, 80 rows 62 / 57, 128 rows
-    // 86 / 64; 64 of up to 1024 64 rows 70 / 78, 80 rows 84 / 70; 16 float32 ones of up to 4096 96 rows 74 / 90, 128 rows 96 / 95, 192 rows 126 / 135
-    // but 240 rows 152 / 145; one float16 sequence of 16 384 80 rows 39 / 42, 128 rows 36 / 46, 192 rows 51 / 48.
+    // rows.  us, rows / chunk kernel, 8 heads of 128, 8 bits: 16 float16 sequences of up to 4096 keys 64 rows 62 / 59, 80 rows 76 / 64, 128 rows
+    // 93 / 78; 64 of up to 1024 64 rows 70 / 77, 80 rows 92 / 82; 16 float32 ones of up to 4096 80 rows 87 / 89, 96 rows 90 / 89, 128 rows 104 / 103, 192 rows
+    // 152 / 144; one float16 sequence of 16 384 80 rows 39 / 49, 128 rows 41 / 52, 192 rows 57 / 58.  Heads of 64 and 256 cross over at the same rows within
+    // some 10 % of the time, but for float32 above 128 (128 rows of 16 sequences 198 / 291: the chunk kernel's registers spill).
     // Where there can be both, both are launched and each takes its own; otherwise either takes all (one prompt of 8192 among 31 single tokens: the chunk
     // kernel alone 1245 us, both 1000).  There are chunks alone where the longest leaves no room for a sequence without tokens, and
     // 512 rows in the mean: an idle launch is lost for little otherwise.

@@ -198,3 +198,20 @@ def test_prompts_beside_single_tokens(chunks, lengths, max_chunk, dtype):
     for kw in ({}, dict(window=130)):
         b = Batch(chunks, lengths, 4, 1, 64, bits=4 if len(kw) else 8, dtype=dtype, seed=len(chunks), tail=3)
         held(b, b.run(max_chunk=max_chunk, **kw), **kw)
+
+
+KINDS = {"16 rows": ([1, 1], [300, 45]), "32 rows": ([5, 2], [200, 64]), "chunks": ([40, 70], [40, 300]), "one prompt": ([260], [1100])}
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 160, 224, 256])
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("bits", [8, 4])
+def test_every_kernel(bits, symmetric, dtype, dim, kind):
+    """Each kernel for codes, scheme, type, head dims up to 64, 128 and 256 and rows of a sequence at a whole and a cut head dim: pages within a step and
+    beyond it, a window, all keys."""
+    chunks, lengths = KINDS[kind]
+    b = Batch(chunks, lengths, 4, 1, dim, 16 if dim % 64 else 64, bits, symmetric, dtype, seed=dim + bits, tail=1)
+    kw = (dict(), dict(window=21), dict(causal=False, scale=-0.4 / np.sqrt(dim)))[(dim // 32 + bits + symmetric) % 3]
+    held(b, b.run(max_chunk=max(chunks), **kw), **kw)
