@@ -399,6 +399,7 @@ def held_by_a_graph(calls):
     """Bytes of the pool that a graph of these calls holds."""
     used = C.c_size_t()
     L.synchronize()
+    _C.call("lq_empty_cache")  # (a kept block of up to twice the size would be taken for one that is asked for)
     _C.call("lq_memory_stats", C.byref(used), None)
     before = used.value
     with L.graph.capture() as g:
