@@ -481,7 +481,9 @@ int lq_kv_cache_read(const lq_kv_cache* cache, const int32_t* slots, size_t toke
  * seen; lengths beyond the table are cut to it.  Scores, sums and products are float32: codes enter the matrix products as the
  * whole numbers they are, scales after them; float16 queries as they are, float32 ones as two float16 of 22 bits together; probabilities times
  * v_scale as two as well, against the largest that the row itself sees: keys that it does not see, or gives no weight, take none of
- * its bits.  max_chunk: the most queries of a sequence, or 0; the work is divided by it, and results differ by rounding alone. */
+ * its bits.  max_chunk: the most queries of a sequence, or 0; the work is divided by it, and results differ by rounding alone.
+ * tokens * heads is at most 2^25, table_width * page_size 2^30.  Pieces of split sequences take up to some 145 MB of scratch for a
+ * stream, or for a stream of a graph. */
 int lq_paged_attention(const lq_kv_cache* cache, const void* q, size_t ldq, void* out, int dtype, int tokens, int heads, int batch,
                        const int32_t* page_table, int table_width, const int32_t* q_starts, const int32_t* kv_lens, float scale, int causal,
                        int window, int max_chunk, lq_stream stream);

@@ -1,9 +1,10 @@
 // Attention of many rows (a chunk of a prompt) over paged quantized keys and values.
 //
-// Bound by the vector unit, by what it does for each score (an exponent, a maximum, an exponential, a sum, a scale, a rounding: some ten issue
-// slots beside four cycles of a matrix product) and for each code, and then by the matrix pipe: of 8192 tokens of 16 384 (32 heads
-// of 128 on 8, float16, 8 bits, 1885 to 2000 us: up to 0.87 PFLOP/s of the 1.16 that a large library product reaches) the one is busy 50 % of
-// the time, the other 37 %.  So a code is turned into float16 once for a block's 128 or 256 rows, on its way into LDS, and a wavefront has 32 rows, whose
+// Bound by what the vector unit does for each score (an exponent, a maximum, an exponential, a sum, a scale, two roundings) and each code, and
+// by the matrix products, on wavefronts that do not quite fill each other's gaps: of 8192 tokens of 16 384 (32 heads of 128 on 8, float16, 8 bits, 2400 us,
+// three products where the result needs two: 1.03 PFLOP/s of the 1.16 that a large library product reaches) vector instructions take 50 % of
+// the SIMDs' cycles and matrix ones 45; a wavefront issues for 42 % of its time, waits for its turn for 31 and for LDS, memory or the others of
+// its block for 28.  So a code is turned into float16 once for a block's 128 or 256 rows, on its way into LDS, and a wavefront has 32 rows, whose
 // accumulators, maxima and sums stay in its registers:
 //
 //   S^T = K Q^T    v_mfma_f32_32x32x16_f16, A: K from LDS, lane (h, n) key n of 32, columns 8h..8h+7 of 16; B: Q in registers.
@@ -36,7 +37,7 @@ struct ChunkKernel {
     static constexpr bool F32 = std::is_same_v<T, float>;
     static constexpr int PARTS = F32 ? 2 : 1;  // float16 parts of a query
     // Probabilities are two float16 for float16 results as well: with one alone the error is 1.4 times that of the result's own rounding, and
-    // would depend on which kernel has a row.  (8192 of 16 384, float16, 1893 us with one, 2450 so: half as many products again.)
+    // would depend on which kernel has a row (8192 of 16 384, float16, 1893 us with one, 2400 so).
     static constexpr int P_PARTS = 2;
     static constexpr int THREADS = 64 * WAVES, R = 32 * WAVES, KEYS = 64;
     static constexpr int SLABS = DIM / 16, TILES = DIM / 32;

@@ -62,16 +62,16 @@ extern "C" int lq_paged_attention(const lq_kv_cache* c, const void* q, size_t ld
         // Tiles of 128 rows, two blocks a CU, one of which has the CU to itself when the other has ended; or of 256, one block a CU, in
         // which a code is turned into float16 for twice as many rows.  The latter where blocks are alike and fill the places: one
         // sequence of 1024 rows or more, in two rounds of blocks or more or behind three times as many keys.  us, 128 / 256 rows, 32 heads of 128 on
-        // 8, float16: 8192 tokens of 16 384 2070 / 1949, 8192 of 8192 742 / 701, 1000 of 16 000 362 / 334, 2048 of 8192 331 / 327; but 2048 of 4096
-        // 164 / 172, 1000 of 1000 52.5 / 55.9, and of four sequences of 1934 to 8192 keys 274 / 311 (of four of 8192 372 / 342: their lengths are
-        // on the device).
+        // 8, float16: 8192 tokens of 16 384 2425 / 2347, 8192 of 8192 887 / 826, 1000 of 16 000 420 / 401, 2048 of 8192 403 / 397; but 2048 of 4096
+        // 187 / 205, 1000 of 1000 50 / 57, and of four sequences of 1934 to 8192 keys 308 / 351 (of four of 8192 429 / 401: their lengths are
+        // on the device).  float32: 3183 / 2855, 1123 / 1011, 544 / 486, 512 / 479, 259 / 248, 64 / 63.
         const int64_t rows = int64_t(chunk) * group;
         const bool wide = dim == 128 && batch == 1 && rows >= 1024 && (rows * c->kv_heads >= 512 * 256 || most >= 4 * int64_t(chunk));
         const int R = wide ? 256 : 128;
         a.min_rows = few ? few_rows + 1 : 1, a.max_rows = 0x7fffffff;
         // (a block at least: of no sequence it clears the rows)
         const int tiles = std::max(1, int(std::min<int64_t>(sequences, all_rows / a.min_rows) + all_rows / R));
-        // (parts of 256 / 384 / 512 keys at least: 3 chunks of 333, float32, 52 / 50.5 / 61 us; 8 of 300 over up to 700 keys 69 / 63 / 64)
+        // (parts of 256 / 384 / 512 keys at least: 3 chunks of 333, float32, 53 / 50 / 60 us; 8 of 300 over up to 700 keys 80 / 72 / 72)
         a.each = (dim > 128 || wide ? 1 : 2) * 256, a.least = 384;
         // (four rounds of blocks of one sequence are left whole: joining none of 129 tiles of 8 heads takes 25 us)
         const bool join = most > a.least && !(batch == 1 && rows * c->kv_heads >= int64_t(4) * a.each * R);

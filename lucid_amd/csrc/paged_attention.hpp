@@ -228,7 +228,7 @@ __device__ __forceinline__ unsigned parts_of(unsigned extent, unsigned most) {
 // the blocks that end early then take another.  (Tiles of several parts, each longer than one, then have 4 a.each parts at most, for all heads.)  Up to 64 sequences of about the same length (one a lane; 0 tiles: not this launch's)
 // have equal parts, which come in whole rounds: a lane each tries the longest in 1, 2, 3, ... parts, and the shortest sum of the rounds'
 // lengths counts, in keys, of which a block costs kBlock besides its own and one whose part is joined kPart more (us, parts of the share / in
-// rounds: 4 chunks of 512 over 8192 keys 400 / 387, one of 300 101 / 85; but 4 over 1934 to 8192 keys 281 / 292).
+// rounds: 4 chunks of 512 over 8192 keys 458 / 440, one of 300 115 / 92; but 4 over 1934 to 8192 keys 310 / 321).
 constexpr float kBlock = 128.f, kPart = 320.f, kAlike = 0.8f;
 __device__ __forceinline__ unsigned part_keys(const AttnArgs& a, float keys, unsigned tiles, unsigned extent, int lane) {
     const float heads = float(a.kv_heads), places = float(a.each);
