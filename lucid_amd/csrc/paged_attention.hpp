@@ -13,7 +13,8 @@
 // results too (one float16 alone makes the error 1.4 times that of the result's own rounding).  The sums of the p_j are not rounded.
 // What keeps a w_j's 22 bits whatever the scales is that a row's m goes by the keys that the row itself has seen, and by their w_j: it is
 // renewed where one may pass 2^15, so that it is 2^7 then, and two float16 hold a number to 2^-25 of 1.  Mostly the scales of the keys of a step
-// are within 2^8 of each other; then the exponents' maximum and one `Level` for all of them bound the w_j.  In other steps each key's scale counts.
+// are within 2^8 of each other; then the exponents' maximum and one `Level` for all of them bound the w_j.  In other steps each key's scale counts
+// (scales of all keys 2^-3 to 2^3 times as large, at random: chunks take a quarter longer, few rows up to 6 %).
 #pragma once
 #include "kv_cache.hpp"
 #include "wave_reduce.hpp"
