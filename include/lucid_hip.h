@@ -444,6 +444,25 @@ int lq_wq_matmul(const float* x, const uint32_t* packed, const float* scales, co
  * (lucid/nn/quantized/mlx_linear.py forward). */
 int lq_bias_act_f32(float* y, const float* bias, size_t M, int N, int relu, lq_stream stream);
 
+/* Both projections of a gated feed-forward block on such weights, with the activation and the product (no counterpart in Lucid):
+ *     out[m, n] = act(x[m] . w_gate[n] + bias_gate[n]) * (x[m] . w_up[n] + bias_up[n])
+ * x [M, K] and out [M, N] are both LQ_F32 or both LQ_F16; weights as lq_wq_matmul takes them, 16-byte aligned; index 0 is the gate, 1 the way up.  act: 0
+ * silu v / (1 + exp(-v)), 1 gelu (erf form), 2 relu, 3 sigmoid.  Codes enter the products as whole numbers, scales and sums are float32:
+ * nothing of a weight is rounded, a float32 x keeps 22 bits or more of its row's largest value, float16 results are rounded once.  A
+ * non-finite x gives a non-finite row before the activation.  May take scratch of the stream. */
+typedef struct lq_wq_gated_args {
+    const void* x;
+    void* out;
+    const uint32_t* packed[2]; /* [N, K * bits / 32]         */
+    const float* scales[2];    /* [N, K / group_size]        */
+    const float* biases[2];
+    const float* bias[2];      /* [N], or NULL               */
+    int M, N, K;
+    int group_size, bits;      /* 32, 64 or 128; 4 or 8      */
+    int act, dtype;
+} lq_wq_gated_args;
+int lq_wq_gated_matmul(const lq_wq_gated_args* args, lq_stream stream);
+
 /* ------------------------------------------------- quantized key / value cache
  * No counterpart in Lucid.  Pages of page_size tokens; a page holds, per key / value head, page_size rows of head_dim codes,
  * so that a head's rows of a page are contiguous: codes [num_pages, kv_heads, page_size, head_dim * bits / 8] bytes, scale and
@@ -487,6 +506,56 @@ int lq_kv_cache_read(const lq_kv_cache* cache, const int32_t* slots, size_t toke
 int lq_paged_attention(const lq_kv_cache* cache, const void* q, size_t ldq, void* out, int dtype, int tokens, int heads, int batch,
                        const int32_t* page_table, int table_width, const int32_t* q_starts, const int32_t* kv_lens, float scale, int causal,
                        int window, int max_chunk, lq_stream stream);
+
+/* Copies whole pages, keys, values and their numbers: page src[i] into page dst[i], for `pages` pairs (int32).  A pair with a page
+ * that is negative or beyond the cache is skipped.  A page may be the source of several pairs; the destinations are distinct,
+ * and none is another pair's source. */
+int lq_kv_cache_copy(const lq_kv_cache* cache, const int32_t* src, const int32_t* dst, size_t pages, lq_stream stream);
+/* Moves the rows that sequences keep to their beginnings.  Sequence b keeps the places keep[starts[b]] .. keep[starts[b + 1] - 1]
+ * of the pages page_table[b, :] (int32 [batch, table_width]; keep int32 [kept], from 0 and rising within a sequence; starts int32 [batch + 1],
+ * rising from 0 to kept): the i-th of them moves to place i, all heads, as if all were read before any is written.  Places behind
+ * the kept ones stay as they are.  A row whose old or new place is beyond the table or on a page that is negative or beyond the
+ * cache is not moved; one that stays in its place is neither read nor written, so sequences may share the pages that hold only such.
+ * Takes scratch of the stream. */
+int lq_kv_cache_compact(const lq_kv_cache* cache, const int32_t* page_table, int table_width, int batch, const int32_t* keep, size_t kept,
+                        const int32_t* starts, lq_stream stream);
+
+/* ------------------------------------------------- around a decoder's attention
+ * No counterpart in Lucid.  The residual connection between two blocks with the norms beside it, over rows of `cols` values (at most
+ * 32768):  t = post(x), or x when post == 0;  r' = r + gate * scale * t;  y = pre(r').  Norms: v / sqrt(mean(v^2) + eps) * weight + bias,
+ * when layer == 1 of v - mean(v) in v's place (lucid/_C/backend/cpu/Norm.cpp:35-65).  Everything float32 in between; y is made from r'
+ * before that is rounded to its type. */
+typedef struct lq_residual_norm_args {
+    const void* x;            /* [rows, cols], LQ_F32 or LQ_F16                      */
+    const void* r;            /* [rows, cols] of r_dtype, or NULL: zeros             */
+    const void* gate;         /* [gate_rows, cols] of x's type: row g for the g-th rows / gate_rows rows; NULL: ones */
+    const float* scale;       /* [cols], or NULL: ones                               */
+    const float* weight;      /* [cols], or NULL: ones                               */
+    const float* bias;        /* [cols], or NULL: zeros                              */
+    const float* post_weight; /* likewise, of post                                   */
+    const float* post_bias;
+    void* y;     /* [rows, cols] of x's type; may be x                               */
+    void* r_out; /* [rows, cols] of r_dtype, may be r; NULL: not wanted              */
+    int64_t rows;
+    int64_t gate_rows; /* divides rows; 0 without a gate                             */
+    int cols;
+    int x_dtype, r_dtype; /* r_dtype: LQ_F32, or x_dtype                             */
+    int layer, post;
+    float eps;
+} lq_residual_norm_args;
+int lq_residual_norm(const lq_residual_norm_args* args, lq_stream stream);
+/* Drafted tokens against the target's probabilities, from given random numbers.  Sequence b has the rows starts[b] .. starts[b + 1] - 1
+ * (int32 [batch + 1], rising, within `rows`) of a step: its last token, and behind it the drafted ones (tokens int32 [rows]).  Row i of
+ * target ([rows, vocab], LQ_F32 or LQ_F16) holds the probabilities p of the token behind row i, row i of draft (the same type) those, q,
+ * that token i + 1 was drawn from; draft NULL: q = 1.  In order, x = tokens[i + 1] is accepted if uniforms[i] * q[x] < p[x] (exactly; a
+ * token outside the vocabulary is refused).  Behind the accepted tokens comes one drawn with last[b]: from max(p - q, 0) of the row that
+ * refused (draft NULL: from p without x), from p of the last row where none did, or where nothing of p - q is positive: the lowest
+ * token of positive weight at which the weights' running sum passes last[b] times their sum, in float64 (the last of positive weight if
+ * none does; -1 if there is none).  Weights that are not positive and finite count as 0.  new_tokens (int32 [rows]): in a sequence's
+ * rows its new tokens, then -1; rows of no sequence stay.  counts (int32 [batch]): how many; 0 of an empty sequence.  At most
+ * 65535 sequences, 2^24 tokens.  Takes scratch of the stream. */
+int lq_verify_drafts(const void* target, const void* draft, int dtype, int rows, int vocab, const int32_t* tokens, const int32_t* starts,
+                     int batch, const float* uniforms, const float* last, int32_t* new_tokens, int32_t* counts, lq_stream stream);
 
 /* ------------------------------------------------- ranges kept by the producer */
 /* Dynamic per-tensor quantization of a small tensor (n <= 262144) in one launch:

@@ -269,6 +269,34 @@ class KvCache(C.Structure):
 _SIGNATURES["lq_kv_cache_write"] = [C.POINTER(KvCache), _vp, _vp, _i, _sz, _sz, _vp, _sz, _vp]
 _SIGNATURES["lq_kv_cache_read"] = [C.POINTER(KvCache), _vp, _sz, _vp, _vp, _i, _vp]
 _SIGNATURES["lq_paged_attention"] = [C.POINTER(KvCache), _vp, _sz, _vp, _i, _i, _i, _i, _vp, _i, _vp, _vp, _f, _i, _i, _i, _vp]
+_SIGNATURES["lq_kv_cache_copy"] = [C.POINTER(KvCache), _vp, _vp, _sz, _vp]
+_SIGNATURES["lq_kv_cache_compact"] = [C.POINTER(KvCache), _vp, _i, _i, _vp, _sz, _vp, _vp]
+
+
+class ResidualNormArgs(C.Structure):
+    """``lq_residual_norm_args`` of ``include/lucid_hip.h``."""
+
+    _fields_ = [
+        ("x", _vp), ("r", _vp), ("gate", _vp), ("scale", _vp), ("weight", _vp), ("bias", _vp), ("post_weight", _vp), ("post_bias", _vp),
+        ("y", _vp), ("r_out", _vp), ("rows", C.c_int64), ("gate_rows", C.c_int64), ("cols", _i), ("x_dtype", _i), ("r_dtype", _i), ("layer", _i),
+        ("post", _i), ("eps", _f),
+    ]
+
+
+_SIGNATURES["lq_residual_norm"] = [C.POINTER(ResidualNormArgs), _vp]
+_SIGNATURES["lq_verify_drafts"] = [_vp, _vp, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp]
+
+
+class WqGatedArgs(C.Structure):
+    """``lq_wq_gated_args`` of ``include/lucid_hip.h``."""
+
+    _fields_ = [
+        ("x", _vp), ("out", _vp), ("packed", _vp * 2), ("scales", _vp * 2), ("biases", _vp * 2), ("bias", _vp * 2), ("M", _i), ("N", _i), ("K", _i),
+        ("group_size", _i), ("bits", _i), ("act", _i), ("dtype", _i),
+    ]
+
+
+_SIGNATURES["lq_wq_gated_matmul"] = [C.POINTER(WqGatedArgs), _vp]
 _SIGNATURES["lq_lstm_sequence_pays"] = [_i] * 3 + [C.POINTER(_i)]
 _SIGNATURES["lq_lstm_fused_layers"] = [_i] * 6 + [C.POINTER(_i)]
 _SIGNATURES["lq_lstm_sequence_f32"] = [C.POINTER(LstmArgs), _vp]

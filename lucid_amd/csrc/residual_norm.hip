@@ -1,0 +1,213 @@
+// The residual connection between two blocks, with the norms beside it, in one pass:
+//
+//   t  = post(x), or x            post, pre: rms    v / sqrt(mean(v^2) + eps) * weight (+ bias)
+//   r' = r + gate * scale * t                layer  (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps) * weight (+ bias)
+//   y  = pre(r')
+//
+// A row stays in the registers of the TPR threads that have it: x and r are read once, r' and y written once, whatever norms are
+// asked for; a layer norm's variance is taken about its mean from the registers.  y comes from r' as it is in float32, before that
+// is rounded to its own type.  Bound by memory.
+#include <type_traits>
+
+#include "common.hpp"
+
+using namespace lq;
+
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+
+struct Norm {
+    const float *weight, *bias;  // NULL: ones, zeros
+};
+
+struct Args {
+    const void *x, *r, *gate;  // r NULL: no residual; gate NULL: ones
+    const float* scale;        // [cols], NULL: ones
+    Norm pre, post;
+    void *y, *r_out;  // r_out NULL: not wanted
+    unsigned rows, cols;
+    float eps;
+    FastDiv per_gate{1};  // rows of a row of the gate
+};
+
+// Four values of a row from column c on, zeros past its end.
+template <class T>
+__device__ __forceinline__ f4 load4(const T* row, unsigned c, unsigned cols) {
+    if (c + 4 <= cols) {  // (not always 8 or 16-byte aligned)
+        if constexpr (std::is_same_v<T, float>) {
+            f4 v;
+            __builtin_memcpy(&v, row + c, 16);
+            return v;
+        } else {
+            h4 v;
+            __builtin_memcpy(&v, row + c, 8);
+            return f4{float(v[0]), float(v[1]), float(v[2]), float(v[3])};
+        }
+    }
+    f4 v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (unsigned i = 0; i < 3; ++i)
+        if (c + i < cols) v[i] = float(row[c + i]);
+    return v;
+}
+template <class T>
+__device__ __forceinline__ void store4(T* row, unsigned c, unsigned cols, f4 v) {
+    if (c + 4 <= cols) {
+        if constexpr (std::is_same_v<T, float>) {
+            __builtin_memcpy(row + c, &v, 16);
+        } else {
+            const h4 h{_Float16(v[0]), _Float16(v[1]), _Float16(v[2]), _Float16(v[3])};
+            __builtin_memcpy(row + c, &h, 8);
+        }
+        return;
+    }
+#pragma unroll
+    for (unsigned i = 0; i < 3; ++i)
+        if (c + i < cols) row[c + i] = T(v[i]);
+}
+
+// The sum over the TPR threads of a row, to all of them.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* s) {
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
+    if constexpr (TPR > 64) {
+        __syncthreads();  // (the sums before have been read)
+        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = s[threadIdx.x & (TPR / 64 - 1)];
+#pragma unroll
+        for (int d = TPR / 128; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
+    }
+    return v;
+}
+
+template <bool LAYER, int TPR, int NV>
+__device__ __forceinline__ void normalize(f4 (&v)[NV], const Norm& n, unsigned at, unsigned cols, float eps, float* s) {
+    const float inverse = 1.0f / float(cols);
+    float sum = 0.f;
+    if constexpr (LAYER) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) sum += (v[i][0] + v[i][1]) + (v[i][2] + v[i][3]);
+        const float mean = row_sum<TPR>(sum, s) * inverse;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][e] = at + i * TPR * 4 + e < cols ? v[i][e] - mean : 0.f;
+        sum = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) sum += (v[i][0] * v[i][0] + v[i][1] * v[i][1]) + (v[i][2] * v[i][2] + v[i][3] * v[i][3]);
+    const float f = 1.0f / sqrtf(row_sum<TPR>(sum, s) * inverse + eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const unsigned c = at + i * TPR * 4;
+        v[i] *= f;
+        if (n.weight && c < cols) v[i] *= load4(n.weight, c, cols);
+        if (n.bias && c < cols) v[i] += load4(n.bias, c, cols);
+    }
+}
+
+template <class TX, class TR, bool LAYER, bool POST, int TPR, int NV>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void residual_norm_kernel(Args a) {
+    __shared__ float s[TPR / 64];
+    const unsigned row = blockIdx.x * (TPR < 256 ? 256 / TPR : 1) + threadIdx.x / TPR, at = threadIdx.x % TPR * 4;
+    if (row >= a.rows) return;  // (rows of TPR = 64: no barrier follows)
+    const size_t base = size_t(row) * a.cols;
+    f4 x[NV], r[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x[i] = load4(static_cast<const TX*>(a.x) + base, at + i * TPR * 4, a.cols);
+    if (a.r) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) r[i] = load4(static_cast<const TR*>(a.r) + base, at + i * TPR * 4, a.cols);
+    }
+    if constexpr (POST) normalize<LAYER, TPR, NV>(x, a.post, at, a.cols, a.eps, s);
+    if (a.scale) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) x[i] *= load4(a.scale, at + i * TPR * 4, a.cols);
+    }
+    if (a.gate) {
+        const TX* gate = static_cast<const TX*>(a.gate) + size_t(a.per_gate(row)) * a.cols;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) x[i] *= load4(gate, at + i * TPR * 4, a.cols);
+    }
+    if (a.r) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) x[i] += r[i];
+    }
+    if (a.r_out) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) store4(static_cast<TR*>(a.r_out) + base, at + i * TPR * 4, a.cols, x[i]);
+    }
+    normalize<LAYER, TPR, NV>(x, a.pre, at, a.cols, a.eps, s);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) store4(static_cast<TX*>(a.y) + base, at + i * TPR * 4, a.cols, x[i]);
+}
+
+template <int V>
+using Int = std::integral_constant<int, V>;
+
+// f with the threads of a row and the fours of values that each has.
+template <class F>
+void by_shape(unsigned rows, unsigned cols, F&& f) {
+    const unsigned fours = (cols + 3) / 4;
+    if (fours <= 64) f(Int<64>{}, Int<1>{});
+    else if (fours <= 128) f(Int<64>{}, Int<2>{});
+    else if (fours <= 192) f(Int<64>{}, Int<3>{});
+    else if (fours <= 256) f(Int<64>{}, Int<4>{});
+    else if (fours <= 512) f(Int<256>{}, Int<2>{});
+    else if (fours <= 1024) f(Int<256>{}, Int<4>{});
+    else if (fours <= 2048) f(Int<1024>{}, Int<2>{});
+    else if (fours <= 4096) f(Int<1024>{}, Int<4>{});
+    else f(Int<1024>{}, Int<8>{});
+}
+
+template <class TX, class TR, bool LAYER>
+void launch(const Args& a, bool post, hipStream_t st) {
+    by_shape(a.rows, a.cols, [&](auto tpr, auto nv) {
+        constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, BLOCK = TPR < 256 ? 256 : TPR;
+        const unsigned per = BLOCK / TPR;
+        const auto kernel = post ? residual_norm_kernel<TX, TR, LAYER, true, TPR, NV> : residual_norm_kernel<TX, TR, LAYER, false, TPR, NV>;
+        kernel<<<(a.rows + per - 1) / per, BLOCK, 0, st>>>(a);
+    });
+}
+
+constexpr int kMaxCols = 32768;  // 1024 threads with 32 values each
+
+}  // namespace
+
+extern "C" int lq_residual_norm(const lq_residual_norm_args* n, lq_stream stream) {
+    LQ_REQUIRE(n, LQ_ERR_VALUE, "residual_norm: args is NULL");
+    LQ_REQUIRE(n->rows >= 0 && n->cols >= 0, LQ_ERR_SHAPE, "residual_norm: %lld rows of %d", (long long)n->rows, n->cols);
+    LQ_REQUIRE(n->layer == 0 || n->layer == 1, LQ_ERR_VALUE, "residual_norm: norm %d; 0 is rms, 1 is layer", n->layer);
+    LQ_REQUIRE((n->x_dtype == LQ_F32 || n->x_dtype == LQ_F16) && (n->r_dtype == LQ_F32 || n->r_dtype == n->x_dtype), LQ_ERR_DTYPE,
+               "residual_norm: x is float32 or float16, the residual float32 or of its type");
+    LQ_REQUIRE(n->gate_rows >= 0 && (n->gate ? n->gate_rows > 0 : n->gate_rows == 0), LQ_ERR_VALUE, "residual_norm: a gate of %lld rows",
+               (long long)n->gate_rows);
+    if (n->rows == 0 || n->cols == 0) return LQ_OK;
+    LQ_REQUIRE(n->x && n->y, LQ_ERR_VALUE, "residual_norm: x or y is NULL");
+    LQ_REQUIRE(n->gate_rows == 0 || n->rows % n->gate_rows == 0, LQ_ERR_SHAPE, "residual_norm: a gate of %lld rows for %lld", (long long)n->gate_rows,
+               (long long)n->rows);
+    LQ_REQUIRE(n->cols <= kMaxCols, LQ_ERR_NOT_IMPLEMENTED, "residual_norm: rows of %d; at most %d are built", n->cols, kMaxCols);
+    LQ_REQUIRE(n->rows < int64_t(1) << 31, LQ_ERR_SHAPE, "residual_norm: %lld rows", (long long)n->rows);
+    Args a;
+    a.x = n->x, a.r = n->r, a.gate = n->gate, a.scale = n->scale;
+    a.pre = Norm{n->weight, n->bias}, a.post = Norm{n->post_weight, n->post_bias};
+    a.y = n->y, a.r_out = n->r_out, a.rows = unsigned(n->rows), a.cols = unsigned(n->cols), a.eps = n->eps;
+    if (n->gate) a.per_gate = FastDiv(unsigned(n->rows / n->gate_rows));
+    const hipStream_t st = as_stream(stream);
+    const bool post = n->post != 0;
+    auto of_norm = [&](auto tx, auto tr) {
+        using TX = decltype(tx);
+        using TR = decltype(tr);
+        if (n->layer) launch<TX, TR, true>(a, post, st);
+        else launch<TX, TR, false>(a, post, st);
+    };
+    if (n->x_dtype == LQ_F32) of_norm(float{}, float{});
+    else if (n->r_dtype == LQ_F32) of_norm(_Float16{}, float{});
+    else of_norm(_Float16{}, _Float16{});
+    LQ_CHECK_LAUNCH("residual_norm");
+    return LQ_OK;
+}

@@ -1,0 +1,101 @@
+// Both projections of a gated feed-forward block on group-wise int4 / int8 weights, with the activation and the product:
+//
+//   h[m, n] = act(g[m, n] + bg[n]) * (u[m, n] + bu[n])
+//   g, u [m, n] = sum over groups of  s[n, group] * (sum_{k in group} c[n, k] x[m, k])  +  b[n, group] * (sum_{k in group} x[m, k])
+//
+// for the weights of the gate and of the way up.  Codes enter the matrix instructions as the whole numbers c - 2^(bits-1) that they are
+// (the rest of the code goes to b), so that nothing of a weight is rounded: scales follow in float32, on the sums of a group.  float16 x
+// enters as it is; float32 x as three bfloat16 of 24 bits together (wq_pack.hpp), or as two float16 of 22 (wq_gated_gemm.hip).
+#pragma once
+#include "wq_pack.hpp"
+
+namespace lq {
+namespace gated {
+
+enum Act { kSilu = 0, kGelu = 1, kRelu = 2, kSigmoid = 3 };
+
+struct Weight {
+    const uint32_t* packed;      // [N, K * bits / 32]
+    const float *scales, *biases;  // [N, K / group]
+    const float* bias;           // [N] or NULL
+};
+
+struct Args {
+    const void* x;
+    void* out;
+    Weight w[2];  // gate, up
+    int M, N, K, gs_shift, act;
+};
+
+namespace {
+
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ float activate(int act, float g) {
+    if (act == kSilu) return g / (1.0f + expf(-g));
+    if (act == kGelu) return 0.5f * g * erfcf(g * -0.70710678118654752440f);  // (erfc: nothing cancels below zero)
+    if (act == kRelu) return g < 0.0f ? 0.0f : g;
+    return 1.0f / (1.0f + expf(-g));
+}
+
+// The codes of instruction i of a window (see wq_codes) as float16: c - 2^(bits-1), exactly.  A 4-bit code under the upper bits of 1024
+// is 1024 + c; four bits further up 1024 + 16 c, a sixteenth of which is 64 + c.  Slots as wq_codes has them.
+template <int BITS>
+__device__ __forceinline__ v8h codes_f16(const uint32_t (&wd)[4], int i) {
+    union { v2h h[4]; v8h all; } f;
+    auto half2 = [](uint32_t u) { return __builtin_bit_cast(v2h, u); };
+    if constexpr (BITS == 4) {
+        uint32_t low = 0x000f000fu, high = 0x00f000f0u, one = 0x64006400u;
+        asm("" : "+s"(low));  // in registers: an AND-OR takes one literal at most
+        asm("" : "+s"(high));
+        asm("" : "+v"(one));
+        const uint32_t c = wd[i], d = c >> 8;
+        const v2h off{_Float16(-1032.f), _Float16(-1032.f)}, unit{_Float16(0.0625f), _Float16(0.0625f)}, off16{_Float16(-72.f), _Float16(-72.f)};
+        f.h[0] = half2((c & low) | one) + off;
+        f.h[1] = __builtin_elementwise_fma(half2((c & high) | one), unit, off16);
+        f.h[2] = half2((d & low) | one) + off;
+        f.h[3] = __builtin_elementwise_fma(half2((d & high) | one), unit, off16);
+    } else {
+        const v2h off{_Float16(-1152.f), _Float16(-1152.f)};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t c = wd[(2 * i + j) & 3];
+            f.h[2 * j] = half2(__builtin_amdgcn_perm(0x64646464u, c, 0x04010400u)) + off;
+            f.h[2 * j + 1] = half2(__builtin_amdgcn_perm(0x64646464u, c, 0x04030402u)) + off;
+        }
+    }
+    return f.all;
+}
+
+// Eight consecutive x in the slots of the codes: of 4 bits element d beside d + 4.
+template <int BITS>
+__device__ __forceinline__ v8h slots_f16(uint4 x) {
+    if constexpr (BITS == 8) return __builtin_bit_cast(v8h, x);
+    auto low = [](uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); };
+    auto high = [](uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); };
+    return __builtin_bit_cast(v8h, uint4{low(x.x, x.z), high(x.x, x.z), low(x.y, x.w), high(x.y, x.w)});
+}
+
+// f(BITS, SW) as constants: what a window of 64 lanes x 16 bytes is made of (wq_pack.hpp)
+template <class F>
+int by_window(int bits, int gs, F&& f) {
+    const int sw = wq_swap_mode(bits, gs);
+    using std::integral_constant;
+    if (bits == 4) {
+        if (sw == 0) return f(integral_constant<int, 4>{}, integral_constant<int, 0>{});
+        if (sw == 1) return f(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+        return f(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+    }
+    if (sw == 0) return f(integral_constant<int, 8>{}, integral_constant<int, 0>{});
+    return f(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+}
+
+}  // namespace
+
+// Few rows (wq_gated_rows.hip).  bits 4 or 8, groups of 32, 64 or 128.
+int launch_rows_f16(const Args& a, int bits, hipStream_t st);
+int launch_rows_f32(const Args& a, int bits, hipStream_t st);
+
+}  // namespace gated
+}  // namespace lq

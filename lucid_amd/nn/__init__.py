@@ -379,6 +379,22 @@ class LayerNorm(Module):
         return F.layer_norm(x, self.normalized_shape, self.weight, self.bias, self.eps, self.track_range)
 
 
+class RMSNorm(Module):
+    """``functional.rms_norm`` over the last axis; float32 or float16 in, the same out.  ``residual_norm`` takes ``weight`` and ``eps`` where
+    the norm stands behind a residual connection."""
+
+    def __init__(self, normalized_shape: int, eps: float = 1e-6) -> None:
+        super().__init__()
+        self.normalized_shape, self.eps = int(normalized_shape), float(eps)
+        self.register_buffer("weight", T.tensor(np.ones(normalized_shape, np.float32)))
+
+    def forward(self, x):
+        from . import functional as F
+
+        weight = self.weight if self.weight.device == "hip" else self.weight.to("hip")
+        return F.rms_norm(x, self.normalized_shape, weight, self.eps)
+
+
 class GELU(Module):
     def forward(self, x):
         from . import functional as F

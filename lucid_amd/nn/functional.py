@@ -186,6 +186,149 @@ def paged_attention_qkv(qkv: Tensor, num_heads: int, cache, page_table: Tensor, 
     return out
 
 
+def _vector(name: str, what: str, t, cols: int):
+    """The address of a float32 ``(cols,)`` vector, or None."""
+    if t is None:
+        return None
+    _require_f32_hip(name, t)
+    if t.shape != (cols,):
+        raise _C.ShapeMismatch(f"{name}: {what} has shape {t.shape}, expected {(cols,)}")
+    return t.data_ptr
+
+
+_NORMS = {"rms": 0, "layer": 1}
+
+
+def _residual_norm(name, x, residual, weight, bias, norm, eps, post, post_weight, post_bias, gate, scale, out, residual_out):
+    if not isinstance(x, Tensor) or x.ndim < 1:
+        raise _C.ShapeMismatch(f"{name}: x is a (..., features) tensor")
+    _check_rows(name, "x", x, x.shape)
+    if norm not in _NORMS:
+        raise ValueError(f"{name}: norm {norm!r}; 'rms' or 'layer'")
+    if not post and (post_weight is not None or post_bias is not None):
+        raise ValueError(f"{name}: post_weight and post_bias belong to post=True")
+    cols = x.shape[-1]
+    rows = x.numel // cols if cols else 0
+    gate_rows = 0
+    if residual is not None:
+        _check_rows(name, "residual", residual, x.shape)
+        if residual.dtype != x.dtype and residual.dtype != T.float32:
+            raise _C.DtypeMismatch(f"{name}: x is {x.dtype}, residual {residual.dtype} (x's type or float32)")
+    if gate is not None:
+        if not isinstance(gate, Tensor) or gate.ndim < 1 or gate.shape[-1] != cols:
+            raise _C.ShapeMismatch(f"{name}: gate is a (..., {cols}) tensor")
+        _check_rows(name, "gate", gate, gate.shape)
+        if gate.dtype != x.dtype:
+            raise _C.DtypeMismatch(f"{name}: x is {x.dtype}, gate {gate.dtype}")
+        gate_rows = gate.numel // cols if cols else 0
+        if rows and (gate_rows == 0 or rows % gate_rows):
+            raise _C.ShapeMismatch(f"{name}: a gate of {gate_rows} rows for {rows}")
+    vectors = [_vector(name, what, t, cols) for what, t in (("scale", scale), ("weight", weight), ("bias", bias), ("post_weight", post_weight),
+                                                            ("post_bias", post_bias))]
+    if out is not None:
+        _check_rows(name, "out", out, x.shape)
+        if out.dtype != x.dtype:
+            raise _C.DtypeMismatch(f"{name}: x is {x.dtype}, out {out.dtype}")
+    if residual_out is not None:
+        _check_rows(name, "residual_out", residual_out, x.shape)
+        if residual_out.dtype != residual.dtype:
+            raise _C.DtypeMismatch(f"{name}: residual is {residual.dtype}, residual_out {residual_out.dtype}")
+        if out is not None and residual_out.data_ptr == out.data_ptr and x.numel:
+            raise ValueError(f"{name}: out and residual_out are one tensor")
+    if out is None:
+        out = Tensor.empty(x.shape, x.dtype, "hip")
+    if residual_out is None and residual is not None:
+        residual_out = Tensor.empty(x.shape, residual.dtype, "hip")
+    args = _C.ResidualNormArgs(
+        x.data_ptr, residual.data_ptr if residual is not None else None, gate.data_ptr if rows and gate is not None else None, *vectors, out.data_ptr,
+        residual_out.data_ptr if residual is not None else None, rows, gate_rows if rows else 0, cols, x.dtype.code,
+        (residual if residual is not None else x).dtype.code, _NORMS[norm], 1 if post else 0, float(eps))
+    _C.call("lq_residual_norm", _C.C.byref(args), None)
+    _written(out)
+    if residual is not None:
+        _written(residual_out)
+    return out, residual_out
+
+
+def rms_norm(x: Tensor, normalized_shape, weight: Tensor | None = None, eps: float = 1e-6, out: Tensor | None = None) -> Tensor:
+    """``x / sqrt(mean(x^2) + eps) * weight`` over the last axis; ``x`` float32 or float16, ``weight`` float32 or ``None``.
+    ``out`` may be ``x``."""
+    cols = normalized_shape if isinstance(normalized_shape, int) else int(normalized_shape[-1])
+    if isinstance(x, Tensor) and x.ndim and x.shape[-1] != cols:
+        raise _C.ShapeMismatch(f"rms_norm: last dim {x.shape[-1]} vs normalized_shape {cols}")
+    return _residual_norm("rms_norm", x, None, weight, None, "rms", eps, False, None, None, None, None, out, None)[0]
+
+
+def residual_norm(x: Tensor, residual: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, norm: str = "rms", eps: float = 1e-6,
+                  post: bool = False, post_weight: Tensor | None = None, post_bias: Tensor | None = None, gate: Tensor | None = None,
+                  scale: Tensor | None = None, out: Tensor | None = None, residual_out: Tensor | None = None) -> tuple[Tensor, Tensor]:
+    """The residual connection between two blocks with the norms beside it, in one pass: ``(y, r)`` with
+
+        r = residual + gate * scale * post(x)        y = pre(r)
+
+    ``x`` ``(..., features)`` is what a block gives, float32 or float16, ``residual`` what went past it, of that type or float32; ``y`` has
+    ``x``'s type, ``r`` the residual's.  ``pre``, in front of the next block, has ``weight`` and ``bias``; ``post``, behind this one, is left
+    out without ``post=True`` and has ``post_weight`` and ``post_bias``.  Both are ``norm``: ``"rms"``, ``v / sqrt(mean(v^2) + eps) * weight +
+    bias``, or ``"layer"``, the same of ``v - mean(v)``.  ``gate`` ``(..., features)``, of ``x``'s type, has a row for each of equal runs of
+    ``x``'s rows: one for all, one for each sequence of a batch, one for each token.  ``scale``, the weights and biases are float32
+    ``(features,)``.  In between everything is float32, and ``y`` is made from ``r`` before that is rounded.  At most 32768 features.
+    ``out`` and ``residual_out`` take the results; they may be ``x`` and ``residual``."""
+    if residual is None:
+        raise _C.ShapeMismatch("residual_norm: residual is a tensor of x's shape")
+    return _residual_norm("residual_norm", x, residual, weight, bias, norm, eps, post, post_weight, post_bias, gate, scale, out, residual_out)
+
+
+def verify_drafts(target: Tensor, tokens: Tensor, starts: Tensor, uniforms: Tensor, last_uniforms: Tensor, draft: Tensor | None = None,
+                  out: tuple[Tensor, Tensor] | None = None) -> tuple[Tensor, Tensor]:
+    """Drafted tokens against the target's probabilities: ``(new_tokens, counts)``.
+
+    Sequence ``b`` has the rows ``starts[b]`` to ``starts[b + 1]`` (int32 ``(batch + 1,)``, rising: ``q_starts`` of ``paged_attention``) of a step,
+    its last token and behind it the drafted ones: ``tokens`` int32 ``(rows,)``, what the step was run on.  Row ``i`` of ``target`` ``(rows,
+    vocab)``, float32 or float16, holds the probabilities ``p`` of the token behind row ``i``; row ``i`` of ``draft``, of the same shape and
+    type, those that token ``i + 1`` was drawn from, ``q``.  Without ``draft`` that token was not drawn (``q`` is 1 there and 0 elsewhere).
+
+    In order, token ``x`` behind row ``i`` is accepted if ``uniforms[i] * q[x] < p[x]`` (float32 ``(rows,)`` in [0, 1)).  Behind the accepted
+    ones comes a token drawn with ``last_uniforms[b]`` (float32 ``(batch,)``): from ``max(p - q, 0)`` of the row that refused, from ``p`` of the
+    last row where none did, so that all are distributed as the target's.  It is the lowest token at which the running sum of the
+    weights passes ``last_uniforms[b]`` times their sum, in float64.  Neither ``p`` nor ``q`` need sum to one; what is not positive and finite
+    counts as 0; where no ``p - q`` is positive the token comes from ``p``, and is -1 where no ``p`` is.  A drafted token
+    outside the vocabulary is refused.
+
+    ``new_tokens`` int32 ``(rows,)`` has a sequence's new tokens from ``starts[b]`` on and -1 behind them; ``counts`` int32 ``(batch,)`` says how many
+    they are, at least 1, and 0 of a sequence without rows.  The cache then holds ``counts[b] - 1`` of the drafted tokens' rows.
+    Rows of no sequence (a padded batch) are left as they are in ``out``, which takes the results."""
+    if not isinstance(target, Tensor) or target.ndim != 2:
+        raise _C.ShapeMismatch("verify_drafts: target is a (rows, vocab) tensor")
+    rows, vocab = target.shape
+    _check_rows("verify_drafts", "target", target, target.shape)
+    _check_ids("verify_drafts", "tokens", tokens, (rows,))
+    if not isinstance(starts, Tensor) or starts.ndim != 1 or starts.shape[0] < 1:
+        raise _C.ShapeMismatch("verify_drafts: starts is a (batch + 1,) tensor")
+    batch = starts.shape[0] - 1
+    _check_ids("verify_drafts", "starts", starts, (batch + 1,))
+    for what, t, n in (("uniforms", uniforms, rows), ("last_uniforms", last_uniforms, batch)):
+        _require_f32_hip("verify_drafts", t)
+        if t.shape != (n,):
+            raise _C.ShapeMismatch(f"verify_drafts: {what} has shape {t.shape}, expected {(n,)}")
+    if draft is not None:
+        _check_rows("verify_drafts", "draft", draft, target.shape)
+        if draft.dtype != target.dtype:
+            raise _C.DtypeMismatch(f"verify_drafts: target is {target.dtype}, draft {draft.dtype}")
+    if out is None:
+        new_tokens, counts = Tensor.empty((rows,), T.int32, "hip"), Tensor.empty((batch,), T.int32, "hip")
+        _C.call("lq_fill_bytes", new_tokens.data_ptr, 0xff, new_tokens.nbytes, None)
+    else:
+        new_tokens, counts = out
+        _check_ids("verify_drafts", "out[0]", new_tokens, (rows,))
+        _check_ids("verify_drafts", "out[1]", counts, (batch,))
+    if max(rows, batch, vocab) > _INT_MAX:
+        raise _C.ShapeMismatch(f"verify_drafts: {rows} rows of {vocab} tokens, {batch} sequences")
+    _C.call("lq_verify_drafts", target.data_ptr, draft.data_ptr if draft is not None else None, target.dtype.code, rows, vocab, tokens.data_ptr,
+            starts.data_ptr, batch, uniforms.data_ptr, last_uniforms.data_ptr, new_tokens.data_ptr, counts.data_ptr, None)
+    _written(new_tokens), _written(counts)
+    return new_tokens, counts
+
+
 def conv2d_f32(x: Tensor, weight: Tensor, bias: Tensor | None = None, stride=(1, 1), padding=(0, 0),
                dilation=(1, 1), groups: int = 1) -> Tensor:
     """``F.conv2d`` in float32 with zero padding (``CpuBackend.h:8124-8257``): NCHW input, OIHW

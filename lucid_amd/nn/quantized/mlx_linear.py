@@ -61,3 +61,50 @@ class QuantizedLinearMLX(Module):
     def extra_repr(self) -> str:
         return (f"in_features={self.in_features}, out_features={self.out_features}, bits={self.bits}, "
                 f"group_size={self.group_size}")
+
+
+class QuantizedGatedLinearMLX(Module):
+    """Both projections of a gated feed-forward block, ``act(gate(x)) * up(x)``, on group-wise int4 / int8 weights in one call
+    (``_qgemm.quantized_gated_matmul``); a ``QuantizedLinearMLX`` takes the result back.  Buffers: ``gate_packed_weight``, ``gate_scales``,
+    ``gate_biases``, ``gate_bias`` and the same of ``up``, each as ``QuantizedLinearMLX`` has it.  ``x`` is float32 or float16."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, bits: int = 8, group_size: int = 64,
+                 activation: str = "silu") -> None:
+        super().__init__()
+        if bits not in (4, 8):
+            raise ValueError(f"bits must be 4 or 8, got {bits}")
+        if in_features % group_size:
+            raise ValueError(f"group_size {group_size} must divide in_features {in_features}")
+        if activation not in _qgemm._GATES:
+            raise ValueError(f"activation must be one of {', '.join(_qgemm._GATES)}, got {activation!r}")
+        self.in_features, self.out_features = in_features, out_features
+        self.bits, self.group_size, self.activation = bits, group_size, activation
+        zeros = lambda shape, dt: T.tensor(np.zeros(shape, dt), device="hip")
+        for name in ("gate", "up"):
+            self.register_buffer(f"{name}_packed_weight", zeros((out_features, in_features * bits // 32), np.int32))
+            self.register_buffer(f"{name}_scales", zeros((out_features, in_features // group_size), np.float32))
+            self.register_buffer(f"{name}_biases", zeros((out_features, in_features // group_size), np.float32))
+            self.register_buffer(f"{name}_bias", zeros(out_features, np.float32) if bias else None)
+
+    def forward(self, x: Tensor) -> Tensor:
+        return _qgemm.quantized_gated_matmul(x, (self.gate_packed_weight, self.gate_scales, self.gate_biases),
+                                             (self.up_packed_weight, self.up_scales, self.up_biases), self.activation, self.group_size, self.bits,
+                                             self.gate_bias, self.up_bias)
+
+    @classmethod
+    def from_float(cls, gate, up, bits: int = 8, group_size: int = 64, activation: str = "silu") -> "QuantizedGatedLinearMLX":
+        """Pack the weights of two float ``Linear`` of one shape."""
+        if (gate.in_features, gate.out_features) != (up.in_features, up.out_features):
+            raise _C.ShapeMismatch(f"gate is {gate.in_features} -> {gate.out_features}, up {up.in_features} -> {up.out_features}")
+        q = cls(gate.in_features, gate.out_features, bias=gate.bias is not None or up.bias is not None, bits=bits, group_size=group_size,
+                activation=activation)
+        for name, mod in (("gate", gate), ("up", up)):
+            for part, t in zip(("packed_weight", "scales", "biases"), _qgemm.quantize(mod.weight.to("hip"), group_size, bits)):
+                q.register_buffer(f"{name}_{part}", t)
+            if mod.bias is not None:
+                q.register_buffer(f"{name}_bias", mod.bias.to("hip"))
+        return q
+
+    def extra_repr(self) -> str:
+        return (f"in_features={self.in_features}, out_features={self.out_features}, bits={self.bits}, group_size={self.group_size}, "
+                f"activation={self.activation}")

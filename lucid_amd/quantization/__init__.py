@@ -4,7 +4,7 @@ Names and signatures follow ``lucid/quantization/__init__.py:67-118``.
 """
 
 from ._functional import dequantize, fake_quantize, minmax, quantize, quantize_rows_dynamic
-from ._kv_cache import PagedKVCache, kv_cache_read, kv_cache_write, kv_cache_write_qkv
+from ._kv_cache import PagedKVCache, kv_cache_compact, kv_cache_copy, kv_cache_read, kv_cache_write, kv_cache_write_qkv
 from ._qparams import QParams, calculate_qparams
 from ._qscheme import (
     QDtype,
@@ -46,5 +46,5 @@ __all__ = [
     "QScheme", "per_tensor_affine", "per_tensor_symmetric", "per_channel_affine",
     "per_channel_symmetric", "QDtype", "qint8", "quint8", "qint32", "qint4", "QParams",
     "calculate_qparams", "quantize", "dequantize", "fake_quantize", "minmax", "quantize_rows_dynamic",
-    "PagedKVCache", "kv_cache_write", "kv_cache_write_qkv", "kv_cache_read",
+    "PagedKVCache", "kv_cache_write", "kv_cache_write_qkv", "kv_cache_read", "kv_cache_copy", "kv_cache_compact",
 ]

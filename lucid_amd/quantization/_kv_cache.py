@@ -178,3 +178,38 @@ def kv_cache_read(cache: PagedKVCache, slots: Tensor, dtype=T.float32, out: tupl
     _C.call("lq_kv_cache_read", cache._ref, slots.data_ptr, shape[0], k.data_ptr, v.data_ptr, k.dtype.code, None)
     _written(k), _written(v)
     return k, v
+
+
+def kv_cache_copy(cache: PagedKVCache, src: Tensor, dst: Tensor) -> None:
+    """Copies page ``src[i]`` into page ``dst[i]`` (int32 ``(pages,)``), keys, values and their scales and zero points: what forks a
+    sequence, whose whole pages both then share and whose last one each has for itself.  A pair with a page that is negative or
+    beyond the cache is skipped: what pads a list.  A page may be copied several times; the destinations are distinct, and none is
+    another pair's source."""
+    _check_cache("kv_cache_copy", cache)
+    if not isinstance(src, Tensor) or src.ndim != 1:
+        raise _C.ShapeMismatch("kv_cache_copy: src is a (pages,) tensor")
+    _check_ids("kv_cache_copy", "src", src, src.shape)
+    _check_ids("kv_cache_copy", "dst", dst, src.shape)
+    _C.call("lq_kv_cache_copy", cache._ref, src.data_ptr, dst.data_ptr, src.shape[0], None)
+
+
+def kv_cache_compact(cache: PagedKVCache, page_table: Tensor, keep: Tensor, starts: Tensor) -> None:
+    """Moves the tokens that sequences keep to their beginnings, so that the pages behind them are free.
+
+    Sequence ``b`` keeps the places ``keep[starts[b]:starts[b + 1]]`` (int32 ``(kept,)``, from 0 and rising within a sequence; ``starts`` int32
+    ``(batch + 1,)``, rising from 0 to ``kept``) of its pages ``page_table[b]`` (int32 ``(batch, pages)``); the ``i``-th of them becomes
+    its token ``i``, and its length the number of them (``kv_lens`` of ``paged_attention``).  What lies behind stays as it was.  A token
+    whose old or new place is beyond ``page_table``, or on a page that is negative or beyond the cache, is not moved; one that stays
+    in its place is neither read nor written, so sequences may share pages of such tokens.  Other pages belong to one sequence."""
+    _check_cache("kv_cache_compact", cache)
+    if not isinstance(page_table, Tensor) or page_table.ndim != 2:
+        raise _C.ShapeMismatch("kv_cache_compact: page_table is a (batch, pages) tensor")
+    _check_ids("kv_cache_compact", "page_table", page_table, page_table.shape)
+    if not isinstance(keep, Tensor) or keep.ndim != 1:
+        raise _C.ShapeMismatch("kv_cache_compact: keep is a (kept,) tensor")
+    _check_ids("kv_cache_compact", "keep", keep, keep.shape)
+    batch, width = page_table.shape
+    _check_ids("kv_cache_compact", "starts", starts, (batch + 1,))
+    if max(batch, width) > 0x7fffffff:  # (ctypes takes the low 32 bits of a longer int)
+        raise _C.ShapeMismatch(f"kv_cache_compact: {batch} sequences of {width} pages")
+    _C.call("lq_kv_cache_compact", cache._ref, page_table.data_ptr, width, batch, keep.data_ptr, keep.shape[0], starts.data_ptr, None)

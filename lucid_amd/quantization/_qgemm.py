@@ -66,3 +66,60 @@ def quantized_matmul(x: Tensor, wq: Tensor, scales: Tensor, biases: Tensor, tran
     _C.call("lq_wq_matmul", x.data_ptr, wq.data_ptr, scales.data_ptr, biases.data_ptr, M, N, K,
             int(group_size), int(bits), out.data_ptr, None)
     return out
+
+
+_GATES = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
+
+
+def quantized_gated_matmul(x: Tensor, gate: tuple[Tensor, Tensor, Tensor], up: tuple[Tensor, Tensor, Tensor], activation: str = "silu",
+                           group_size: int = 64, bits: int = 8, gate_bias: Tensor | None = None, up_bias: Tensor | None = None,
+                           out: Tensor | None = None) -> Tensor:
+    """``act(x @ w_gate.T + gate_bias) * (x @ w_up.T + up_bias)``: both projections of a gated feed-forward block, its activation and its
+    product in one call.  ``gate`` and ``up`` are what ``quantize`` gives of ``(out, in)`` weights of one shape; ``x`` ``(..., in)`` is float32 or
+    float16 and so is the result ``(..., out)``, the biases are float32 ``(out,)``.  ``activation``: ``"silu"``, ``"gelu"`` (erf form), ``"relu"`` or
+    ``"sigmoid"``.  Nothing of a weight is rounded beyond its codes.  ``out`` takes the result.  No counterpart in Lucid."""
+    name = "quantized_gated_matmul"
+    if activation not in _GATES:
+        raise ValueError(f"{name}: activation {activation!r}; one of {', '.join(_GATES)}")
+    _check(name, x, *gate, *up)
+    if x.dtype != T.float32 and x.dtype != T.float16:
+        raise _C.DtypeMismatch(f"{name} expects a float32 or float16 activation, got {x.dtype}")
+    if bits not in (4, 8) or group_size not in (32, 64, 128):
+        raise ValueError(f"{name}: bits {bits}, group_size {group_size}; 4 or 8, and 32, 64 or 128")
+    if gate[0].ndim != 2:
+        raise _C.ShapeMismatch(f"{name}: a packed weight is 2-d, got {gate[0].shape}")
+    N = gate[0].shape[0]
+    K = gate[0].shape[1] * 32 // bits
+    for what, (packed, scales, biases), bias in (("gate", gate, gate_bias), ("up", up, up_bias)):
+        if packed.shape != gate[0].shape or K % group_size or scales.shape != (N, K // group_size) or biases.shape != scales.shape:
+            raise _C.ShapeMismatch(f"{name}: {what} is packed {packed.shape}, scales {scales.shape}, biases {biases.shape} in groups of {group_size}; "
+                                   f"gate is packed {gate[0].shape}")
+        if packed.dtype != T.int32 or scales.dtype != T.float32 or biases.dtype != T.float32:
+            raise _C.DtypeMismatch(f"{name}: {what} is int32, float32 and float32, got {packed.dtype}, {scales.dtype} and {biases.dtype}")
+        if bias is not None:
+            _check(name, bias)
+            if bias.dtype != T.float32:
+                raise _C.DtypeMismatch(f"{name}: {what}_bias is float32, got {bias.dtype}")
+            if bias.shape != (N,):
+                raise _C.ShapeMismatch(f"{name}: {what}_bias has shape {bias.shape}, expected {(N,)}")
+    if x.ndim < 1 or x.shape[-1] != K:
+        raise _C.ShapeMismatch(f"{name}: activation {x.shape} against packed ({N}, {K}) weights")
+    shape = (*x.shape[:-1], N)
+    if out is None:
+        out = Tensor.empty(shape, x.dtype, "hip")
+    else:
+        _check(name, out)
+        if out.dtype != x.dtype:
+            raise _C.DtypeMismatch(f"{name}: x is {x.dtype}, out {out.dtype}")
+        if out.shape != shape:
+            raise _C.ShapeMismatch(f"{name}: out has shape {out.shape}, expected {shape}")
+    M = x.numel // K if K else 0
+    if max(M, N, K) > 0x7fffffff:  # (ctypes takes the low 32 bits of a longer int)
+        raise _C.ShapeMismatch(f"{name}: {M} x {N} x {K}")
+    pair = _C.C.c_void_p * 2
+    args = _C.WqGatedArgs(x.data_ptr, out.data_ptr, pair(gate[0].data_ptr, up[0].data_ptr), pair(gate[1].data_ptr, up[1].data_ptr),
+                          pair(gate[2].data_ptr, up[2].data_ptr), pair(*(b.data_ptr if b is not None else None for b in (gate_bias, up_bias))), M, N, K,
+                          int(group_size), int(bits), _GATES[activation], x.dtype.code)
+    _C.call("lq_wq_gated_matmul", _C.C.byref(args), None)
+    out._grid = out._range = None
+    return out

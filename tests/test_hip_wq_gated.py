@@ -1,0 +1,194 @@
+"""Gated projections on group-wise weights against float64: exactly on numbers that float32 holds, and within its rounding on others."""
+
+import numpy as np
+import pytest
+from scipy.special import erfc
+
+import lucid_amd as L
+import lucid_amd.nn as nn
+import lucid_amd.nn.quantized as nnq
+import oracle.wq_group as W
+from lucid_amd.quantization import _qgemm
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24  # half a step of float32, relative
+
+
+def hip(a):
+    return L.tensor(np.ascontiguousarray(a), device="hip")
+
+
+ACTS = {"silu": lambda g: g / (1 + np.exp(-g)), "gelu": lambda g: 0.5 * g * erfc(-g / np.sqrt(2)), "relu": lambda g: np.maximum(g, 0),
+        "sigmoid": lambda g: 1 / (1 + np.exp(-g))}
+
+
+def weight64(packed, s, b, gs, bits):
+    return W.unpack(packed, bits) * np.repeat(s.astype(np.float64), gs, 1) + np.repeat(b.astype(np.float64), gs, 1)
+
+
+# rows on both sides of every number of row tiles, columns that end inside one, K of part of a window, of odd numbers of windows and of groups
+SHAPES = [(1, 1, 32, 32), (1, 16, 64, 64), (1, 17, 128, 128), (1, 11008, 4096, 64), (2, 100, 96, 32), (3, 33, 1056, 32), (15, 48, 640, 128), (16, 31, 2112, 64),
+          (17, 130, 1024, 128), (31, 64, 480, 32), (32, 65, 512, 64), (33, 257, 384, 128), (48, 1033, 4608, 64), (63, 40, 320, 64), (64, 129, 256, 128),
+          (65, 256, 544, 32), (97, 300, 1152, 128), (128, 128, 4096, 64), (129, 511, 192, 64), (200, 96, 96, 32), (256, 257, 1024, 64), (257, 640, 640, 128),
+          (333, 1033, 576, 32), (400, 2049, 256, 128)]
+
+
+@pytest.mark.parametrize("M,N,K,gs", SHAPES)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_exact_on_exact_numbers(M, N, K, gs, bits, dtype):
+    """Small whole x, scales of powers of two and whole biases keep every sum a multiple of 1/64 below 2^18: one code, scale, group or row out of place
+    shows.  (Codes of 8 bits in a band of 32 about the middle and at its ends, so that sums stay small.)"""
+    rng = np.random.default_rng(M + N + K + bits)
+    x = rng.integers(-3, 4, (M, K)).astype(dtype)
+    x[rng.random((M, K)) < 0.5] = 0
+    packs, g64 = [], []
+    for scale in (1.0, 2.0 ** -6):
+        codes = rng.integers(0, 16, (N, K)) if bits == 4 else rng.integers(112, 144, (N, K))
+        codes[rng.random((N, K)) < 0.01] = (1 << bits) - 1
+        codes[rng.random((N, K)) < 0.01] = 0
+        per = 32 // bits
+        packed = (codes.astype(np.uint32).reshape(N, K // per, per) << (np.arange(per, dtype=np.uint32) * np.uint32(bits))).sum(-1, dtype=np.uint64).astype(np.uint32).view(np.int32)
+        s = (scale * rng.integers(1, 3, (N, K // gs))).astype(np.float32)
+        b = (-(1 << (bits - 1)) * s + scale * rng.integers(-4, 5, s.shape)).astype(np.float32)
+        packs.append((packed, s, b))
+        bias = (scale * rng.integers(-50, 51, N)).astype(np.float32)
+        g64.append((x.astype(np.float64) @ weight64(packed, s, b, gs, bits).T + bias, bias))
+    y = _qgemm.quantized_gated_matmul(hip(x), *(tuple(map(hip, p)) for p in packs), activation="relu", group_size=gs, bits=bits,
+                                      gate_bias=hip(g64[0][1]), up_bias=hip(g64[1][1]))
+    assert y.shape == (M, N) and y.dtype.np == dtype
+    assert max(abs(g).max() for g, _ in g64) < 2 ** 18
+    with np.errstate(over="ignore"):
+        want = (np.maximum(g64[0][0], 0) * g64[1][0]).astype(np.float32).astype(dtype)
+    assert np.array_equal(y.numpy(), want)
+
+
+def bound(x, parts, gs, bits, act, bias):
+    """The result in float64 and how far float32 arithmetic may be from it.  A projection is a sum of products (c - half) s x and of group terms
+    (b + half s) (sum of x), accumulated in at most K / 8 roundings (a matrix instruction has 32 k, a group two multiply-adds): of random signs
+    they stay below 4 sqrt(K / 8) U of the terms' magnitudes together, four deviations and more.  b + half s rounds once, x to 22 bits, and at 2^-38 of its
+    row's largest value."""
+    half, K = 1 << (bits - 1), x.shape[1]
+    out = []
+    for (packed, s, b), bb in zip(parts, bias):
+        s64, b64 = np.repeat(s.astype(np.float64), gs, 1), np.repeat(b.astype(np.float64), gs, 1)
+        c = W.unpack(packed, bits).astype(np.float64) - half
+        size = abs(x) @ (abs(c * s64) + abs(b64) + half * abs(s64)).T + abs(bb)
+        floor = 2.0 ** -38 * abs(x).max(-1, keepdims=True) * abs(c * s64).sum(-1)
+        out.append((x @ (c * s64 + b64 + half * s64).T + bb, (4 * np.sqrt(K / 8) + 8) * U * size + floor))
+    (g, eg), (u, eu) = out
+    a = ACTS[act](g)
+    # slopes of the activations are at most 1.13; exp and erfc round by a few units, and exp(-g) by U |g| more through its argument
+    ea = 1.13 * eg + 8 * U * (1 + abs(g)) * abs(a) + U * 2.0 ** -20
+    return a * u, ea * abs(u) + abs(a) * eu + ea * eu + U * abs(a * u)
+
+
+@pytest.mark.parametrize("M,N,K,gs", [(1, 256, 512, 64), (1, 300, 4096, 128), (5, 100, 256, 32), (16, 512, 4096, 64), (40, 96, 256, 64), (64, 257, 2048, 64),
+                                      (96, 128, 1024, 32), (150, 333, 1152, 128), (300, 96, 4096, 128), (513, 200, 768, 64)])
+@pytest.mark.parametrize("bits,dtype", [(4, np.float32), (8, np.float32), (4, np.float16), (8, np.float16)])
+@pytest.mark.parametrize("act", list(ACTS))
+def test_against_float64(M, N, K, gs, bits, dtype, act):
+    rng = np.random.default_rng(M + N + K + bits)
+    x = (rng.standard_normal((M, K)) * (1 + 9 * (rng.random(K) < 0.02)) + 0.3).astype(dtype)
+    parts = [W.quantize((0.03 * rng.standard_normal((N, K))).astype(np.float32), gs, bits) for _ in range(2)]
+    bias = [(0.2 * rng.standard_normal(N)).astype(np.float32) for _ in range(2)]
+    with_bias = act in ("silu", "relu")
+    y = _qgemm.quantized_gated_matmul(hip(x), *(tuple(map(hip, p)) for p in parts), activation=act, group_size=gs, bits=bits,
+                                      **({"gate_bias": hip(bias[0]), "up_bias": hip(bias[1])} if with_bias else {})).numpy()
+    want, e = bound(x.astype(np.float64), parts, gs, bits, act, bias if with_bias else [np.zeros(N)] * 2)
+    info = np.finfo(dtype)
+    assert (abs(y - want) <= e + (abs(want) + e) * info.eps / 2 + info.tiny * info.eps).all()
+
+
+@pytest.mark.parametrize("M", [3, 100, 300])
+def test_rows_of_all_sizes_side_by_side(M):
+    """Each float32 row keeps its own bits: rows of 1e-30 to 1e30, a row of zeros, rows with one value far above the others."""
+    rng = np.random.default_rng(M)
+    N, K, gs = 70, 256, 64
+    x = rng.standard_normal((M, K))
+    x *= 10.0 ** rng.integers(-12, 13, (M, 1))
+    x[0], x[1, 7] = 0, 3e4 * abs(x[1]).max()
+    x = x.astype(np.float32)
+    parts = [W.quantize((0.03 * rng.standard_normal((N, K))).astype(np.float32), gs, 8) for _ in range(2)]
+    y = _qgemm.quantized_gated_matmul(hip(x), *(tuple(map(hip, p)) for p in parts), activation="relu", group_size=gs, bits=8).numpy()
+    want, e = bound(x.astype(np.float64), parts, gs, 8, "relu", [np.zeros(N)] * 2)
+    assert (abs(y - want) <= e + abs(want) * U + 1e-45).all()
+
+
+@pytest.mark.parametrize("M", [2, 90, 300])
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_what_is_not_finite_stays_in_its_row(M, dtype):
+    rng = np.random.default_rng(M)
+    parts = [tuple(map(hip, W.quantize(rng.standard_normal((50, 192)).astype(np.float32), 64, 4))) for _ in range(2)]
+    x = rng.standard_normal((M, 192)).astype(dtype)
+    clean = _qgemm.quantized_gated_matmul(hip(x), *parts, activation="sigmoid", group_size=64, bits=4).numpy()
+    x[0, 3] = np.nan
+    x[M - 1, 100] = np.inf
+    y = _qgemm.quantized_gated_matmul(hip(x), *parts, activation="sigmoid", group_size=64, bits=4).numpy()
+    assert np.isnan(y[0]).all() and not np.isfinite(y[M - 1]).any()
+    assert np.array_equal(y[1:M - 1], clean[1:M - 1])
+
+
+def test_results_in_a_given_place():
+    """Rows in the middle of a larger tensor: those around them stay."""
+    rng = np.random.default_rng(1)
+    parts = [tuple(map(hip, W.quantize(rng.standard_normal((33, 128)).astype(np.float32), 32, 8))) for _ in range(2)]
+    for M in (5, 70, 260):
+        x = hip(rng.standard_normal((M, 128)).astype(np.float32))
+        big = hip(np.full((M + 5, 33), 7, np.float32))
+        out = big.row_range(2, M + 2)
+        got = _qgemm.quantized_gated_matmul(x, *parts, group_size=32, bits=8, out=out)
+        assert got is out
+        want = _qgemm.quantized_gated_matmul(x, *parts, group_size=32, bits=8).numpy()
+        all_rows = big.numpy()
+        assert np.array_equal(all_rows[2:M + 2], want) and (all_rows[:2] == 7).all() and (all_rows[M + 2:] == 7).all()
+
+
+def test_no_rows_no_columns_and_leading_axes():
+    rng = np.random.default_rng(2)
+    w = lambda n: tuple(map(hip, W.quantize(rng.standard_normal((n, 64)).astype(np.float32), 32, 4)))
+    gate, up = w(20), w(20)
+    assert _qgemm.quantized_gated_matmul(hip(np.zeros((0, 64), np.float32)), gate, up, group_size=32, bits=4).shape == (0, 20)
+    x = rng.standard_normal((2, 3, 64)).astype(np.float32)
+    y = _qgemm.quantized_gated_matmul(hip(x), gate, up, group_size=32, bits=4).numpy()
+    flat = _qgemm.quantized_gated_matmul(hip(x.reshape(6, 64)), gate, up, group_size=32, bits=4).numpy()
+    assert y.shape == (2, 3, 20) and np.array_equal(y.reshape(6, 20), flat)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_the_block_as_modules(bits):
+    """A gated feed-forward block on packed weights: the module's result is the call's, and the way back takes it."""
+    gate, up, down = nn.Linear(256, 672), nn.Linear(256, 672, bias=False), nn.Linear(672, 256)
+    m = nnq.QuantizedGatedLinearMLX.from_float(gate, up, bits=bits, group_size=32)
+    back = nnq.QuantizedLinearMLX.from_float(down, bits=bits, group_size=32)
+    x = np.random.default_rng(bits).standard_normal((9, 256)).astype(np.float32)
+    h = m(hip(x))
+    parts = [W.quantize(lin.weight.numpy(), 32, bits) for lin in (gate, up)]
+    want, e = bound(x.astype(np.float64), parts, 32, bits, "silu", [gate.bias.numpy(), np.zeros(672)])
+    assert (abs(h.numpy() - want) <= e + abs(want) * U).all()
+    y = back(h).numpy()
+    w = weight64(*W.quantize(down.weight.numpy(), 32, bits), 32, bits)
+    assert (abs(y - (h.numpy() @ w.T + down.bias.numpy())) <= 1e-4 * max(1.0, abs(y).max())).all()
+    q = nnq.QuantizedGatedLinearMLX(256, 672, bits=bits, group_size=32)
+    q.load_state_dict(m.state_dict())
+    assert np.array_equal(q(hip(x)).numpy(), h.numpy())
+
+
+@pytest.mark.parametrize("M", [1, 20, 300])
+def test_replayed_from_two_graphs(M):
+    rng = np.random.default_rng(M)
+    graphs = []
+    for N, dtype in ((300, np.float32), (170, np.float16)):
+        parts = [tuple(map(hip, W.quantize(rng.standard_normal((N, 256)).astype(np.float32), 64, 4))) for _ in range(2)]
+        x = hip(rng.standard_normal((M, 256)).astype(dtype))
+        call = lambda x=x, parts=parts: _qgemm.quantized_gated_matmul(x, *parts, group_size=64, bits=4)
+        call()
+        with L.graph.capture() as g:
+            y = call()
+        graphs.append((g, x, y, call))
+    for _ in range(3):
+        for g, x, y, call in graphs:
+            x.copy_from(rng.standard_normal((M, 256)).astype(x.dtype.np))
+            g.replay()
+            L.synchronize()
+            assert np.array_equal(y.numpy(), call().numpy())
