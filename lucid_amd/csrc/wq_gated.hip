@@ -25,5 +25,10 @@ extern "C" int lq_wq_gated_matmul(const lq_wq_gated_args* g, lq_stream stream) {
     LQ_REQUIRE(a.x && a.out, LQ_ERR_VALUE, "quantized_gated_matmul: NULL pointer");
     LQ_REQUIRE(a.x != a.out, LQ_ERR_VALUE, "quantized_gated_matmul: the result cannot take x's place");
     const hipStream_t st = as_stream(stream);
+    // (offsets of codes are 32-bit in the kernel of many rows)
+    if (a.M > 64 && size_t(a.N) * a.K * g->bits / 8 < 0x7fffffffull) {
+        if (g->dtype == LQ_F16) return g->bits == 4 ? gated::launch_gemm_f16_4(a, st) : gated::launch_gemm_f16_8(a, st);
+        return g->bits == 4 ? gated::launch_gemm_f32_4(a, st) : gated::launch_gemm_f32_8(a, st);
+    }
     return g->dtype == LQ_F16 ? gated::launch_rows_f16(a, g->bits, st) : gated::launch_rows_f32(a, g->bits, st);
 }

@@ -5,7 +5,7 @@
 //
 // for the weights of the gate and of the way up.  Codes enter the matrix instructions as the whole numbers c - 2^(bits-1) that they are
 // (the rest of the code goes to b), so that nothing of a weight is rounded: scales follow in float32, on the sums of a group.  float16 x
-// enters as it is; float32 x as three bfloat16 of 24 bits together (wq_pack.hpp), or as two float16 of 22 (wq_gated_gemm.hip).
+// enters as it is; float32 x as three bfloat16 of 24 bits together (wq_pack.hpp), or as two float16 of 22 (wq_gated_gemm.hpp).
 #pragma once
 #include "wq_pack.hpp"
 
@@ -96,6 +96,11 @@ int by_window(int bits, int gs, F&& f) {
 // Few rows (wq_gated_rows.hip).  bits 4 or 8, groups of 32, 64 or 128.
 int launch_rows_f16(const Args& a, int bits, hipStream_t st);
 int launch_rows_f32(const Args& a, int bits, hipStream_t st);
+// Many rows (wq_gated_gemm.hpp), by type and bits; weights below 2 GiB.
+int launch_gemm_f16_4(const Args& a, hipStream_t st);
+int launch_gemm_f16_8(const Args& a, hipStream_t st);
+int launch_gemm_f32_4(const Args& a, hipStream_t st);
+int launch_gemm_f32_8(const Args& a, hipStream_t st);
 
 }  // namespace gated
 }  // namespace lq

@@ -1,0 +1,368 @@
+// Gated projections of many rows (wq_gated.hpp has the mathematics): bound by the matrix cores and the vector work beside them.
+//
+// gated_prepare_kernel lays out, once a call, what every block would otherwise make again: x in operand order (a fragment = 16 rows x 32 k
+// of one part = 1 KiB, the lanes' 16 bytes in lane order), its sums over the groups and the groups' b + 2^(bits-1) s as operands of bfloat16
+// parts, and the scales group after group.  float16 x enters as it is; a float32 row is multiplied by the power of two that brings its
+// largest value below 2^15 and enters as two float16, hi = x rounded, lo = x - hi rounded: 22 bits, or 2^-39 of the largest value.
+//
+// gated_gemm_kernel: a block of four wavefronts takes 16 MT rows x 128 columns of both weights, a wavefront all rows x 32 columns of each, so
+// that no code is turned into float16 twice in a block.  What a stage of 64 k needs comes from memory straight into LDS in pieces of
+// 1 KiB per wavefront and instruction, in a ring of stages: every wavefront issues as many loads per stage, so that "stage s has arrived"
+// is a count of outstanding loads.  The products of a group (at most 64 k) go to accumulators of their own, and from there with their scale to
+// the sums.  The terms of b come last, as a product over the groups of three bfloat16 parts of each side, which leaves 2^-24 of them; of a
+// float16 x two parts, 2^-16, a sixteenth of what the result rounds.
+#pragma once
+#include <algorithm>
+
+#include "wq_gated.hpp"
+
+namespace lq {
+namespace gated {
+namespace {
+
+constexpr int kPiece = 1024;  // bytes one wavefront moves into LDS with one instruction
+constexpr int kCols = 128;    // of a block, of each weight
+
+__host__ __device__ constexpr int sum_parts(int parts) { return parts == 1 ? 2 : 3; }
+
+struct Prepared {
+    char* x;          // [stage][row tile][2][part] pieces
+    char* sums;       // [row tile][group step][sum part] pieces: groups as k
+    char* biases;     // [weight][column tile of 16][group step][sum part] pieces
+    float* scales;    // [group][block of columns][weight][128]
+    float* unscale;   // [row] of float32 x: what its row was multiplied by, inverse
+    int mtiles, stages, group_steps, tiles_n;
+};
+
+// The power of two of each row: one wavefront a row.
+__global__ __launch_bounds__(256) void gated_row_scale_kernel(const float* __restrict__ x, int M, int K, float* __restrict__ unscale) {
+    const int m = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (m >= M) return;
+    const float* row = x + size_t(m) * K;
+    float top = 0.f;
+    for (int k = lane * 4; k < K; k += 256) {  // K is a multiple of 32
+        float4 v;
+        __builtin_memcpy(&v, row + k, 16);
+        top = fmaxf(fmaxf(fmaxf(top, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    if (lane == 0) {
+        // top = 2^e t with t in [0.5, 1): times 2^(15 - e), within what a float32 can say.  (Infinite rows stay: they give no number.)
+        int e = 15;
+        if (top > 0.f && top < __builtin_inff()) frexpf(top, &e);
+        e = e < -111 ? -111 : e;
+        unscale[m] = ldexpf(1.0f, e - 15);
+    }
+}
+
+// Two kinds of blocks.  The first `x_blocks`: 16 rows x 128 k, a thread has eight k.  The others: 64 columns of a weight, a wavefront eight groups.
+template <class T, int PARTS, int BITS>
+__global__ __launch_bounds__(256) void gated_prepare_kernel(Args a, Prepared p, unsigned x_blocks) {
+    constexpr int SP = sum_parts(PARTS);
+    const int gs = 1 << a.gs_shift;
+    if (blockIdx.x >= x_blocks) {
+        const unsigned i = blockIdx.x - x_blocks, across = unsigned(p.tiles_n) * (kCols / 64), which = (i / across) & 1, lane = threadIdx.x & 63;
+        const int octet = int(i / across / 2) * 4 + int(threadIdx.x >> 6), n = int(i % across) * 64 + int(lane), groups = a.K >> a.gs_shift;
+        if (octet >= p.group_steps * 4) return;
+        const Weight& w = a.w[which];
+        float b[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int g = octet * 8 + e;
+            const bool there = n < a.N && g < groups;
+            const float s = there ? w.scales[size_t(n) * groups + g] : 0.f;
+            b[e] = there ? w.biases[size_t(n) * groups + g] - float(kWqCentre<BITS>) * s : 0.f;
+            // (what a stage past K asks for lies within group_steps * 32 groups)
+            p.scales[(size_t(g) * p.tiles_n + n / kCols) * (2 * kCols) + which * kCols + n % kCols] = s;
+        }
+        uint32_t d[3][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) wq_split3x2(b[2 * j], b[2 * j + 1], d[0][j], d[1][j], d[2][j]);
+        const size_t tile = size_t(which) * p.tiles_n * (kCols / 16) + n / 16;
+#pragma unroll
+        for (int part = 0; part < SP; ++part)
+            reinterpret_cast<uint4*>(p.biases)[((tile * p.group_steps + octet / 4) * SP + part) * 64 + n % 16 + 16 * (octet % 4)] =
+                uint4{d[part][0], d[part][1], d[part][2], d[part][3]};
+        return;
+    }
+    const int mt = int(blockIdx.x % unsigned(p.mtiles)), pair = int(blockIdx.x / unsigned(p.mtiles));
+    const int oct = threadIdx.x & 15, row = threadIdx.x >> 4, m = mt * 16 + row, k = pair * 128 + oct * 8, stage = pair * 2 + (oct >> 3);
+    const bool there = m < a.M && k < a.K;  // K is a multiple of 32
+    float v[8];
+    uint4 piece[PARTS];
+    if constexpr (PARTS == 1) {
+        uint4 raw{0u, 0u, 0u, 0u};
+        if (there) __builtin_memcpy(&raw, static_cast<const _Float16*>(a.x) + size_t(m) * a.K + k, 16);
+        const v8h h = __builtin_bit_cast(v8h, raw);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = float(h[e]);
+        piece[0] = __builtin_bit_cast(uint4, slots_f16<BITS>(raw));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        if (there) {
+            __builtin_memcpy(v, static_cast<const float*>(a.x) + size_t(m) * a.K + k, 32);
+            const float f = 1.0f / p.unscale[m];  // (powers of two)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= f;
+        }
+        v8h hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) hi[e] = _Float16(v[e]), lo[e] = _Float16(v[e] - float(hi[e]));
+        piece[0] = __builtin_bit_cast(uint4, slots_f16<BITS>(__builtin_bit_cast(uint4, hi)));
+        piece[1] = __builtin_bit_cast(uint4, slots_f16<BITS>(__builtin_bit_cast(uint4, lo)));
+    }
+    if (stage < p.stages) {
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part)
+            reinterpret_cast<uint4*>(p.x)[(((size_t(stage) * p.mtiles + mt) * 2 + ((oct >> 2) & 1)) * PARTS + part) * 64 + row + 16 * (oct & 3)] = piece[part];
+    }
+    float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    sum += __shfl_xor(sum, 1, 64);
+    sum += __shfl_xor(sum, 2, 64);
+    if (gs >= 64) sum += __shfl_xor(sum, 4, 64);
+    if (gs == 128) sum += __shfl_xor(sum, 8, 64);
+    const int g = k >> a.gs_shift;
+    if ((oct & (gs / 8 - 1)) == 0 && g < p.group_steps * 32) {
+        uint32_t d[3];
+        wq_split3x2(sum, 0.f, d[0], d[1], d[2]);
+#pragma unroll
+        for (int part = 0; part < SP; ++part)
+            reinterpret_cast<uint16_t*>(p.sums)[(((size_t(mt) * p.group_steps + g / 32) * SP + part) * 64 + row + 16 * (g % 32 / 8)) * 8 + g % 8] = uint16_t(d[part]);
+    }
+}
+
+// What a stage of one block is made of, in pieces.
+template <int PARTS, int BITS, int GS, int MT>
+struct Stage {
+    static constexpr int SEGS = GS == 32 ? 2 : 1;     // groups of a stage
+    static constexpr int X = 2 * MT * PARTS;          // fragments
+    static constexpr int S = SEGS;                    // 128 scales of both weights
+    static constexpr int W = 2 * BITS;                // 128 rows of 8 BITS bytes, of both
+    static constexpr int PIECES = X + S + W;
+    static constexpr int PER_WAVE = (PIECES + 3) / 4;
+    static constexpr int FIT = 80 / PIECES;  // two blocks a CU
+    static constexpr int RING = FIT > 4 ? 4 : FIT;
+    static_assert(RING >= 2 && PER_WAVE * (RING - 2) <= 63, "");
+};
+
+// s_waitcnt immediate for vmcnt <= n and every LDS read done
+constexpr int vmcnt_lds(int n) { return (n & 0xF) | ((n >> 4) << 14) | (0x7 << 4); }
+
+template <class T, int PARTS, int BITS, int GS, int MT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void gated_gemm_kernel(Args a, Prepared p, int tiles_m) {
+    using S = Stage<PARTS, BITS, GS, MT>;
+    constexpr int SP = sum_parts(PARTS);
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = lane & 15, q = lane >> 4;
+    // every XCD gets a contiguous range of tiles, row tiles first: its L2 then reads a weight row once
+    const int nblk = gridDim.x, xcd = blockIdx.x & 7, quot = nblk >> 3, rem = nblk & 7;
+    const int lid = xcd * quot + (xcd < rem ? xcd : rem) + (int(blockIdx.x) >> 3);
+    const int tn = lid / tiles_m, tm = lid - tn * tiles_m;
+
+    // ---- the loads of a stage: piece u * 4 + wave (the last round repeats pieces: the counts stay equal)
+    constexpr int ROW = 8 * BITS, CH = ROW / 16;  // bytes of codes per row and stage; 16-byte chunks
+    const unsigned row_bytes = unsigned(a.K) * BITS / 8, w_last = unsigned(a.N) * row_bytes - 16;
+    const char* src[S::PER_WAVE];
+    unsigned off[S::PER_WAVE];
+#pragma unroll
+    for (int u = 0; u < S::PER_WAVE; ++u) {
+        int at = u * 4 + wave;
+        at = at < S::PIECES ? at : at - 4;
+        off[u] = unsigned(lane) * 16;
+        if (at < S::X) {
+            src[u] = p.x + size_t(tm) * (S::X * kPiece) + at * kPiece;
+        } else if (at < S::X + S::S) {
+            src[u] = reinterpret_cast<const char*>(p.scales) + (size_t(at - S::X) * p.tiles_n + tn) * kPiece;
+        } else {
+            // the chunks of a row change places with its number, so that the 16 rows of an operand lie in different banks
+            const int i = at - (S::X + S::S), which = i / BITS, r = (i - which * BITS) * (64 / CH) + lane / CH;
+            const int n = tn * kCols + r < a.N ? tn * kCols + r : a.N - 1;
+            src[u] = reinterpret_cast<const char*>(which ? a.w[1].packed : a.w[0].packed);
+            off[u] = unsigned(n) * row_bytes + unsigned((lane % CH) ^ ((r / (16 / CH)) % CH)) * 16;
+        }
+    }
+    auto load_stage = [&](int s, int slot) {
+        const int sc = s < p.stages ? s : p.stages - 1;  // past the end: any stage, to keep the count
+#pragma unroll
+        for (int u = 0; u < S::PER_WAVE; ++u) {
+            int at = u * 4 + wave;
+            at = at < S::PIECES ? at : at - 4;
+            const char* base = src[u];
+            unsigned o = off[u];
+            if (at < S::X) {
+                base += size_t(sc) * p.mtiles * (2 * PARTS * kPiece);
+            } else if (at < S::X + S::S) {
+                base += size_t(GS == 128 ? sc >> 1 : sc * S::SEGS) * p.tiles_n * kPiece;
+            } else {
+                // a stage past K runs past its row: into the next ones, or at the end of the weight onto its last bytes (its x is zero)
+                const unsigned from = unsigned(sc) * ROW + o;
+                o = from < w_last ? from : w_last;
+            }
+            __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(base + o),
+                                             (__attribute__((address_space(3))) void*)(smem + (slot * S::PIECES + at) * kPiece), 16, 0, 0);
+        }
+    };
+
+    v4f y[4][MT];  // columns 0 .. 15 and 16 .. 31 of the gate, then of the other
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) y[j][i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < S::RING - 1; ++s) load_stage(s, s);
+    int slot = 0;
+    for (int s = 0; s < p.stages; ++s) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(vmcnt_lds(S::PER_WAVE * (S::RING - 2)));
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        load_stage(s + S::RING - 1, slot == 0 ? S::RING - 1 : slot - 1);  // (the slot that everybody has just left)
+        const char* base = smem + slot * (S::PIECES * kPiece);
+        slot = slot + 1 == S::RING ? 0 : slot + 1;
+        const char* codes = base + (S::X + S::S) * kPiece;
+        v8h x[2][MT][PARTS];
+#pragma unroll
+        for (int ii = 0; ii < 2; ++ii)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part)
+                    x[ii][i][part] = *reinterpret_cast<const v8h*>(base + ((i * 2 + ii) * PARTS + part) * kPiece + lane * 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int which = j >> 1, r = wave * 32 + (j & 1) * 16 + ln;
+            v8h c[2];
+            float f[S::SEGS];
+#pragma unroll
+            for (int ii = 0; ii < 2; ++ii) {
+                uint32_t wd[4] = {0u, 0u, 0u, 0u};
+                const char* row = codes + which * (BITS * kPiece) + r * ROW;
+                if constexpr (BITS == 4) wd[0] = *reinterpret_cast<const uint32_t*>(row + (ii ^ ((r >> 3) & 1)) * 16 + q * 4);
+                else __builtin_memcpy(wd, __builtin_assume_aligned(row + ((ii * 2 + (q >> 1)) ^ ((r >> 2) & 3)) * 16 + (q & 1) * 8, 8), 8);
+                c[ii] = codes_f16<BITS>(wd, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < S::SEGS; ++e) f[e] = *reinterpret_cast<const float*>(base + (S::X + e) * kPiece + (which * kCols + r) * 4);
+            v4f acc[S::SEGS][MT];
+#pragma unroll
+            for (int ii = 0; ii < 2; ++ii)
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        const int e = S::SEGS == 2 ? ii : 0;
+                        const bool first = part == 0 && (S::SEGS == 2 || ii == 0);
+                        acc[e][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[ii][i][part], c[ii], first ? v4f{0.f, 0.f, 0.f, 0.f} : acc[e][i], 0, 0, 0);
+                    }
+#pragma unroll
+            for (int e = 0; e < S::SEGS; ++e)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int r4 = 0; r4 < 4; ++r4) y[j][i][r4] = __builtin_fmaf(f[e], acc[e][i][r4], y[j][i][r4]);
+        }
+    }
+    // the terms of b: hi hi, then what is 2^-8 of it, then (three parts) 2^-16
+#pragma unroll 1
+    for (int g = 0; g < p.group_steps; ++g) {
+        v8bf sums[MT][SP];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int part = 0; part < SP; ++part)
+                sums[i][part] = __builtin_bit_cast(v8bf, reinterpret_cast<const uint4*>(p.sums)[((size_t(tm * MT + i) * p.group_steps + g) * SP + part) * 64 + lane]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const size_t tile = size_t(j >> 1) * p.tiles_n * (kCols / 16) + tn * (kCols / 16) + wave * 2 + (j & 1);
+            v8bf b[SP];
+#pragma unroll
+            for (int part = 0; part < SP; ++part)
+                b[part] = __builtin_bit_cast(v8bf, reinterpret_cast<const uint4*>(p.biases)[((tile * p.group_steps + g) * SP + part) * 64 + lane]);
+#pragma unroll
+            for (int order = SP - 1; order >= 0; --order)
+#pragma unroll
+                for (int part = 0; part <= order; ++part)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) y[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sums[i][part], b[order - part], y[j][i], 0, 0, 0);
+        }
+    }
+    __builtin_amdgcn_s_waitcnt(vmcnt_lds(0));  // the loads past the end have landed before the LDS is given up
+    // accumulator element r of a lane: row 4 * quarter + r, column lane % 16
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj) {
+        const int n = tn * kCols + wave * 32 + jj * 16 + ln;
+        if (n >= a.N) continue;
+        const float bg = a.w[0].bias ? a.w[0].bias[n] : 0.f, bu = a.w[1].bias ? a.w[1].bias[n] : 0.f;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int m = (tm * MT + i) * 16 + q * 4 + r;
+                if (m >= a.M) continue;
+                const float f = PARTS == 1 ? 1.0f : p.unscale[m];
+                const float g = y[jj][i][r] * f + bg, v = y[2 + jj][i][r] * f + bu;
+                static_cast<T*>(a.out)[size_t(m) * a.N + n] = T(activate(a.act, g) * v);
+            }
+    }
+}
+
+template <class T, int PARTS, int BITS, int GS, int MT>
+int launch_gemm_tile(const Args& a, hipStream_t st) {
+    using S = Stage<PARTS, BITS, GS, MT>;
+    constexpr int SP = sum_parts(PARTS);
+    Prepared p;
+    const int tiles_m = (a.M + 16 * MT - 1) / (16 * MT);
+    p.mtiles = tiles_m * MT, p.stages = (a.K + 63) / 64, p.group_steps = (a.K / GS + 31) / 32, p.tiles_n = (a.N + kCols - 1) / kCols;
+    const size_t x_bytes = size_t(p.stages) * p.mtiles * (2 * PARTS * kPiece), sum_bytes = size_t(p.mtiles) * p.group_steps * (SP * kPiece);
+    const size_t bias_bytes = size_t(2) * p.tiles_n * (kCols / 16) * p.group_steps * (SP * kPiece);
+    const size_t scale_bytes = size_t(p.group_steps) * 32 * p.tiles_n * kPiece, unscale_bytes = PARTS == 1 ? 0 : size_t(a.M) * 4;
+    const auto lock = scratch_lock(st);
+    void* ws = nullptr;
+    if (const int rc = call_buffer(11, x_bytes + sum_bytes + bias_bytes + scale_bytes + unscale_bytes, st, &ws)) return rc;
+    p.x = static_cast<char*>(ws), p.sums = p.x + x_bytes, p.biases = p.sums + sum_bytes;
+    p.scales = reinterpret_cast<float*>(p.biases + bias_bytes), p.unscale = reinterpret_cast<float*>(p.biases + bias_bytes + scale_bytes);
+    if constexpr (PARTS == 2) {
+        gated_row_scale_kernel<<<unsigned((a.M + 3) / 4), 256, 0, st>>>(static_cast<const float*>(a.x), a.M, a.K, p.unscale);
+        LQ_CHECK_LAUNCH("quantized_gated_matmul");
+    }
+    // 128 k a block, all that the sums' steps of 32 groups reach over
+    const unsigned x_blocks = unsigned(p.mtiles) * unsigned(p.group_steps * 32 * GS / 128);
+    const unsigned w_blocks = unsigned(p.tiles_n) * (kCols / 64) * 2 * unsigned(p.group_steps);
+    gated_prepare_kernel<T, PARTS, BITS><<<x_blocks + w_blocks, 256, 0, st>>>(a, p, x_blocks);
+    LQ_CHECK_LAUNCH("quantized_gated_matmul");
+    static DeviceOnce once;
+    constexpr int lds = S::RING * S::PIECES * kPiece;
+    const auto kernel = gated_gemm_kernel<T, PARTS, BITS, GS, MT>;
+    if (const int rc = allow_dynamic_lds(once, reinterpret_cast<const void*>(kernel), lds)) return rc;
+    kernel<<<unsigned(tiles_m) * unsigned(p.tiles_n), 256, lds, st>>>(a, p, tiles_m);
+    LQ_CHECK_LAUNCH("quantized_gated_matmul");
+    return LQ_OK;
+}
+
+// Rows in chunks whose prepared x stays below 2^30 bytes; whole tiles, so that the bits do not depend on them.
+template <class T, int PARTS, int BITS, int GS, int MT>
+int launch_gemm_chunks(Args a, hipStream_t st) {
+    const size_t tile = size_t((a.K + 63) / 64) * (2 * PARTS * MT) * kPiece, tiles = tile < size_t(1) << 30 ? (size_t(1) << 30) / tile : 1;
+    const int M = a.M, rows = int(std::min<size_t>(tiles * 16 * MT, size_t(M)));
+    for (int m0 = 0; m0 < M; m0 += a.M) {
+        a.M = std::min(rows, M - m0);
+        if (const int rc = launch_gemm_tile<T, PARTS, BITS, GS, MT>(a, st)) return rc;
+        a.x = static_cast<const T*>(a.x) + size_t(a.M) * a.K, a.out = static_cast<T*>(a.out) + size_t(a.M) * a.N;
+    }
+    return LQ_OK;
+}
+
+template <class T, int PARTS, int BITS>
+int launch_gemm(const Args& a, hipStream_t st) {
+    constexpr int MT = PARTS == 1 ? 6 : 4;
+    const int gs = 1 << a.gs_shift;
+    if (gs == 32) return launch_gemm_chunks<T, PARTS, BITS, 32, MT>(a, st);
+    if (gs == 64) return launch_gemm_chunks<T, PARTS, BITS, 64, MT>(a, st);
+    return launch_gemm_chunks<T, PARTS, BITS, 128, MT>(a, st);
+}
+
+}  // namespace
+}  // namespace gated
+}  // namespace lq
