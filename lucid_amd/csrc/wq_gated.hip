@@ -21,8 +21,11 @@ extern "C" int lq_wq_gated_matmul(const lq_wq_gated_args* g, lq_stream stream) {
         a.w[i] = gated::Weight{g->packed[i], g->scales[i], g->biases[i], g->bias[i]};
         LQ_REQUIRE(a.w[i].packed && a.w[i].scales && a.w[i].biases, LQ_ERR_VALUE, "quantized_gated_matmul: NULL pointer");
         LQ_REQUIRE(aligned16(a.w[i].packed), LQ_ERR_VALUE, "quantized_gated_matmul: packed weights must be 16-byte aligned");
+        LQ_REQUIRE((reinterpret_cast<uintptr_t>(a.w[i].scales) | reinterpret_cast<uintptr_t>(a.w[i].biases)) % 4 == 0, LQ_ERR_VALUE,
+                   "quantized_gated_matmul: scales must be aligned");
     }
     LQ_REQUIRE(a.x && a.out, LQ_ERR_VALUE, "quantized_gated_matmul: NULL pointer");
+    LQ_REQUIRE(aligned16(a.x), LQ_ERR_VALUE, "quantized_gated_matmul: x must be 16-byte aligned");
     LQ_REQUIRE(a.x != a.out, LQ_ERR_VALUE, "quantized_gated_matmul: the result cannot take x's place");
     const hipStream_t st = as_stream(stream);
     // (offsets of codes are 32-bit in the kernel of many rows)

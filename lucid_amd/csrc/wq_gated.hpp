@@ -5,7 +5,7 @@
 //
 // for the weights of the gate and of the way up.  Codes enter the matrix instructions as the whole numbers c - 2^(bits-1) that they are
 // (the rest of the code goes to b), so that nothing of a weight is rounded: scales follow in float32, on the sums of a group.  float16 x
-// enters as it is; float32 x as three bfloat16 of 24 bits together (wq_pack.hpp), or as two float16 of 22 (wq_gated_gemm.hpp).
+// enters as it is; a float32 row times a power of two as two float16 of 22 bits together.
 #pragma once
 #include "wq_pack.hpp"
 
@@ -77,18 +77,19 @@ __device__ __forceinline__ v8h slots_f16(uint4 x) {
     return __builtin_bit_cast(v8h, uint4{low(x.x, x.z), high(x.x, x.z), low(x.y, x.w), high(x.y, x.w)});
 }
 
-// f(BITS, SW) as constants: what a window of 64 lanes x 16 bytes is made of (wq_pack.hpp)
-template <class F>
-int by_window(int bits, int gs, F&& f) {
-    const int sw = wq_swap_mode(bits, gs);
-    using std::integral_constant;
-    if (bits == 4) {
-        if (sw == 0) return f(integral_constant<int, 4>{}, integral_constant<int, 0>{});
-        if (sw == 1) return f(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-        return f(integral_constant<int, 4>{}, integral_constant<int, 2>{});
-    }
-    if (sw == 0) return f(integral_constant<int, 8>{}, integral_constant<int, 0>{});
-    return f(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+// What undoes the factor of a float32 row whose largest value is `top` = 2^e t, t in [0.5, 1): 2^(e - 15), within what a float32 and its
+// inverse can say.  (A row that is not finite keeps its values, and gives no number.)
+__device__ __forceinline__ float row_unscale(float top) {
+    int e = 15;
+    if (top > 0.f && top < __builtin_inff()) frexpf(top, &e);
+    return ldexpf(1.0f, (e < -111 ? -111 : e) - 15);
+}
+// Eight values times f as two float16 each
+__device__ __forceinline__ void split_f16(const float (&v)[8], float f, uint4 (&part)[2]) {
+    v8h hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) hi[e] = _Float16(v[e] * f), lo[e] = _Float16(v[e] * f - float(hi[e]));
+    part[0] = __builtin_bit_cast(uint4, hi), part[1] = __builtin_bit_cast(uint4, lo);
 }
 
 }  // namespace

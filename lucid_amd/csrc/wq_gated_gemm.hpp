@@ -20,6 +20,8 @@ namespace lq {
 namespace gated {
 namespace {
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));  // (see wq_gated_rows.hpp on types in LDS)
+
 constexpr int kPiece = 1024;  // bytes one wavefront moves into LDS with one instruction
 constexpr int kCols = 128;    // of a block, of each weight
 
@@ -47,13 +49,7 @@ __global__ __launch_bounds__(256) void gated_row_scale_kernel(const float* __res
     }
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-    if (lane == 0) {
-        // top = 2^e t with t in [0.5, 1): times 2^(15 - e), within what a float32 can say.  (Infinite rows stay: they give no number.)
-        int e = 15;
-        if (top > 0.f && top < __builtin_inff()) frexpf(top, &e);
-        e = e < -111 ? -111 : e;
-        unscale[m] = ldexpf(1.0f, e - 15);
-    }
+    if (lane == 0) unscale[m] = row_unscale(top);
 }
 
 // Two kinds of blocks.  The first `x_blocks`: 16 rows x 128 k, a thread has eight k.  The others: 64 columns of a weight, a wavefront eight groups.
@@ -101,17 +97,17 @@ __global__ __launch_bounds__(256) void gated_prepare_kernel(Args a, Prepared p, 
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        float f = 1.0f;
         if (there) {
             __builtin_memcpy(v, static_cast<const float*>(a.x) + size_t(m) * a.K + k, 32);
-            const float f = 1.0f / p.unscale[m];  // (powers of two)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= f;
+            f = 1.0f / p.unscale[m];  // (powers of two)
         }
-        v8h hi, lo;
+        uint4 part[2];
+        split_f16(v, f, part);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) hi[e] = _Float16(v[e]), lo[e] = _Float16(v[e] - float(hi[e]));
-        piece[0] = __builtin_bit_cast(uint4, slots_f16<BITS>(__builtin_bit_cast(uint4, hi)));
-        piece[1] = __builtin_bit_cast(uint4, slots_f16<BITS>(__builtin_bit_cast(uint4, lo)));
+        for (int i = 0; i < 2; ++i) piece[i] = __builtin_bit_cast(uint4, slots_f16<BITS>(part[i]));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= f;
     }
     if (stage < p.stages) {
 #pragma unroll
@@ -240,7 +236,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 uint32_t wd[4] = {0u, 0u, 0u, 0u};
                 const char* row = codes + which * (BITS * kPiece) + r * ROW;
                 if constexpr (BITS == 4) wd[0] = *reinterpret_cast<const uint32_t*>(row + (ii ^ ((r >> 3) & 1)) * 16 + q * 4);
-                else __builtin_memcpy(wd, __builtin_assume_aligned(row + ((ii * 2 + (q >> 1)) ^ ((r >> 2) & 3)) * 16 + (q & 1) * 8, 8), 8);
+                else {
+                    const u32x2 t = *reinterpret_cast<const u32x2*>(row + ((ii * 2 + (q >> 1)) ^ ((r >> 2) & 3)) * 16 + (q & 1) * 8);
+                    wd[0] = t[0], wd[1] = t[1];
+                }
                 c[ii] = codes_f16<BITS>(wd, 0);
             }
 #pragma unroll

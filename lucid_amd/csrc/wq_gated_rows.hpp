@@ -1,10 +1,21 @@
 // Gated projections of few rows (wq_gated.hpp has the mathematics): bound by reading the weights.
 //
-// A block has 16 columns of both weights and 16 MT rows of x; its four wavefronts have windows of k of their own (64 lanes x 16 bytes: 128
-// or 64 k of 16 weight rows, every fourth window a wavefront), so that each x that a wavefront loads meets both weights and nothing is
-// shared until the sums are added in LDS.  One window is under way while another is multiplied.  Scales come with the codes: a
-// lane has those of its own 16 bytes, which lie in one group, and where a window has several groups the others' come from the lanes that have
-// them.  The sums of x of a group are a product with ones.
+// A wavefront has 16 columns of both weights and steps of 128 k; the wavefronts of a block that have the same columns and other steps add
+// their sums in LDS at the end.  What a step needs goes from memory straight into LDS, into a ring of steps, with neighbouring lanes on
+// neighbouring bytes: a load whose lanes are an operand's (row = lane % 16) costs the address unit a cycle a lane, whatever it carries (1 x 11008 x
+// 4096 of 4 bits took 24 us that way, with half or all of the vector work and whatever was under way).  In LDS the 16-byte chunks of a row
+// change places with its number, so that the 16 rows of an operand lie in different banks.  The sums of x of a group are a product with ones.
+//
+// x as it enters the matrix instructions: float16 as it is; a float32 row times the power of two that brings its largest value below 2^15,
+// as two float16, hi = x rounded, lo = x - hi rounded: 22 bits, or 2^-39 of the largest value.
+//
+// gated_few_kernel, up to 4 rows of up to 64 KB: a block has 16 columns, its four wavefronts every fourth step each.  It brings x into LDS itself, while
+// its first weights are under way, and nothing else is shared, so that there is no barrier in the loop.  A row of x lies on every fourth row of the
+// instruction: a lane then has one element of each result.
+//
+// gated_rows_kernel, up to 64 rows: a block has 64 columns, its eight wavefronts 16 of them and every other step each, so that four share
+// an x (16 rows of float32 are as many bytes as the codes of 16 columns of both weights in 8 bits, and come from the L2 for every block again:
+// 16 x 11008 x 4096, 16 columns a block and no x shared, 41 us).  float32 rows are split by a launch of their own.
 #pragma once
 #include <type_traits>
 
@@ -14,173 +25,427 @@ namespace lq {
 namespace gated {
 namespace {
 
-constexpr int kWaves = 4;
+// (The compiler waits for every load under way into LDS before it reads there through a type that aliases all others, as the vector types of HIP's
+// headers are copied: these are types of the language.)
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-template <class T, int BITS, int SW, int MT>
-__global__ __launch_bounds__(64 * kWaves) void gated_rows_kernel(Args a) {
-    using G = WqGeom<BITS>;
-    constexpr int CODES = G::CODES, WK = G::WK, NI = G::NI, GW = 1 << SW, SEG = WK / GW, IPS = NI / GW;
-    constexpr bool F16 = std::is_same_v<T, _Float16>;
-    constexpr int QUADS = F16 ? 1 : 2;  // 16-byte loads of x per fragment
-    constexpr float UNIT = F16 ? 1.0f : kWqUnit<BITS>;
-    __shared__ v4f s_y[kWaves][2][MT][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = lane & 15, q = lane >> 4;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MT);
-    const int windows = (a.K + WK - 1) / WK, groups = a.K >> a.gs_shift;
-    const int n = n0 + ln < a.N ? n0 + ln : a.N - 1;
+constexpr int kStep = 128;  // k of a step
+constexpr size_t kFewLds = 64 * 1024;
+constexpr int kFewWaves = 4;
+constexpr int kColumnGroups = 4, kStepGroups = 2, kRowsWaves = kColumnGroups * kStepGroups;
+
+struct RowsX {
+    const _Float16* part[2];  // [M, K]; float16 x: the first
+    const float* unscale;     // [M], of float32 x
+};
+
+// A wavefront's part of a step in LDS: the codes of 16 rows of both weights, 16 BITS bytes each, then [weight][scales, biases][row][group].
+template <int BITS, int GS>
+struct Codes {
+    static constexpr int LOADS = 2 * BITS / 4, GROUPS = kStep / GS;  // instructions that move 1 KiB; and 256 bytes
+    static constexpr int BYTES = LOADS * 1024 + GROUPS * 256;
+    static constexpr int ROW = 16 * BITS, CHUNKS = ROW / 16;
+    static __device__ __forceinline__ int swizzle(int r) { return CHUNKS == 4 ? (r >> 2) & 3 : (r >> 1) & 7; }
+};
+
+typedef __attribute__((address_space(1))) void* gptr;
+typedef __attribute__((address_space(3))) void* lptr;
+
+// What a wavefront keeps to load them (rows past N: the last one's bytes; their results go nowhere).
+template <int BITS, int GS>
+struct CodesFrom {
+    using C = Codes<BITS, GS>;
     const char* codes[2];
-    const float *scales[2], *biases[2];
+    const float* numbers[C::GROUPS];
+    unsigned row_bytes;
+    int last, groups, lane;
+    __device__ __forceinline__ CodesFrom(const Args& a, int n0, int lane_) {
+        n0 = n0 < a.N ? n0 : a.N - 1;  // (a wavefront past N)
+        lane = lane_, last = a.N - 1 - n0, groups = a.K / GS, row_bytes = unsigned(a.K) * BITS / 8;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        codes[i] = reinterpret_cast<const char*>(a.w[i].packed) + size_t(n) * (size_t(a.K) * BITS / 8);
-        scales[i] = a.w[i].scales + size_t(n) * groups;
-        biases[i] = a.w[i].biases + size_t(n) * groups;
+        for (int i = 0; i < 2; ++i) codes[i] = reinterpret_cast<const char*>(a.w[i].packed) + size_t(n0) * row_bytes;
+#pragma unroll
+        for (int u = 0; u < C::GROUPS; ++u) {
+            const int which = (u * 64 + lane) / (16 * C::GROUPS);
+            const float *of0 = which & 1 ? a.w[0].biases : a.w[0].scales, *of1 = which & 1 ? a.w[1].biases : a.w[1].scales;
+            numbers[u] = (which & 2 ? of1 : of0) + size_t(n0) * groups;
+        }
     }
-    const T* x[MT];
+    __device__ __forceinline__ void load(int s, char* to) const {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) x[t] = static_cast<const T*>(a.x) + size_t(m0 + t * 16 + ln) * a.K;
-    struct Window {
-        uint4 w[2];
-        float s[2], b[2];
-        uint4 x[MT][NI][QUADS];
+        for (int u = 0; u < C::LOADS; ++u) {
+            constexpr int HALF = C::LOADS / 2;
+            const int r = u % HALF * (64 / C::CHUNKS) + lane / C::CHUNKS, chunk = (lane % C::CHUNKS) ^ C::swizzle(r);
+            const unsigned at = unsigned(s) * C::ROW + unsigned(chunk) * 16;  // (past K: the row's first bytes, which meet zeros of x)
+            __builtin_amdgcn_global_load_lds((gptr)(codes[u / HALF] + (unsigned(r < last ? r : last) * row_bytes + (at < row_bytes ? at : 0))),
+                                             (lptr)(to + u * 1024), 16, 0, 0);
+        }
+#pragma unroll
+        for (int u = 0; u < C::GROUPS; ++u) {
+            const int i = u * 64 + lane, r = i / C::GROUPS % 16, g = s * C::GROUPS + i % C::GROUPS;
+            const int at = (r < last ? r : last) * groups + (g < groups ? g : groups - 1);
+            __builtin_amdgcn_global_load_lds((gptr)(numbers[u] + at), (lptr)(to + C::LOADS * 1024 + u * 256), 4, 0, 0);
+        }
+    }
+};
+
+// y += the products of a step; x_at(k, part, tile) is eight x from k on, in the codes' slots.
+template <int PARTS, int BITS, int GS, int MT, int RU, class F>
+__device__ __forceinline__ void multiply(const char* at, int lane, float (&y)[2][MT][RU], F&& x_at) {
+    using C = Codes<BITS, GS>;
+    constexpr int SEGS = C::GROUPS, IPS = 4 / SEGS, BYTES = IPS * BITS;  // instructions (32 k) of a group; a lane's bytes of one, consecutive
+    const int ln = lane & 15, q = lane >> 4;
+    const _Float16 o = _Float16(1.f);
+    const v8h one{o, o, o, o, o, o, o, o};
+#pragma unroll
+    for (int e = 0; e < SEGS; ++e) {
+        uint32_t wd[2][8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int b = 0; b < (BYTES + 15) / 16; ++b) {
+                const int byte = e * (C::ROW / SEGS) + q * BYTES + b * 16;
+                const char* from = at + i * (C::LOADS / 2 * 1024) + (lane & 15) * C::ROW + ((byte >> 4) ^ C::swizzle(ln)) * 16 + (byte & 15);
+                if constexpr (BYTES >= 16) {
+                    const u32x4 t = *reinterpret_cast<const u32x4*>(from);
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) wd[i][b * 4 + d] = t[d];
+                } else if constexpr (BYTES == 8) {
+                    const u32x2 t = *reinterpret_cast<const u32x2*>(from);
+                    wd[i][0] = t[0], wd[i][1] = t[1];
+                } else {
+                    wd[i][0] = *reinterpret_cast<const uint32_t*>(from);
+                }
+            }
+        v4f acc[2][MT], sum[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[0][t] = acc[1][t] = sum[t] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ii = 0; ii < IPS; ++ii) {
+            constexpr int W = BITS / 4;  // words of eight codes
+            const uint32_t wg[4] = {wd[0][ii * W], wd[0][ii * W + W - 1], 0u, 0u}, wu[4] = {wd[1][ii * W], wd[1][ii * W + W - 1], 0u, 0u};
+            const v8h cg = codes_f16<BITS>(wg, 0), cu = codes_f16<BITS>(wu, 0);
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    const v8h f = x_at(e * GS + q * (IPS * 8) + ii * 8, p, t);
+                    acc[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, cg, acc[0][t], 0, 0, 0);
+                    acc[1][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, cu, acc[1][t], 0, 0, 0);
+                    sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, one, sum[t], 0, 0, 0);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float* numbers = reinterpret_cast<const float*>(at + C::LOADS * 1024) + (i * 32 + ln) * SEGS + e;
+            const float sc = numbers[0], b = __builtin_fmaf(-float(kWqCentre<BITS>), sc, numbers[16 * SEGS]);
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int r = 0; r < RU; ++r) y[i][t][r] = __builtin_fmaf(sc, acc[i][t][r], __builtin_fmaf(b, sum[t][r], y[i][t][r]));
+        }
+    }
+}
+
+// s_waitcnt immediates: vmcnt <= n alone, and with every LDS read done; every LDS read done
+constexpr int vmcnt_only(int n) { return (n & 0xF) | ((n >> 4) << 14) | (0x7 << 4) | (0xF << 8); }
+constexpr int vmcnt_and_lds(int n) { return (n & 0xF) | ((n >> 4) << 14) | (0x7 << 4); }
+constexpr int kLdsDone = 0xF | (0x3 << 14) | (0x7 << 4);
+
+__device__ __forceinline__ void pin() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// ---------------------------------------------------------------- up to four rows
+// (as many steps as three blocks a CU have room for)
+template <int BITS>
+constexpr int kFewRing = BITS == 4 ? 3 : 2;
+
+template <class T, int PARTS, int BITS, int GS>
+__global__ __launch_bounds__(64 * kFewWaves) void gated_few_kernel(Args a) {
+    using C = Codes<BITS, GS>;
+    constexpr int RING = kFewRing<BITS>, LOADS = C::LOADS + C::GROUPS;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];  // the wavefronts' rings, then x: [part][row][K rounded up to steps, and 8]
+    __shared__ float s_y[kFewWaves][2][64];
+    __shared__ float s_unscale[4], s_top[kFewWaves];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * 16, steps = (a.K + kStep - 1) / kStep;
+    char* const ring = smem + wave * (RING * C::BYTES);
+    char* const s_x = smem + kFewWaves * RING * C::BYTES;
+    const unsigned stride = unsigned(steps) * (kStep * 2) + 16, x_part = unsigned(a.M) * stride;  // bytes of a row, of a part
+    const CodesFrom<BITS, GS> from(a, n0, lane);
+    auto load = [&](int s, char* to) { from.load(s < steps ? s : steps - 1, to); };  // (past the end: any step, to keep the count)
+    constexpr int QUADS = PARTS == 1 ? 1 : 2;
+    const unsigned octets = unsigned(steps) * (kStep / 8), total = unsigned(a.M) * octets;
+    auto fetch = [&](unsigned u, uint4 (&raw)[QUADS]) {
+        u = u < total ? u : 0;
+        const unsigned m = u / octets, k = (u - m * octets) * 8;
+        __builtin_memcpy(raw, static_cast<const T*>(a.x) + size_t(m) * a.K + (k < unsigned(a.K) ? k : 0), 16 * QUADS);
     };
-    auto load = [&](int w, Window& v) {
-        // (past K: the row's first bytes, which meet zeros of x)
-        const int k = w * WK + q * CODES, kc = k < a.K ? k : 0, g = kc >> a.gs_shift;
+    auto place = [&](unsigned u, uint4 (&raw)[QUADS]) {
+        if (u >= total) return;
+        const unsigned m = u / octets, o = u - m * octets, at = m * stride + o * 16;
+        if (o * 8 >= unsigned(a.K))
+#pragma unroll
+            for (int h = 0; h < QUADS; ++h) raw[h] = uint4{0u, 0u, 0u, 0u};
+        if constexpr (PARTS == 1) {
+            *reinterpret_cast<v8h*>(s_x + at) = slots_f16<BITS>(raw[0]);
+        } else {
+            float f[8];
+            __builtin_memcpy(f, raw, 32);
+            uint4 part[2];
+            split_f16(f, 1.0f / s_unscale[m], part);
+#pragma unroll
+            for (int p = 0; p < 2; ++p) *reinterpret_cast<v8h*>(s_x + p * x_part + at) = slots_f16<BITS>(part[p]);
+        }
+    };
+    if constexpr (PARTS == 2) {
+        for (int m = 0; m < a.M; ++m) {
+            float top = 0.f;
+            for (unsigned c = threadIdx.x; c < unsigned(a.K) / 8; c += 64 * kFewWaves) {
+                float f[8];
+                __builtin_memcpy(f, static_cast<const float*>(a.x) + size_t(m) * a.K + c * 8, 32);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
+            }
+#pragma unroll
+            for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+            __syncthreads();  // (the row before has been read)
+            if (lane == 0) s_top[wave] = top;
+            __syncthreads();
+            if (threadIdx.x == 0) s_unscale[m] = row_unscale(fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3])));
+        }
+        __syncthreads();
+    }
+    // the first octets of a thread are under way before the weights
+    uint4 first[2][QUADS];
+    fetch(threadIdx.x, first[0]);
+    fetch(threadIdx.x + 64 * kFewWaves, first[1]);
+    pin();
+#pragma unroll
+    for (int d = 0; d < RING; ++d) load(wave + d * kFewWaves, ring + d * C::BYTES);
+    pin();
+    place(threadIdx.x, first[0]);
+    place(threadIdx.x + 64 * kFewWaves, first[1]);
+    for (unsigned u = threadIdx.x + 2 * 64 * kFewWaves; u < total; u += 64 * kFewWaves) {
+        fetch(u, first[0]);
+        place(u, first[0]);
+    }
+    lds_barrier();
+    const char* const x_row = s_x + unsigned(((lane & 15) >> 2) < a.M ? (lane & 15) >> 2 : 0) * stride;
+    float y[2][1][1] = {};
+    int slot = 0;
+    for (int s = wave; s < steps; s += kFewWaves) {
+        char* const at = ring + slot * C::BYTES;
+        slot = slot + 1 == RING ? 0 : slot + 1;
+        pin();
+        __builtin_amdgcn_s_waitcnt(vmcnt_only(LOADS * (RING - 1)));
+        pin();
+        multiply<PARTS, BITS, GS, 1, 1>(at, lane, y, [&](int k, int p, int) {
+            return *reinterpret_cast<const v8h*>(x_row + p * x_part + unsigned(s * kStep + k) * 2);
+        });
+        pin();
+        __builtin_amdgcn_s_waitcnt(kLdsDone);  // the step has been read
+        pin();
+        load(s + RING * kFewWaves, at);
+    }
+    s_y[wave][0][lane] = y[0][0][0], s_y[wave][1][lane] = y[1][0][0];
+    __syncthreads();  // (and the loads past the end have landed)
+    // a thread has a column and row q that lane column + 16 q holds
+    const int n = n0 + (threadIdx.x & 15), m = threadIdx.x >> 4;
+    if (n >= a.N || m >= a.M) return;
+    float g = 0.f, u = 0.f;
+#pragma unroll
+    for (int p = 0; p < kFewWaves; ++p) g += s_y[p][0][threadIdx.x], u += s_y[p][1][threadIdx.x];
+    if constexpr (PARTS == 2) g *= s_unscale[m & 3], u *= s_unscale[m & 3];
+    if (a.w[0].bias) g += a.w[0].bias[n];
+    if (a.w[1].bias) u += a.w[1].bias[n];
+    static_cast<T*>(a.out)[size_t(m) * a.N + n] = T(activate(a.act, g) * u);
+}
+
+// ---------------------------------------------------------------- up to 64 rows
+template <int PARTS, int BITS, int GS, int MT>
+struct RowsStep {
+    using C = Codes<BITS, GS>;
+    static constexpr int X = PARTS * MT * 4096;  // of each group of steps: [part][tile][16 rows of 256 bytes]
+    static constexpr int BYTES = kRowsWaves * C::BYTES + kStepGroups * X;
+    static constexpr int LOADS = C::LOADS + C::GROUPS + PARTS * MT;
+    static constexpr int FIT = 158 * 1024 / BYTES, RING = FIT > 3 ? 3 : FIT;
+    static constexpr bool POSSIBLE = RING >= 2 && LOADS * (RING - 2) <= 63;
+};
+
+template <class T, int PARTS, int BITS, int GS, int MT>
+__global__ __launch_bounds__(64 * kRowsWaves) void gated_rows_kernel(Args a, RowsX rx) {
+    using S = RowsStep<PARTS, BITS, GS, MT>;
+    using C = Codes<BITS, GS>;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];  // the ring of steps; at the end the sums
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = lane & 15;
+    const int cg = wave % kColumnGroups, sg = wave / kColumnGroups;
+    const int n0 = (blockIdx.x * kColumnGroups + cg) * 16, m0 = blockIdx.y * (16 * MT), steps = (a.K + kStep - 1) / kStep;
+    const CodesFrom<BITS, GS> from(a, n0, lane);
+    // four rows of each tile of x are this wavefront's to load (rows past M: the last one's bytes)
+    const int xr = cg * 4 + (lane >> 4);
+    size_t x_off[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int m = m0 + t * 16 + xr;
+        x_off[t] = size_t(m < a.M ? m : a.M - 1) * a.K;
+    }
+    auto load = [&](int i, int slot) {
+        const int want = i * kStepGroups + sg, s = want < steps ? want : steps - 1;  // past the end: any step, to keep the count
+        char* const to = smem + slot * S::BYTES;
+        from.load(s, to + wave * C::BYTES);
+        const int k = s * kStep + ((lane & 15) ^ xr) * 8;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                __builtin_amdgcn_global_load_lds((gptr)(rx.part[p] + x_off[t] + (k < a.K ? k : 0)),
+                                                 (lptr)(to + kRowsWaves * C::BYTES + sg * S::X + ((p * MT + t) * 4 + cg) * 1024), 16, 0, 0);
+    };
+    float y[2][MT][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                int q_src, j_src;
-                wq_source(SW, BITS == 4 ? i : 2 * i, q, q_src, j_src);
-                const int at = w * WK + q_src * CODES + j_src * (32 / BITS);
+            for (int r = 0; r < 4; ++r) y[i][t][r] = 0.f;
 #pragma unroll
-                for (int h = 0; h < QUADS; ++h) {
-                    v.x[t][i][h] = uint4{0u, 0u, 0u, 0u};
-                    if (m0 + t * 16 + ln < a.M && at < a.K) __builtin_memcpy(&v.x[t][i][h], x[t] + at + h * 4, 16);
-                }
-            }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            v.w[i] = *reinterpret_cast<const uint4*>(codes[i] + size_t(kc) * BITS / 8);
-            v.s[i] = scales[i][g], v.b[i] = biases[i][g];
-        }
-    };
-    v4f y[2][MT];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) y[i][t] = v4f{0.f, 0.f, 0.f, 0.f};
-    auto multiply = [&](Window& v) {
-        uint32_t wd[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            wd[i][0] = v.w[i].x, wd[i][1] = v.w[i].y, wd[i][2] = v.w[i].z, wd[i][3] = v.w[i].w;
-            wq_exchange<SW>(wd[i]);
-        }
-#pragma unroll
-        for (int e = 0; e < GW; ++e) {
-            v4f acc[2][MT], sum[MT];
-#pragma unroll
-            for (int t = 0; t < MT; ++t) acc[0][t] = acc[1][t] = sum[t] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int ii = 0; ii < IPS; ++ii) {
-                const int i = e * IPS + ii;
-                if constexpr (F16) {
-                    const _Float16 o = _Float16(1.f);
-                    const v8h one{o, o, o, o, o, o, o, o}, cg = codes_f16<BITS>(wd[0], i), cu = codes_f16<BITS>(wd[1], i);
-#pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        const v8h f = slots_f16<BITS>(v.x[t][i][0]);
-                        acc[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, cg, acc[0][t], 0, 0, 0);
-                        acc[1][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, cu, acc[1][t], 0, 0, 0);
-                        sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, one, sum[t], 0, 0, 0);
-                    }
-                } else {
-                    const v8bf one = __builtin_bit_cast(v8bf, uint4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
-                    const v8bf cg = __builtin_bit_cast(v8bf, wq_codes<BITS>(wd[0], i)), cu = __builtin_bit_cast(v8bf, wq_codes<BITS>(wd[1], i));
-#pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        float f[8];
-                        __builtin_memcpy(f, v.x[t][i], 32);
-                        uint32_t part[3][4];
-#pragma unroll
-                        for (int d = 0; d < 4; ++d)
-                            wq_split3x2(BITS == 4 ? f[d] : f[2 * d], BITS == 4 ? f[d + 4] : f[2 * d + 1], part[0][d], part[1][d], part[2][d]);
-#pragma unroll
-                        for (int p = 0; p < 3; ++p) {
-                            const v8bf fp = __builtin_bit_cast(v8bf, uint4{part[p][0], part[p][1], part[p][2], part[p][3]});
-                            acc[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp, cg, acc[0][t], 0, 0, 0);
-                            acc[1][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp, cu, acc[1][t], 0, 0, 0);
-                            sum[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp, one, sum[t], 0, 0, 0);
-                        }
-                    }
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                // of the segment's first quarter
-                const float s = SW == 0 ? v.s[i] : __shfl(v.s[i], ln + 16 * (e * (4 / GW)), 64);
-                const float b = (SW == 0 ? v.b[i] : __shfl(v.b[i], ln + 16 * (e * (4 / GW)), 64)) - float(kWqCentre<BITS>) * s, us = UNIT * s;
-#pragma unroll
-                for (int t = 0; t < MT; ++t)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) y[i][t][r] = __builtin_fmaf(us, acc[i][t][r], __builtin_fmaf(b, sum[t][r], y[i][t][r]));
-            }
-        }
-    };
-    auto pin = [] {
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    Window v0, v1;
-    int w = wave;
-    if (w < windows) {
-        load(w, v0);
-        for (;;) {
-            load(w + kWaves, v1);  // (past the last: bytes of the row that are not used)
-            pin();
-            multiply(v0);
-            pin();
-            if ((w += kWaves) >= windows) break;
-            load(w + kWaves, v0);
-            pin();
-            multiply(v1);
-            pin();
-            if ((w += kWaves) >= windows) break;
-        }
+    for (int d = 0; d < S::RING - 1; ++d) load(d, d);
+    int slot = 0;
+    for (int i = 0; i * kStepGroups < steps; ++i) {
+        pin();
+        __builtin_amdgcn_s_waitcnt(vmcnt_and_lds(S::LOADS * (S::RING - 2)));
+        __builtin_amdgcn_s_barrier();
+        pin();
+        load(i + S::RING - 1, slot == 0 ? S::RING - 1 : slot - 1);  // (the slot that everybody has just left)
+        const char* const at = smem + slot * S::BYTES;
+        slot = slot + 1 == S::RING ? 0 : slot + 1;
+        const int s = i * kStepGroups + sg;
+        if (s >= steps) continue;  // uniform: the other group's last step
+        const char* const x = at + kRowsWaves * C::BYTES + sg * S::X + ln * 256;
+        const int end = a.K - s * kStep;
+        multiply<PARTS, BITS, GS, MT, 4>(at + wave * C::BYTES, lane, y, [&](int k, int p, int t) {
+            u32x4 raw = *reinterpret_cast<const u32x4*>(x + (p * MT + t) * 4096 + ((k >> 3) ^ ln) * 16);
+            if (k >= end) raw = u32x4{0u, 0u, 0u, 0u};
+            return slots_f16<BITS>(uint4{raw[0], raw[1], raw[2], raw[3]});
+        });
     }
+    __builtin_amdgcn_s_waitcnt(vmcnt_and_lds(0));  // the loads past the end have landed
+    __syncthreads();
+    float(*const s_y)[2][MT][4][64] = reinterpret_cast<float(*)[2][MT][4][64]>(smem);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int t = 0; t < MT; ++t) s_y[wave][i][t][lane] = y[i][t];
-    __syncthreads();
-    // a thread has row tid / 16 of each tile: element row % 4 of lane column + 16 (row / 4)
-    const int col = threadIdx.x & 15, row = threadIdx.x >> 4, from = col + 16 * (row >> 2);
-    if (n0 + col >= a.N) return;
-    const float bg = a.w[0].bias ? a.w[0].bias[n0 + col] : 0.f, bu = a.w[1].bias ? a.w[1].bias[n0 + col] : 0.f;
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int m = m0 + t * 16 + row;
+            for (int r = 0; r < 4; ++r) s_y[wave][i][t][r][lane] = y[i][t][r];
+    __syncthreads();
+    // a thread has a column of 64 and rows 8 apart: element row % 4 of lane column + 16 (row / 4)
+    const int col = threadIdx.x & 63, n = blockIdx.x * (kColumnGroups * 16) + col;
+    if (n >= a.N) return;
+    const float bg = a.w[0].bias ? a.w[0].bias[n] : 0.f, bu = a.w[1].bias ? a.w[1].bias[n] : 0.f;
+#pragma unroll
+    for (int j = 0; j < 2 * MT; ++j) {
+        const int row = j * 8 + (threadIdx.x >> 6), m = m0 + row, t = row >> 4, from_lane = (col & 15) + 16 * ((row >> 2) & 3);
         if (m >= a.M) return;
         float g = 0.f, u = 0.f;
 #pragma unroll
-        for (int p = 0; p < kWaves; ++p) g += s_y[p][0][t][from][row & 3], u += s_y[p][1][t][from][row & 3];
-        static_cast<T*>(a.out)[size_t(m) * a.N + n0 + col] = T(activate(a.act, g + bg) * (u + bu));
+        for (int p = 0; p < kStepGroups; ++p) {
+            g += s_y[p * kColumnGroups + (col >> 4)][0][t][row & 3][from_lane];
+            u += s_y[p * kColumnGroups + (col >> 4)][1][t][row & 3][from_lane];
+        }
+        if constexpr (PARTS == 2) g *= rx.unscale[m], u *= rx.unscale[m];
+        static_cast<T*>(a.out)[size_t(m) * a.N + n] = T(activate(a.act, g + bg) * (u + bu));
     }
+}
+
+// A float32 row as two float16, and what undoes its factor: a block a row.
+__global__ __launch_bounds__(256) void gated_split_kernel(const float* __restrict__ x, int K, _Float16* __restrict__ hi, _Float16* __restrict__ lo,
+                                                          float* __restrict__ unscale) {
+    __shared__ float s_top[4];
+    const size_t base = size_t(blockIdx.x) * K;
+    const unsigned octets = unsigned(K) / 8;
+    float f[8], top = 0.f;
+    for (unsigned c = threadIdx.x; c < octets; c += 256) {
+        __builtin_memcpy(f, x + base + c * 8, 32);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = top;
+    __syncthreads();
+    const float u = row_unscale(fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3])));
+    if (threadIdx.x == 0) unscale[blockIdx.x] = u;
+    for (unsigned c = threadIdx.x; c < octets; c += 256) {
+        __builtin_memcpy(f, x + base + c * 8, 32);
+        uint4 part[2];
+        split_f16(f, 1.0f / u, part);
+        *reinterpret_cast<uint4*>(hi + base + c * 8) = part[0], *reinterpret_cast<uint4*>(lo + base + c * 8) = part[1];
+    }
+}
+
+// f(BITS, GS) as constants
+template <class F>
+int by_group(int bits, int gs, F&& f) {
+    using std::integral_constant;
+    auto of_bits = [&](auto b) {
+        if (gs == 32) return f(b, integral_constant<int, 32>{});
+        if (gs == 64) return f(b, integral_constant<int, 64>{});
+        return f(b, integral_constant<int, 128>{});
+    };
+    return bits == 4 ? of_bits(integral_constant<int, 4>{}) : of_bits(integral_constant<int, 8>{});
 }
 
 template <class T>
 int launch_rows(const Args& a, int bits, hipStream_t st) {
-    return by_window(bits, 1 << a.gs_shift, [&](auto bits_c, auto sw) -> int {
-        constexpr int BITS = decltype(bits_c)::value, SW = decltype(sw)::value;
-        const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
-        const dim3 grid(unsigned((a.N + 15) / 16), unsigned((a.M + 16 * mt - 1) / (16 * mt)));
-        LQ_REQUIRE(grid.y <= 65535, LQ_ERR_SHAPE, "quantized_gated_matmul: %d rows", a.M);
-        const auto kernel = mt == 1 ? gated_rows_kernel<T, BITS, SW, 1> : mt == 2 ? gated_rows_kernel<T, BITS, SW, 2> : gated_rows_kernel<T, BITS, SW, 4>;
-        kernel<<<grid, 64 * kWaves, 0, st>>>(a);
+    constexpr int PARTS = std::is_same_v<T, float> ? 2 : 1;
+    LQ_REQUIRE(a.K < 1 << 26, LQ_ERR_SHAPE, "quantized_gated_matmul: K = %d", a.K);  // (offsets of 16 rows are 32-bit)
+    const size_t few = size_t(PARTS) * a.M * ((a.K + kStep - 1) / kStep * (kStep * 2) + 16);
+    if (a.M <= 4 && few <= kFewLds)
+        return by_group(bits, 1 << a.gs_shift, [&](auto bits_c, auto gs_c) -> int {
+            constexpr int BITS = decltype(bits_c)::value, GS = decltype(gs_c)::value;
+            const auto kernel = gated_few_kernel<T, PARTS, BITS, GS>;
+            constexpr size_t ring = size_t(kFewWaves) * kFewRing<BITS> * Codes<BITS, GS>::BYTES;
+            static DeviceOnce once;
+            if (const int rc = allow_dynamic_lds(once, reinterpret_cast<const void*>(kernel), ring + kFewLds)) return rc;
+            kernel<<<unsigned((a.N + 15) / 16), 64 * kFewWaves, ring + few, st>>>(a);
+            LQ_CHECK_LAUNCH("quantized_gated_matmul");
+            return LQ_OK;
+        });
+    const auto lock = scratch_lock(st);
+    RowsX rx{{static_cast<const _Float16*>(a.x), nullptr}, nullptr};
+    if constexpr (PARTS == 2) {
+        void* ws = nullptr;
+        const size_t part = size_t(a.M) * a.K;
+        if (const int rc = call_buffer(11, part * 4 + size_t(a.M) * 4, st, &ws)) return rc;
+        _Float16* const hi = static_cast<_Float16*>(ws);
+        float* const unscale = reinterpret_cast<float*>(hi + 2 * part);
+        gated_split_kernel<<<unsigned(a.M), 256, 0, st>>>(static_cast<const float*>(a.x), a.K, hi, hi + part, unscale);
         LQ_CHECK_LAUNCH("quantized_gated_matmul");
-        return LQ_OK;
+        rx = RowsX{{hi, hi + part}, unscale};
+    }
+    return by_group(bits, 1 << a.gs_shift, [&](auto bits_c, auto gs_c) -> int {
+        constexpr int BITS = decltype(bits_c)::value, GS = decltype(gs_c)::value;
+        auto launch = [&](auto tiles) -> int {
+            constexpr int MT = decltype(tiles)::value;
+            using S = RowsStep<PARTS, BITS, GS, MT>;
+            const dim3 grid(unsigned((a.N + kColumnGroups * 16 - 1) / (kColumnGroups * 16)), unsigned((a.M + 16 * MT - 1) / (16 * MT)));
+            LQ_REQUIRE(grid.y <= 65535, LQ_ERR_SHAPE, "quantized_gated_matmul: %d rows", a.M);
+            const auto kernel = gated_rows_kernel<T, PARTS, BITS, GS, MT>;
+            constexpr int lds = S::RING * S::BYTES > kRowsWaves * MT * 2048 ? S::RING * S::BYTES : kRowsWaves * MT * 2048;
+            static DeviceOnce once;
+            if (const int rc = allow_dynamic_lds(once, reinterpret_cast<const void*>(kernel), lds)) return rc;
+            kernel<<<grid, 64 * kRowsWaves, lds, st>>>(a, rx);
+            LQ_CHECK_LAUNCH("quantized_gated_matmul");
+            return LQ_OK;
+        };
+        if constexpr (RowsStep<PARTS, BITS, GS, 4>::POSSIBLE)
+            if (a.M > 32) return launch(std::integral_constant<int, 4>{});
+        return a.M > 16 ? launch(std::integral_constant<int, 2>{}) : launch(std::integral_constant<int, 1>{});
     });
 }
 
