@@ -10,8 +10,9 @@
 // sums would move one in a thousand draws.
 //
 // A block has a run of the vocabulary of one sequence; every block judges the drafts itself (two numbers each), so that it knows the row
-// to read.  Sums go to the last block that arrives, which finds the run and in it the token.  Each probability is read once, the run of
-// the token twice.  Bound by memory.
+// to read, and asks for up to 8192 of its probabilities at once.  Sums go to the last block that arrives, which finds the run, in it the piece of
+// 512 that a wavefront reads with one instruction, the lane and the token.  Each probability is read once, the run of the token twice.  Bound by
+// memory in the large (128 rows of 131 072 float16), by a chain of eight trips to memory in the small.
 #include <type_traits>
 
 #include "common.hpp"
@@ -20,7 +21,8 @@ using namespace lq;
 
 namespace {
 
-constexpr unsigned kThreads = 256, kVec = 8;
+constexpr unsigned kThreads = 256, kWaves = kThreads / 64, kVec = 8, kPiece = 64 * kVec, kAtOnce = 4, kRound = kThreads * kVec;  // tokens
+constexpr unsigned kNone = 0xffffffffu;
 
 struct Args {
     const void *target, *draft;  // [rows, vocab]; draft NULL: q is 1 at the drafted token
@@ -32,15 +34,14 @@ struct Args {
     int* arrived;               // [batch], zero between launches
 };
 
-// what counts of a weight: a positive finite number
-__device__ __forceinline__ double positive(double d) { return d > 0.0 && d < __builtin_inf() ? d : 0.0; }
+// what counts of a probability: a positive finite number
+__device__ __forceinline__ float counted(float p) { return p < __builtin_inff() ? fmaxf(p, 0.f) : 0.f; }  // (fmaxf of a NaN is 0)
 
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
     return v;
 }
-
 // the sum over the lanes up to this one
 __device__ __forceinline__ double wave_scan(double v, unsigned lane) {
 #pragma unroll
@@ -51,39 +52,78 @@ __device__ __forceinline__ double wave_scan(double v, unsigned lane) {
     return v;
 }
 
-// eight values from v on, zeros from `end` on
+// Eight values from v on, as they lie in memory; zeros from `end` on.
 template <class T>
-__device__ __forceinline__ void load8(const T* row, unsigned v, unsigned end, float (&p)[kVec]) {
+struct Raw {
+    T v[kVec];
+};
+template <class T>
+__device__ __forceinline__ Raw<T> load8(const T* row, unsigned v, unsigned end) {
+    Raw<T> raw;
     if (v + kVec <= end) {
-        T raw[kVec];
-        __builtin_memcpy(raw, row + v, sizeof raw);  // (rows of odd length are not 16-byte aligned)
-#pragma unroll
-        for (unsigned e = 0; e < kVec; ++e) p[e] = float(raw[e]);
+        __builtin_memcpy(&raw, row + v, sizeof raw);  // (rows of odd length are not 16-byte aligned)
     } else {
 #pragma unroll
-        for (unsigned e = 0; e < kVec; ++e) p[e] = v + e < end ? float(row[v + e]) : 0.f;
+        for (unsigned e = 0; e < kVec; ++e) raw.v[e] = v + e < end ? row[v + e] : T(0.f);
     }
+    return raw;
 }
 
-// The weights of eight tokens: those of the row's distribution, and of what a refused draft leaves of it.
-template <class T>
-__device__ __forceinline__ void weights8(const T* p_row, const T* q_row, bool refused, unsigned x, unsigned v, unsigned end, double (&all)[kVec],
-                                         double (&rest)[kVec]) {
-    float p[kVec], q[kVec];
-    load8(p_row, v, end, p);
-    if (refused && q_row) load8(q_row, v, end, q);
+// The row that a sequence's next token is drawn from: p alone, without token x (kNone: with all), or p - q.
+template <class T, bool DRAFT>
+struct Row {
+    const T *p, *q;  // q NULL: p alone
+    unsigned x;
+    struct Eight {
+        Raw<T> p, q[DRAFT ? 1 : 0];
+    };
+    __device__ __forceinline__ Eight load(unsigned v, unsigned end) const {
+        Eight r;
+        r.p = load8(p, v, end);
+        if constexpr (DRAFT)
+            if (q) r.q[0] = load8(q, v, end);
+        return r;
+    }
+    // the weights; all: those of p where q is there
+    __device__ __forceinline__ void weights(const Eight& r, unsigned v, double (&w)[kVec], double& all) const {
+        all = 0.0;
 #pragma unroll
-    for (unsigned e = 0; e < kVec; ++e) {
-        all[e] = positive(double(p[e]));
-        rest[e] = !refused ? 0.0 : q_row ? positive(double(p[e]) - positive(double(q[e]))) : v + e == x ? 0.0 : all[e];
+        for (unsigned e = 0; e < kVec; ++e) w[e] = double(counted(float(r.p.v[e])));
+        if constexpr (DRAFT) {
+            if (q) {
+#pragma unroll
+                for (unsigned e = 0; e < kVec; ++e) {
+                    all += w[e];
+                    w[e] = fmax(w[e] - double(counted(float(r.q[0].v[e]))), 0.0);
+                }
+            }
+        } else if (x - v < kVec) {
+#pragma unroll
+            for (unsigned e = 0; e < kVec; ++e)
+                if (v + e == x) w[e] = 0.0;
+        }
     }
+};
+
+// The lane that the running sum passes `goal` in, of `v` with `before` in front, and what is in front of it: the lowest with something in it that does,
+// else the last with something in it; -1 without any.  The same for all lanes.
+__device__ __forceinline__ int passing(double v, double goal, unsigned lane, double& before) {
+    const double upto = before + wave_scan(v, lane);
+    const uint64_t some = __builtin_amdgcn_ballot_w64(v > 0.0), over = __builtin_amdgcn_ballot_w64(v > 0.0 && upto > goal);
+    if (!some) return -1;
+    const int at = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
+    if (at) before = __shfl(upto, at - 1, 64);
+    return at;
 }
 
-template <class T>
-__global__ __launch_bounds__(256) void verify_drafts_kernel(Args a) {
-    __shared__ double s_sum[2][kThreads / 64], s_scan[kThreads / 64];
-    __shared__ unsigned s_first, s_found, s_last;
-    __shared__ int s_is_last;
+template <bool DRAFT>
+constexpr int kBlocks = DRAFT ? 4 : 6;  // of a CU: what their registers leave room for
+
+template <class T, bool DRAFT>
+__global__ __launch_bounds__(256, kBlocks<DRAFT>) void verify_drafts_kernel(Args a) {
+    __shared__ double s_sum[2][kWaves], s_piece[kAtOnce * kWaves];
+    __shared__ unsigned s_first;
+    __shared__ int s_is_last, s_next;
     const unsigned b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, runs = gridDim.x;
     const long lo = a.starts[b], hi = a.starts[b + 1];
     const unsigned from = unsigned(lo < 0 ? 0 : lo > long(a.rows) ? long(a.rows) : lo), to = unsigned(hi < lo ? from : hi > long(a.rows) ? long(a.rows) : hi < 0 ? 0 : hi);
@@ -102,11 +142,12 @@ __global__ __launch_bounds__(256) void verify_drafts_kernel(Args a) {
         const unsigned i = i0 + tid;
         if (i + 1 < n) {
             const unsigned x = unsigned(a.tokens[from + i + 1]);
+            const float u = a.uniforms[from + i];
             bool ok = false;
             if (x < a.vocab) {
                 const double p = double(float(target[size_t(from + i) * a.vocab + x]));
-                const double q = draft ? double(float(draft[size_t(from + i) * a.vocab + x])) : 1.0;
-                ok = double(a.uniforms[from + i]) * q < p;
+                const double q = DRAFT ? double(float(draft[size_t(from + i) * a.vocab + x])) : 1.0;
+                ok = double(u) * q < p;
             }
             if (!ok) atomicMin(&s_first, i);
         }
@@ -116,77 +157,106 @@ __global__ __launch_bounds__(256) void verify_drafts_kernel(Args a) {
         __syncthreads();
     }
     const bool refused = accepted < n - 1;
-    const unsigned x = refused ? unsigned(a.tokens[from + accepted + 1]) : 0;
-    const T* const p_row = target + size_t(from + accepted) * a.vocab;
-    const T* const q_row = draft ? draft + size_t(from + accepted) * a.vocab : nullptr;
+    Row<T, DRAFT> row{target + size_t(from + accepted) * a.vocab, refused && DRAFT ? draft + size_t(from + accepted) * a.vocab : nullptr,
+               refused && !DRAFT ? unsigned(a.tokens[from + accepted + 1]) : kNone};
 
     // sums of this run
     const unsigned begin = blockIdx.x * a.run, end = begin + a.run < a.vocab ? begin + a.run : a.vocab;
     double all = 0.0, rest = 0.0;
-    for (unsigned v = begin + tid * kVec; v < end; v += kThreads * kVec) {
-        double wa[kVec], wr[kVec];
-        weights8(p_row, q_row, refused, x, v, end, wa, wr);
+    for (unsigned v0 = begin; v0 < end; v0 += kAtOnce * kRound) {
+        typename Row<T, DRAFT>::Eight r[kAtOnce];
 #pragma unroll
-        for (unsigned e = 0; e < kVec; ++e) all += wa[e], rest += wr[e];
+        for (unsigned u = 0; u < kAtOnce; ++u)
+            if (v0 + u * kRound < end) r[u] = row.load(v0 + u * kRound + tid * kVec, end);
+#pragma unroll
+        for (unsigned u = 0; u < kAtOnce; ++u) {
+            if (v0 + u * kRound >= end) continue;  // uniform
+            double w[kVec], some;
+            row.weights(r[u], v0 + u * kRound + tid * kVec, w, some);
+            all += some;
+            rest += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+        }
     }
-    all = wave_sum(all), rest = wave_sum(rest);
-    if (lane == 0) s_sum[0][wave] = all, s_sum[1][wave] = rest;
+    rest = wave_sum(rest);
+    if (row.q) all = wave_sum(all);
+    if (lane == 0) s_sum[0][wave] = rest, s_sum[1][wave] = all;
     __syncthreads();
     if (tid == 0) {
-        all = (s_sum[0][0] + s_sum[0][1]) + (s_sum[0][2] + s_sum[0][3]), rest = (s_sum[1][0] + s_sum[1][1]) + (s_sum[1][2] + s_sum[1][3]);
+        rest = (s_sum[0][0] + s_sum[0][1]) + (s_sum[0][2] + s_sum[0][3]), all = (s_sum[1][0] + s_sum[1][1]) + (s_sum[1][2] + s_sum[1][3]);
         double* const out = a.sums + (size_t(b) * runs + blockIdx.x) * 2;
         // (through to where every block sees it)
-        __hip_atomic_store(out, all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(out + 1, rest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s_is_last = __hip_atomic_fetch_add(&a.arrived[b], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == int(runs) - 1;
+        __hip_atomic_store(out, rest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(out + 1, all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // (both go past the caches, and the last block reads them so: that they have arrived is order enough, no cache need be written back)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        s_is_last = __hip_atomic_fetch_add(&a.arrived[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == int(runs) - 1;
     }
     __syncthreads();
     if (!s_is_last) return;
 
-    // the last block of the sequence: which weights, which run (a lane has the sums of one), which token
+    // the last block of the sequence: a lane has the sums of one run
     const double* const sums = a.sums + (size_t(b) * runs + lane) * 2;
-    const double run_all = lane < runs ? __hip_atomic_load(sums, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
-    const double run_rest = lane < runs ? __hip_atomic_load(sums + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
-    const bool of_rest = refused && wave_sum(run_rest) > 0.0;
-    const double run_sum = of_rest ? run_rest : run_all;
-    const double upto = wave_scan(run_sum, lane), goal = double(a.last[b]) * __shfl(upto, 63, 64);
-    const uint64_t some = __builtin_amdgcn_ballot_w64(run_sum > 0.0), over = __builtin_amdgcn_ballot_w64(run_sum > 0.0 && upto > goal);
-    // (none is over with numbers of 1 and more, and NaN: the last token then)
-    const int run = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : 0;
-    const double before = run ? __shfl(upto, run - 1, 64) : 0.0;
-    // a thread has consecutive tokens of the run
-    const unsigned first = unsigned(run) * a.run, stop = first + a.run < a.vocab ? first + a.run : a.vocab;
-    const unsigned each = (a.run + kThreads * kVec - 1) / (kThreads * kVec) * kVec, mine = first + tid * each;
-    auto over_mine = [&](auto&& f) {
-        for (unsigned v = mine; v < mine + each && v < stop; v += kVec) {
-            double wa[kVec], wr[kVec];
-            weights8(p_row, q_row, refused, x, v, stop, wa, wr);
-#pragma unroll
-            for (unsigned e = 0; e < kVec; ++e) f(v + e, of_rest ? wr[e] : wa[e]);
+    double run_sum = lane < runs ? __hip_atomic_load(sums, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+    const double run_all = lane < runs ? __hip_atomic_load(sums + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+    double total = wave_sum(run_sum), before = 0.0;
+    if (tid == 0) s_next = -1;
+    if (refused && !(total > 0.0)) {
+        // nothing is left of p: from p itself (without a draft that is x alone)
+        if (row.q) {
+            row.q = nullptr, run_sum = run_all, total = wave_sum(run_all);
+        } else if (row.x < a.vocab && counted(float(row.p[row.x])) > 0.f) {
+            __syncthreads();
+            if (tid == 0) s_next = int(row.x);
         }
-    };
-    double sum = 0.0;
-    over_mine([&](unsigned, double w) { sum += w; });
-    // what the threads before it have
-    const double scan = wave_scan(sum, lane);
-    if (lane == 63) s_scan[wave] = scan;
-    if (tid == 0) s_found = 0xffffffffu, s_last = 0;
-    __syncthreads();
-    double at = before + (scan - sum);
-    for (unsigned i = 0; i < wave; ++i) at += s_scan[i];
-    unsigned found = 0xffffffffu, last = 0;
-    if (sum > 0.0)
-        over_mine([&](unsigned v, double w) {
-            if (w > 0.0) {
-                at += w, last = v + 1;
-                if (at > goal && found == 0xffffffffu) found = v;
+    }
+    const double goal = double(a.last[b]) * total;
+    const int run = passing(run_sum, goal, lane, before);
+    if (run >= 0) {
+        const unsigned first = unsigned(run) * a.run, stop = first + a.run < a.vocab ? first + a.run : a.vocab;
+        for (unsigned v0 = first; v0 < stop; v0 += kAtOnce * kRound) {
+            double sum[kAtOnce];
+            typename Row<T, DRAFT>::Eight r[kAtOnce];
+#pragma unroll
+            for (unsigned u = 0; u < kAtOnce; ++u) r[u] = row.load(v0 + u * kRound + tid * kVec, stop);
+            __syncthreads();  // (the pieces' sums before have been read)
+#pragma unroll
+            for (unsigned u = 0; u < kAtOnce; ++u) {
+                double w[kVec], some;
+                row.weights(r[u], v0 + u * kRound + tid * kVec, w, some);
+                sum[u] = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+                const double piece = wave_sum(sum[u]);
+                if (lane == 0) s_piece[u * kWaves + wave] = piece;
             }
-        });
-    if (found != 0xffffffffu) atomicMin(&s_found, found);
-    if (last) atomicMax(&s_last, last);
+            __syncthreads();
+            const double piece_sum = lane < kAtOnce * kWaves ? s_piece[lane] : 0.0, here = wave_sum(piece_sum);
+            // (the last of a run's rounds with something in it decides if none passes)
+            double at_piece = before;
+            const int piece = passing(piece_sum, goal, lane, at_piece);
+            if (piece >= 0 && unsigned(piece) % kWaves == wave) {
+                const unsigned u = unsigned(piece) / kWaves;
+                double mine = sum[0];
+#pragma unroll
+                for (unsigned k = 1; k < kAtOnce; ++k) mine = u == k ? sum[k] : mine;
+                const int at_lane = passing(mine, goal, lane, at_piece);
+                if (at_lane == int(lane)) {
+                    const unsigned v = v0 + u * kRound + tid * kVec;
+                    double w[kVec], some;
+                    row.weights(row.load(v, stop), v, w, some);
+                    int next = -1;
+                    bool passed = false;
+#pragma unroll
+                    for (unsigned e = 0; e < kVec; ++e)
+                        if (w[e] > 0.0 && !passed) at_piece += w[e], next = int(v + e), passed = at_piece > goal;
+                    s_next = next;
+                }
+            }
+            before += here;
+            if (before > goal) break;  // uniform
+        }
+    }
     __syncthreads();
     if (tid == 0) a.arrived[b] = 0;
-    const int next = s_found != 0xffffffffu ? int(s_found) : int(s_last) - 1;  // (-1: no weight at all)
+    const int next = s_next;
     for (unsigned i = tid; i < n; i += kThreads) a.new_tokens[from + i] = i < accepted ? a.tokens[from + i + 1] : i == accepted ? next : -1;
     if (tid == 0) a.counts[b] = int(accepted) + 1;
 }
@@ -202,11 +272,12 @@ extern "C" int lq_verify_drafts(const void* target, const void* draft, int dtype
     LQ_REQUIRE(starts && last && counts, LQ_ERR_VALUE, "verify_drafts: starts, last or counts is NULL");
     LQ_REQUIRE(new_tokens != tokens || !tokens, LQ_ERR_VALUE, "verify_drafts: the new tokens cannot take the drafted ones' place");
     LQ_REQUIRE(rows == 0 || (target && tokens && uniforms && new_tokens), LQ_ERR_VALUE, "verify_drafts: a NULL pointer");
-    // Runs of 8192 tokens, shorter ones of few sequences, so that some 512 blocks share the work, and 64 of a sequence at most.
-    unsigned runs = unsigned(vocab + 8191) / 8192;
-    const unsigned fill = 512 / unsigned(batch), most = unsigned(vocab + 2047) / 2048;
-    if (runs < fill) runs = fill < most ? fill : most;
-    if (runs > 64) runs = 64;
+    // As many blocks as are resident, a round of 2048 tokens at least each; 64 of a sequence at most.  (128 rows of 131 072: three rounds of blocks of
+    // 8192 tokens 50 us, one of 16 384 39, before the sums went on without a write-back of the caches.)
+    unsigned runs = 256u * unsigned(draft ? kBlocks<true> : kBlocks<false>) / unsigned(batch);
+    const unsigned most = (unsigned(vocab) + kRound - 1) / kRound;
+    runs = runs < 1 ? 1 : runs > 64 ? 64 : runs;
+    if (runs > most) runs = most;
     const unsigned run = ((unsigned(vocab) + runs - 1) / runs + kVec - 1) / kVec * kVec;
     runs = (unsigned(vocab) + run - 1) / run;
     const hipStream_t st = as_stream(stream);
@@ -216,8 +287,9 @@ extern "C" int lq_verify_drafts(const void* target, const void* draft, int dtype
     const Args a{target, draft, tokens, starts, uniforms, last, new_tokens, counts, unsigned(rows), unsigned(vocab), run,
                  reinterpret_cast<double*>(scratch.slabs), scratch.counters};
     const dim3 grid(runs, unsigned(batch));
-    if (dtype == LQ_F32) verify_drafts_kernel<float><<<grid, kThreads, 0, st>>>(a);
-    else verify_drafts_kernel<_Float16><<<grid, kThreads, 0, st>>>(a);
+    const auto kernel = dtype == LQ_F32 ? (draft ? verify_drafts_kernel<float, true> : verify_drafts_kernel<float, false>)
+                                        : (draft ? verify_drafts_kernel<_Float16, true> : verify_drafts_kernel<_Float16, false>);
+    kernel<<<grid, kThreads, 0, st>>>(a);
     LQ_CHECK_LAUNCH("verify_drafts");
     return LQ_OK;
 }
