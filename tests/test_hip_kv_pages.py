@@ -88,7 +88,7 @@ def test_compacted_sequences(bits, symmetric, dim, heads, page, lengths, part):
     check(c, table, np.concatenate(keep), np.cumsum([0] + [len(k) for k in keep]))
 
 
-@pytest.mark.parametrize("n", [63, 64, 65, 128, 129, 1000, 5000])
+@pytest.mark.parametrize("n", [63, 64, 65, 255, 256, 257, 513, 1000, 5000])
 @pytest.mark.parametrize("kind", ["first evicted", "a window", "sinks and a window", "every other", "all", "none of the second half", "one each"])
 def test_what_sequences_keep(n, kind):
     """Rows that move by one, by the most, not at all; a tile's old places taken by tiles far behind it."""
