@@ -29,20 +29,29 @@ __global__ __launch_bounds__(256) void kv_copy_kernel(Buffers b, const int* __re
                                                       unsigned num_pages, unsigned codes, unsigned numbers, FastDiv units, FastDiv blocks,
                                                       unsigned pages) {
     const unsigned group = blocks(blockIdx.x), chunk = (blockIdx.x - group * blocks.d) * kCopyChunk, first = group * pages;
+    constexpr unsigned EACH = kCopyChunk / 256;
+    u4 v[EACH];
+    u4* to[EACH];
+    // (no branch around the loads: all of a thread's are under way at once)
 #pragma unroll
-    for (unsigned u = 0; u < kCopyChunk; u += 256) {
-        const unsigned i = chunk + u + threadIdx.x, pair = first + units(i);
-        unsigned unit = i - units(i) * units.d;
-        if (pair >= n || (pages == 1 ? pair != first : pair >= first + pages)) continue;
-        const unsigned from = unsigned(src[pair]), to = unsigned(dst[pair]);
-        if (from >= num_pages || to >= num_pages) continue;  // (negative ones too)
-        unsigned which = 0, length = codes;
+    for (unsigned u = 0; u < EACH; ++u) {
+        const unsigned i = chunk + u * 256 + threadIdx.x, in_group = units(i), pair = first + in_group;
+        unsigned unit = i - in_group * units.d, length = codes;
+        bool there = pair < n && in_group < pages;
+        const unsigned from_page = unsigned(src[there ? pair : 0]), to_page = unsigned(dst[there ? pair : 0]);
+        there = there && from_page < num_pages && to_page < num_pages;  // (negative ones too)
+        unsigned which = 0;
         if (unit >= 2 * codes) unit -= 2 * codes, which = 2, length = numbers;
-        while (unit >= length) unit -= length, ++which;
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            if (unit >= length) unit -= length, ++which;
         char* const base = b.at[which];
-        const u4 v = __builtin_nontemporal_load(reinterpret_cast<const u4*>(base + (size_t(from) * length + unit) * 16));
-        __builtin_nontemporal_store(v, reinterpret_cast<u4*>(base + (size_t(to) * length + unit) * 16));
+        v[u] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(base + (size_t(there ? from_page : 0) * length + unit) * 16));
+        to[u] = there ? reinterpret_cast<u4*>(base + (size_t(to_page) * length + unit) * 16) : nullptr;
     }
+#pragma unroll
+    for (unsigned u = 0; u < EACH; ++u)
+        if (to[u]) __builtin_nontemporal_store(v[u], to[u]);
 }
 
 // ---------------------------------------------------------------- rows

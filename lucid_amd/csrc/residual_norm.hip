@@ -6,7 +6,9 @@
 //
 // A row stays in the registers of the TPR threads that have it: x and r are read once, r' and y written once, whatever norms are
 // asked for; a layer norm's variance is taken about its mean from the registers.  y comes from r' as it is in float32, before that
-// is rounded to its own type.  Bound by memory.
+// is rounded to its own type.  Bound by memory: what passes once leaves the caches to others (12 608 x 768 float32, both layer norms, a gate of
+// 64 rows and a scale 36 -> 29 us, 5.3 TB/s; sums over lane patterns 37 -> 36).  Keeping weights and scales in registers from row to row, with the next
+// row under way, gains nothing: 37 to 40 us.
 #include <type_traits>
 
 #include "common.hpp"
@@ -17,6 +19,8 @@ namespace {
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef f4 f4u __attribute__((aligned(4)));  // (rows need not be aligned)
+typedef h4 h4u __attribute__((aligned(2)));
 
 struct Norm {
     const float *weight, *bias;  // NULL: ones, zeros
@@ -32,47 +36,61 @@ struct Args {
     FastDiv per_gate{1};  // rows of a row of the gate
 };
 
-// Four values of a row from column c on, zeros past its end.
-template <class T>
+// Four values of a row from column c on, zeros past its end.  WHOLE: rows of a multiple of four.  No branch: the compiler waits for a load where two
+// paths that give its register a value meet.
+template <bool WHOLE, bool STREAM = false, class T>
 __device__ __forceinline__ f4 load4(const T* row, unsigned c, unsigned cols) {
-    if (c + 4 <= cols) {  // (not always 8 or 16-byte aligned)
+    f4 v;
+    if constexpr (WHOLE) {
+        const T* const from = row + (c < cols ? c : 0);
         if constexpr (std::is_same_v<T, float>) {
-            f4 v;
-            __builtin_memcpy(&v, row + c, 16);
-            return v;
+            v = STREAM ? __builtin_nontemporal_load(reinterpret_cast<const f4u*>(from)) : *reinterpret_cast<const f4u*>(from);
         } else {
-            h4 v;
-            __builtin_memcpy(&v, row + c, 8);
-            return f4{float(v[0]), float(v[1]), float(v[2]), float(v[3])};
+            const h4 h = STREAM ? __builtin_nontemporal_load(reinterpret_cast<const h4u*>(from)) : *reinterpret_cast<const h4u*>(from);
+            v = f4{float(h[0]), float(h[1]), float(h[2]), float(h[3])};
         }
-    }
-    f4 v{0.f, 0.f, 0.f, 0.f};
+        return c < cols ? v : f4{0.f, 0.f, 0.f, 0.f};
+    } else {
 #pragma unroll
-    for (unsigned i = 0; i < 3; ++i)
-        if (c + i < cols) v[i] = float(row[c + i]);
-    return v;
+        for (unsigned i = 0; i < 4; ++i) {
+            const float e = float(row[c + i < cols ? c + i : 0]);
+            v[i] = c + i < cols ? e : 0.f;
+        }
+        return v;
+    }
 }
-template <class T>
+template <bool WHOLE, class T>
 __device__ __forceinline__ void store4(T* row, unsigned c, unsigned cols, f4 v) {
-    if (c + 4 <= cols) {
+    if constexpr (WHOLE) {
+        if (c >= cols) return;
         if constexpr (std::is_same_v<T, float>) {
-            __builtin_memcpy(row + c, &v, 16);
+            __builtin_nontemporal_store(f4u(v), reinterpret_cast<f4u*>(row + c));
         } else {
             const h4 h{_Float16(v[0]), _Float16(v[1]), _Float16(v[2]), _Float16(v[3])};
-            __builtin_memcpy(row + c, &h, 8);
+            __builtin_nontemporal_store(h4u(h), reinterpret_cast<h4u*>(row + c));
         }
-        return;
-    }
+    } else {
 #pragma unroll
-    for (unsigned i = 0; i < 3; ++i)
-        if (c + i < cols) row[c + i] = T(v[i]);
+        for (unsigned i = 0; i < 4; ++i)
+            if (c + i < cols) row[c + i] = T(v[i]);
+    }
 }
 
+// A lane's neighbour by the vector unit's own patterns, zeros where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float moved(float v) {
+    return __uint_as_float(unsigned(__builtin_amdgcn_update_dpp(0, int(__float_as_uint(v)), CTRL, ROWS, 0xf, false)));
+}
 // The sum over the TPR threads of a row, to all of them.
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* s) {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
+    v += moved<0x111, 0xf>(v);  // over rows of 16 lanes: from 1, 2, 4, 8 lanes before
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);  // lane 15 into rows 1 and 3, lane 31 into rows 2 and 3: lane 63 has the sum
+    v += moved<0x143, 0xc>(v);
+    v = __uint_as_float(unsigned(__builtin_amdgcn_readlane(int(__float_as_uint(v)), 63)));
     if constexpr (TPR > 64) {
         __syncthreads();  // (the sums before have been read)
         if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
@@ -84,7 +102,7 @@ __device__ __forceinline__ float row_sum(float v, float* s) {
     return v;
 }
 
-template <bool LAYER, int TPR, int NV>
+template <bool LAYER, bool WHOLE, int TPR, int NV>
 __device__ __forceinline__ void normalize(f4 (&v)[NV], const Norm& n, unsigned at, unsigned cols, float eps, float* s) {
     const float inverse = 1.0f / float(cols);
     float sum = 0.f;
@@ -102,36 +120,39 @@ __device__ __forceinline__ void normalize(f4 (&v)[NV], const Norm& n, unsigned a
     for (int i = 0; i < NV; ++i) sum += (v[i][0] * v[i][0] + v[i][1] * v[i][1]) + (v[i][2] * v[i][2] + v[i][3] * v[i][3]);
     const float f = 1.0f / sqrtf(row_sum<TPR>(sum, s) * inverse + eps);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const unsigned c = at + i * TPR * 4;
-        v[i] *= f;
-        if (n.weight && c < cols) v[i] *= load4(n.weight, c, cols);
-        if (n.bias && c < cols) v[i] += load4(n.bias, c, cols);
+    for (int i = 0; i < NV; ++i) v[i] *= f;
+    if (n.weight) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] *= load4<WHOLE>(n.weight, at + i * TPR * 4, cols);
+    }
+    if (n.bias) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] += load4<WHOLE>(n.bias, at + i * TPR * 4, cols);
     }
 }
 
-template <class TX, class TR, bool LAYER, bool POST, int TPR, int NV>
+template <class TX, class TR, bool LAYER, bool POST, bool WHOLE, int TPR, int NV>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void residual_norm_kernel(Args a) {
     __shared__ float s[TPR / 64];
     const unsigned row = blockIdx.x * (TPR < 256 ? 256 / TPR : 1) + threadIdx.x / TPR, at = threadIdx.x % TPR * 4;
-    if (row >= a.rows) return;  // (rows of TPR = 64: no barrier follows)
+    if (row >= a.rows) return;  // (rows of 64 threads: no barrier follows)
     const size_t base = size_t(row) * a.cols;
     f4 x[NV], r[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) x[i] = load4(static_cast<const TX*>(a.x) + base, at + i * TPR * 4, a.cols);
+    for (int i = 0; i < NV; ++i) x[i] = load4<WHOLE, true>(static_cast<const TX*>(a.x) + base, at + i * TPR * 4, a.cols);
     if (a.r) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) r[i] = load4(static_cast<const TR*>(a.r) + base, at + i * TPR * 4, a.cols);
+        for (int i = 0; i < NV; ++i) r[i] = load4<WHOLE, true>(static_cast<const TR*>(a.r) + base, at + i * TPR * 4, a.cols);
     }
-    if constexpr (POST) normalize<LAYER, TPR, NV>(x, a.post, at, a.cols, a.eps, s);
+    if constexpr (POST) normalize<LAYER, WHOLE, TPR, NV>(x, a.post, at, a.cols, a.eps, s);
     if (a.scale) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) x[i] *= load4(a.scale, at + i * TPR * 4, a.cols);
+        for (int i = 0; i < NV; ++i) x[i] *= load4<WHOLE>(a.scale, at + i * TPR * 4, a.cols);
     }
     if (a.gate) {
         const TX* gate = static_cast<const TX*>(a.gate) + size_t(a.per_gate(row)) * a.cols;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) x[i] *= load4(gate, at + i * TPR * 4, a.cols);
+        for (int i = 0; i < NV; ++i) x[i] *= load4<WHOLE>(gate, at + i * TPR * 4, a.cols);
     }
     if (a.r) {
 #pragma unroll
@@ -139,37 +160,45 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void residual_norm_kernel(Ar
     }
     if (a.r_out) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) store4(static_cast<TR*>(a.r_out) + base, at + i * TPR * 4, a.cols, x[i]);
+        for (int i = 0; i < NV; ++i) store4<WHOLE>(static_cast<TR*>(a.r_out) + base, at + i * TPR * 4, a.cols, x[i]);
     }
-    normalize<LAYER, TPR, NV>(x, a.pre, at, a.cols, a.eps, s);
+    normalize<LAYER, WHOLE, TPR, NV>(x, a.pre, at, a.cols, a.eps, s);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) store4(static_cast<TX*>(a.y) + base, at + i * TPR * 4, a.cols, x[i]);
+    for (int i = 0; i < NV; ++i) store4<WHOLE>(static_cast<TX*>(a.y) + base, at + i * TPR * 4, a.cols, x[i]);
 }
 
 template <int V>
 using Int = std::integral_constant<int, V>;
 
-// f with the threads of a row and the fours of values that each has.
+// f with whether rows are of a multiple of four values, the threads of a row, and the fours of values that each has.
 template <class F>
-void by_shape(unsigned rows, unsigned cols, F&& f) {
+void by_shape(unsigned cols, F&& f) {
     const unsigned fours = (cols + 3) / 4;
-    if (fours <= 64) f(Int<64>{}, Int<1>{});
-    else if (fours <= 128) f(Int<64>{}, Int<2>{});
-    else if (fours <= 192) f(Int<64>{}, Int<3>{});
-    else if (fours <= 256) f(Int<64>{}, Int<4>{});
-    else if (fours <= 512) f(Int<256>{}, Int<2>{});
-    else if (fours <= 1024) f(Int<256>{}, Int<4>{});
-    else if (fours <= 2048) f(Int<1024>{}, Int<2>{});
-    else if (fours <= 4096) f(Int<1024>{}, Int<4>{});
-    else f(Int<1024>{}, Int<8>{});
+    if (cols % 4) {
+        if (fours <= 256) f(std::false_type{}, Int<64>{}, Int<4>{});
+        else if (fours <= 1024) f(std::false_type{}, Int<256>{}, Int<4>{});
+        else f(std::false_type{}, Int<1024>{}, Int<8>{});
+        return;
+    }
+    const std::true_type whole{};
+    if (fours <= 64) f(whole, Int<64>{}, Int<1>{});
+    else if (fours <= 128) f(whole, Int<64>{}, Int<2>{});
+    else if (fours <= 192) f(whole, Int<64>{}, Int<3>{});
+    else if (fours <= 256) f(whole, Int<64>{}, Int<4>{});
+    else if (fours <= 512) f(whole, Int<256>{}, Int<2>{});
+    else if (fours <= 1024) f(whole, Int<256>{}, Int<4>{});
+    else if (fours <= 2048) f(whole, Int<1024>{}, Int<2>{});
+    else if (fours <= 4096) f(whole, Int<1024>{}, Int<4>{});
+    else f(whole, Int<1024>{}, Int<8>{});
 }
 
 template <class TX, class TR, bool LAYER>
 void launch(const Args& a, bool post, hipStream_t st) {
-    by_shape(a.rows, a.cols, [&](auto tpr, auto nv) {
+    by_shape(a.cols, [&](auto whole, auto tpr, auto nv) {
+        constexpr bool WHOLE = decltype(whole)::value;
         constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, BLOCK = TPR < 256 ? 256 : TPR;
         const unsigned per = BLOCK / TPR;
-        const auto kernel = post ? residual_norm_kernel<TX, TR, LAYER, true, TPR, NV> : residual_norm_kernel<TX, TR, LAYER, false, TPR, NV>;
+        const auto kernel = post ? residual_norm_kernel<TX, TR, LAYER, true, WHOLE, TPR, NV> : residual_norm_kernel<TX, TR, LAYER, false, WHOLE, TPR, NV>;
         kernel<<<(a.rows + per - 1) / per, BLOCK, 0, st>>>(a);
     });
 }
