@@ -94,14 +94,30 @@ __device__ __forceinline__ void split_f16(const float (&v)[8], float f, uint4 (&
 
 }  // namespace
 
-// Few rows (wq_gated_rows.hip).  bits 4 or 8, groups of 32, 64 or 128.
+// Few rows (wq_gated_rows.hpp).  bits 4 or 8, groups of 32, 64 or 128.
 int launch_rows_f16(const Args& a, int bits, hipStream_t st);
 int launch_rows_f32(const Args& a, int bits, hipStream_t st);
-// Many rows (wq_gated_gemm.hpp), by type and bits; weights below 2 GiB.
-int launch_gemm_f16_4(const Args& a, hipStream_t st);
-int launch_gemm_f16_8(const Args& a, hipStream_t st);
-int launch_gemm_f32_4(const Args& a, hipStream_t st);
-int launch_gemm_f32_8(const Args& a, hipStream_t st);
+
+// Many rows (wq_gated_gemm.hpp): 16 mt rows x 64 ct columns a block, and what a stage of 64 k takes (us) when a CU has one block, or two: measured
+// with 4-bit codes in groups of 128 at K = 4096, N = 11008 and 64 to 2048 rows.  (8-bit codes of wide blocks leave no room for a ring of stages.)
+struct GemmTile {
+    int mt, ct;
+    float one, two;
+};
+constexpr int kGemmTiles = 5;
+template <int PARTS, int BITS>
+constexpr GemmTile kGemmTile[kGemmTiles] = {{2, 2, 0.73f, 1.03f}, {4, 2, 0.95f, 1.25f}, {6, 2, 1.15f, 1.72f}, {2, 4, 1.15f, 1.75f}, {3, 4, 1.32f, 1.95f}};
+template <>
+inline constexpr GemmTile kGemmTile<1, 8>[kGemmTiles] = {{2, 2, 0.73f, 1.03f}, {3, 2, 0.85f, 1.17f}, {4, 2, 0.95f, 1.25f}, {6, 2, 1.15f, 1.72f}, {2, 4, 1.15f, 1.75f}};
+template <>
+inline constexpr GemmTile kGemmTile<2, 4>[kGemmTiles] = {{1, 2, 0.60f, 0.97f}, {2, 2, 0.95f, 1.30f}, {4, 2, 1.35f, 1.98f}, {2, 4, 1.40f, 2.35f}, {3, 4, 1.70f, 2.95f}};
+template <>
+inline constexpr GemmTile kGemmTile<2, 8>[kGemmTiles] = {{1, 2, 0.60f, 0.97f}, {2, 2, 0.95f, 1.30f}, {3, 2, 1.20f, 1.58f}, {4, 2, 1.35f, 1.98f}, {0, 0, 0.f, 0.f}};
+// By type and bits, `tile` of these; weights below 2 GiB.
+int launch_gemm_f16_4(const Args& a, int tile, hipStream_t st);
+int launch_gemm_f16_8(const Args& a, int tile, hipStream_t st);
+int launch_gemm_f32_4(const Args& a, int tile, hipStream_t st);
+int launch_gemm_f32_8(const Args& a, int tile, hipStream_t st);
 
 }  // namespace gated
 }  // namespace lq

@@ -5,7 +5,7 @@
 // parts, and the scales group after group.  float16 x enters as it is; a float32 row is multiplied by the power of two that brings its
 // largest value below 2^15 and enters as two float16, hi = x rounded, lo = x - hi rounded: 22 bits, or 2^-39 of the largest value.
 //
-// gated_gemm_kernel: a block of four wavefronts takes 16 MT rows x 128 columns of both weights, a wavefront all rows x 32 columns of each, so
+// gated_gemm_kernel: a block of four wavefronts takes 16 MT rows x 64 CT columns of both weights, a wavefront all rows x 16 CT columns of each, so
 // that no code is turned into float16 twice in a block.  What a stage of 64 k needs comes from memory straight into LDS in pieces of
 // 1 KiB per wavefront and instruction, in a ring of stages: every wavefront issues as many loads per stage, so that "stage s has arrived"
 // is a count of outstanding loads.  The products of a group (at most 64 k) go to accumulators of their own, and from there with their scale to
@@ -13,6 +13,7 @@
 // float16 x two parts, 2^-16, a sixteenth of what the result rounds.
 #pragma once
 #include <algorithm>
+#include <type_traits>
 
 #include "wq_gated.hpp"
 
@@ -23,7 +24,6 @@ namespace {
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));  // (see wq_gated_rows.hpp on types in LDS)
 
 constexpr int kPiece = 1024;  // bytes one wavefront moves into LDS with one instruction
-constexpr int kCols = 128;    // of a block, of each weight
 
 __host__ __device__ constexpr int sum_parts(int parts) { return parts == 1 ? 2 : 3; }
 
@@ -31,7 +31,7 @@ struct Prepared {
     char* x;          // [stage][row tile][2][part] pieces
     char* sums;       // [row tile][group step][sum part] pieces: groups as k
     char* biases;     // [weight][column tile of 16][group step][sum part] pieces
-    float* scales;    // [group][block of columns][weight][128]
+    float* scales;    // [group][block of columns][weight][64 CT]
     float* unscale;   // [row] of float32 x: what its row was multiplied by, inverse
     int mtiles, stages, group_steps, tiles_n;
 };
@@ -53,9 +53,9 @@ __global__ __launch_bounds__(256) void gated_row_scale_kernel(const float* __res
 }
 
 // Two kinds of blocks.  The first `x_blocks`: 16 rows x 128 k, a thread has eight k.  The others: 64 columns of a weight, a wavefront eight groups.
-template <class T, int PARTS, int BITS>
+template <class T, int PARTS, int BITS, int CT>
 __global__ __launch_bounds__(256) void gated_prepare_kernel(Args a, Prepared p, unsigned x_blocks) {
-    constexpr int SP = sum_parts(PARTS);
+    constexpr int SP = sum_parts(PARTS), kCols = 64 * CT;
     const int gs = 1 << a.gs_shift;
     if (blockIdx.x >= x_blocks) {
         const unsigned i = blockIdx.x - x_blocks, across = unsigned(p.tiles_n) * (kCols / 64), which = (i / across) & 1, lane = threadIdx.x & 63;
@@ -130,12 +130,12 @@ __global__ __launch_bounds__(256) void gated_prepare_kernel(Args a, Prepared p, 
 }
 
 // What a stage of one block is made of, in pieces.
-template <int PARTS, int BITS, int GS, int MT>
+template <int PARTS, int BITS, int GS, int MT, int CT>
 struct Stage {
     static constexpr int SEGS = GS == 32 ? 2 : 1;     // groups of a stage
     static constexpr int X = 2 * MT * PARTS;          // fragments
-    static constexpr int S = SEGS;                    // 128 scales of both weights
-    static constexpr int W = 2 * BITS;                // 128 rows of 8 BITS bytes, of both
+    static constexpr int S = SEGS * CT / 2;           // 64 CT scales of both weights
+    static constexpr int W = CT * BITS;               // 64 CT rows of 8 BITS bytes, of both
     static constexpr int PIECES = X + S + W;
     static constexpr int PER_WAVE = (PIECES + 3) / 4;
     static constexpr int FIT = 80 / PIECES;  // two blocks a CU
@@ -146,10 +146,10 @@ struct Stage {
 // s_waitcnt immediate for vmcnt <= n and every LDS read done
 constexpr int vmcnt_lds(int n) { return (n & 0xF) | ((n >> 4) << 14) | (0x7 << 4); }
 
-template <class T, int PARTS, int BITS, int GS, int MT>
+template <class T, int PARTS, int BITS, int GS, int MT, int CT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void gated_gemm_kernel(Args a, Prepared p, int tiles_m) {
-    using S = Stage<PARTS, BITS, GS, MT>;
-    constexpr int SP = sum_parts(PARTS);
+    using S = Stage<PARTS, BITS, GS, MT, CT>;
+    constexpr int SP = sum_parts(PARTS), kCols = 64 * CT, JT = 2 * CT;  // column tiles of a wavefront: the gate's, then the other's
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = lane & 15, q = lane >> 4;
     // every XCD gets a contiguous range of tiles, row tiles first: its L2 then reads a weight row once
@@ -159,62 +159,82 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
     // ---- the loads of a stage: piece u * 4 + wave (the last round repeats pieces: the counts stay equal)
     constexpr int ROW = 8 * BITS, CH = ROW / 16;  // bytes of codes per row and stage; 16-byte chunks
-    const unsigned row_bytes = unsigned(a.K) * BITS / 8, w_last = unsigned(a.N) * row_bytes - 16;
+    const unsigned row_bytes = unsigned(a.K) * BITS / 8;
+    // A piece's address is a scalar, which goes on by `step` from stage to stage, and a lane's offset: no branch, next to no vector work.
     const char* src[S::PER_WAVE];
-    unsigned off[S::PER_WAVE];
+    size_t step[S::PER_WAVE];
+    unsigned off[S::PER_WAVE], back[S::PER_WAVE];
+    bool twice[S::PER_WAVE];  // (scales of groups of 128: every second stage)
 #pragma unroll
     for (int u = 0; u < S::PER_WAVE; ++u) {
         int at = u * 4 + wave;
         at = at < S::PIECES ? at : at - 4;
-        off[u] = unsigned(lane) * 16;
+        off[u] = unsigned(lane) * 16, back[u] = 0, twice[u] = false;
         if (at < S::X) {
             src[u] = p.x + size_t(tm) * (S::X * kPiece) + at * kPiece;
+            step[u] = size_t(p.mtiles) * (2 * PARTS * kPiece);
         } else if (at < S::X + S::S) {
-            src[u] = reinterpret_cast<const char*>(p.scales) + (size_t(at - S::X) * p.tiles_n + tn) * kPiece;
+            const int i = at - S::X;  // CT / 2 pieces a group
+            src[u] = reinterpret_cast<const char*>(p.scales) + (size_t(i / (CT / 2)) * p.tiles_n + tn) * (CT / 2 * kPiece) + i % (CT / 2) * kPiece;
+            step[u] = size_t(S::SEGS) * p.tiles_n * (CT / 2 * kPiece), twice[u] = GS == 128;
         } else {
             // the chunks of a row change places with its number, so that the 16 rows of an operand lie in different banks
-            const int i = at - (S::X + S::S), which = i / BITS, r = (i - which * BITS) * (64 / CH) + lane / CH;
-            const int n = tn * kCols + r < a.N ? tn * kCols + r : a.N - 1;
+            const int i = at - (S::X + S::S), which = i / (S::W / 2), r = i % (S::W / 2) * (64 / CH) + lane / CH;
+            const int n = tn * kCols + r < a.N ? tn * kCols + r : a.N - 1, chunk = (lane % CH) ^ ((r / (16 / CH)) % CH);
             src[u] = reinterpret_cast<const char*>(which ? a.w[1].packed : a.w[0].packed);
-            off[u] = unsigned(n) * row_bytes + unsigned((lane % CH) ^ ((r / (16 / CH)) % CH)) * 16;
+            step[u] = ROW;
+            off[u] = unsigned(n) * row_bytes + unsigned(chunk) * 16;
+            // the second half of a stage that ends half-way is past the row: the first half again (its x is zero)
+            back[u] = GS == 32 && chunk >= CH / 2 && a.K % 64 ? ROW / 2 : 0;
         }
     }
-    auto load_stage = [&](int s, int slot) {
-        const int sc = s < p.stages ? s : p.stages - 1;  // past the end: any stage, to keep the count
+    int loaded = 0;  // the stage that src is at
+    auto load_stage = [&](int slot) {
+        const bool last = loaded >= p.stages - 1;
 #pragma unroll
         for (int u = 0; u < S::PER_WAVE; ++u) {
             int at = u * 4 + wave;
             at = at < S::PIECES ? at : at - 4;
-            const char* base = src[u];
             unsigned o = off[u];
-            if (at < S::X) {
-                base += size_t(sc) * p.mtiles * (2 * PARTS * kPiece);
-            } else if (at < S::X + S::S) {
-                base += size_t(GS == 128 ? sc >> 1 : sc * S::SEGS) * p.tiles_n * kPiece;
-            } else {
-                // a stage past K runs past its row: into the next ones, or at the end of the weight onto its last bytes (its x is zero)
-                const unsigned from = unsigned(sc) * ROW + o;
-                o = from < w_last ? from : w_last;
-            }
-            __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(base + o),
+            if constexpr (GS == 32) o -= last ? back[u] : 0;  // (K is a multiple of 64 otherwise)
+            __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void*)(src[u] + o),
                                              (__attribute__((address_space(3))) void*)(smem + (slot * S::PIECES + at) * kPiece), 16, 0, 0);
+            // past the end: the last stage again, to keep the count
+            src[u] += last || (GS == 128 && twice[u] && loaded % 2 == 0) ? 0 : step[u];
         }
+        ++loaded;
     };
 
-    v4f y[4][MT];  // columns 0 .. 15 and 16 .. 31 of the gate, then of the other
+    v4f y[JT][MT];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < JT; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) y[j][i] = v4f{0.f, 0.f, 0.f, 0.f};
+    v4f acc[2][S::SEGS][MT];
+    float f_last[S::SEGS];
 #pragma unroll
-    for (int s = 0; s < S::RING - 1; ++s) load_stage(s, s);
+    for (int e = 0; e < S::SEGS; ++e) {
+        f_last[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[1][e][i] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    auto scale_sums = [&](int j, const float(&f)[S::SEGS], const v4f(&sums)[S::SEGS][MT]) {
+#pragma unroll
+        for (int e = 0; e < S::SEGS; ++e)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[j][i][r] = __builtin_fmaf(f[e], sums[e][i][r], y[j][i][r]);
+    };
+#pragma unroll
+    for (int s = 0; s < S::RING - 1; ++s) load_stage(s);
     int slot = 0;
     for (int s = 0; s < p.stages; ++s) {
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(vmcnt_lds(S::PER_WAVE * (S::RING - 2)));
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        load_stage(s + S::RING - 1, slot == 0 ? S::RING - 1 : slot - 1);  // (the slot that everybody has just left)
+        load_stage(slot == 0 ? S::RING - 1 : slot - 1);  // (the slot that everybody has just left)
         const char* base = smem + slot * (S::PIECES * kPiece);
         slot = slot + 1 == S::RING ? 0 : slot + 1;
         const char* codes = base + (S::X + S::S) * kPiece;
@@ -226,25 +246,41 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
                 for (int part = 0; part < PARTS; ++part)
                     x[ii][i][part] = *reinterpret_cast<const v8h*>(base + ((i * 2 + ii) * PARTS + part) * kPiece + lane * 16);
+        // Column tile j is multiplied while the sums of the one before it are scaled (of the last: in the next stage) and the codes of the one
+        // behind it are decoded.
+        uint32_t raw[JT][2][BITS / 4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int which = j >> 1, r = wave * 32 + (j & 1) * 16 + ln;
-            v8h c[2];
-            float f[S::SEGS];
+        for (int j = 0; j < JT; ++j) {
+            const int r = (wave * CT + j % CT) * 16 + ln;
+            const char* row = codes + j / CT * (S::W / 2 * kPiece) + r * ROW;
 #pragma unroll
             for (int ii = 0; ii < 2; ++ii) {
-                uint32_t wd[4] = {0u, 0u, 0u, 0u};
-                const char* row = codes + which * (BITS * kPiece) + r * ROW;
-                if constexpr (BITS == 4) wd[0] = *reinterpret_cast<const uint32_t*>(row + (ii ^ ((r >> 3) & 1)) * 16 + q * 4);
-                else {
+                if constexpr (BITS == 4) {
+                    raw[j][ii][0] = *reinterpret_cast<const uint32_t*>(row + (ii ^ ((r >> 3) & 1)) * 16 + q * 4);
+                } else {
                     const u32x2 t = *reinterpret_cast<const u32x2*>(row + ((ii * 2 + (q >> 1)) ^ ((r >> 2) & 3)) * 16 + (q & 1) * 8);
-                    wd[0] = t[0], wd[1] = t[1];
+                    raw[j][ii][0] = t[0], raw[j][ii][BITS / 4 - 1] = t[1];
                 }
+            }
+        }
+        auto decode = [&](int j, v8h(&c)[2]) {
+#pragma unroll
+            for (int ii = 0; ii < 2; ++ii) {
+                const uint32_t wd[4] = {raw[j][ii][0], raw[j][ii][BITS / 4 - 1], 0u, 0u};
                 c[ii] = codes_f16<BITS>(wd, 0);
             }
+        };
+        float f[JT][S::SEGS];
 #pragma unroll
-            for (int e = 0; e < S::SEGS; ++e) f[e] = *reinterpret_cast<const float*>(base + (S::X + e) * kPiece + (which * kCols + r) * 4);
-            v4f acc[S::SEGS][MT];
+        for (int j = 0; j < JT; ++j)
+#pragma unroll
+            for (int e = 0; e < S::SEGS; ++e)
+                f[j][e] = *reinterpret_cast<const float*>(base + (S::X + e * (CT / 2)) * kPiece + (j / CT * kCols + (wave * CT + j % CT) * 16 + ln) * 4);
+        v8h c[2][2];
+        decode(0, c[0]);
+#pragma unroll
+        for (int j = 0; j < JT; ++j) {
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int ii = 0; ii < 2; ++ii)
 #pragma unroll
@@ -253,16 +289,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                     for (int i = 0; i < MT; ++i) {
                         const int e = S::SEGS == 2 ? ii : 0;
                         const bool first = part == 0 && (S::SEGS == 2 || ii == 0);
-                        acc[e][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[ii][i][part], c[ii], first ? v4f{0.f, 0.f, 0.f, 0.f} : acc[e][i], 0, 0, 0);
+                        acc[j & 1][e][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[ii][i][part], c[j & 1][ii], first ? v4f{0.f, 0.f, 0.f, 0.f} : acc[j & 1][e][i], 0, 0, 0);
                     }
+            scale_sums(j == 0 ? JT - 1 : j - 1, j == 0 ? f_last : f[j - 1], acc[(j & 1) ^ 1]);
+            if (j < JT - 1) decode(j + 1, c[(j & 1) ^ 1]);
+            constexpr int MFMAS = 2 * PARTS * MT, VALU = (4 * MT * S::SEGS + 2 * (BITS == 4 ? 9 : 8)) / MFMAS + 1;
 #pragma unroll
-            for (int e = 0; e < S::SEGS; ++e)
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int r4 = 0; r4 < 4; ++r4) y[j][i][r4] = __builtin_fmaf(f[e], acc[e][i][r4], y[j][i][r4]);
+            for (int k = 0; k < MFMAS; ++k) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+            }
         }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < S::SEGS; ++e) f_last[e] = f[JT - 1][e];
     }
+    scale_sums(JT - 1, f_last, acc[1]);
     // the terms of b: hi hi, then what is 2^-8 of it, then (three parts) 2^-16
 #pragma unroll 1
     for (int g = 0; g < p.group_steps; ++g) {
@@ -273,8 +315,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             for (int part = 0; part < SP; ++part)
                 sums[i][part] = __builtin_bit_cast(v8bf, reinterpret_cast<const uint4*>(p.sums)[((size_t(tm * MT + i) * p.group_steps + g) * SP + part) * 64 + lane]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const size_t tile = size_t(j >> 1) * p.tiles_n * (kCols / 16) + tn * (kCols / 16) + wave * 2 + (j & 1);
+        for (int j = 0; j < JT; ++j) {
+            const size_t tile = size_t(j / CT) * p.tiles_n * (kCols / 16) + tn * (kCols / 16) + wave * CT + j % CT;
             v8bf b[SP];
 #pragma unroll
             for (int part = 0; part < SP; ++part)
@@ -290,8 +332,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __builtin_amdgcn_s_waitcnt(vmcnt_lds(0));  // the loads past the end have landed before the LDS is given up
     // accumulator element r of a lane: row 4 * quarter + r, column lane % 16
 #pragma unroll
-    for (int jj = 0; jj < 2; ++jj) {
-        const int n = tn * kCols + wave * 32 + jj * 16 + ln;
+    for (int jj = 0; jj < CT; ++jj) {
+        const int n = tn * kCols + (wave * CT + jj) * 16 + ln;
         if (n >= a.N) continue;
         const float bg = a.w[0].bias ? a.w[0].bias[n] : 0.f, bu = a.w[1].bias ? a.w[1].bias[n] : 0.f;
 #pragma unroll
@@ -301,22 +343,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 const int m = (tm * MT + i) * 16 + q * 4 + r;
                 if (m >= a.M) continue;
                 const float f = PARTS == 1 ? 1.0f : p.unscale[m];
-                const float g = y[jj][i][r] * f + bg, v = y[2 + jj][i][r] * f + bu;
+                const float g = y[jj][i][r] * f + bg, v = y[CT + jj][i][r] * f + bu;
                 static_cast<T*>(a.out)[size_t(m) * a.N + n] = T(activate(a.act, g) * v);
             }
     }
 }
 
-template <class T, int PARTS, int BITS, int GS, int MT>
+template <class T, int PARTS, int BITS, int GS, int MT, int CT>
 int launch_gemm_tile(const Args& a, hipStream_t st) {
-    using S = Stage<PARTS, BITS, GS, MT>;
-    constexpr int SP = sum_parts(PARTS);
+    using S = Stage<PARTS, BITS, GS, MT, CT>;
+    constexpr int SP = sum_parts(PARTS), kCols = 64 * CT;
     Prepared p;
     const int tiles_m = (a.M + 16 * MT - 1) / (16 * MT);
     p.mtiles = tiles_m * MT, p.stages = (a.K + 63) / 64, p.group_steps = (a.K / GS + 31) / 32, p.tiles_n = (a.N + kCols - 1) / kCols;
     const size_t x_bytes = size_t(p.stages) * p.mtiles * (2 * PARTS * kPiece), sum_bytes = size_t(p.mtiles) * p.group_steps * (SP * kPiece);
     const size_t bias_bytes = size_t(2) * p.tiles_n * (kCols / 16) * p.group_steps * (SP * kPiece);
-    const size_t scale_bytes = size_t(p.group_steps) * 32 * p.tiles_n * kPiece, unscale_bytes = PARTS == 1 ? 0 : size_t(a.M) * 4;
+    const size_t scale_bytes = size_t(p.group_steps) * 32 * p.tiles_n * (CT / 2 * kPiece), unscale_bytes = PARTS == 1 ? 0 : size_t(a.M) * 4;
     const auto lock = scratch_lock(st);
     void* ws = nullptr;
     if (const int rc = call_buffer(11, x_bytes + sum_bytes + bias_bytes + scale_bytes + unscale_bytes, st, &ws)) return rc;
@@ -329,11 +371,11 @@ int launch_gemm_tile(const Args& a, hipStream_t st) {
     // 128 k a block, all that the sums' steps of 32 groups reach over
     const unsigned x_blocks = unsigned(p.mtiles) * unsigned(p.group_steps * 32 * GS / 128);
     const unsigned w_blocks = unsigned(p.tiles_n) * (kCols / 64) * 2 * unsigned(p.group_steps);
-    gated_prepare_kernel<T, PARTS, BITS><<<x_blocks + w_blocks, 256, 0, st>>>(a, p, x_blocks);
+    gated_prepare_kernel<T, PARTS, BITS, CT><<<x_blocks + w_blocks, 256, 0, st>>>(a, p, x_blocks);
     LQ_CHECK_LAUNCH("quantized_gated_matmul");
     static DeviceOnce once;
     constexpr int lds = S::RING * S::PIECES * kPiece;
-    const auto kernel = gated_gemm_kernel<T, PARTS, BITS, GS, MT>;
+    const auto kernel = gated_gemm_kernel<T, PARTS, BITS, GS, MT, CT>;
     if (const int rc = allow_dynamic_lds(once, reinterpret_cast<const void*>(kernel), lds)) return rc;
     kernel<<<unsigned(tiles_m) * unsigned(p.tiles_n), 256, lds, st>>>(a, p, tiles_m);
     LQ_CHECK_LAUNCH("quantized_gated_matmul");
@@ -341,25 +383,37 @@ int launch_gemm_tile(const Args& a, hipStream_t st) {
 }
 
 // Rows in chunks whose prepared x stays below 2^30 bytes; whole tiles, so that the bits do not depend on them.
-template <class T, int PARTS, int BITS, int GS, int MT>
+template <class T, int PARTS, int BITS, int GS, int MT, int CT>
 int launch_gemm_chunks(Args a, hipStream_t st) {
     const size_t tile = size_t((a.K + 63) / 64) * (2 * PARTS * MT) * kPiece, tiles = tile < size_t(1) << 30 ? (size_t(1) << 30) / tile : 1;
     const int M = a.M, rows = int(std::min<size_t>(tiles * 16 * MT, size_t(M)));
     for (int m0 = 0; m0 < M; m0 += a.M) {
         a.M = std::min(rows, M - m0);
-        if (const int rc = launch_gemm_tile<T, PARTS, BITS, GS, MT>(a, st)) return rc;
+        if (const int rc = launch_gemm_tile<T, PARTS, BITS, GS, MT, CT>(a, st)) return rc;
         a.x = static_cast<const T*>(a.x) + size_t(a.M) * a.K, a.out = static_cast<T*>(a.out) + size_t(a.M) * a.N;
     }
     return LQ_OK;
 }
 
 template <class T, int PARTS, int BITS>
-int launch_gemm(const Args& a, hipStream_t st) {
-    constexpr int MT = PARTS == 1 ? 6 : 4;
+int launch_gemm(const Args& a, int tile, hipStream_t st) {
+    auto of_group = [&](auto gs_c) -> int {
+        constexpr int GS = decltype(gs_c)::value;
+        auto is = [&](auto index) -> int {
+            constexpr GemmTile t = kGemmTile<PARTS, BITS>[decltype(index)::value];
+            if constexpr (t.mt > 0) return launch_gemm_chunks<T, PARTS, BITS, GS, t.mt, t.ct>(a, st);
+            return fail(LQ_ERR_VALUE, "quantized_gated_matmul: no tile");
+        };
+        if (tile == 0) return is(std::integral_constant<int, 0>{});
+        if (tile == 1) return is(std::integral_constant<int, 1>{});
+        if (tile == 2) return is(std::integral_constant<int, 2>{});
+        if (tile == 3) return is(std::integral_constant<int, 3>{});
+        return is(std::integral_constant<int, 4>{});
+    };
     const int gs = 1 << a.gs_shift;
-    if (gs == 32) return launch_gemm_chunks<T, PARTS, BITS, 32, MT>(a, st);
-    if (gs == 64) return launch_gemm_chunks<T, PARTS, BITS, 64, MT>(a, st);
-    return launch_gemm_chunks<T, PARTS, BITS, 128, MT>(a, st);
+    if (gs == 32) return of_group(std::integral_constant<int, 32>{});
+    if (gs == 64) return of_group(std::integral_constant<int, 64>{});
+    return of_group(std::integral_constant<int, 128>{});
 }
 
 }  // namespace
