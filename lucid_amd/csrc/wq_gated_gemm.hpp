@@ -62,15 +62,26 @@ __global__ __launch_bounds__(256) void gated_prepare_kernel(Args a, Prepared p, 
         const int octet = int(i / across / 2) * 4 + int(threadIdx.x >> 6), n = int(i % across) * 64 + int(lane), groups = a.K >> a.gs_shift;
         if (octet >= p.group_steps * 4) return;
         const Weight& w = a.w[which];
-        float b[8];
+        float s[8], b[8];
+        const size_t row = size_t(n < a.N ? n : a.N - 1) * groups;
+        if (groups % 8 == 0 && aligned16(w.scales) && aligned16(w.biases)) {  // (a lane has a row: as few requests as can be)
+            const size_t from = row + (octet * 8 < groups ? octet * 8 : 0);
+            __builtin_memcpy(s, __builtin_assume_aligned(w.scales + from, 16), 32);
+            __builtin_memcpy(b, __builtin_assume_aligned(w.biases + from, 16), 32);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const size_t from = row + (octet * 8 + e < groups ? octet * 8 + e : 0);
+                s[e] = w.scales[from], b[e] = w.biases[from];
+            }
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int g = octet * 8 + e;
             const bool there = n < a.N && g < groups;
-            const float s = there ? w.scales[size_t(n) * groups + g] : 0.f;
-            b[e] = there ? w.biases[size_t(n) * groups + g] - float(kWqCentre<BITS>) * s : 0.f;
+            s[e] = there ? s[e] : 0.f, b[e] = there ? b[e] - float(kWqCentre<BITS>) * s[e] : 0.f;
             // (what a stage past K asks for lies within group_steps * 32 groups)
-            p.scales[(size_t(g) * p.tiles_n + n / kCols) * (2 * kCols) + which * kCols + n % kCols] = s;
+            p.scales[(size_t(g) * p.tiles_n + n / kCols) * (2 * kCols) + which * kCols + n % kCols] = s[e];
         }
         uint32_t d[3][4];
 #pragma unroll
