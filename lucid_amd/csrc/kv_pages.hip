@@ -130,6 +130,7 @@ __global__ __launch_bounds__(kTileThreads, kTileThreads / 256) void kv_compact_k
     __syncthreads();
     const unsigned tile = r.by_group(s_ticket), head0 = (s_ticket - tile * r.by_group.d) * r.together, launch = s_launch;
     const unsigned head_end = head0 + r.together < r.heads ? head0 + r.together : r.heads;
+    if (tile >= r.tiles) return;  // (no block of this launch)
     // the sequence whose tiles this one is among
     const unsigned upto = how_many(r.batch, lane, [&](unsigned b) { return first_tile(r, b) <= tile; }), seq = upto ? upto - 1 : 0;
     const unsigned begin0 = unsigned(r.starts[seq]), end0 = unsigned(r.starts[seq + 1]), own_tile = tile - first_tile(r, seq);

@@ -55,7 +55,10 @@ extern "C" int lq_wq_gated_matmul(const lq_wq_gated_args* g, lq_stream stream) {
     }
     LQ_REQUIRE(a.x && a.out, LQ_ERR_VALUE, "quantized_gated_matmul: NULL pointer");
     LQ_REQUIRE(aligned16(a.x), LQ_ERR_VALUE, "quantized_gated_matmul: x must be 16-byte aligned");
-    LQ_REQUIRE(a.x != a.out, LQ_ERR_VALUE, "quantized_gated_matmul: the result cannot take x's place");
+    const size_t item = g->dtype == LQ_F16 ? 2 : 4;
+    const uintptr_t x0 = reinterpret_cast<uintptr_t>(a.x), out0 = reinterpret_cast<uintptr_t>(a.out);
+    LQ_REQUIRE(x0 + size_t(a.M) * a.K * item <= out0 || out0 + size_t(a.M) * a.N * item <= x0, LQ_ERR_VALUE,
+               "quantized_gated_matmul: the result cannot take x's place");
     const hipStream_t st = as_stream(stream);
     const bool half = g->dtype == LQ_F16;
     const Choice c = choose(a, half, g->bits);

@@ -193,8 +193,8 @@ def gated_args(**kw):
 
 
 @pytest.mark.parametrize("kw,error", [
-    (dict(x=None), ValueError), (dict(out=None), ValueError), (dict(out=P), ValueError), (dict(packed=(P, None)), ValueError), (dict(packed=(P + 8, P)), ValueError),
-    (dict(scales=(None, P)), ValueError), (dict(biases=(P, None)), ValueError), (dict(M=-1), L.ShapeMismatch), (dict(N=-1), L.ShapeMismatch), (dict(K=0), L.ShapeMismatch),
+    (dict(x=None), ValueError), (dict(out=None), ValueError), (dict(out=P), ValueError), (dict(out=P + 2 * 64 * 4 - 16), ValueError), (dict(out=P - 2 * 8 * 4 + 16), ValueError), (dict(x=P + 4), ValueError), (dict(packed=(P, None)), ValueError), (dict(packed=(P + 8, P)), ValueError),
+    (dict(scales=(None, P)), ValueError), (dict(scales=(P, P + 2)), ValueError), (dict(biases=(P, None)), ValueError), (dict(M=-1), L.ShapeMismatch), (dict(N=-1), L.ShapeMismatch), (dict(K=0), L.ShapeMismatch),
     (dict(K=96, group_size=64), L.ShapeMismatch), (dict(K=1 << 30), L.ShapeMismatch), (dict(group_size=16), ValueError), (dict(bits=2), ValueError), (dict(act=4), ValueError),
     (dict(act=-1), ValueError), (dict(dtype=_C.BF16), L.DtypeMismatch)])
 def test_c_gated_refuses(kw, error):
