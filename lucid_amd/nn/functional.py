@@ -6,6 +6,7 @@ kernel; inputs and outputs are float32 tensors on the ``hip`` device.
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 from .. import _C
@@ -186,10 +187,10 @@ def paged_attention_qkv(qkv: Tensor, num_heads: int, cache, page_table: Tensor, 
     return out
 
 
-def _vector(name: str, what: str, t, cols: int):
-    """The address of a float32 ``(cols,)`` vector, or None."""
-    if t is None:
-        return None
+def _vector(name: str, what: str, t, cols: int) -> int:
+    """The address of a float32 ``(cols,)`` vector."""
+    if t.__class__ is Tensor and t.device == "hip" and t.dtype is T.float32 and t.shape == (cols,):
+        return t.data_ptr
     _require_f32_hip(name, t)
     if t.shape != (cols,):
         raise _C.ShapeMismatch(f"{name}: {what} has shape {t.shape}, expected {(cols,)}")
@@ -223,8 +224,11 @@ def _residual_norm(name, x, residual, weight, bias, norm, eps, post, post_weight
         gate_rows = gate.numel // cols if cols else 0
         if rows and (gate_rows == 0 or rows % gate_rows):
             raise _C.ShapeMismatch(f"{name}: a gate of {gate_rows} rows for {rows}")
-    vectors = [_vector(name, what, t, cols) for what, t in (("scale", scale), ("weight", weight), ("bias", bias), ("post_weight", post_weight),
-                                                            ("post_bias", post_bias))]
+    scale = None if scale is None else _vector(name, "scale", scale, cols)
+    weight = None if weight is None else _vector(name, "weight", weight, cols)
+    bias = None if bias is None else _vector(name, "bias", bias, cols)
+    post_weight = None if post_weight is None else _vector(name, "post_weight", post_weight, cols)
+    post_bias = None if post_bias is None else _vector(name, "post_bias", post_bias, cols)
     if out is not None:
         _check_rows(name, "out", out, x.shape)
         if out.dtype != x.dtype:
@@ -240,10 +244,11 @@ def _residual_norm(name, x, residual, weight, bias, norm, eps, post, post_weight
     if residual_out is None and residual is not None:
         residual_out = Tensor.empty(x.shape, residual.dtype, "hip")
     args = _C.ResidualNormArgs(
-        x.data_ptr, residual.data_ptr if residual is not None else None, gate.data_ptr if rows and gate is not None else None, *vectors, out.data_ptr,
+        x.data_ptr, residual.data_ptr if residual is not None else None, gate.data_ptr if rows and gate is not None else None, scale, weight, bias,
+        post_weight, post_bias, out.data_ptr,
         residual_out.data_ptr if residual is not None else None, rows, gate_rows if rows else 0, cols, x.dtype.code,
-        (residual if residual is not None else x).dtype.code, _NORMS[norm], 1 if post else 0, float(eps))
-    _C.call("lq_residual_norm", _C.C.byref(args), None)
+        x.dtype.code if residual is None else residual.dtype.code, _NORMS[norm], 1 if post else 0, eps)
+    _C.call("lq_residual_norm", ctypes.byref(args), None)
     _written(out)
     if residual is not None:
         _written(residual_out)

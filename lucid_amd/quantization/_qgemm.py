@@ -8,6 +8,8 @@ The packed tensor is int32-tagged (Lucid has no uint32 dtype either,
 
 from __future__ import annotations
 
+import ctypes
+
 from .. import _C
 from .. import _tensor as T
 from .._tensor import Tensor
@@ -116,10 +118,10 @@ def quantized_gated_matmul(x: Tensor, gate: tuple[Tensor, Tensor, Tensor], up: t
     M = x.numel // K if K else 0
     if max(M, N, K) > 0x7fffffff:  # (ctypes takes the low 32 bits of a longer int)
         raise _C.ShapeMismatch(f"{name}: {M} x {N} x {K}")
-    pair = _C.C.c_void_p * 2
-    args = _C.WqGatedArgs(x.data_ptr, out.data_ptr, pair(gate[0].data_ptr, up[0].data_ptr), pair(gate[1].data_ptr, up[1].data_ptr),
-                          pair(gate[2].data_ptr, up[2].data_ptr), pair(*(b.data_ptr if b is not None else None for b in (gate_bias, up_bias))), M, N, K,
-                          int(group_size), int(bits), _GATES[activation], x.dtype.code)
-    _C.call("lq_wq_gated_matmul", _C.C.byref(args), None)
+    args = _C.WqGatedArgs(x.data_ptr, out.data_ptr, (gate[0].data_ptr, up[0].data_ptr), (gate[1].data_ptr, up[1].data_ptr),
+                          (gate[2].data_ptr, up[2].data_ptr),
+                          (None if gate_bias is None else gate_bias.data_ptr, None if up_bias is None else up_bias.data_ptr), M, N, K, group_size, bits,
+                          _GATES[activation], x.dtype.code)
+    _C.call("lq_wq_gated_matmul", ctypes.byref(args), None)
     out._grid = out._range = None
     return out
