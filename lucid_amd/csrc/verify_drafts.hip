@@ -10,7 +10,7 @@
 // sums would move one in a thousand draws.
 //
 // A block has a run of the vocabulary of one sequence; every block judges the drafts itself (two numbers each), so that it knows the row
-// to read, and asks for up to 8192 of its probabilities at once.  Sums go to the last block that arrives, which finds the run, in it the piece of
+// to read, and asks for 8192 of its probabilities at once, or 16 384.  Sums go to the last block that arrives, which finds the run, in it the piece of
 // 512 that a wavefront reads with one instruction, the lane and the token.  Each probability is read once, the run of the token twice.  Bound by
 // memory in the large (128 rows of 131 072 float16), by a chain of eight trips to memory in the small.
 #include <type_traits>
@@ -21,7 +21,7 @@ using namespace lq;
 
 namespace {
 
-constexpr unsigned kThreads = 256, kWaves = kThreads / 64, kVec = 8, kPiece = 64 * kVec, kAtOnce = 4, kRound = kThreads * kVec;  // tokens
+constexpr unsigned kThreads = 256, kWaves = kThreads / 64, kVec = 8, kRound = kThreads * kVec;  // tokens
 constexpr unsigned kNone = 0xffffffffu;
 
 struct Args {
@@ -116,11 +116,13 @@ __device__ __forceinline__ int passing(double v, double goal, unsigned lane, dou
     return at;
 }
 
-template <bool DRAFT>
-constexpr int kBlocks = DRAFT ? 4 : 6;  // of a CU: what their registers leave room for
+constexpr int kBlocks = 4;  // of a CU: what their registers leave room for
+template <class T, bool DRAFT>
+constexpr unsigned kAhead = sizeof(T) == 2 && !DRAFT ? 8 : 4;  // times eight probabilities that a thread asks for at once
 
 template <class T, bool DRAFT>
-__global__ __launch_bounds__(256, kBlocks<DRAFT>) void verify_drafts_kernel(Args a) {
+__global__ __launch_bounds__(256, kBlocks) void verify_drafts_kernel(Args a) {
+    constexpr unsigned kAtOnce = kAhead<T, DRAFT>;
     __shared__ double s_sum[2][kWaves], s_piece[kAtOnce * kWaves];
     __shared__ unsigned s_first;
     __shared__ int s_is_last, s_next;
@@ -272,9 +274,9 @@ extern "C" int lq_verify_drafts(const void* target, const void* draft, int dtype
     LQ_REQUIRE(starts && last && counts, LQ_ERR_VALUE, "verify_drafts: starts, last or counts is NULL");
     LQ_REQUIRE(new_tokens != tokens || !tokens, LQ_ERR_VALUE, "verify_drafts: the new tokens cannot take the drafted ones' place");
     LQ_REQUIRE(rows == 0 || (target && tokens && uniforms && new_tokens), LQ_ERR_VALUE, "verify_drafts: a NULL pointer");
-    // As many blocks as are resident, a round of 2048 tokens at least each; 64 of a sequence at most.  (128 rows of 131 072: three rounds of blocks of
-    // 8192 tokens 50 us, one of 16 384 39, before the sums went on without a write-back of the caches.)
-    unsigned runs = 256u * unsigned(draft ? kBlocks<true> : kBlocks<false>) / unsigned(batch);
+    // As many blocks as are resident, 2048 tokens at least each; 64 of a sequence at most.  (128 rows of 131 072 float16: 8 blocks a sequence that ask
+    // for all of their run at once 23.5 us, 12 and 16 of smaller runs 26 and 24.5, in rounds of 8192 tokens 29.)
+    unsigned runs = 256u * unsigned(kBlocks) / unsigned(batch);
     const unsigned most = (unsigned(vocab) + kRound - 1) / kRound;
     runs = runs < 1 ? 1 : runs > 64 ? 64 : runs;
     if (runs > most) runs = most;
