@@ -244,7 +244,7 @@ int lq_kv_cache_copy(const lq_kv_cache* cache, const int32_t* src, const int32_t
     LQ_REQUIRE(units < size_t(1) << 30, LQ_ERR_SHAPE, "kv_cache_copy: pages of %zu bytes", units * 16);
     const size_t blocks = (units + kCopyChunk - 1) / kCopyChunk, together = blocks == 1 ? kCopyChunk / units : 1;
     const size_t grid = (pages + together - 1) / together * blocks;
-    LQ_REQUIRE(pages < size_t(1) << 31 && grid < size_t(1) << 31, LQ_ERR_SHAPE, "kv_cache_copy: %zu pages of %zu bytes", pages, units * 16);
+    LQ_REQUIRE(pages < size_t(1) << 31 && grid < size_t(1) << 24, LQ_ERR_SHAPE, "kv_cache_copy: %zu pages of %zu bytes", pages, units * 16);
     kv_copy_kernel<<<unsigned(grid), 256, 0, as_stream(stream)>>>(buffers_of(cache), src, dst, unsigned(pages), unsigned(cache->num_pages),
                                                                    unsigned(codes), unsigned(numbers), FastDiv(unsigned(units)),
                                                                    FastDiv(unsigned(blocks)), unsigned(together));
@@ -259,8 +259,7 @@ int lq_kv_cache_compact(const lq_kv_cache* cache, const int32_t* page_table, int
     LQ_REQUIRE(batch >= 0 && table_width >= 0, LQ_ERR_SHAPE, "kv_cache_compact: %d sequences of %d pages", batch, table_width);
     if (kept == 0 || batch == 0 || table_width == 0) return LQ_OK;
     LQ_REQUIRE(page_table && keep && starts, LQ_ERR_VALUE, "kv_cache_compact: a list is NULL");
-    LQ_REQUIRE(kept <= size_t(cache->num_pages) * cache->page_size, LQ_ERR_SHAPE, "kv_cache_compact: %zu rows kept of a cache of %zu", kept,
-               size_t(cache->num_pages) * cache->page_size);
+    LQ_REQUIRE(kept < size_t(1) << 31, LQ_ERR_SHAPE, "kv_cache_compact: %zu rows kept", kept);  // (more than the cache has, where pages are shared)
     Rows r;
     r.b = buffers_of(cache), r.table = page_table, r.keep = keep, r.starts = starts, r.batch = unsigned(batch), r.width = unsigned(table_width);
     r.n = unsigned(kept), r.num_pages = unsigned(cache->num_pages), r.heads = unsigned(cache->kv_heads);
@@ -271,7 +270,8 @@ int lq_kv_cache_compact(const lq_kv_cache* cache, const int32_t* page_table, int
     const unsigned groups = (r.heads + r.together - 1) / r.together;
     r.by_group = FastDiv(groups);
     const size_t grid = size_t(r.tiles) * groups, words_needed = size_t(r.tiles) * r.heads;
-    LQ_REQUIRE(grid < size_t(1) << 31, LQ_ERR_SHAPE, "kv_cache_compact: %zu rows of %u heads", kept, r.heads);
+    LQ_REQUIRE(grid < (size_t(1) << 32) / kTileThreads, LQ_ERR_SHAPE, "kv_cache_compact: %zu rows of %u sequences and %u heads", kept, r.batch,
+               r.heads);  // (a launch has fewer than 2^32 threads)
     const hipStream_t st = as_stream(stream);
     const auto lock = scratch_lock(st);
     void* words = nullptr;

@@ -118,6 +118,16 @@ def test_shared_pages_whose_rows_stay():
     check(c, table, np.concatenate(keep), [0, 35, 69])
 
 
+def test_more_rows_kept_than_the_cache_has():
+    """Sequences that share most of their pages keep more between them than there are rows."""
+    rng = np.random.default_rng(6)
+    c = filled(rng, 8, 16, 2, 32, False, 8)
+    table = np.array([[0, 1, 2 + b] for b in range(6)], np.int32)
+    keep = [np.concatenate([np.arange(32), np.sort(32 + rng.permutation(16)[:5])]) for _ in range(6)]
+    assert 6 * 37 > 8 * 16
+    check(c, table, np.concatenate(keep), np.arange(7) * 37)
+
+
 def test_nothing_to_move():
     rng = np.random.default_rng(4)
     c = filled(rng, 3, 16, 1, 16, True, 8)
