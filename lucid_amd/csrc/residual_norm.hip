@@ -134,7 +134,7 @@ __device__ __forceinline__ void normalize(f4 (&v)[NV], const Norm& n, unsigned a
 template <class TX, class TR, bool LAYER, bool POST, bool WHOLE, int TPR, int NV>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void residual_norm_kernel(Args a) {
     __shared__ float s[TPR / 64];
-    const unsigned row = blockIdx.x * (TPR < 256 ? 256 / TPR : 1) + threadIdx.x / TPR, at = threadIdx.x % TPR * 4;
+    const unsigned row = (blockIdx.y * gridDim.x + blockIdx.x) * (TPR < 256 ? 256 / TPR : 1) + threadIdx.x / TPR, at = threadIdx.x % TPR * 4;
     if (row >= a.rows) return;  // (rows of 64 threads: no barrier follows)
     const size_t base = size_t(row) * a.cols;
     f4 x[NV], r[NV];
@@ -197,9 +197,10 @@ void launch(const Args& a, bool post, hipStream_t st) {
     by_shape(a.cols, [&](auto whole, auto tpr, auto nv) {
         constexpr bool WHOLE = decltype(whole)::value;
         constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, BLOCK = TPR < 256 ? 256 : TPR;
-        const unsigned per = BLOCK / TPR;
+        // (2^32 threads and more are several rows of blocks: a launch has fewer along its first axis)
+        const unsigned per = BLOCK / TPR, blocks = (a.rows + per - 1) / per, across = blocks < 1u << 21 ? blocks : 1u << 21;
         const auto kernel = post ? residual_norm_kernel<TX, TR, LAYER, true, WHOLE, TPR, NV> : residual_norm_kernel<TX, TR, LAYER, false, WHOLE, TPR, NV>;
-        kernel<<<(a.rows + per - 1) / per, BLOCK, 0, st>>>(a);
+        kernel<<<dim3(across, (blocks + across - 1) / across), BLOCK, 0, st>>>(a);
     });
 }
 

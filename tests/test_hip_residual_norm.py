@@ -6,6 +6,7 @@ import pytest
 import lucid_amd as L
 import lucid_amd.nn as nn
 import lucid_amd.nn.functional as F
+from lucid_amd import _C
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24  # half a step of float32, relative
@@ -154,3 +155,13 @@ def test_replayed_from_a_graph():
         L.synchronize()
         want = [t.numpy() for t in F.residual_norm(x, r, post=True)]
         assert np.array_equal(y.numpy(), want[0]) and np.array_equal(r2.numpy(), want[1])
+
+
+@pytest.mark.parametrize("rows,cols", [((1 << 22) + 3, 4100), ((1 << 24) + 5, 1028)])
+def test_rows_of_more_threads_than_a_launch_has_along_an_axis(rows, cols):
+    """34 GB of one number, in place; each value's norm is 1 within half a step of float16."""
+    x = L.Tensor.empty((rows, cols), L.float16, "hip")
+    _C.call("lq_fill_bytes", x.data_ptr, 0x3c, x.nbytes, None)
+    F.rms_norm(x, cols, eps=0.0, out=x)
+    for at in (0, 1 << 20, 1 << 21, (1 << 21) + 1, rows // 2, (rows - 3) // 2, rows - 3):
+        assert (x.row_range(at, at + 3).numpy() == 1.0).all()
