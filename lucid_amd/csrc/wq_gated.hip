@@ -17,13 +17,13 @@ struct Choice {
 Choice choose(const gated::Args& a, bool half, int bits) {
     const gated::GemmTile* const tiles = half ? (bits == 4 ? gated::kGemmTile<1, 4> : gated::kGemmTile<1, 8>) : (bits == 4 ? gated::kGemmTile<2, 4> : gated::kGemmTile<2, 8>);
     const int few_tiles = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
-    const int64_t few_blocks = int64_t((a.N + 63) / 64) * ((a.M + 16 * few_tiles - 1) / (16 * few_tiles)), stages = (a.K + 63) / 64;
+    const int64_t few_blocks = (int64_t(a.N) + 63) / 64 * ((int64_t(a.M) + 16 * few_tiles - 1) / (16 * few_tiles)), stages = (a.K + 63) / 64;
     const float per_stage = half ? (few_tiles == 1 ? 0.30f : few_tiles == 2 ? 0.36f : 0.53f) : (few_tiles == 1 ? 0.40f : few_tiles == 2 ? 0.50f : 1.0f);
     Choice best{-1, (half ? 0.f : 5.f) + float((few_blocks + 255) / 256) * float(stages) * per_stage};
     if (size_t(a.N) * a.K * bits / 8 >= 0x7fffffffull) return best;  // (offsets of codes are 32-bit in the kernel of many rows)
     for (int t = 0; t < gated::kGemmTiles && tiles[t].mt; ++t) {
         const gated::GemmTile& tile = tiles[t];
-        const int64_t blocks = int64_t((a.M + 16 * tile.mt - 1) / (16 * tile.mt)) * ((a.N + 64 * tile.ct - 1) / (64 * tile.ct)), rest = blocks % 512;
+        const int64_t blocks = (int64_t(a.M) + 16 * tile.mt - 1) / (16 * tile.mt) * ((int64_t(a.N) + 64 * tile.ct - 1) / (64 * tile.ct)), rest = blocks % 512;
         const float us = (half ? 6.f : 12.f) + float(stages) * (float(blocks / 512) * tile.two + (rest == 0 ? 0.f : rest <= 256 ? tile.one : tile.two));
         if (us < best.us) best = Choice{t, us};
     }

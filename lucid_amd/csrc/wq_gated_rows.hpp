@@ -296,7 +296,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void gated_few_kernel(Args a) {
         load(s + RING * kFewWaves, at);
     }
     s_y[wave][0][lane] = y[0][0][0], s_y[wave][1][lane] = y[1][0][0];
-    __syncthreads();  // (and the loads past the end have landed)
+    __builtin_amdgcn_s_waitcnt(vmcnt_and_lds(0));  // the loads past the end have landed before the LDS is given up
+    __syncthreads();
     // a thread has a column and row q that lane column + 16 q holds
     const int n = n0 + (threadIdx.x & 15), m = threadIdx.x >> 4;
     if (n >= a.N || m >= a.M) return;
@@ -495,7 +496,7 @@ int launch_rows(const Args& a, int bits, hipStream_t st) {
             const auto kernel = gated_few_kernel<T, PARTS, BITS, GS>;
             static DeviceOnce once;
             if (const int rc = allow_dynamic_lds(once, reinterpret_cast<const void*>(kernel), kFewFixed<BITS> + int(kFewLds))) return rc;
-            kernel<<<unsigned((a.N + 15) / 16), 64 * kFewWaves, kFewFixed<BITS> + few, st>>>(a);
+            kernel<<<(unsigned(a.N) + 15) / 16, 64 * kFewWaves, kFewFixed<BITS> + few, st>>>(a);
             LQ_CHECK_LAUNCH("quantized_gated_matmul");
             return LQ_OK;
         });
@@ -516,7 +517,7 @@ int launch_rows(const Args& a, int bits, hipStream_t st) {
         auto launch = [&](auto tiles) -> int {
             constexpr int MT = decltype(tiles)::value;
             using S = RowsStep<PARTS, BITS, GS, MT>;
-            const dim3 grid(unsigned((a.N + kColumnGroups * 16 - 1) / (kColumnGroups * 16)), unsigned((a.M + 16 * MT - 1) / (16 * MT)));
+            const dim3 grid((unsigned(a.N) + kColumnGroups * 16 - 1) / (kColumnGroups * 16), (unsigned(a.M) + 16 * MT - 1) / (16 * MT));
             LQ_REQUIRE(grid.y <= 65535, LQ_ERR_SHAPE, "quantized_gated_matmul: %d rows", a.M);
             const auto kernel = gated_rows_kernel<T, PARTS, BITS, GS, MT>;
             constexpr int need = 2 * S::TABLE + S::RING * S::BYTES, sums = kRowsWaves * MT * 2048, lds = need > sums ? need : sums;

@@ -2,6 +2,8 @@
 packed weights, probabilities, verified drafts; sequences that are forked and that evict tokens between the steps.  Every stage is held to float64
 (or to the byte) on what it was given, so that what one operator hands to the next is seen."""
 
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -10,10 +12,12 @@ import lucid_amd.nn as nn
 import lucid_amd.nn.functional as F
 import lucid_amd.nn.quantized as nnq
 import lucid_amd.quantization as Q
+from lucid_amd import _C
+from lucid_amd.quantization import _qgemm
 import oracle.kv_cache as K
 import oracle.wq_group as W
 from test_hip_kv_cache import buffers, same
-from test_hip_kv_pages import compacted, copied
+from test_hip_kv_pages import compacted, copied, filled
 from test_hip_residual_norm import norm
 from test_hip_verify_drafts import verified
 from test_hip_wq_gated import bound
@@ -179,3 +183,55 @@ def test_steps_with_drafts_forks_and_evictions(bits, given):
         if turn == 2:
             d.evict(32)
     assert told > 0  # (some drafts were accepted)
+
+
+def test_each_call_on_two_streams_at_once():
+    """Every call that takes scratch, on two streams of different inputs without a wait between: each has what it gives alone."""
+    rng = np.random.default_rng(9)
+    some = lambda *s: rng.standard_normal(s).astype(np.float32)
+    parts = [[tuple(map(hip, W.quantize(some(n, 512), 64, 4))) for _ in range(2)] for n in (700, 90)]
+    calls = [[], []]
+    for i in (0, 1):
+        for rows, dtype in ((3, np.float32), (20, np.float32), (300, np.float32), (300, np.float16)):
+            x = hip(some(rows + i, 512).astype(dtype))
+            calls[i].append(lambda x=x, w=parts[i]: _qgemm.quantized_gated_matmul(x, *w, group_size=64, bits=4))
+        vocab, n = (60000, 700)[i], 12
+        p, q = (hip(rng.random((n, vocab)).astype(np.float32)) for _ in range(2))
+        t, starts, u, w = ids(rng.integers(0, vocab, n)), ids([0, 5, 6, n]), hip(rng.random(n).astype(np.float32)), hip(rng.random(3).astype(np.float32))
+        calls[i].append(lambda p=p, q=q, t=t, s=starts, u=u, w=w: F.verify_drafts(p, t, s, u, w, draft=q)[0])
+        calls[i].append(lambda p=p, t=t, s=starts, u=u, w=w: F.verify_drafts(p, t, s, u, w)[0])
+        x, r = hip(some(50 + i, 1000)), hip(some(50 + i, 1000))
+        calls[i].append(lambda x=x, r=r: F.residual_norm(x, r, norm="layer", post=True)[0])
+    alone = [[f().numpy() for f in c] for c in calls]
+    # a cache each, compacted again and again: a row is evicted at a time
+    tokens, turns = (900, 3000), 4
+    caches, befores = [], []
+    for i in (0, 1):
+        pages = tokens[i] // PAGE + 1
+        c, table = filled(rng, pages, PAGE, KV_HEADS, DIM, False, 8), ids([rng.permutation(pages)])
+        want = buffers(c)
+        for turn in range(turns):
+            keep = np.delete(np.arange(tokens[i] - turn), turn * 7)
+            want = compacted(want, PAGE, table.numpy(), keep, [0, len(keep)])
+            calls[i].append(lambda c=c, t=table, k=ids(keep), s=ids([0, len(keep)]): Q.kv_cache_compact(c, t, k, s))
+        caches.append(c), befores.append(want)
+    streams = []
+    for _ in range(2):
+        s = C.c_void_p()
+        _C.call("lq_stream_create", C.byref(s))
+        streams.append(s)
+    L.synchronize()
+    prev, got = _C.current_stream(), [[], []]
+    try:
+        for a, b in zip(*calls):
+            for i, f in enumerate((a, b)):
+                _C.set_current_stream(streams[i])
+                got[i].append(f())
+        for s in streams:
+            _C.call("lq_sync", s)
+    finally:
+        _C.set_current_stream(prev)
+    for i in (0, 1):
+        for g, want in zip(got[i], alone[i]):
+            assert np.array_equal(g.numpy(), want)
+        same(buffers(caches[i]), befores[i])

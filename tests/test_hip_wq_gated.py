@@ -174,6 +174,23 @@ def test_the_block_as_modules(bits):
     assert np.array_equal(q(hip(x)).numpy(), h.numpy())
 
 
+@pytest.mark.parametrize("M", [1, 4, 5, 20, 64, 300])
+@pytest.mark.parametrize("K,gs", [(96, 32), (320, 64), (640, 128), (2112, 64)])
+@pytest.mark.parametrize("bits,dtype", [(4, np.float16), (8, np.float32)])
+def test_rows_out_of_the_middle(M, K, gs, bits, dtype):
+    """Weights that are some rows of larger ones, whose scales lie at any multiple of four bytes; x and the result likewise."""
+    rng = np.random.default_rng(M + K)
+    parts = [W.quantize(rng.standard_normal((90, K)).astype(np.float32), gs, bits) for _ in range(2)]
+    x = rng.standard_normal((M + 3, K)).astype(dtype)
+    want = _qgemm.quantized_gated_matmul(hip(x[1:M + 1]), *[tuple(hip(p[5:82]) for p in w) for w in parts], group_size=gs, bits=bits).numpy()
+    filled = np.full((M + 2, 77), 7, dtype)
+    out = hip(filled)
+    views = [tuple(hip(p).row_range(5, 82) for p in w) for w in parts]
+    _qgemm.quantized_gated_matmul(hip(x).row_range(1, M + 1), *views, group_size=gs, bits=bits, out=out.row_range(1, M + 1))
+    filled[1:M + 1] = want
+    assert np.array_equal(out.numpy(), filled)
+
+
 @pytest.mark.parametrize("M", [1, 20, 300])
 def test_replayed_from_two_graphs(M):
     rng = np.random.default_rng(M)
