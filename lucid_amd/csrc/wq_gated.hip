@@ -6,26 +6,33 @@ using namespace lq;
 namespace {
 
 struct Choice {
-    int tile;  // of the kernel of many rows; -1: the one of few
+    bool rows;  // the kernel of few rows
+    int tile;
     float us;
 };
 
-// The kernel, and of the one of many rows the tile, that takes the least time as rounds of blocks: for few rows one block a CU, for many two, or one
-// where a last round has no more than 256.  Few rows take 0.3 to 0.53 us for 64 k (float32, two parts of x: 0.4 to 1), and 5 us before for splitting
-// float32; many rows 6 or 12 us before for laying out their operands.  us, few / many, 4 bits in groups of 128, K = 4096: 64 x 11008 float16 34 / 52, 65
-// 64 / 60, 128 66 / 69, 128 x 4096 (8 bits) 36 / 57; 64 x 11008 float32 70 / 72, 65 125 / 77.
-Choice choose(const gated::Args& a, bool half, int bits) {
-    const gated::GemmTile* const tiles = half ? (bits == 4 ? gated::kGemmTile<1, 4> : gated::kGemmTile<1, 8>) : (bits == 4 ? gated::kGemmTile<2, 4> : gated::kGemmTile<2, 8>);
-    const int few_tiles = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
-    const int64_t few_blocks = (int64_t(a.N) + 63) / 64 * ((int64_t(a.M) + 16 * few_tiles - 1) / (16 * few_tiles)), stages = (a.K + 63) / 64;
-    const float per_stage = half ? (few_tiles == 1 ? 0.30f : few_tiles == 2 ? 0.36f : 0.53f) : (few_tiles == 1 ? 0.40f : few_tiles == 2 ? 0.50f : 1.0f);
-    Choice best{-1, (half ? 0.f : 5.f) + float((few_blocks + 255) / 256) * float(stages) * per_stage};
-    if (size_t(a.N) * a.K * bits / 8 >= 0x7fffffffull) return best;  // (offsets of codes are 32-bit in the kernel of many rows)
-    for (int t = 0; t < gated::kGemmTiles && tiles[t].mt; ++t) {
-        const gated::GemmTile& tile = tiles[t];
-        const int64_t blocks = (int64_t(a.M) + 16 * tile.mt - 1) / (16 * tile.mt) * ((int64_t(a.N) + 64 * tile.ct - 1) / (64 * tile.ct)), rest = blocks % 512;
-        const float us = (half ? 6.f : 12.f) + float(stages) * (float(blocks / 512) * tile.two + (rest == 0 ? 0.f : rest <= 256 ? tile.one : tile.two));
-        if (us < best.us) best = Choice{t, us};
+// The kernel and the tile that take the least time as rounds of blocks.  Of few rows a CU has one block, which takes 2.5 us (3.5: float32) beside its
+// stages of 64 k; many small blocks end sooner as long as they are one round (16 x 4096 x 4096, 4 bits, float16: 64, 32, 16 columns a block 16.7, 11.3,
+// 8.8 us; 16 x 11008 x 4096 18.1, 21.6, 20.5).  Of many rows a CU has two blocks, or one where a last round has no more than 256; what comes before and
+// behind, a launch that lays out the operands among it, takes 12 us.  us, few / many, 4 bits in groups of 128: 128 x 11008 x 4096 float16 64 / 66, 200
+// 95 / 93, 333 155 / 118, 512 x 4096 x 4096 63 / 66, 1024 x 2816 x 1024 33 / 40; 65 x 11008 x 4096 float32 82 / 82, 128 94 / 88, 512 x 4096 x 4096 127 / 98.
+template <int PARTS, int BITS>
+Choice choose(const gated::Args& a) {
+    constexpr bool half = PARTS == 1;
+    const float stages = float((int64_t(a.K) + 63) / 64);
+    const auto blocks_of = [&](int rows, int cols) { return (int64_t(a.M) + rows - 1) / rows * ((int64_t(a.N) + cols - 1) / cols); };
+    Choice best{true, 0, 3.4e38f};
+    for (size_t t = 0; t < gated::kRowsTiles<PARTS>.size(); ++t) {
+        const gated::RowsTile& tile = gated::kRowsTiles<PARTS>[t];
+        const float us = (half ? 1.f : 3.5f) + float((blocks_of(16 * tile.mt, 16 * tile.cg) + 255) / 256) * ((half ? 2.5f : 3.5f) + stages * tile.us);
+        if (us < best.us) best = Choice{true, int(t), us};
+    }
+    if (size_t(a.N) * a.K * BITS / 8 >= 0x7fffffffull) return best;  // (offsets of codes are 32-bit in the kernel of many rows)
+    for (size_t t = 0; t < gated::kGemmTiles<PARTS, BITS>.size(); ++t) {
+        const gated::GemmTile& tile = gated::kGemmTiles<PARTS, BITS>[t];
+        const int64_t blocks = blocks_of(16 * tile.mt, 64 * tile.ct), rest = blocks % 512;
+        const float us = 12.f + stages * (float(blocks / 512) * tile.two + (rest == 0 ? 0.f : rest <= 256 ? tile.one : tile.two));
+        if (us < best.us) best = Choice{false, int(t), us};
     }
     return best;
 }
@@ -61,8 +68,8 @@ extern "C" int lq_wq_gated_matmul(const lq_wq_gated_args* g, lq_stream stream) {
                "quantized_gated_matmul: the result cannot take x's place");
     const hipStream_t st = as_stream(stream);
     const bool half = g->dtype == LQ_F16;
-    const Choice c = choose(a, half, g->bits);
-    if (c.tile < 0) return half ? gated::launch_rows_f16(a, g->bits, st) : gated::launch_rows_f32(a, g->bits, st);
+    const Choice c = half ? (g->bits == 4 ? choose<1, 4>(a) : choose<1, 8>(a)) : (g->bits == 4 ? choose<2, 4>(a) : choose<2, 8>(a));
+    if (c.rows) return half ? gated::launch_rows_f16(a, g->bits, c.tile, st) : gated::launch_rows_f32(a, g->bits, c.tile, st);
     if (half) return g->bits == 4 ? gated::launch_gemm_f16_4(a, c.tile, st) : gated::launch_gemm_f16_8(a, c.tile, st);
     return g->bits == 4 ? gated::launch_gemm_f32_4(a, c.tile, st) : gated::launch_gemm_f32_8(a, c.tile, st);
 }

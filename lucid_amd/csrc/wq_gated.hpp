@@ -7,6 +7,8 @@
 // (the rest of the code goes to b), so that nothing of a weight is rounded: scales follow in float32, on the sums of a group.  float16 x
 // enters as it is; a float32 row times a power of two as two float16 of 22 bits together.
 #pragma once
+#include <array>
+
 #include "wq_pack.hpp"
 
 namespace lq {
@@ -94,9 +96,19 @@ __device__ __forceinline__ void split_f16(const float (&v)[8], float f, uint4 (&
 
 }  // namespace
 
-// Few rows (wq_gated_rows.hpp).  bits 4 or 8, groups of 32, 64 or 128.
-int launch_rows_f16(const Args& a, int bits, hipStream_t st);
-int launch_rows_f32(const Args& a, int bits, hipStream_t st);
+// Few rows or columns (wq_gated_rows.hpp): 16 mt rows x 16 cg columns a block, and what 64 k of it take (us), on average of 4 and 8 bits: measured with
+// 6 to 256 rows and 512 to 11008 columns at K = 4096 and 14336.  bits 4 or 8, groups of 32, 64 or 128; `tile` of these.
+struct RowsTile {
+    int mt, cg;
+    float us;
+};
+template <int PARTS>  // (of a float32 x there is no room for more)
+constexpr std::array<RowsTile, 6> kRowsTiles = {{{4, 4, 0.80f}, {2, 4, 0.47f}, {2, 2, 0.28f}, {1, 4, 0.30f}, {1, 2, 0.175f}, {1, 1, 0.112f}}};
+template <>
+inline constexpr std::array<RowsTile, 7> kRowsTiles<1> = {
+    {{4, 4, 0.45f}, {2, 4, 0.27f}, {2, 2, 0.152f}, {2, 1, 0.109f}, {1, 4, 0.21f}, {1, 2, 0.115f}, {1, 1, 0.0625f}}};
+int launch_rows_f16(const Args& a, int bits, int tile, hipStream_t st);
+int launch_rows_f32(const Args& a, int bits, int tile, hipStream_t st);
 
 // Many rows (wq_gated_gemm.hpp): 16 mt rows x 64 ct columns a block, and what a stage of 64 k takes (us) when a CU has one block, or two: measured
 // with 4-bit codes in groups of 128 at K = 4096, N = 11008 and 64 to 2048 rows.  (8-bit codes of wide blocks leave no room for a ring of stages.)
@@ -104,15 +116,14 @@ struct GemmTile {
     int mt, ct;
     float one, two;
 };
-constexpr int kGemmTiles = 5;
 template <int PARTS, int BITS>
-constexpr GemmTile kGemmTile[kGemmTiles] = {{2, 2, 0.73f, 1.03f}, {4, 2, 0.95f, 1.25f}, {6, 2, 1.15f, 1.72f}, {2, 4, 1.15f, 1.75f}, {3, 4, 1.32f, 1.95f}};
+constexpr std::array<GemmTile, 3> kGemmTiles = {{{4, 2, 0.95f, 1.25f}, {6, 2, 1.15f, 1.72f}, {3, 4, 1.32f, 1.95f}}};
 template <>
-inline constexpr GemmTile kGemmTile<1, 8>[kGemmTiles] = {{2, 2, 0.73f, 1.03f}, {3, 2, 0.85f, 1.17f}, {4, 2, 0.95f, 1.25f}, {6, 2, 1.15f, 1.72f}, {2, 4, 1.15f, 1.75f}};
+inline constexpr std::array<GemmTile, 2> kGemmTiles<1, 8> = {{{4, 2, 0.95f, 1.25f}, {6, 2, 1.15f, 1.72f}}};
 template <>
-inline constexpr GemmTile kGemmTile<2, 4>[kGemmTiles] = {{1, 2, 0.60f, 0.97f}, {2, 2, 0.95f, 1.30f}, {4, 2, 1.35f, 1.98f}, {2, 4, 1.40f, 2.35f}, {3, 4, 1.70f, 2.95f}};
+inline constexpr std::array<GemmTile, 4> kGemmTiles<2, 4> = {{{2, 2, 0.95f, 1.30f}, {4, 2, 1.35f, 1.98f}, {2, 4, 1.40f, 2.35f}, {3, 4, 1.70f, 2.95f}}};
 template <>
-inline constexpr GemmTile kGemmTile<2, 8>[kGemmTiles] = {{1, 2, 0.60f, 0.97f}, {2, 2, 0.95f, 1.30f}, {3, 2, 1.20f, 1.58f}, {4, 2, 1.35f, 1.98f}, {0, 0, 0.f, 0.f}};
+inline constexpr std::array<GemmTile, 3> kGemmTiles<2, 8> = {{{2, 2, 0.95f, 1.30f}, {3, 2, 1.20f, 1.58f}, {4, 2, 1.35f, 1.98f}}};
 // By type and bits, `tile` of these; weights below 2 GiB.
 int launch_gemm_f16_4(const Args& a, int tile, hipStream_t st);
 int launch_gemm_f16_8(const Args& a, int tile, hipStream_t st);

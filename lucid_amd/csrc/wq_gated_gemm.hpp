@@ -406,20 +406,24 @@ int launch_gemm_chunks(Args a, hipStream_t st) {
     return LQ_OK;
 }
 
+// f(MT, CT) of a tile of kGemmTiles
+template <int PARTS, int BITS, int AT = 0, class F>
+int by_gemm_tile(int tile, F&& f) {
+    if constexpr (AT < kGemmTiles<PARTS, BITS>.size()) {
+        constexpr GemmTile t = kGemmTiles<PARTS, BITS>[AT];
+        if (tile == AT) return f(std::integral_constant<int, t.mt>{}, std::integral_constant<int, t.ct>{});
+        return by_gemm_tile<PARTS, BITS, AT + 1>(tile, f);
+    }
+    return fail(LQ_ERR_VALUE, "quantized_gated_matmul: no tile");
+}
+
 template <class T, int PARTS, int BITS>
 int launch_gemm(const Args& a, int tile, hipStream_t st) {
     auto of_group = [&](auto gs_c) -> int {
         constexpr int GS = decltype(gs_c)::value;
-        auto is = [&](auto index) -> int {
-            constexpr GemmTile t = kGemmTile<PARTS, BITS>[decltype(index)::value];
-            if constexpr (t.mt > 0) return launch_gemm_chunks<T, PARTS, BITS, GS, t.mt, t.ct>(a, st);
-            return fail(LQ_ERR_VALUE, "quantized_gated_matmul: no tile");
-        };
-        if (tile == 0) return is(std::integral_constant<int, 0>{});
-        if (tile == 1) return is(std::integral_constant<int, 1>{});
-        if (tile == 2) return is(std::integral_constant<int, 2>{});
-        if (tile == 3) return is(std::integral_constant<int, 3>{});
-        return is(std::integral_constant<int, 4>{});
+        return by_gemm_tile<PARTS, BITS>(tile, [&](auto mt, auto ct) -> int {
+            return launch_gemm_chunks<T, PARTS, BITS, GS, decltype(mt)::value, decltype(ct)::value>(a, st);
+        });
     };
     const int gs = 1 << a.gs_shift;
     if (gs == 32) return of_group(std::integral_constant<int, 32>{});

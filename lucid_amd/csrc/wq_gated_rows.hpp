@@ -11,14 +11,17 @@
 // x as it enters the matrix instructions: float16 as it is; a float32 row times the power of two that brings its largest value below 2^15,
 // as two float16, hi = x rounded, lo = x - hi rounded: 22 bits, or 2^-39 of the largest value.
 //
-// gated_few_kernel, up to 4 rows of up to 64 KB: a block has 16 columns, its four wavefronts every fourth step each.  It brings x into LDS itself, while
+// gated_few_kernel, up to 4 rows that leave room for two blocks a CU: a block has 16 columns, its four wavefronts every fourth step each.  It brings x into LDS itself, while
 // its first weights are under way, and nothing else is shared, so that there is no barrier in the loop.  A row of x lies on every fourth row of the
 // instruction: a lane then has one element of each result.
 //
-// gated_rows_kernel, up to 64 rows: a block has 64 columns, its eight wavefronts 16 of them and every other step each, so that four share
+// gated_rows_kernel: a block of eight wavefronts has CG times 16 columns, a wavefront 16 of them and every SG-th step (CG SG = 8), so that CG share
 // an x (16 rows of float32 are as many bytes as the codes of 16 columns of both weights in 8 bits, and come from the L2 for every block again:
-// 16 x 11008 x 4096, 16 columns a block and no x shared, 41 us).  float32 rows are split by a launch of their own.
+// 16 x 11008 x 4096, 16 columns a block and no x shared, 41 us).  What a block takes is a chain of steps, so with few columns steps are dealt
+// to more wavefronts as far as the blocks are one a CU: 16 x 2048 x 4096, 4 bits, float16, 16 us with CG = 4, 10.6 with 2, 8.0 with 1.  float32 rows
+// are split by a launch of their own.
 #pragma once
+#include <algorithm>
 #include <type_traits>
 
 #include "wq_gated.hpp"
@@ -32,9 +35,7 @@ namespace {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr size_t kFewLds = 64 * 1024;
 constexpr int kFewWaves = 4, kFewStep = 128;  // k of a step
-constexpr int kColumnGroups = 4, kStepGroups = 2, kRowsWaves = kColumnGroups * kStepGroups, kRowsTable = 16;  // (groups)
 
 struct RowsX {
     const _Float16* part[2];  // [M, K]; float16 x: the first
@@ -190,6 +191,9 @@ template <int BITS>
 constexpr int kFewRing = BITS == 4 ? 3 : 2;
 template <int BITS>
 constexpr int kFewFixed = kFewWaves * kFewRing<BITS> * Codes<BITS, kFewStep>::BYTES + 2 * Numbers<kFewTable>::BYTES;  // bytes of LDS without x
+// For x where a CU has two blocks.  (One: 2 x 11008 x 4096, float32 and 8 bits, 37.3 us, by the other kernel 25.7; two: 4 bits, 26.4 and 27.7.)
+template <int BITS>
+constexpr int kFewRoom = 77 * 1024 - kFewFixed<BITS>;
 
 template <class T, int PARTS, int BITS, int GS>
 __global__ __launch_bounds__(64 * kFewWaves) void gated_few_kernel(Args a) {
@@ -310,36 +314,37 @@ __global__ __launch_bounds__(64 * kFewWaves) void gated_few_kernel(Args a) {
     static_cast<T*>(a.out)[size_t(m) * a.N + n] = T(activate(a.act, g) * u);
 }
 
-// ---------------------------------------------------------------- up to 64 rows
+// ---------------------------------------------------------------- more rows
 // A step is 128 k where LDS has room for two of them beside the tables, else 64 (16 x 11008 x 4096, 8 bits, float32, without the launch that
 // splits x: 25.2 us, 28.9 with steps of 64 and a ring of four).
-template <int PARTS, int BITS, int MT, int STEP>
-constexpr int kRowsBytes = kRowsWaves * Codes<BITS, STEP>::BYTES + kStepGroups * PARTS * MT * STEP * 32;
-template <int PARTS, int BITS, int GS, int MT>
+template <int PARTS, int BITS, int MT, int CG, int SG, int STEP>
+constexpr int kRowsBytes = CG * SG * Codes<BITS, STEP>::BYTES + SG * PARTS * MT * STEP * 32;
+template <int PARTS, int BITS, int GS, int MT, int CG, int SG>
 struct RowsStep {
-    static constexpr int TABLE = kColumnGroups * Numbers<kRowsTable>::BYTES, ROOM = 158 * 1024 - 2 * TABLE;  // a table of the block's columns
-    static constexpr int STEP = 2 * kRowsBytes<PARTS, BITS, MT, 128> <= ROOM ? 128 : 64, BYTES = kRowsBytes<PARTS, BITS, MT, STEP>;
+    static constexpr int WAVES = CG * SG, GROUPS = SG == 8 ? 32 : 16;  // of a table
+    static constexpr int TABLE = CG * Numbers<GROUPS>::BYTES, ROOM = 158 * 1024 - 2 * TABLE;  // a table of the block's columns
+    static constexpr int STEP = 2 * kRowsBytes<PARTS, BITS, MT, CG, SG, 128> <= ROOM ? 128 : 64, BYTES = kRowsBytes<PARTS, BITS, MT, CG, SG, STEP>;
     using C = Codes<BITS, STEP>;
     // x of each group of steps: [part][tile][16 rows of 2 STEP bytes], 1 KiB has 512 / STEP rows
     static constexpr int OCTETS = STEP / 8, ROWS = 512 / STEP, PIECES = PARTS * MT * 16 / ROWS;
-    static constexpr int PER_WAVE = (PIECES + kColumnGroups - 1) / kColumnGroups;
+    static constexpr int PER_WAVE = (PIECES + CG - 1) / CG;
     static constexpr int LOADS = C::LOADS + PER_WAVE;
-    static constexpr int FIT = ROOM / BYTES, RING = FIT > 4 ? 4 : FIT;
-    static constexpr int TURN = kRowsTable * GS / (STEP * kStepGroups);  // iterations for a table: it has landed when RING - 2 are under way
+    static constexpr int TURN = GROUPS * GS / (STEP * SG);  // iterations for a table: it has landed when RING - 2 are under way
+    static constexpr int FIT = ROOM / BYTES, MOST = TURN < 2 ? TURN + 2 : 4, RING = FIT > MOST ? MOST : FIT;
     static_assert(RING >= 2 && LOADS * (RING - 2) <= 63 && TURN >= RING - 2, "");
     static __device__ __forceinline__ int swizzle(int r) { return STEP == 128 ? r : r >> 1; }
 };
 
 __device__ const uint4 kZeros = {0u, 0u, 0u, 0u};  // what a step past K has for x
 
-template <class T, int PARTS, int BITS, int GS, int MT>
-__global__ __launch_bounds__(64 * kRowsWaves) void gated_rows_kernel(Args a, RowsX rx) {
-    using S = RowsStep<PARTS, BITS, GS, MT>;
+template <class T, int PARTS, int BITS, int GS, int MT, int CG, int SG>
+__global__ __launch_bounds__(64 * CG * SG) void gated_rows_kernel(Args a, RowsX rx) {
+    using S = RowsStep<PARTS, BITS, GS, MT, CG, SG>;
     using C = typename S::C;
     extern __shared__ __attribute__((aligned(1024))) char smem[];  // the tables, the ring of steps; at the end the sums
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = lane & 15;
-    const int cg = wave % kColumnGroups, sg = wave / kColumnGroups;
-    const int n0 = (blockIdx.x * kColumnGroups + cg) * 16, m0 = blockIdx.y * (16 * MT), steps = (a.K + S::STEP - 1) / S::STEP;
+    const int cg = wave % CG, sg = wave / CG;
+    const int n0 = (blockIdx.x * CG + cg) * 16, m0 = blockIdx.y * (16 * MT), steps = (a.K + S::STEP - 1) / S::STEP;
     const CodesFrom<BITS, S::STEP> from(a, n0, lane);
     const bool aligned = numbers_aligned(a);
     // this wavefront's pieces of x (rows past M: the last one's bytes; one that there is not: another's again)
@@ -347,20 +352,20 @@ __global__ __launch_bounds__(64 * kRowsWaves) void gated_rows_kernel(Args a, Row
     int x_piece[S::PER_WAVE], x_k[S::PER_WAVE];
 #pragma unroll
     for (int u = 0; u < S::PER_WAVE; ++u) {
-        x_piece[u] = (u * kColumnGroups + cg) % S::PIECES;
+        x_piece[u] = (u * CG + cg) % S::PIECES;
         const int tile = x_piece[u] * S::ROWS / 16, r = x_piece[u] * S::ROWS % 16 + lane / S::OCTETS, m = m0 + tile % MT * 16 + r;
         x_from[u] = (tile / MT ? rx.part[PARTS - 1] : rx.part[0]) + size_t(m < a.M ? m : a.M - 1) * a.K;
         x_k[u] = ((lane % S::OCTETS) ^ (S::swizzle(r) % S::OCTETS)) * 8;
     }
     auto load = [&](int i, int slot) {
-        const int want = i * kStepGroups + sg, s = want < steps ? want : steps - 1;  // past the end: any step, to keep the count
+        const int want = i * SG + sg, s = want < steps ? want : steps - 1;  // past the end: any step, to keep the count
         char* const to = smem + 2 * S::TABLE + slot * S::BYTES;
         from.load(s, to + wave * C::BYTES);
 #pragma unroll
         for (int u = 0; u < S::PER_WAVE; ++u) {
             const int k = s * S::STEP + x_k[u];
             __builtin_amdgcn_global_load_lds((gptr)(k < a.K ? reinterpret_cast<const char*>(x_from[u] + k) : reinterpret_cast<const char*>(&kZeros)),
-                                             (lptr)(to + kRowsWaves * C::BYTES + (sg * S::PIECES + x_piece[u]) * 1024), 16, 0, 0);
+                                             (lptr)(to + S::WAVES * C::BYTES + (sg * S::PIECES + x_piece[u]) * 1024), 16, 0, 0);
         }
     };
     float y[2][MT][4];
@@ -372,28 +377,29 @@ __global__ __launch_bounds__(64 * kRowsWaves) void gated_rows_kernel(Args a, Row
             for (int r = 0; r < 4; ++r) y[i][t][r] = 0.f;
     // two arrays of its columns' tables are each wavefront's to load
     auto load_table = [&](int j) {
-        char* const table = smem + (j & 1) * S::TABLE + cg * Numbers<kRowsTable>::BYTES;
+        char* const table = smem + (j & 1) * S::TABLE + cg * Numbers<S::GROUPS>::BYTES;
 #pragma unroll
-        for (int u = 0; u < 4 / kStepGroups; ++u) load_numbers<kRowsTable>(a, sg * (4 / kStepGroups) + u, n0, j * kRowsTable, table, lane, aligned);
+        for (int u = 0; u < (SG > 4 ? 1 : 4 / SG); ++u)
+            load_numbers<S::GROUPS>(a, SG > 4 ? sg % 4 : sg * (4 / SG) + u, n0, j * S::GROUPS, table, lane, aligned);
     };
     load_table(0);
 #pragma unroll
     for (int d = 0; d < S::RING - 1; ++d) load(d, d);
     int slot = 0;
-    for (int i = 0; i * kStepGroups < steps; ++i) {
+    for (int i = 0; i * SG < steps; ++i) {
         pin();
         __builtin_amdgcn_s_waitcnt(vmcnt_and_lds(S::LOADS * (S::RING - 2)));
         __builtin_amdgcn_s_barrier();
         pin();
-        if (i % S::TURN == 0 && (i + S::TURN) * kStepGroups < steps) load_table(i / S::TURN + 1);
+        if (i % S::TURN == 0 && (i + S::TURN) * SG < steps) load_table(i / S::TURN + 1);
         load(i + S::RING - 1, slot == 0 ? S::RING - 1 : slot - 1);  // (the slot that everybody has just left)
         const char* const at = smem + 2 * S::TABLE + slot * S::BYTES;
         slot = slot + 1 == S::RING ? 0 : slot + 1;
-        const int s = i * kStepGroups + sg;
+        const int s = i * SG + sg;
         if (s >= steps) continue;  // uniform: the other group's last step
-        const char* const x = at + kRowsWaves * C::BYTES + sg * (S::PIECES * 1024) + ln * (2 * S::STEP);
-        const char* const table = smem + (i / S::TURN & 1) * S::TABLE + cg * Numbers<kRowsTable>::BYTES;
-        multiply<PARTS, BITS, GS, S::STEP, kRowsTable, MT, 4>(at + wave * C::BYTES, table, s * S::STEP / GS % kRowsTable, lane, y, [&](int k, int p, int t) {
+        const char* const x = at + S::WAVES * C::BYTES + sg * (S::PIECES * 1024) + ln * (2 * S::STEP);
+        const char* const table = smem + (i / S::TURN & 1) * S::TABLE + cg * Numbers<S::GROUPS>::BYTES;
+        multiply<PARTS, BITS, GS, S::STEP, S::GROUPS, MT, 4>(at + wave * C::BYTES, table, s * S::STEP / GS % S::GROUPS, lane, y, [&](int k, int p, int t) {
             const u32x4 raw = *reinterpret_cast<const u32x4*>(x + (p * MT + t) * (32 * S::STEP) + ((k >> 3) ^ (S::swizzle(ln) % S::OCTETS)) * 16);
             return slots_f16<BITS>(uint4{raw[0], raw[1], raw[2], raw[3]});
         });
@@ -408,19 +414,20 @@ __global__ __launch_bounds__(64 * kRowsWaves) void gated_rows_kernel(Args a, Row
 #pragma unroll
             for (int r = 0; r < 4; ++r) s_y[wave][i][t][r][lane] = y[i][t][r];
     __syncthreads();
-    // a thread has a column of 64 and rows 8 apart: element row % 4 of lane column + 16 (row / 4)
-    const int col = threadIdx.x & 63, n = blockIdx.x * (kColumnGroups * 16) + col;
+    // a thread has a column and rows ROWS apart: element row % 4 of lane column + 16 (row / 4)
+    constexpr int COLS = CG * 16, ROWS = 4 * SG;
+    const int col = threadIdx.x % COLS, n = blockIdx.x * COLS + col;
     if (n >= a.N) return;
     const float bg = a.w[0].bias ? a.w[0].bias[n] : 0.f, bu = a.w[1].bias ? a.w[1].bias[n] : 0.f;
 #pragma unroll
-    for (int j = 0; j < 2 * MT; ++j) {
-        const int row = j * 8 + (threadIdx.x >> 6), m = m0 + row, t = row >> 4, from_lane = (col & 15) + 16 * ((row >> 2) & 3);
-        if (m >= a.M) return;
+    for (int j = 0; j < (16 * MT + ROWS - 1) / ROWS; ++j) {
+        const int row = j * ROWS + threadIdx.x / COLS, m = m0 + row, t = row >> 4, from_lane = (col & 15) + 16 * ((row >> 2) & 3);
+        if ((16 * MT % ROWS && row >= 16 * MT) || m >= a.M) return;
         float g = 0.f, u = 0.f;
 #pragma unroll
-        for (int p = 0; p < kStepGroups; ++p) {
-            g += s_y[p * kColumnGroups + (col >> 4)][0][t][row & 3][from_lane];
-            u += s_y[p * kColumnGroups + (col >> 4)][1][t][row & 3][from_lane];
+        for (int p = 0; p < SG; ++p) {
+            g += s_y[p * CG + (col >> 4)][0][t][row & 3][from_lane];
+            u += s_y[p * CG + (col >> 4)][1][t][row & 3][from_lane];
         }
         if constexpr (PARTS == 2) g *= rx.unscale[m], u *= rx.unscale[m];
         static_cast<T*>(a.out)[size_t(m) * a.N + n] = T(activate(a.act, g + bg) * (u + bu));
@@ -485,22 +492,20 @@ int by_group(int bits, int gs, F&& f) {
     return bits == 4 ? of_bits(integral_constant<int, 4>{}) : of_bits(integral_constant<int, 8>{});
 }
 
-template <class T>
-int launch_rows(const Args& a, int bits, hipStream_t st) {
-    constexpr int PARTS = std::is_same_v<T, float> ? 2 : 1;
-    LQ_REQUIRE(a.K < 1 << 26, LQ_ERR_SHAPE, "quantized_gated_matmul: K = %d", a.K);  // (offsets of 16 rows are 32-bit)
-    const size_t few = size_t(PARTS) * a.M * ((a.K + kFewStep - 1) / kFewStep * (kFewStep * 2) + 16);
-    if (a.M <= 4 && few <= kFewLds)
-        return by_group(bits, 1 << a.gs_shift, [&](auto bits_c, auto gs_c) -> int {
-            constexpr int BITS = decltype(bits_c)::value, GS = decltype(gs_c)::value;
-            const auto kernel = gated_few_kernel<T, PARTS, BITS, GS>;
-            static DeviceOnce once;
-            if (const int rc = allow_dynamic_lds(once, reinterpret_cast<const void*>(kernel), kFewFixed<BITS> + int(kFewLds))) return rc;
-            kernel<<<(unsigned(a.N) + 15) / 16, 64 * kFewWaves, kFewFixed<BITS> + few, st>>>(a);
-            LQ_CHECK_LAUNCH("quantized_gated_matmul");
-            return LQ_OK;
-        });
-    const auto lock = scratch_lock(st);
+// f(MT, CG, SG) of a tile of kRowsTiles: eight wavefronts
+template <int PARTS, int AT = 0, class F>
+int by_tile(int tile, F&& f) {
+    if constexpr (AT < kRowsTiles<PARTS>.size()) {
+        using std::integral_constant;
+        constexpr RowsTile t = kRowsTiles<PARTS>[AT];
+        if (tile == AT) return f(integral_constant<int, t.mt>{}, integral_constant<int, t.cg>{}, integral_constant<int, 8 / t.cg>{});
+        return by_tile<PARTS, AT + 1>(tile, f);
+    }
+    return fail(LQ_ERR_VALUE, "quantized_gated_matmul: no tile");
+}
+
+template <class T, int PARTS>
+int launch_rows_chunk(const Args& a, int bits, int tile, hipStream_t st) {
     RowsX rx{{static_cast<const _Float16*>(a.x), nullptr}, nullptr};
     if constexpr (PARTS == 2) {
         void* ws = nullptr;
@@ -514,22 +519,45 @@ int launch_rows(const Args& a, int bits, hipStream_t st) {
     }
     return by_group(bits, 1 << a.gs_shift, [&](auto bits_c, auto gs_c) -> int {
         constexpr int BITS = decltype(bits_c)::value, GS = decltype(gs_c)::value;
-        auto launch = [&](auto tiles) -> int {
-            constexpr int MT = decltype(tiles)::value;
-            using S = RowsStep<PARTS, BITS, GS, MT>;
-            const dim3 grid((unsigned(a.N) + kColumnGroups * 16 - 1) / (kColumnGroups * 16), (unsigned(a.M) + 16 * MT - 1) / (16 * MT));
-            LQ_REQUIRE(grid.y <= 65535, LQ_ERR_SHAPE, "quantized_gated_matmul: %d rows", a.M);
-            const auto kernel = gated_rows_kernel<T, PARTS, BITS, GS, MT>;
-            constexpr int need = 2 * S::TABLE + S::RING * S::BYTES, sums = kRowsWaves * MT * 2048, lds = need > sums ? need : sums;
+        return by_tile<PARTS>(tile, [&](auto mt, auto cg, auto sg) -> int {
+            constexpr int MT = decltype(mt)::value, CG = decltype(cg)::value, SG = decltype(sg)::value;
+            using S = RowsStep<PARTS, BITS, GS, MT, CG, SG>;
+            const dim3 grid((unsigned(a.N) + CG * 16 - 1) / (CG * 16), (unsigned(a.M) + 16 * MT - 1) / (16 * MT));
+            const auto kernel = gated_rows_kernel<T, PARTS, BITS, GS, MT, CG, SG>;
+            constexpr int need = 2 * S::TABLE + S::RING * S::BYTES, sums = S::WAVES * MT * 2048, lds = need > sums ? need : sums;
             static DeviceOnce once;
             if (const int rc = allow_dynamic_lds(once, reinterpret_cast<const void*>(kernel), lds)) return rc;
-            kernel<<<grid, 64 * kRowsWaves, lds, st>>>(a, rx);
+            kernel<<<grid, 64 * S::WAVES, lds, st>>>(a, rx);
             LQ_CHECK_LAUNCH("quantized_gated_matmul");
             return LQ_OK;
-        };
-        if (a.M > 32) return launch(std::integral_constant<int, 4>{});
-        return a.M > 16 ? launch(std::integral_constant<int, 2>{}) : launch(std::integral_constant<int, 1>{});
+        });
     });
+}
+
+template <class T>
+int launch_rows(Args a, int bits, int tile, hipStream_t st) {
+    constexpr int PARTS = std::is_same_v<T, float> ? 2 : 1;
+    LQ_REQUIRE(a.K < 1 << 26, LQ_ERR_SHAPE, "quantized_gated_matmul: K = %d", a.K);  // (offsets of 16 rows are 32-bit)
+    const size_t few = size_t(PARTS) * a.M * ((a.K + kFewStep - 1) / kFewStep * (kFewStep * 2) + 16);
+    if (a.M <= 4 && few <= size_t(bits == 4 ? kFewRoom<4> : kFewRoom<8>))
+        return by_group(bits, 1 << a.gs_shift, [&](auto bits_c, auto gs_c) -> int {
+            constexpr int BITS = decltype(bits_c)::value, GS = decltype(gs_c)::value;
+            const auto kernel = gated_few_kernel<T, PARTS, BITS, GS>;
+            static DeviceOnce once;
+            if (const int rc = allow_dynamic_lds(once, reinterpret_cast<const void*>(kernel), kFewFixed<BITS> + kFewRoom<BITS>)) return rc;
+            kernel<<<(unsigned(a.N) + 15) / 16, 64 * kFewWaves, kFewFixed<BITS> + few, st>>>(a);
+            LQ_CHECK_LAUNCH("quantized_gated_matmul");
+            return LQ_OK;
+        });
+    const auto lock = scratch_lock(st);
+    // rows in chunks of whole tiles whose parts stay below 2^30 bytes
+    const int M = a.M, most = int(std::clamp<size_t>((size_t(1) << 28) / a.K / 64 * 64, 64, 65535 * 16));
+    for (int m0 = 0; m0 < M; m0 += a.M) {
+        a.M = std::min(most, M - m0);
+        if (const int rc = launch_rows_chunk<T, PARTS>(a, bits, tile, st)) return rc;
+        a.x = static_cast<const T*>(a.x) + size_t(a.M) * a.K, a.out = static_cast<T*>(a.out) + size_t(a.M) * a.N;
+    }
+    return LQ_OK;
 }
 
 }  // namespace

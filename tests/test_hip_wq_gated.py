@@ -33,10 +33,7 @@ SHAPES = [(1, 1, 32, 32), (1, 16, 64, 64), (1, 17, 128, 128), (1, 11008, 4096, 6
           (333, 1033, 576, 32), (400, 2049, 256, 128)]
 
 
-@pytest.mark.parametrize("M,N,K,gs", SHAPES)
-@pytest.mark.parametrize("bits", [4, 8])
-@pytest.mark.parametrize("dtype", [np.float32, np.float16])
-def test_exact_on_exact_numbers(M, N, K, gs, bits, dtype):
+def exact_numbers(M, N, K, gs, bits, dtype, columns=slice(None)):
     """Small whole x, scales of powers of two and whole biases keep every sum a multiple of 1/64 below 2^18: one code, scale, group or row out of place
     shows.  (Codes of 8 bits in a band of 32 about the middle and at its ends, so that sums stay small.)"""
     rng = np.random.default_rng(M + N + K + bits)
@@ -53,21 +50,45 @@ def test_exact_on_exact_numbers(M, N, K, gs, bits, dtype):
         b = (-(1 << (bits - 1)) * s + scale * rng.integers(-4, 5, s.shape)).astype(np.float32)
         packs.append((packed, s, b))
         bias = (scale * rng.integers(-50, 51, N)).astype(np.float32)
-        g64.append((x.astype(np.float64) @ weight64(packed, s, b, gs, bits).T + bias, bias))
+        g64.append((x.astype(np.float64) @ weight64(packed[columns], s[columns], b[columns], gs, bits).T + bias[columns], bias))
     y = _qgemm.quantized_gated_matmul(hip(x), *(tuple(map(hip, p)) for p in packs), activation="relu", group_size=gs, bits=bits,
                                       gate_bias=hip(g64[0][1]), up_bias=hip(g64[1][1]))
     assert y.shape == (M, N) and y.dtype.np == dtype
     assert max(abs(g).max() for g, _ in g64) < 2 ** 18
     with np.errstate(over="ignore"):
         want = (np.maximum(g64[0][0], 0) * g64[1][0]).astype(np.float32).astype(dtype)
-    assert np.array_equal(y.numpy(), want)
+    assert np.array_equal(y.numpy()[:, columns], want)
 
 
-def bound(x, parts, gs, bits, act, bias):
+@pytest.mark.parametrize("M,N,K,gs", SHAPES)
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_exact_on_exact_numbers(M, N, K, gs, bits, dtype):
+    exact_numbers(M, N, K, gs, bits, dtype)
+
+
+# few rows of columns that fill the device with 16, 32 or 64 a block; more rows than that takes, in tiles of every size
+WIDE = [(16, 4090), (16, 5630), (16, 11001), (32, 4000), (31, 8010), (32, 11008), (63, 11001), (325, 11009), (97, 8690), (195, 8850), (227, 8200), (325, 8250), (670, 4475), (685, 8410),
+        (1219, 2311)]
+
+
+def some_columns(N):
+    return np.r_[0:40, N // 3:N // 3 + 150, N - 70:N]
+
+
+@pytest.mark.parametrize("M,N", WIDE)
+@pytest.mark.parametrize("K,gs", [(160, 32), (320, 64), (640, 128)])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_many_columns(M, N, K, gs, bits, dtype):
+    exact_numbers(M, N, K, gs, bits, dtype, some_columns(N))
+
+
+def bound(x, parts, gs, bits, act, bias, two_parts=False):
     """The result in float64 and how far float32 arithmetic may be from it.  A projection is a sum of products (c - half) s x and of group terms
     (b + half s) (sum of x), accumulated in at most K / 8 roundings (a matrix instruction has 32 k, a group two multiply-adds): of random signs
     they stay below 4 sqrt(K / 8) U of the terms' magnitudes together, four deviations and more.  b + half s rounds once, x to 22 bits, and at 2^-38 of its
-    row's largest value."""
+    row's largest value.  two_parts: b + half s and the sums of x as two bfloat16 of 2^-18 together, whose lower ones are not multiplied."""
     half, K = 1 << (bits - 1), x.shape[1]
     out = []
     for (packed, s, b), bb in zip(parts, bias):
@@ -75,7 +96,8 @@ def bound(x, parts, gs, bits, act, bias):
         c = W.unpack(packed, bits).astype(np.float64) - half
         size = abs(x) @ (abs(c * s64) + abs(b64) + half * abs(s64)).T + abs(bb)
         floor = 2.0 ** -38 * abs(x).max(-1, keepdims=True) * abs(c * s64).sum(-1)
-        out.append((x @ (c * s64 + b64 + half * s64).T + bb, (4 * np.sqrt(K / 8) + 8) * U * size + floor))
+        lost = 3 * 2.0 ** -18 * abs(x.reshape(len(x), -1, gs).sum(-1)) @ abs(b.astype(np.float64) + half * s).T if two_parts else 0.0
+        out.append((x @ (c * s64 + b64 + half * s64).T + bb, (4 * np.sqrt(K / 8) + 8) * U * size + floor + lost))
     (g, eg), (u, eu) = out
     a = ACTS[act](g)
     # slopes of the activations are at most 1.13; exp and erfc round by a few units, and exp(-g) by U |g| more through its argument
@@ -98,6 +120,49 @@ def test_against_float64(M, N, K, gs, bits, dtype, act):
     want, e = bound(x.astype(np.float64), parts, gs, bits, act, bias if with_bias else [np.zeros(N)] * 2)
     info = np.finfo(dtype)
     assert (abs(y - want) <= e + (abs(want) + e) * info.eps / 2 + info.tiny * info.eps).all()
+
+
+@pytest.mark.parametrize("M,N,K,gs", [(33, 11008, 1152, 32), (195, 8850, 1024, 64), (333, 8200, 1152, 128)])
+@pytest.mark.parametrize("bits,dtype", [(4, np.float32), (8, np.float32), (4, np.float16), (8, np.float16)])
+def test_many_columns_against_float64(M, N, K, gs, bits, dtype):
+    rng = np.random.default_rng(M + bits)
+    x = (rng.standard_normal((M, K)) * (1 + 30 * (rng.random(K) < 0.01))).astype(dtype)
+    parts = [W.quantize((0.05 * rng.standard_normal((N, K))).astype(np.float32), gs, bits) for _ in range(2)]
+    y = _qgemm.quantized_gated_matmul(hip(x), *(tuple(map(hip, p)) for p in parts), group_size=gs, bits=bits).numpy()
+    cols = some_columns(N)
+    want, e = bound(x.astype(np.float64), [tuple(a[cols] for a in p) for p in parts], gs, bits, "silu", [np.zeros(len(cols))] * 2,
+                    two_parts=dtype is np.float16)
+    half = np.finfo(dtype).eps / 2
+    assert (abs(y[:, cols] - want) <= e + half * (abs(want) + e) + np.finfo(dtype).tiny * np.finfo(dtype).eps).all()
+
+
+@pytest.mark.parametrize("M", [16, 63, 325])
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_many_columns_in_graphs_and_with_rows_that_are_not_finite(M, dtype):
+    rng = np.random.default_rng(M)
+    graphs = []
+    for N in (8250, 11008):
+        parts = [tuple(map(hip, W.quantize(rng.standard_normal((N, 160)).astype(np.float32), 32, 4))) for _ in range(2)]
+        x = hip(rng.standard_normal((M, 160)).astype(dtype))
+        call = lambda x=x, parts=parts: _qgemm.quantized_gated_matmul(x, *parts, group_size=32, bits=4)
+        call()
+        with L.graph.capture() as g:
+            y = call()
+        graphs.append((g, x, y, call))
+    for _ in range(3):
+        for g, x, y, call in graphs:
+            clean = rng.standard_normal((M, 160)).astype(dtype)
+            x.copy_from(clean)
+            g.replay()
+            L.synchronize()
+            want = call().numpy()
+            assert np.isfinite(want).all() and np.array_equal(y.numpy(), want)
+            clean[3, 5], clean[9, 159] = np.nan, np.inf
+            x.copy_from(clean)
+            g.replay()
+            L.synchronize()
+            rest = np.delete(np.arange(M), [3, 9])
+            assert np.array_equal(y.numpy()[rest], want[rest]) and np.isnan(y.numpy()[3]).all() and not np.isfinite(y.numpy()[9]).any()
 
 
 @pytest.mark.parametrize("M", [3, 100, 300])
