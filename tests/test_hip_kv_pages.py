@@ -101,6 +101,19 @@ def test_what_sequences_keep(n, kind):
     check(c, table, np.concatenate([keep, keep]), [0, len(keep), 2 * len(keep)])
 
 
+@pytest.mark.parametrize("bits,symmetric,dim,heads", [(8, True, 16, 1), (8, False, 64, 3), (4, False, 32, 1), (4, True, 128, 2), (8, False, 80, 1)])
+@pytest.mark.parametrize("part", [0.3, 0.98])
+def test_many_sequences_and_long_ones(bits, symmetric, dim, heads, part):
+    """Sequences that end on both sides of a tile, and many that have none to themselves."""
+    rng = np.random.default_rng(dim + heads)
+    lengths = list(rng.integers(0, 20, 560)) + [1023, 1024, 1025, 1400, 4000, 2049, 1]
+    pages, table = sequences(rng, lengths, 16)
+    c = filled(rng, pages, 16, heads, dim, symmetric, bits)
+    keep = [np.sort(rng.permutation(n)[:round(part * n)]) for n in lengths]
+    keep[-5], keep[-3] = np.arange(1, 1025), np.concatenate([np.arange(1024), np.arange(1030, 4000)])
+    check(c, table, np.concatenate(keep), np.cumsum([0] + [len(k) for k in keep]))
+
+
 def test_places_that_are_none():
     """Beyond the table, on a page that is negative or beyond the cache, old or new: not moved.  Entries of no sequence are not looked at."""
     rng = np.random.default_rng(2)

@@ -63,7 +63,7 @@ def check(rows, cols, layer=False, post=False, gate_rows=0, scale=False, x_type=
 
 
 # rows of every number of threads and of values a thread, whole and not
-WIDTHS = [1, 2, 3, 5, 16, 255, 256, 257, 512, 513, 768, 1000, 1024, 1025, 2047, 2048, 4095, 4096, 4097, 8192, 8195, 16384, 16385, 32767, 32768]
+WIDTHS = [1, 2, 3, 5, 16, 255, 256, 257, 512, 513, 768, 1000, 1024, 1025, 2047, 2048, 2501, 2910, 3000, 4095, 4096, 4097, 5999, 6140, 6146, 8191, 8192, 8195, 16384, 16385, 32767, 32768]
 
 
 @pytest.mark.parametrize("cols", WIDTHS)
