@@ -52,31 +52,34 @@ __device__ __forceinline__ double wave_scan(double v, unsigned lane) {
     return v;
 }
 
-// Eight values from v on, as they lie in memory; zeros from `end` on.
+// Eight values of a row as they lie in memory.
 template <class T>
 struct Raw {
     T v[kVec];
 };
-template <class T>
-__device__ __forceinline__ Raw<T> load8(const T* row, unsigned v, unsigned end) {
-    Raw<T> raw;
-    if (v + kVec <= end) {
-        __builtin_memcpy(&raw, row + v, sizeof raw);  // (rows of odd length are not 16-byte aligned)
-    } else {
-#pragma unroll
-        for (unsigned e = 0; e < kVec; ++e) raw.v[e] = v + e < end ? row[v + e] : T(0.f);
-    }
-    return raw;
-}
 
-// The row that a sequence's next token is drawn from: p alone, without token x (kNone: with all), or p - q.
-template <class T, bool DRAFT>
+// The row that a sequence's next token is drawn from: p alone, without token x (kNone: with all), or p - q.  A lane's eight tokens from v on: of
+// those that reach past `end` the last eight before it are loaded, and what is before v does not count, so that no load has a branch (code
+// that a block runs once comes from memory: one row of 540 float32 by value with branches 10.2 us, so
+// 8.9; 128 rows of 131 072, which are bound by memory, 33.5 and 34.7).  TINY: rows of fewer than eight, by value.
+template <class T, bool DRAFT, bool TINY>
 struct Row {
     const T *p, *q;  // q NULL: p alone
     unsigned x;
     struct Eight {
         Raw<T> p, q[DRAFT ? 1 : 0];
     };
+    static __device__ __forceinline__ unsigned place(unsigned v, unsigned end) { return !TINY && v + kVec > end ? end - kVec : v; }
+    static __device__ __forceinline__ Raw<T> load8(const T* row, unsigned v, unsigned end) {
+        Raw<T> raw;
+        if constexpr (TINY) {
+#pragma unroll
+            for (unsigned e = 0; e < kVec; ++e) raw.v[e] = row[v + e < end ? v + e : 0];
+        } else {
+            __builtin_memcpy(&raw, row + place(v, end), sizeof raw);  // (rows of odd length are not 16-byte aligned)
+        }
+        return raw;
+    }
     __device__ __forceinline__ Eight load(unsigned v, unsigned end) const {
         Eight r;
         r.p = load8(p, v, end);
@@ -84,11 +87,15 @@ struct Row {
             if (q) r.q[0] = load8(q, v, end);
         return r;
     }
-    // the weights; all: those of p where q is there
-    __device__ __forceinline__ void weights(const Eight& r, unsigned v, double (&w)[kVec], double& all) const {
+    // the weights of tokens place(v, end) + e; all: those of p where q is there
+    __device__ __forceinline__ void weights(const Eight& r, unsigned v, unsigned end, double (&w)[kVec], double& all) const {
         all = 0.0;
+        const unsigned at = place(v, end);
 #pragma unroll
-        for (unsigned e = 0; e < kVec; ++e) w[e] = double(counted(float(r.p.v[e])));
+        for (unsigned e = 0; e < kVec; ++e) {
+            const bool own = TINY ? v + e < end : at + e >= v;
+            w[e] = own ? double(counted(float(r.p.v[e]))) : 0.0;
+        }
         if constexpr (DRAFT) {
             if (q) {
 #pragma unroll
@@ -97,10 +104,10 @@ struct Row {
                     w[e] = fmax(w[e] - double(counted(float(r.q[0].v[e]))), 0.0);
                 }
             }
-        } else if (x - v < kVec) {
+        } else if (x - at < kVec) {
 #pragma unroll
             for (unsigned e = 0; e < kVec; ++e)
-                if (v + e == x) w[e] = 0.0;
+                if (at + e == x) w[e] = 0.0;
         }
     }
 };
@@ -120,9 +127,9 @@ constexpr int kBlocks = 4;  // of a CU: what their registers leave room for
 template <class T, bool DRAFT>
 constexpr unsigned kAhead = sizeof(T) == 2 && !DRAFT ? 8 : 4;  // times eight probabilities that a thread asks for at once
 
-template <class T, bool DRAFT>
+template <class T, bool DRAFT, bool TINY>
 __global__ __launch_bounds__(256, kBlocks) void verify_drafts_kernel(Args a) {
-    constexpr unsigned kAtOnce = kAhead<T, DRAFT>;
+    constexpr unsigned kAtOnce = TINY ? 1 : kAhead<T, DRAFT>;
     __shared__ double s_sum[2][kWaves], s_piece[kAtOnce * kWaves];
     __shared__ unsigned s_first;
     __shared__ int s_is_last, s_next;
@@ -159,14 +166,14 @@ __global__ __launch_bounds__(256, kBlocks) void verify_drafts_kernel(Args a) {
         __syncthreads();
     }
     const bool refused = accepted < n - 1;
-    Row<T, DRAFT> row{target + size_t(from + accepted) * a.vocab, refused && DRAFT ? draft + size_t(from + accepted) * a.vocab : nullptr,
+    Row<T, DRAFT, TINY> row{target + size_t(from + accepted) * a.vocab, refused && DRAFT ? draft + size_t(from + accepted) * a.vocab : nullptr,
                refused && !DRAFT ? unsigned(a.tokens[from + accepted + 1]) : kNone};
 
     // sums of this run
     const unsigned begin = blockIdx.x * a.run, end = begin + a.run < a.vocab ? begin + a.run : a.vocab;
     double all = 0.0, rest = 0.0;
     for (unsigned v0 = begin; v0 < end; v0 += kAtOnce * kRound) {
-        typename Row<T, DRAFT>::Eight r[kAtOnce];
+        typename Row<T, DRAFT, TINY>::Eight r[kAtOnce];
 #pragma unroll
         for (unsigned u = 0; u < kAtOnce; ++u)
             if (v0 + u * kRound < end) r[u] = row.load(v0 + u * kRound + tid * kVec, end);
@@ -174,7 +181,7 @@ __global__ __launch_bounds__(256, kBlocks) void verify_drafts_kernel(Args a) {
         for (unsigned u = 0; u < kAtOnce; ++u) {
             if (v0 + u * kRound >= end) continue;  // uniform
             double w[kVec], some;
-            row.weights(r[u], v0 + u * kRound + tid * kVec, w, some);
+            row.weights(r[u], v0 + u * kRound + tid * kVec, end, w, some);
             all += some;
             rest += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
         }
@@ -183,23 +190,25 @@ __global__ __launch_bounds__(256, kBlocks) void verify_drafts_kernel(Args a) {
     if (row.q) all = wave_sum(all);
     if (lane == 0) s_sum[0][wave] = rest, s_sum[1][wave] = all;
     __syncthreads();
-    if (tid == 0) {
-        rest = (s_sum[0][0] + s_sum[0][1]) + (s_sum[0][2] + s_sum[0][3]), all = (s_sum[1][0] + s_sum[1][1]) + (s_sum[1][2] + s_sum[1][3]);
-        double* const out = a.sums + (size_t(b) * runs + blockIdx.x) * 2;
-        // (through to where every block sees it)
-        __hip_atomic_store(out, rest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(out + 1, all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        // (both go past the caches, and the last block reads them so: that they have arrived is order enough, no cache need be written back)
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        s_is_last = __hip_atomic_fetch_add(&a.arrived[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == int(runs) - 1;
+    rest = (s_sum[0][0] + s_sum[0][1]) + (s_sum[0][2] + s_sum[0][3]), all = (s_sum[1][0] + s_sum[1][1]) + (s_sum[1][2] + s_sum[1][3]);
+    double run_sum = lane == 0 ? rest : 0.0, run_all = lane == 0 ? all : 0.0;  // a lane has the sums of one run
+    if (runs > 1) {
+        if (tid == 0) {
+            double* const out = a.sums + (size_t(b) * runs + blockIdx.x) * 2;
+            // (through to where every block sees it)
+            __hip_atomic_store(out, rest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(out + 1, all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            // (both go past the caches, and the last block reads them so: that they have arrived is order enough, no cache need be written back)
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            s_is_last = __hip_atomic_fetch_add(&a.arrived[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == int(runs) - 1;
+        }
+        __syncthreads();
+        if (!s_is_last) return;
+        // the last block of the sequence
+        const double* const sums = a.sums + (size_t(b) * runs + lane) * 2;
+        run_sum = lane < runs ? __hip_atomic_load(sums, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+        run_all = lane < runs ? __hip_atomic_load(sums + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
     }
-    __syncthreads();
-    if (!s_is_last) return;
-
-    // the last block of the sequence: a lane has the sums of one run
-    const double* const sums = a.sums + (size_t(b) * runs + lane) * 2;
-    double run_sum = lane < runs ? __hip_atomic_load(sums, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
-    const double run_all = lane < runs ? __hip_atomic_load(sums + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
     double total = wave_sum(run_sum), before = 0.0;
     if (tid == 0) s_next = -1;
     if (refused && !(total > 0.0)) {
@@ -217,14 +226,14 @@ __global__ __launch_bounds__(256, kBlocks) void verify_drafts_kernel(Args a) {
         const unsigned first = unsigned(run) * a.run, stop = first + a.run < a.vocab ? first + a.run : a.vocab;
         for (unsigned v0 = first; v0 < stop; v0 += kAtOnce * kRound) {
             double sum[kAtOnce];
-            typename Row<T, DRAFT>::Eight r[kAtOnce];
+            typename Row<T, DRAFT, TINY>::Eight r[kAtOnce];
 #pragma unroll
             for (unsigned u = 0; u < kAtOnce; ++u) r[u] = row.load(v0 + u * kRound + tid * kVec, stop);
             __syncthreads();  // (the pieces' sums before have been read)
 #pragma unroll
             for (unsigned u = 0; u < kAtOnce; ++u) {
                 double w[kVec], some;
-                row.weights(r[u], v0 + u * kRound + tid * kVec, w, some);
+                row.weights(r[u], v0 + u * kRound + tid * kVec, stop, w, some);
                 sum[u] = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
                 const double piece = wave_sum(sum[u]);
                 if (lane == 0) s_piece[u * kWaves + wave] = piece;
@@ -243,12 +252,12 @@ __global__ __launch_bounds__(256, kBlocks) void verify_drafts_kernel(Args a) {
                 if (at_lane == int(lane)) {
                     const unsigned v = v0 + u * kRound + tid * kVec;
                     double w[kVec], some;
-                    row.weights(row.load(v, stop), v, w, some);
+                    row.weights(row.load(v, stop), v, stop, w, some);
                     int next = -1;
                     bool passed = false;
 #pragma unroll
                     for (unsigned e = 0; e < kVec; ++e)
-                        if (w[e] > 0.0 && !passed) at_piece += w[e], next = int(v + e), passed = at_piece > goal;
+                        if (w[e] > 0.0 && !passed) at_piece += w[e], next = int(row.place(v, stop) + e), passed = at_piece > goal;
                     s_next = next;
                 }
             }
@@ -257,7 +266,7 @@ __global__ __launch_bounds__(256, kBlocks) void verify_drafts_kernel(Args a) {
         }
     }
     __syncthreads();
-    if (tid == 0) a.arrived[b] = 0;
+    if (runs > 1 && tid == 0) a.arrived[b] = 0;
     const int next = s_next;
     for (unsigned i = tid; i < n; i += kThreads) a.new_tokens[from + i] = i < accepted ? a.tokens[from + i + 1] : i == accepted ? next : -1;
     if (tid == 0) a.counts[b] = int(accepted) + 1;
@@ -274,10 +283,11 @@ extern "C" int lq_verify_drafts(const void* target, const void* draft, int dtype
     LQ_REQUIRE(starts && last && counts, LQ_ERR_VALUE, "verify_drafts: starts, last or counts is NULL");
     LQ_REQUIRE(new_tokens != tokens || !tokens, LQ_ERR_VALUE, "verify_drafts: the new tokens cannot take the drafted ones' place");
     LQ_REQUIRE(rows == 0 || (target && tokens && uniforms && new_tokens), LQ_ERR_VALUE, "verify_drafts: a NULL pointer");
-    // As many blocks as are resident, 2048 tokens at least each; 64 of a sequence at most.  (128 rows of 131 072 float16: 8 blocks a sequence that ask
-    // for all of their run at once 23.5 us, 12 and 16 of smaller runs 26 and 24.5, in rounds of 8192 tokens 29.)
+    // As many blocks as are resident, 8192 tokens at least each: what a block asks for at once, where one that is alone need not wait for others; 64 of
+    // a sequence at most.  (16 x 131 072 float32 22 us of 2048 tokens, 13.2 of 8192; 16 x 32 000 12.5 and 11.1.  128 rows of 131 072
+    // float16: 8 blocks a sequence that ask for all of their run at once 23.5 us, 12 and 16 of smaller runs 26 and 24.5, in rounds of 8192 tokens 29.)
     unsigned runs = 256u * unsigned(kBlocks) / unsigned(batch);
-    const unsigned most = (unsigned(vocab) + kRound - 1) / kRound;
+    const unsigned most = (unsigned(vocab) + 4 * kRound - 1) / (4 * kRound);
     runs = runs < 1 ? 1 : runs > 64 ? 64 : runs;
     if (runs > most) runs = most;
     const unsigned run = ((unsigned(vocab) + runs - 1) / runs + kVec - 1) / kVec * kVec;
@@ -289,8 +299,13 @@ extern "C" int lq_verify_drafts(const void* target, const void* draft, int dtype
     const Args a{target, draft, tokens, starts, uniforms, last, new_tokens, counts, unsigned(rows), unsigned(vocab), run,
                  reinterpret_cast<double*>(scratch.slabs), scratch.counters};
     const dim3 grid(runs, unsigned(batch));
-    const auto kernel = dtype == LQ_F32 ? (draft ? verify_drafts_kernel<float, true> : verify_drafts_kernel<float, false>)
-                                        : (draft ? verify_drafts_kernel<_Float16, true> : verify_drafts_kernel<_Float16, false>);
+    const auto of = [&](auto value, auto tiny) {
+        using T = decltype(value);
+        return draft ? verify_drafts_kernel<T, true, decltype(tiny)::value> : verify_drafts_kernel<T, false, decltype(tiny)::value>;
+    };
+    const bool tiny = unsigned(vocab) < kVec;
+    const auto kernel = dtype == LQ_F32 ? (tiny ? of(0.f, std::true_type{}) : of(0.f, std::false_type{}))
+                                        : (tiny ? of(_Float16(0.f), std::true_type{}) : of(_Float16(0.f), std::false_type{}));
     kernel<<<grid, kThreads, 0, st>>>(a);
     LQ_CHECK_LAUNCH("verify_drafts");
     return LQ_OK;
