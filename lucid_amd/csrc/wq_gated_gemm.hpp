@@ -154,6 +154,9 @@ struct Stage {
     static_assert(RING >= 2 && PER_WAVE * (RING - 2) <= 63, "");
 };
 
+// Row tiles of sums that a block has in LDS at once: all, or a half or a third, so that two blocks fit a CU.
+__host__ __device__ constexpr int epilogue_rows(int mt, int ct) { return mt * ct <= 8 ? mt : mt % 2 == 0 ? mt / 2 : mt / 3; }
+
 // s_waitcnt immediate for vmcnt <= n and every LDS read done
 constexpr int vmcnt_lds(int n) { return (n & 0xF) | ((n >> 4) << 14) | (0x7 << 4); }
 
@@ -340,23 +343,47 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                     for (int i = 0; i < MT; ++i) y[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(sums[i][part], b[order - part], y[j][i], 0, 0, 0);
         }
     }
-    __builtin_amdgcn_s_waitcnt(vmcnt_lds(0));  // the loads past the end have landed before the LDS is given up
-    // accumulator element r of a lane: row 4 * quarter + r, column lane % 16
+    // A wavefront's sums go through LDS, ROWS tiles at a time, so that a lane has four columns of a row and the activations stand in the code once: a block's
+    // first instructions come from memory (sigmoid of each accumulator by itself: 2048 x 11008 x 4096 float16 465 us, so 453; 2896 x 3864 x 128 51 and 44).
+    constexpr int ROWS = epilogue_rows(MT, CT), STRIDE = 16 * CT + 4, QUADS = 4 * CT;
+    __builtin_amdgcn_s_waitcnt(vmcnt_lds(0));  // the loads past the end have landed
+    __syncthreads();                           // and everybody has left the ring
+    float(*const s_y)[16 * ROWS][STRIDE] = reinterpret_cast<float(*)[16 * ROWS][STRIDE]>(smem) + 2 * wave;
+    const int col = lane % QUADS * 4, n = tn * kCols + wave * (16 * CT) + col;
+    float bias[2][4];
 #pragma unroll
-    for (int jj = 0; jj < CT; ++jj) {
-        const int n = tn * kCols + (wave * CT + jj) * 16 + ln;
-        if (n >= a.N) continue;
-        const float bg = a.w[0].bias ? a.w[0].bias[n] : 0.f, bu = a.w[1].bias ? a.w[1].bias[n] : 0.f;
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int e = 0; e < 4; ++e) bias[i][e] = a.w[i].bias ? a.w[i].bias[n + e < a.N ? n + e : a.N - 1] : 0.f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int m = (tm * MT + i) * 16 + q * 4 + r;
-                if (m >= a.M) continue;
-                const float f = PARTS == 1 ? 1.0f : p.unscale[m];
-                const float g = y[jj][i][r] * f + bg, v = y[CT + jj][i][r] * f + bu;
-                static_cast<T*>(a.out)[size_t(m) * a.N + n] = T(activate(a.act, g) * v);
+    for (int i0 = 0; i0 < MT; i0 += ROWS) {
+        // accumulator element r of a lane: row 4 * quarter + r, column lane % 16
+#pragma unroll
+        for (int j = 0; j < JT; ++j)
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s_y[j / CT][i * 16 + q * 4 + r][j % CT * 16 + ln] = y[j][i0 + i][r];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (of this wavefront alone)
+#pragma unroll 1
+        for (int row = lane / QUADS; row < 16 * ROWS; row += 64 / QUADS) {
+            const int m = (tm * MT + i0) * 16 + row;
+            if (m >= a.M) break;
+            const v4f g4 = *reinterpret_cast<const v4f*>(&s_y[0][row][col]), u4 = *reinterpret_cast<const v4f*>(&s_y[1][row][col]);
+            const float f = PARTS == 1 ? 1.0f : p.unscale[m];
+            T h[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = T(activate(a.act, g4[e] * f + bias[0][e]) * (u4[e] * f + bias[1][e]));
+            T* const to = static_cast<T*>(a.out) + size_t(m) * a.N + n;
+            if (n + 4 <= a.N) {
+                __builtin_memcpy(to, h, sizeof h);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n + e < a.N) to[e] = h[e];
             }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 }
 
@@ -385,7 +412,7 @@ int launch_gemm_tile(const Args& a, hipStream_t st) {
     gated_prepare_kernel<T, PARTS, BITS, CT><<<x_blocks + w_blocks, 256, 0, st>>>(a, p, x_blocks);
     LQ_CHECK_LAUNCH("quantized_gated_matmul");
     static DeviceOnce once;
-    constexpr int lds = S::RING * S::PIECES * kPiece;
+    constexpr int ring = S::RING * S::PIECES * kPiece, sums = 4 * 2 * 16 * epilogue_rows(MT, CT) * (16 * CT + 4) * 4, lds = ring > sums ? ring : sums;
     const auto kernel = gated_gemm_kernel<T, PARTS, BITS, GS, MT, CT>;
     if (const int rc = allow_dynamic_lds(once, reinterpret_cast<const void*>(kernel), lds)) return rc;
     kernel<<<unsigned(tiles_m) * unsigned(p.tiles_n), 256, lds, st>>>(a, p, tiles_m);

@@ -419,7 +419,7 @@ __global__ __launch_bounds__(64 * CG * SG) void gated_rows_kernel(Args a, RowsX 
     const int col = threadIdx.x % COLS, n = blockIdx.x * COLS + col;
     if (n >= a.N) return;
     const float bg = a.w[0].bias ? a.w[0].bias[n] : 0.f, bu = a.w[1].bias ? a.w[1].bias[n] : 0.f;
-#pragma unroll
+#pragma unroll 1  // (one copy of the activations: a block's first instructions come from memory)
     for (int j = 0; j < (16 * MT + ROWS - 1) / ROWS; ++j) {
         const int row = j * ROWS + threadIdx.x / COLS, m = m0 + row, t = row >> 4, from_lane = (col & 15) + 16 * ((row >> 2) & 3);
         if ((16 * MT % ROWS && row >= 16 * MT) || m >= a.M) return;
