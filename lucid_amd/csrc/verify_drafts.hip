@@ -9,7 +9,7 @@
 // in float64, where p - q is exact or nearly so and the order of the additions moves a border by some 1e-15.  Half-precision
 // sums would move one in a thousand draws.
 //
-// A block has a run of the vocabulary of one sequence; every block judges the drafts itself (two numbers each), so that it knows the row
+// A block has a run of the vocabulary of one sequence; every block checks the drafts itself (two numbers each), so that it knows the row
 // to read, and asks for 8192 of its probabilities at once, or 16 384.  Sums go to the last block that arrives, which finds the run, in it the piece of
 // 512 that a wavefront reads with one instruction, the lane and the token.  Each probability is read once, the run of the token twice.  Bound by
 // memory in the large (128 rows of 131 072 float16), by a chain of eight trips to memory in the small.
