@@ -64,7 +64,7 @@ def test_c_copy_refuses(args, error):
 
 
 @pytest.mark.parametrize("at,value,error", [
-    (1, None, ValueError), (2, -1, L.ShapeMismatch), (3, -1, L.ShapeMismatch), (4, None, ValueError), (5, 65, L.ShapeMismatch), (5, 1 << 40, L.ShapeMismatch),
+    (1, None, ValueError), (2, -1, L.ShapeMismatch), (3, -1, L.ShapeMismatch), (4, None, ValueError), (5, 1 << 31, L.ShapeMismatch), (5, 1 << 40, L.ShapeMismatch),
     (6, None, ValueError)])
 def test_c_compact_refuses(at, value, error):
     args = [C.byref(struct()), P, 4, 1, P, 64, P, None]
