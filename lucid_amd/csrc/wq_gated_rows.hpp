@@ -506,6 +506,7 @@ int by_tile(int tile, F&& f) {
 
 template <class T, int PARTS>
 int launch_rows_chunk(const Args& a, int bits, int tile, hipStream_t st) {
+    const auto lock = scratch_lock(st);
     RowsX rx{{static_cast<const _Float16*>(a.x), nullptr}, nullptr};
     if constexpr (PARTS == 2) {
         void* ws = nullptr;
@@ -549,7 +550,6 @@ int launch_rows(Args a, int bits, int tile, hipStream_t st) {
             LQ_CHECK_LAUNCH("quantized_gated_matmul");
             return LQ_OK;
         });
-    const auto lock = scratch_lock(st);
     // rows in chunks of whole tiles whose parts stay below 2^30 bytes
     const int M = a.M, most = int(std::clamp<size_t>((size_t(1) << 28) / a.K / 64 * 64, 64, 65535 * 16));
     for (int m0 = 0; m0 < M; m0 += a.M) {
