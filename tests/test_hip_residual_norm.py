@@ -97,6 +97,13 @@ def test_in_the_places_of_x_and_residual(types):
     assert np.array_equal(y, y2) and np.array_equal(r, r2)
 
 
+@pytest.mark.parametrize("cols", [5, 258, 1233, 4555, 9002, 20003])
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("types", [(np.float32, np.float32), (np.float16, np.float16), (np.float16, np.float32)])
+def test_ragged_rows_in_their_own_places(cols, post, types):
+    check(70, cols, layer=True, post=post, x_type=types[0], r_type=types[1], in_place=True)
+
+
 def test_rows_of_zeros_and_of_one_value():
     x, r = np.zeros((3, 700), np.float32), np.zeros((3, 700), np.float32)
     r[1], r[2] = 1e4, -3e-3

@@ -83,7 +83,7 @@ COUNTS = [[1], [6], [2, 1, 0, 5, 3], [0, 0], [0, 4, 0], [5] * 16, [300, 2], [1] 
 
 
 @pytest.mark.parametrize("counts", COUNTS)
-@pytest.mark.parametrize("vocab", [1, 7, 64, 1000])
+@pytest.mark.parametrize("vocab", [1, 7, 8, 9, 15, 64, 1000])
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])
 @pytest.mark.parametrize("given", [True, False])
 def test_sequences_of_all_kinds(counts, vocab, dtype, given):
