@@ -11,11 +11,12 @@ struct Choice {
     float us;
 };
 
-// The kernel and the tile that take the least time as rounds of blocks.  Of few rows a CU has one block, which takes 2.5 us (3.5: float32) beside its
+// The kernel and the tile that take the least time as rounds of blocks.  Of few rows a CU has one block, which takes 4 us (6: float32) beside its
 // stages of 64 k; many small blocks end sooner as long as they are one round (16 x 4096 x 4096, 4 bits, float16: 64, 32, 16 columns a block 16.7, 11.3,
-// 8.8 us; 16 x 11008 x 4096 18.1, 21.6, 20.5).  Of many rows a CU has two blocks, or one where a last round has no more than 256; what comes before and
-// behind, a launch that lays out the operands among it, takes 12 us.  us, few / many, 4 bits in groups of 128: 128 x 11008 x 4096 float16 64 / 66, 200
-// 95 / 93, 333 155 / 118, 512 x 4096 x 4096 63 / 66, 1024 x 2816 x 1024 33 / 40; 65 x 11008 x 4096 float32 82 / 82, 128 94 / 88, 512 x 4096 x 4096 127 / 98.
+// 8.8 us; 16 x 11008 x 4096 18.1, 21.6, 20.5).  Of many rows a CU has two blocks, which take 9 us (14) beside their stages, or one (4, 7) where a last round
+// has no more than 256; the launch before them and what is once 12 us.  us, few / many, 4 bits, float16: 128 x 11008 x 4096 64 / 66, 200 96 / 89, 512
+// 190 / 137, 1024 x 2816 x 1024 33 / 37, 4056 x 1088 x 256 32 / 34, 435 x 9023 x 256 26 / 23, 1024 x 1024 x 14336 107 / 186; float32: 65 x 11008 x 4096
+// 82 / 82, 128 94 / 88, 512 x 4096 x 4096 127 / 98, 435 x 9023 x 320 46 / 33.
 template <int PARTS, int BITS>
 Choice choose(const gated::Args& a) {
     constexpr bool half = PARTS == 1;
@@ -24,14 +25,15 @@ Choice choose(const gated::Args& a) {
     Choice best{true, 0, 3.4e38f};
     for (size_t t = 0; t < gated::kRowsTiles<PARTS>.size(); ++t) {
         const gated::RowsTile& tile = gated::kRowsTiles<PARTS>[t];
-        const float us = (half ? 1.f : 3.5f) + float((blocks_of(16 * tile.mt, 16 * tile.cg) + 255) / 256) * ((half ? 2.5f : 3.5f) + stages * tile.us);
+        const float us = (half ? -0.5f : 1.f) + float((blocks_of(16 * tile.mt, 16 * tile.cg) + 255) / 256) * ((half ? 4.f : 6.f) + stages * tile.us);
         if (us < best.us) best = Choice{true, int(t), us};
     }
     if (size_t(a.N) * a.K * BITS / 8 >= 0x7fffffffull) return best;  // (offsets of codes are 32-bit in the kernel of many rows)
     for (size_t t = 0; t < gated::kGemmTiles<PARTS, BITS>.size(); ++t) {
         const gated::GemmTile& tile = gated::kGemmTiles<PARTS, BITS>[t];
         const int64_t blocks = blocks_of(16 * tile.mt, 64 * tile.ct), rest = blocks % 512;
-        const float us = 12.f + stages * (float(blocks / 512) * tile.two + (rest == 0 ? 0.f : rest <= 256 ? tile.one : tile.two));
+        const float one = (half ? 4.f : 7.f) + stages * tile.one, two = (half ? 9.f : 14.f) + stages * tile.two;
+        const float us = 12.f + float(blocks / 512) * two + (rest == 0 ? 0.f : rest <= 256 ? one : two);
         if (us < best.us) best = Choice{false, int(t), us};
     }
     return best;

@@ -111,19 +111,19 @@ int launch_rows_f16(const Args& a, int bits, int tile, hipStream_t st);
 int launch_rows_f32(const Args& a, int bits, int tile, hipStream_t st);
 
 // Many rows (wq_gated_gemm.hpp): 16 mt rows x 64 ct columns a block, and what a stage of 64 k takes (us) when a CU has one block, or two: measured
-// with 4-bit codes in groups of 128 at K = 4096, N = 11008 and 64 to 2048 rows.  (8-bit codes of wide blocks leave no room for a ring of stages.)
+// with 4-bit codes in groups of 128 at K = 4096, N = 11008 and 64 to 2048 rows, without what a round takes besides.  (8-bit codes of wide blocks leave no room for a ring of stages.)
 struct GemmTile {
     int mt, ct;
     float one, two;
 };
 template <int PARTS, int BITS>
-constexpr std::array<GemmTile, 3> kGemmTiles = {{{4, 2, 0.95f, 1.25f}, {6, 2, 1.15f, 1.72f}, {3, 4, 1.32f, 1.95f}}};
+constexpr std::array<GemmTile, 3> kGemmTiles = {{{4, 2, 0.89f, 1.11f}, {6, 2, 1.09f, 1.58f}, {3, 4, 1.26f, 1.81f}}};
 template <>
-inline constexpr std::array<GemmTile, 2> kGemmTiles<1, 8> = {{{4, 2, 0.95f, 1.25f}, {6, 2, 1.15f, 1.72f}}};
+inline constexpr std::array<GemmTile, 2> kGemmTiles<1, 8> = {{{4, 2, 0.89f, 1.11f}, {6, 2, 1.09f, 1.58f}}};
 template <>
-inline constexpr std::array<GemmTile, 4> kGemmTiles<2, 4> = {{{2, 2, 0.95f, 1.30f}, {4, 2, 1.35f, 1.98f}, {2, 4, 1.40f, 2.35f}, {3, 4, 1.70f, 2.95f}}};
+inline constexpr std::array<GemmTile, 4> kGemmTiles<2, 4> = {{{2, 2, 0.85f, 1.08f}, {4, 2, 1.25f, 1.76f}, {2, 4, 1.30f, 2.13f}, {3, 4, 1.60f, 2.73f}}};
 template <>
-inline constexpr std::array<GemmTile, 3> kGemmTiles<2, 8> = {{{2, 2, 0.95f, 1.30f}, {3, 2, 1.20f, 1.58f}, {4, 2, 1.35f, 1.98f}}};
+inline constexpr std::array<GemmTile, 3> kGemmTiles<2, 8> = {{{2, 2, 0.85f, 1.08f}, {3, 2, 1.10f, 1.36f}, {4, 2, 1.25f, 1.76f}}};
 // By type and bits, `tile` of these; weights below 2 GiB.
 int launch_gemm_f16_4(const Args& a, int tile, hipStream_t st);
 int launch_gemm_f16_8(const Args& a, int tile, hipStream_t st);

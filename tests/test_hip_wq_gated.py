@@ -69,7 +69,7 @@ def test_exact_on_exact_numbers(M, N, K, gs, bits, dtype):
 
 # few rows of columns that fill the device with 16, 32 or 64 a block; more rows than that takes, in tiles of every size
 WIDE = [(16, 4090), (16, 5630), (16, 11001), (32, 4000), (31, 8010), (32, 11008), (63, 11001), (325, 11009), (97, 8690), (195, 8850), (227, 8200), (325, 8250), (670, 4475), (685, 8410),
-        (1219, 2311)]
+        (1219, 2311), (195, 12336), (193, 13067), (258, 9902), (132, 10968), (482, 11873)]
 
 
 def some_columns(N):
@@ -122,7 +122,8 @@ def test_against_float64(M, N, K, gs, bits, dtype, act):
     assert (abs(y - want) <= e + (abs(want) + e) * info.eps / 2 + info.tiny * info.eps).all()
 
 
-@pytest.mark.parametrize("M,N,K,gs", [(33, 11008, 1152, 32), (195, 8850, 1024, 64), (333, 8200, 1152, 128)])
+@pytest.mark.parametrize("M,N,K,gs", [(33, 11008, 1152, 32), (195, 8850, 1024, 64), (333, 8200, 1152, 128), (412, 4875, 1056, 32), (398, 4946, 1088, 64),
+                                      (415, 4941, 1152, 128)])
 @pytest.mark.parametrize("bits,dtype", [(4, np.float32), (8, np.float32), (4, np.float16), (8, np.float16)])
 def test_many_columns_against_float64(M, N, K, gs, bits, dtype):
     rng = np.random.default_rng(M + bits)
