@@ -120,6 +120,15 @@ def test_c_residual_norm_refuses(kw, error):
         _C.call("lq_residual_norm", norm_args(**kw), None)
 
 
+@pytest.mark.parametrize("kw", [
+    dict(y=0x1004), dict(y=0x1000, r_out=0x1000), dict(y=0x101c, r_out=0x3000), dict(y=0x4000, r_out=0x2020), dict(y=0x4000, r_out=0x403f), dict(y=0x3000, r_out=0x3000),
+    dict(y=0x1000, r_out=0x2000, x_dtype=_C.F16, r=0x1000), dict(y=0x4000, r_out=0x1000, x_dtype=_C.F16), dict(y=0x5010, r_out=0x2000, gate=0x5000, gate_rows=2),
+    dict(y=0x5000, r_out=0x2000, gate=0x5000, gate_rows=1)])
+def test_c_residual_norm_refuses_results_on_what_is_read(kw):
+    with pytest.raises(ValueError, match="residual_norm: a result lies"):
+        _C.call("lq_residual_norm", norm_args(**{"x": 0x1000, "r": 0x2000, "r_out": 0x2000, **kw}), None)
+
+
 def test_c_entries_refuse_no_arguments():
     with pytest.raises(ValueError, match="residual_norm"):
         _C.call("lq_residual_norm", None, None)
