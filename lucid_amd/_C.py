@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "liblucid_hip.so")
@@ -283,7 +284,9 @@ class ResidualNormArgs(C.Structure):
     ]
 
 
-_SIGNATURES["lq_residual_norm"] = [C.POINTER(ResidualNormArgs), _vp]
+# (its fields as bytes in a quarter of the time that an object of the class takes: pointers as numbers, 0 for NULL)
+RESIDUAL_NORM_ARGS = struct.Struct("@10P2q5if0P")
+_SIGNATURES["lq_residual_norm"] = [_vp, _vp]
 _SIGNATURES["lq_verify_drafts"] = [_vp, _vp, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp]
 
 
@@ -296,7 +299,8 @@ class WqGatedArgs(C.Structure):
     ]
 
 
-_SIGNATURES["lq_wq_gated_matmul"] = [C.POINTER(WqGatedArgs), _vp]
+WQ_GATED_ARGS = struct.Struct("@10P7i0P")  # (see RESIDUAL_NORM_ARGS)
+_SIGNATURES["lq_wq_gated_matmul"] = [_vp, _vp]
 _SIGNATURES["lq_lstm_sequence_pays"] = [_i] * 3 + [C.POINTER(_i)]
 _SIGNATURES["lq_lstm_fused_layers"] = [_i] * 6 + [C.POINTER(_i)]
 _SIGNATURES["lq_lstm_sequence_f32"] = [C.POINTER(LstmArgs), _vp]

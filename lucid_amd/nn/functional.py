@@ -6,7 +6,6 @@ kernel; inputs and outputs are float32 tensors on the ``hip`` device.
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 from .. import _C
@@ -213,29 +212,29 @@ def _residual_norm(name, x, residual, weight, bias, norm, eps, post, post_weight
     gate_rows = 0
     if residual is not None:
         _check_rows(name, "residual", residual, x.shape)
-        if residual.dtype != x.dtype and residual.dtype != T.float32:
+        if residual.dtype is not x.dtype and residual.dtype is not T.float32:
             raise _C.DtypeMismatch(f"{name}: x is {x.dtype}, residual {residual.dtype} (x's type or float32)")
     if gate is not None:
         if not isinstance(gate, Tensor) or gate.ndim < 1 or gate.shape[-1] != cols:
             raise _C.ShapeMismatch(f"{name}: gate is a (..., {cols}) tensor")
         _check_rows(name, "gate", gate, gate.shape)
-        if gate.dtype != x.dtype:
+        if gate.dtype is not x.dtype:
             raise _C.DtypeMismatch(f"{name}: x is {x.dtype}, gate {gate.dtype}")
         gate_rows = gate.numel // cols if cols else 0
         if rows and (gate_rows == 0 or rows % gate_rows):
             raise _C.ShapeMismatch(f"{name}: a gate of {gate_rows} rows for {rows}")
-    scale = None if scale is None else _vector(name, "scale", scale, cols)
-    weight = None if weight is None else _vector(name, "weight", weight, cols)
-    bias = None if bias is None else _vector(name, "bias", bias, cols)
-    post_weight = None if post_weight is None else _vector(name, "post_weight", post_weight, cols)
-    post_bias = None if post_bias is None else _vector(name, "post_bias", post_bias, cols)
+    scale = 0 if scale is None else _vector(name, "scale", scale, cols)
+    weight = 0 if weight is None else _vector(name, "weight", weight, cols)
+    bias = 0 if bias is None else _vector(name, "bias", bias, cols)
+    post_weight = 0 if post_weight is None else _vector(name, "post_weight", post_weight, cols)
+    post_bias = 0 if post_bias is None else _vector(name, "post_bias", post_bias, cols)
     if out is not None:
         _check_rows(name, "out", out, x.shape)
-        if out.dtype != x.dtype:
+        if out.dtype is not x.dtype:
             raise _C.DtypeMismatch(f"{name}: x is {x.dtype}, out {out.dtype}")
     if residual_out is not None:
         _check_rows(name, "residual_out", residual_out, x.shape)
-        if residual_out.dtype != residual.dtype:
+        if residual_out.dtype is not residual.dtype:
             raise _C.DtypeMismatch(f"{name}: residual is {residual.dtype}, residual_out {residual_out.dtype}")
         if out is not None and residual_out.data_ptr == out.data_ptr and x.numel:
             raise ValueError(f"{name}: out and residual_out are one tensor")
@@ -243,12 +242,13 @@ def _residual_norm(name, x, residual, weight, bias, norm, eps, post, post_weight
         out = Tensor.empty(x.shape, x.dtype, "hip")
     if residual_out is None and residual is not None:
         residual_out = Tensor.empty(x.shape, residual.dtype, "hip")
-    args = _C.ResidualNormArgs(
-        x.data_ptr, residual.data_ptr if residual is not None else None, gate.data_ptr if rows and gate is not None else None, scale, weight, bias,
-        post_weight, post_bias, out.data_ptr,
-        residual_out.data_ptr if residual is not None else None, rows, gate_rows if rows else 0, cols, x.dtype.code,
+    if cols > 0x7fffffff:
+        raise _C.ShapeMismatch(f"{name}: rows of {cols}")
+    args = _C.RESIDUAL_NORM_ARGS.pack(
+        x.data_ptr, residual.data_ptr if residual is not None else 0, gate.data_ptr if rows and gate is not None else 0, scale, weight, bias,
+        post_weight, post_bias, out.data_ptr, residual_out.data_ptr if residual is not None else 0, rows, gate_rows if rows else 0, cols, x.dtype.code,
         x.dtype.code if residual is None else residual.dtype.code, _NORMS[norm], 1 if post else 0, eps)
-    _C.call("lq_residual_norm", ctypes.byref(args), None)
+    _C.call("lq_residual_norm", args, None)
     _written(out)
     if residual is not None:
         _written(residual_out)

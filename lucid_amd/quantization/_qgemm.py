@@ -8,8 +8,6 @@ The packed tensor is int32-tagged (Lucid has no uint32 dtype either,
 
 from __future__ import annotations
 
-import ctypes
-
 from .. import _C
 from .. import _tensor as T
 from .._tensor import Tensor
@@ -84,44 +82,45 @@ def quantized_gated_matmul(x: Tensor, gate: tuple[Tensor, Tensor, Tensor], up: t
     if activation not in _GATES:
         raise ValueError(f"{name}: activation {activation!r}; one of {', '.join(_GATES)}")
     _check(name, x, *gate, *up)
-    if x.dtype != T.float32 and x.dtype != T.float16:
-        raise _C.DtypeMismatch(f"{name} expects a float32 or float16 activation, got {x.dtype}")
+    dtype = x.dtype
+    if dtype is not T.float16 and dtype is not T.float32:
+        raise _C.DtypeMismatch(f"{name} expects a float32 or float16 activation, got {dtype}")
     if bits not in (4, 8) or group_size not in (32, 64, 128):
         raise ValueError(f"{name}: bits {bits}, group_size {group_size}; 4 or 8, and 32, 64 or 128")
-    if gate[0].ndim != 2:
-        raise _C.ShapeMismatch(f"{name}: a packed weight is 2-d, got {gate[0].shape}")
-    N = gate[0].shape[0]
-    K = gate[0].shape[1] * 32 // bits
+    shape = gate[0].shape
+    if len(shape) != 2:
+        raise _C.ShapeMismatch(f"{name}: a packed weight is 2-d, got {shape}")
+    N, K = shape[0], shape[1] * 32 // bits
+    groups = (N, K // group_size)
     for what, (packed, scales, biases), bias in (("gate", gate, gate_bias), ("up", up, up_bias)):
-        if packed.shape != gate[0].shape or K % group_size or scales.shape != (N, K // group_size) or biases.shape != scales.shape:
+        if packed.shape != shape or K % group_size or scales.shape != groups or biases.shape != groups:
             raise _C.ShapeMismatch(f"{name}: {what} is packed {packed.shape}, scales {scales.shape}, biases {biases.shape} in groups of {group_size}; "
-                                   f"gate is packed {gate[0].shape}")
-        if packed.dtype != T.int32 or scales.dtype != T.float32 or biases.dtype != T.float32:
+                                   f"gate is packed {shape}")
+        if packed.dtype is not T.int32 or scales.dtype is not T.float32 or biases.dtype is not T.float32:
             raise _C.DtypeMismatch(f"{name}: {what} is int32, float32 and float32, got {packed.dtype}, {scales.dtype} and {biases.dtype}")
         if bias is not None:
             _check(name, bias)
-            if bias.dtype != T.float32:
+            if bias.dtype is not T.float32:
                 raise _C.DtypeMismatch(f"{name}: {what}_bias is float32, got {bias.dtype}")
             if bias.shape != (N,):
                 raise _C.ShapeMismatch(f"{name}: {what}_bias has shape {bias.shape}, expected {(N,)}")
-    if x.ndim < 1 or x.shape[-1] != K:
+    if not x.shape or x.shape[-1] != K:
         raise _C.ShapeMismatch(f"{name}: activation {x.shape} against packed ({N}, {K}) weights")
     shape = (*x.shape[:-1], N)
     if out is None:
-        out = Tensor.empty(shape, x.dtype, "hip")
+        out = Tensor.empty(shape, dtype, "hip")
     else:
         _check(name, out)
-        if out.dtype != x.dtype:
-            raise _C.DtypeMismatch(f"{name}: x is {x.dtype}, out {out.dtype}")
+        if out.dtype is not dtype:
+            raise _C.DtypeMismatch(f"{name}: x is {dtype}, out {out.dtype}")
         if out.shape != shape:
             raise _C.ShapeMismatch(f"{name}: out has shape {out.shape}, expected {shape}")
     M = x.numel // K if K else 0
-    if max(M, N, K) > 0x7fffffff:  # (ctypes takes the low 32 bits of a longer int)
+    if max(M, N, K) > 0x7fffffff:  # (more than an int says)
         raise _C.ShapeMismatch(f"{name}: {M} x {N} x {K}")
-    args = _C.WqGatedArgs(x.data_ptr, out.data_ptr, (gate[0].data_ptr, up[0].data_ptr), (gate[1].data_ptr, up[1].data_ptr),
-                          (gate[2].data_ptr, up[2].data_ptr),
-                          (None if gate_bias is None else gate_bias.data_ptr, None if up_bias is None else up_bias.data_ptr), M, N, K, group_size, bits,
-                          _GATES[activation], x.dtype.code)
-    _C.call("lq_wq_gated_matmul", ctypes.byref(args), None)
+    args = _C.WQ_GATED_ARGS.pack(x.data_ptr, out.data_ptr, gate[0].data_ptr, up[0].data_ptr, gate[1].data_ptr, up[1].data_ptr, gate[2].data_ptr,
+                                 up[2].data_ptr, 0 if gate_bias is None else gate_bias.data_ptr, 0 if up_bias is None else up_bias.data_ptr, M, N, K,
+                                 group_size, bits, _GATES[activation], dtype.code)
+    _C.call("lq_wq_gated_matmul", args, None)
     out._grid = out._range = None
     return out

@@ -239,3 +239,15 @@ def test_gated_module_refuses():
             nnq.QuantizedGatedLinearMLX(*args, **kw)
     with pytest.raises(L.ShapeMismatch):
         nnq.QuantizedGatedLinearMLX.from_float(nn.Linear(64, 8), nn.Linear(64, 9))
+
+
+def test_arguments_as_bytes_are_the_structs():
+    """What the wrappers pack lies where the header's structs have it."""
+    for cls, packer in ((_C.ResidualNormArgs, _C.RESIDUAL_NORM_ARGS), (_C.WqGatedArgs, _C.WQ_GATED_ARGS)):
+        n = len(packer.unpack(bytes(packer.size)))
+        values = [i + 1 for i in range(n)]
+        got, flat = cls.from_buffer_copy(packer.pack(*values)), []
+        for field, _ in cls._fields_:
+            v = getattr(got, field)
+            flat += list(v) if isinstance(v, C.Array) else [v]
+        assert C.sizeof(cls) == packer.size and flat == values
