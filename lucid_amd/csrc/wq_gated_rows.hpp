@@ -11,9 +11,9 @@
 // x as it enters the matrix instructions: float16 as it is; a float32 row times the power of two that brings its largest value below 2^15,
 // as two float16, hi = x rounded, lo = x - hi rounded: 22 bits, or 2^-39 of the largest value.
 //
-// gated_few_kernel, up to 4 rows that leave room for two blocks a CU: a block has 16 columns, its four wavefronts every fourth step each.  It brings x into LDS itself, while
-// its first weights are under way, and nothing else is shared, so that there is no barrier in the loop.  A row of x lies on every fourth row of the
-// instruction: a lane then has one element of each result.
+// gated_few_kernel, up to 4 rows that leave room for two blocks a CU: a block has 16 columns, its four wavefronts every fourth step each.  It brings x
+// into LDS itself, while its first weights are under way, and beside that shares the tables alone, so that a barrier comes once a table.  A row of x
+// lies on every fourth row of the instruction: a lane then has one element of each result.
 //
 // gated_rows_kernel: a block of eight wavefronts has CG times 16 columns, a wavefront 16 of them and every SG-th step (CG SG = 8), so that CG share
 // an x (16 rows of float32 are as many bytes as the codes of 16 columns of both weights in 8 bits, and come from the L2 for every block again:
