@@ -4,8 +4,8 @@
 //   g, u [m, n] = sum over groups of  s[n, group] * (sum_{k in group} c[n, k] x[m, k])  +  b[n, group] * (sum_{k in group} x[m, k])
 //
 // for the weights of the gate and of the way up.  Codes enter the matrix instructions as the whole numbers c - 2^(bits-1) that they are
-// (the rest of the code goes to b), so that nothing of a weight is rounded: scales follow in float32, on the sums of a group.  float16 x
-// enters as it is; a float32 row times a power of two as two float16 of 22 bits together.
+// (the rest of the code goes to b, and b + 2^(bits-1) s is rounded to float32), so that nothing else of a weight is rounded: scales follow in float32, on
+// the sums of a group.  float16 x enters as it is; a float32 row times a power of two as two float16 of 22 bits together.
 #pragma once
 #include <array>
 

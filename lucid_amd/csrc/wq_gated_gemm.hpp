@@ -9,8 +9,9 @@
 // that no code is turned into float16 twice in a block.  What a stage of 64 k needs comes from memory straight into LDS in pieces of
 // 1 KiB per wavefront and instruction, in a ring of stages: every wavefront issues as many loads per stage, so that "stage s has arrived"
 // is a count of outstanding loads.  The products of a group (at most 64 k) go to accumulators of their own, and from there with their scale to
-// the sums.  The terms of b come last, as a product over the groups of three bfloat16 parts of each side, which leaves 2^-24 of them; of a
-// float16 x two parts, 2^-16, a sixteenth of what the result rounds.
+// the sums.  The terms of b come last, as a product over the groups of three bfloat16 parts of each side, which leaves 2^-24 of them: whatever
+// x's type, as they cancel against the codes' products wherever a group's middle is far from zero (two parts, 2^-16, left results of float16 off by ten
+// steps and more behind a weight of one among small ones).
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -25,7 +26,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));  // (see wq_gated_ro
 
 constexpr int kPiece = 1024;  // bytes one wavefront moves into LDS with one instruction
 
-__host__ __device__ constexpr int sum_parts(int parts) { return parts == 1 ? 2 : 3; }
+constexpr int kSumParts = 3;
 
 struct Prepared {
     char* x;          // [stage][row tile][2][part] pieces
@@ -55,7 +56,7 @@ __global__ __launch_bounds__(256) void gated_row_scale_kernel(const float* __res
 // Two kinds of blocks.  The first `x_blocks`: 16 rows x 128 k, a thread has eight k.  The others: 64 columns of a weight, a wavefront eight groups.
 template <class T, int PARTS, int BITS, int CT>
 __global__ __launch_bounds__(256) void gated_prepare_kernel(Args a, Prepared p, unsigned x_blocks) {
-    constexpr int SP = sum_parts(PARTS), kCols = 64 * CT;
+    constexpr int SP = kSumParts, kCols = 64 * CT;
     const int gs = 1 << a.gs_shift;
     if (blockIdx.x >= x_blocks) {
         const unsigned i = blockIdx.x - x_blocks, across = unsigned(p.tiles_n) * (kCols / 64), which = (i / across) & 1, lane = threadIdx.x & 63;
@@ -163,7 +164,7 @@ constexpr int vmcnt_lds(int n) { return (n & 0xF) | ((n >> 4) << 14) | (0x7 << 4
 template <class T, int PARTS, int BITS, int GS, int MT, int CT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void gated_gemm_kernel(Args a, Prepared p, int tiles_m) {
     using S = Stage<PARTS, BITS, GS, MT, CT>;
-    constexpr int SP = sum_parts(PARTS), kCols = 64 * CT, JT = 2 * CT;  // column tiles of a wavefront: the gate's, then the other's
+    constexpr int SP = kSumParts, kCols = 64 * CT, JT = 2 * CT;  // column tiles of a wavefront: the gate's, then the other's
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ln = lane & 15, q = lane >> 4;
     // every XCD gets a contiguous range of tiles, row tiles first: its L2 then reads a weight row once
@@ -319,7 +320,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int e = 0; e < S::SEGS; ++e) f_last[e] = f[JT - 1][e];
     }
     scale_sums(JT - 1, f_last, acc[1]);
-    // the terms of b: hi hi, then what is 2^-8 of it, then (three parts) 2^-16
+    // the terms of b, the small ones first: those of 2^-16 of hi hi, of 2^-8, itself
 #pragma unroll 1
     for (int g = 0; g < p.group_steps; ++g) {
         v8bf sums[MT][SP];
@@ -390,7 +391,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 template <class T, int PARTS, int BITS, int GS, int MT, int CT>
 int launch_gemm_tile(const Args& a, hipStream_t st) {
     using S = Stage<PARTS, BITS, GS, MT, CT>;
-    constexpr int SP = sum_parts(PARTS), kCols = 64 * CT;
+    constexpr int SP = kSumParts, kCols = 64 * CT;
     Prepared p;
     const int tiles_m = (a.M + 16 * MT - 1) / (16 * MT);
     p.mtiles = tiles_m * MT, p.stages = (a.K + 63) / 64, p.group_steps = (a.K / GS + 31) / 32, p.tiles_n = (a.N + kCols - 1) / kCols;
