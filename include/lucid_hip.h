@@ -525,7 +525,8 @@ int lq_kv_cache_compact(const lq_kv_cache* cache, const int32_t* page_table, int
  * No counterpart in Lucid.  The residual connection between two blocks with the norms beside it, over rows of `cols` values (at most
  * 32768):  t = post(x), or x when post == 0;  r' = r + gate * scale * t;  y = pre(r').  Norms: v / sqrt(mean(v^2) + eps) * weight + bias,
  * when layer == 1 of v - mean(v) in v's place (lucid/_C/backend/cpu/Norm.cpp:35-65).  Everything float32 in between; y is made from r'
- * before that is rounded to its type. */
+ * before that is rounded to its type.  y and r_out may each lie in the place of x, r or a gate of as many rows, where the types are as wide; on nothing
+ * else that is read, and not on each other. */
 typedef struct lq_residual_norm_args {
     const void* x;            /* [rows, cols], LQ_F32 or LQ_F16                      */
     const void* r;            /* [rows, cols] of r_dtype, or NULL: zeros             */

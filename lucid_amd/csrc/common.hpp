@@ -130,6 +130,16 @@ struct FastDiv {
     __device__ __forceinline__ unsigned operator()(unsigned n) const { return unsigned((uint64_t(n) * m) >> shift); }
 };
 
+// What an argument takes of memory, and whether two of them (NULL: none) have nothing in common.
+struct Span {
+    const void* at;
+    size_t bytes;
+};
+inline bool apart(const Span& a, const Span& b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+    return !x || !y || a.bytes == 0 || b.bytes == 0 || x + a.bytes <= y || y + b.bytes <= x;
+}
+
 __host__ __device__ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // GELU in its erf form, 0.5 x (1 + erf(x / sqrt 2)) (lucid/nn/functional/activations.py:219), erf by Abramowitz & Stegun

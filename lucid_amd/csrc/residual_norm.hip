@@ -232,21 +232,17 @@ extern "C" int lq_residual_norm(const lq_residual_norm_args* n, lq_stream stream
                (long long)n->rows);
     LQ_REQUIRE(n->cols <= kMaxCols, LQ_ERR_NOT_IMPLEMENTED, "residual_norm: rows of %d; at most %d are built", n->cols, kMaxCols);
     LQ_REQUIRE(n->rows < int64_t(1) << 31, LQ_ERR_SHAPE, "residual_norm: %lld rows", (long long)n->rows);
-    // a result is read from where it goes by the lane that has it, so it may lie in its operand's place, and nowhere else on what is read
-    struct Span {
-        const void* at;
-        size_t bytes;
-    };
+    // a row's value is read by the lane that puts a result there, before it does, so a result may lie in such an operand's place, and nowhere else on what is
+    // read: every row reads the vectors, and those of the second norm after r' is written
     const size_t values = size_t(n->rows) * n->cols, x_item = n->x_dtype == LQ_F16 ? 2 : 4, r_item = n->r_dtype == LQ_F16 ? 2 : 4;
     const Span x{n->x, values * x_item}, r{n->r, values * r_item}, gate{n->gate, size_t(n->gate_rows) * n->cols * x_item}, y{n->y, values * x_item},
         r_out{n->r_out, values * r_item};
-    const auto apart = [](const Span& to, const Span& from, bool place) {
-        const uintptr_t t = reinterpret_cast<uintptr_t>(to.at), f = reinterpret_cast<uintptr_t>(from.at);
-        return !t || !f || t + to.bytes <= f || f + from.bytes <= t || (place && t == f && to.bytes == from.bytes);
-    };
-    LQ_REQUIRE(apart(y, x, true) && apart(y, r, true) && apart(y, gate, true) && apart(y, r_out, false) && apart(r_out, x, true) && apart(r_out, r, true) &&
-                   apart(r_out, gate, true),
-               LQ_ERR_VALUE, "residual_norm: a result lies on what is read, but not in its place, or on the other result");
+    bool sound = apart(y, r_out);
+    for (const Span& to : {y, r_out}) {
+        for (const Span& from : {x, r, gate}) sound = sound && (apart(to, from) || (to.at == from.at && to.bytes == from.bytes));
+        for (const float* v : {n->scale, n->weight, n->bias, n->post_weight, n->post_bias}) sound = sound && apart(to, Span{v, size_t(n->cols) * sizeof(float)});
+    }
+    LQ_REQUIRE(sound, LQ_ERR_VALUE, "residual_norm: a result lies on what is read, but not in its place, or on the other result");
     Args a;
     a.x = n->x, a.r = n->r, a.gate = n->gate, a.scale = n->scale;
     a.pre = Norm{n->weight, n->bias}, a.post = Norm{n->post_weight, n->post_bias};

@@ -277,7 +277,7 @@ def residual_norm(x: Tensor, residual: Tensor, weight: Tensor | None = None, bia
     bias``, or ``"layer"``, the same of ``v - mean(v)``.  ``gate`` ``(..., features)``, of ``x``'s type, has a row for each of equal runs of
     ``x``'s rows: one for all, one for each sequence of a batch, one for each token.  ``scale``, the weights and biases are float32
     ``(features,)``.  In between everything is float32, and ``y`` is made from ``r`` before that is rounded.  At most 32768 features.
-    ``out`` and ``residual_out`` take the results; they may be ``x`` and ``residual``."""
+    ``out`` and ``residual_out`` take the results; they may be ``x`` and ``residual``, and lie on nothing else that is read."""
     if residual is None:
         raise _C.ShapeMismatch("residual_norm: residual is a tensor of x's shape")
     return _residual_norm("residual_norm", x, residual, weight, bias, norm, eps, post, post_weight, post_bias, gate, scale, out, residual_out)
