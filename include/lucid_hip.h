@@ -554,7 +554,8 @@ int lq_residual_norm(const lq_residual_norm_args* args, lq_stream stream);
  * refused (draft NULL: from p without x), from p of the last row where none did, or where nothing of p - q is positive: the lowest
  * token of positive weight at which the weights' running sum passes last[b] times their sum, in float64 (the last of positive weight if
  * none does; -1 if there is none).  Weights that are not positive and finite count as 0.  new_tokens (int32 [rows]): in a sequence's
- * rows its new tokens, then -1; rows of no sequence stay.  counts (int32 [batch]): how many; 0 of an empty sequence.  At most
+ * rows its new tokens, then -1; rows of no sequence stay.  counts (int32 [batch]): how many; 0 of an empty sequence.  The results lie apart
+ * from each other and from all that is read.  At most
  * 65535 sequences, 2^24 tokens.  Takes scratch of the stream. */
 int lq_verify_drafts(const void* target, const void* draft, int dtype, int rows, int vocab, const int32_t* tokens, const int32_t* starts,
                      int batch, const float* uniforms, const float* last, int32_t* new_tokens, int32_t* counts, lq_stream stream);

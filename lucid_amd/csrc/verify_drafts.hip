@@ -281,8 +281,16 @@ extern "C" int lq_verify_drafts(const void* target, const void* draft, int dtype
     LQ_REQUIRE(vocab >= 1 && vocab <= 1 << 24, LQ_ERR_SHAPE, "verify_drafts: a vocabulary of %d tokens; 1 to 2^24", vocab);
     if (batch == 0) return LQ_OK;
     LQ_REQUIRE(starts && last && counts, LQ_ERR_VALUE, "verify_drafts: starts, last or counts is NULL");
-    LQ_REQUIRE(new_tokens != tokens || !tokens, LQ_ERR_VALUE, "verify_drafts: the new tokens cannot take the drafted ones' place");
     LQ_REQUIRE(rows == 0 || (target && tokens && uniforms && new_tokens), LQ_ERR_VALUE, "verify_drafts: a NULL pointer");
+    // a sequence's last block writes while other sequences' blocks still read
+    const size_t n = size_t(rows), seqs = size_t(batch), probabilities = n * size_t(vocab) * (dtype == LQ_F16 ? 2 : 4);
+    const Span results[2] = {{new_tokens, n * 4}, {counts, seqs * 4}};
+    bool sound = apart(results[0], results[1]);
+    for (const Span& to : results)
+        for (const Span& from : {Span{target, probabilities}, Span{draft, probabilities}, Span{tokens, n * 4}, Span{starts, (seqs + 1) * 4}, Span{uniforms, n * 4},
+                                 Span{last, seqs * 4}})
+            sound = sound && apart(to, from);
+    LQ_REQUIRE(sound, LQ_ERR_VALUE, "verify_drafts: a result lies on what is read, or on the other result");
     // As many blocks as are resident, 8192 tokens at least each: what a block asks for at once, where one that is alone need not wait for others; 64 of
     // a sequence at most.  (16 x 131 072 float32 22 us of 2048 tokens, 13.2 of 8192; 16 x 32 000 12.5 and 11.1.  128 rows of 131 072
     // float16: 8 blocks a sequence that ask for all of their run at once 23.5 us, 12 and 16 of smaller runs 26 and 24.5, in rounds of 8192 tokens 29.)

@@ -301,7 +301,8 @@ def verify_drafts(target: Tensor, tokens: Tensor, starts: Tensor, uniforms: Tens
 
     ``new_tokens`` int32 ``(rows,)`` has a sequence's new tokens from ``starts[b]`` on and -1 behind them; ``counts`` int32 ``(batch,)`` says how many
     they are, at least 1, and 0 of a sequence without rows.  The cache then holds ``counts[b] - 1`` of the drafted tokens' rows.
-    Rows of no sequence (a padded batch) are left as they are in ``out``, which takes the results."""
+    Rows of no sequence (a padded batch) are left as they are in ``out``, which takes the results: two tensors that share nothing with each other or
+    with what is read."""
     if not isinstance(target, Tensor) or target.ndim != 2:
         raise _C.ShapeMismatch("verify_drafts: target is a (rows, vocab) tensor")
     rows, vocab = target.shape

@@ -35,3 +35,41 @@ def test_residual_norm_of_one_row_refuses_results_in_a_vectors_place(vector, res
 def test_rms_norm_refuses_its_weights_place():
     with pytest.raises(ValueError, match="residual_norm: a result lies"):
         F.rms_norm(Claimed((1, 8), ptr=0x1000), 8, Claimed((8,), ptr=0x7000), out=Claimed((1, 8), ptr=0x7000))
+
+
+# ---------------------------------------------------------------- drafts: 4 rows of 100 float32, 2 sequences
+READ = {"target": (0, 0x10000, 4 * 100 * 4), "draft": (1, 0x20000, 4 * 100 * 4), "tokens": (5, 0x30000, 16), "starts": (6, 0x40000, 12), "uniforms": (8, 0x50000, 16),
+        "last": (9, 0x60000, 8)}
+
+
+def verify_call(**kw):
+    args = [0x10000, 0x20000, _C.F32, 4, 100, 0x30000, 0x40000, 2, 0x50000, 0x60000, 0x70000, 0x80000, None]
+    for at, value in kw.values():
+        args[at] = value
+    _C.call("lq_verify_drafts", *args)
+
+
+@pytest.mark.parametrize("what", list(READ))
+@pytest.mark.parametrize("result,size", [(10, 16), (11, 8)])
+def test_c_verify_refuses_results_on_what_is_read(what, result, size):
+    _, at, n = READ[what]
+    for place in (at, at + n - 4, at - size + 4):
+        with pytest.raises(ValueError, match="verify_drafts: a result lies"):
+            verify_call(result=(result, place))
+
+
+@pytest.mark.parametrize("at", [0x70000, 0x7000c, 0x6fffc])
+def test_c_verify_refuses_one_result_on_the_other(at):
+    with pytest.raises(ValueError, match="verify_drafts: a result lies"):
+        verify_call(counts=(11, at))
+
+
+def test_verify_refuses_rows_beside_those_that_are_read():
+    """Rows of one tensor for the drafted and the new tokens, of another for starts and counts."""
+    i32 = L.int32
+    t = dict(target=Claimed((4, 100), ptr=0x10000), tokens=Claimed((4,), i32, 0x30000), starts=Claimed((3,), i32, 0x40000), uniforms=Claimed((4,), ptr=0x50000),
+             last_uniforms=Claimed((2,), ptr=0x60000))
+    new, counts = Claimed((4,), i32, 0x70000), Claimed((2,), i32, 0x80000)
+    for out in ((Claimed((4,), i32, 0x30004), counts), (Claimed((4,), i32, 0x2fff8), counts), (new, Claimed((2,), i32, 0x40008)), (new, Claimed((2,), i32, 0x70008))):
+        with pytest.raises(ValueError, match="verify_drafts: a result lies"):
+            F.verify_drafts(**t, out=out)
