@@ -446,7 +446,7 @@ int lq_bias_act_f32(float* y, const float* bias, size_t M, int N, int relu, lq_s
 
 /* Both projections of a gated feed-forward block on such weights, with the activation and the product (no counterpart in Lucid):
  *     out[m, n] = act(x[m] . w_gate[n] + bias_gate[n]) * (x[m] . w_up[n] + bias_up[n])
- * x [M, K] and out [M, N] are both LQ_F32 or both LQ_F16; weights as lq_wq_matmul takes them; x and packed are 16-byte aligned; index 0 is the gate, 1 the way up.  act: 0
+ * x [M, K] and out [M, N] are both LQ_F32 or both LQ_F16; weights as lq_wq_matmul takes them; x and packed are 16-byte aligned, out lies on nothing that is read; index 0 is the gate, 1 the way up.  act: 0
  * silu v / (1 + exp(-v)), 1 gelu (erf form), 2 relu, 3 sigmoid.  Codes enter the products as whole numbers; scales and sums are float32, and
  * so are the terms of the biases, in which b + 2^(bits-1) s is rounded once: nothing else of a weight is.  A value of a float32 x is off by at most 2^-22 of
  * itself or 2^-39 of its row's largest, whichever is more; float16 results are rounded once.  A

@@ -64,10 +64,14 @@ extern "C" int lq_wq_gated_matmul(const lq_wq_gated_args* g, lq_stream stream) {
     }
     LQ_REQUIRE(a.x && a.out, LQ_ERR_VALUE, "quantized_gated_matmul: NULL pointer");
     LQ_REQUIRE(aligned16(a.x), LQ_ERR_VALUE, "quantized_gated_matmul: x must be 16-byte aligned");
-    const size_t item = g->dtype == LQ_F16 ? 2 : 4;
-    const uintptr_t x0 = reinterpret_cast<uintptr_t>(a.x), out0 = reinterpret_cast<uintptr_t>(a.out);
-    LQ_REQUIRE(x0 + size_t(a.M) * a.K * item <= out0 || out0 + size_t(a.M) * a.N * item <= x0, LQ_ERR_VALUE,
-               "quantized_gated_matmul: the result cannot take x's place");
+    // (blocks write while others still read)
+    const size_t item = g->dtype == LQ_F16 ? 2 : 4, codes = size_t(a.N) * a.K * g->bits / 8, numbers = size_t(a.N) * (a.K / g->group_size) * 4;
+    const Span out{a.out, size_t(a.M) * a.N * item};
+    bool sound = apart(out, Span{a.x, size_t(a.M) * a.K * item});
+    for (const gated::Weight& w : a.w)
+        sound = sound && apart(out, Span{w.packed, codes}) && apart(out, Span{w.scales, numbers}) && apart(out, Span{w.biases, numbers}) &&
+                apart(out, Span{w.bias, size_t(a.N) * 4});
+    LQ_REQUIRE(sound, LQ_ERR_VALUE, "quantized_gated_matmul: the result cannot lie on x, a weight or a bias");
     const hipStream_t st = as_stream(stream);
     const bool half = g->dtype == LQ_F16;
     const Choice c = half ? (g->bits == 4 ? choose<1, 4>(a) : choose<1, 8>(a)) : (g->bits == 4 ? choose<2, 4>(a) : choose<2, 8>(a));

@@ -78,7 +78,8 @@ def quantized_gated_matmul(x: Tensor, gate: tuple[Tensor, Tensor, Tensor], up: t
     product in one call.  ``gate`` and ``up`` are what ``quantize`` gives of ``(out, in)`` weights of one shape; ``x`` ``(..., in)`` is float32 or
     float16 and so is the result ``(..., out)``, the biases are float32 ``(out,)``.  ``activation``: ``"silu"``, ``"gelu"`` (erf form), ``"relu"`` or
     ``"sigmoid"``.  Beyond its codes nothing of a weight is rounded but ``b + 2^(bits - 1) s`` of a group, to float32.  A value of a float32 ``x`` is off by at most
-    ``2^-22`` of itself or ``2^-39`` of its row's largest; float16 results are rounded once.  ``out`` takes the result.  No counterpart in Lucid."""
+    ``2^-22`` of itself or ``2^-39`` of its row's largest; float16 results are rounded once.  ``out`` takes the result, apart from all that is read.  No counterpart in
+    Lucid."""
     name = "quantized_gated_matmul"
     if activation not in _GATES:
         raise ValueError(f"{name}: activation {activation!r}; one of {', '.join(_GATES)}")

@@ -1,14 +1,13 @@
 """Results that lie on what a call reads are refused, without a device: by the C entry points, whose pointers are never followed, and through the
 wrappers."""
 
-import ctypes as C
-
 import pytest
 
 import lucid_amd as L
 import lucid_amd.nn.functional as F
 from lucid_amd import _C
-from test_host_decoder_step import Claimed, norm_args
+from lucid_amd.quantization import _qgemm
+from test_host_decoder_step import Claimed, gated_args, norm_args
 
 VECTORS = ("scale", "weight", "bias", "post_weight", "post_bias")
 
@@ -73,3 +72,28 @@ def test_verify_refuses_rows_beside_those_that_are_read():
     for out in ((Claimed((4,), i32, 0x30004), counts), (Claimed((4,), i32, 0x2fff8), counts), (new, Claimed((2,), i32, 0x40008)), (new, Claimed((2,), i32, 0x70008))):
         with pytest.raises(ValueError, match="verify_drafts: a result lies"):
             F.verify_drafts(**t, out=out)
+
+
+# ---------------------------------------------------------------- gated projections: 2 x 8 float32 of K = 64 in 4 bits, groups of 32
+OPERANDS = {"x": (0x10000, 2 * 64 * 4), "packed": (0x20000, 8 * 32), "scales": (0x30000, 8 * 2 * 4), "biases": (0x40000, 8 * 2 * 4), "bias": (0x50000, 8 * 4)}
+
+
+def gated_places():
+    """Where each operand lies: the gate's, and the way up's 0x8000 behind."""
+    return {n: at if n == "x" else (at, at + 0x8000) for n, (at, _) in OPERANDS.items()}
+
+
+@pytest.mark.parametrize("what,second", [("x", False)] + [(n, s) for n in list(OPERANDS)[1:] for s in (False, True)])
+def test_c_gated_refuses_a_result_on_what_is_read(what, second):
+    at, size = OPERANDS[what][0] + 0x8000 * second, OPERANDS[what][1]
+    for place in (at, at + size - 4, at - 2 * 8 * 4 + 4):
+        with pytest.raises(ValueError, match="quantized_gated_matmul: the result cannot"):
+            _C.call("lq_wq_gated_matmul", gated_args(**gated_places(), out=place), None)
+
+
+@pytest.mark.parametrize("bias", ["gate_bias", "up_bias"])
+def test_gated_refuses_a_result_in_a_biass_place(bias):
+    at = lambda base: (Claimed((8, 8), L.int32, base), Claimed((8, 2), ptr=base + 0x1000), Claimed((8, 2), ptr=base + 0x2000))
+    with pytest.raises(ValueError, match="quantized_gated_matmul: the result cannot"):
+        _qgemm.quantized_gated_matmul(Claimed((1, 64), ptr=0x10000), at(0x20000), at(0x30000), group_size=32, bits=4, out=Claimed((1, 8), ptr=0x40000),
+                                      **{bias: Claimed((8,), ptr=0x40000)})
