@@ -73,6 +73,8 @@ class QuantizedGatedLinearMLX(Module):
         super().__init__()
         if bits not in (4, 8):
             raise ValueError(f"bits must be 4 or 8, got {bits}")
+        if group_size not in (32, 64, 128):
+            raise ValueError(f"group_size must be 32, 64 or 128, got {group_size}")
         if in_features % group_size:
             raise ValueError(f"group_size {group_size} must divide in_features {in_features}")
         if activation not in _qgemm._GATES:
