@@ -549,11 +549,11 @@ int lq_residual_norm(const lq_residual_norm_args* args, lq_stream stream);
 /* Drafted tokens against the target's probabilities, from given random numbers.  Sequence b has the rows starts[b] .. starts[b + 1] - 1
  * (int32 [batch + 1], rising, within `rows`) of a step: its last token, and behind it the drafted ones (tokens int32 [rows]).  Row i of
  * target ([rows, vocab], LQ_F32 or LQ_F16) holds the probabilities p of the token behind row i, row i of draft (the same type) those, q,
- * that token i + 1 was drawn from; draft NULL: q = 1.  In order, x = tokens[i + 1] is accepted if uniforms[i] * q[x] < p[x] (exactly; a
- * token outside the vocabulary is refused).  Behind the accepted tokens comes one drawn with last[b]: from max(p - q, 0) of the row that
+ * that token i + 1 was drawn from; draft NULL: q = 1.  In order, x = tokens[i + 1] is accepted if uniforms[i] * q[x] < p[x] (exactly, of
+ * the numbers as they are, NaN and infinities too; a token outside the vocabulary is refused).  Behind the accepted tokens comes one drawn with last[b]: from max(p - q, 0) of the row that
  * refused (draft NULL: from p without x), from p of the last row where none did, or where nothing of p - q is positive: the lowest
  * token of positive weight at which the weights' running sum passes last[b] times their sum, in float64 (the last of positive weight if
- * none does; -1 if there is none).  Weights that are not positive and finite count as 0.  new_tokens (int32 [rows]): in a sequence's
+ * none does; -1 if there is none).  There, p and q that are not positive and finite count as 0.  new_tokens (int32 [rows]): in a sequence's
  * rows its new tokens, then -1; rows of no sequence stay.  counts (int32 [batch]): how many; 0 of an empty sequence.  The results lie apart
  * from each other and from all that is read.  At most
  * 65535 sequences, 2^24 tokens.  Takes scratch of the stream. */

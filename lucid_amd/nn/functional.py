@@ -292,11 +292,12 @@ def verify_drafts(target: Tensor, tokens: Tensor, starts: Tensor, uniforms: Tens
     vocab)``, float32 or float16, holds the probabilities ``p`` of the token behind row ``i``; row ``i`` of ``draft``, of the same shape and
     type, those that token ``i + 1`` was drawn from, ``q``.  Without ``draft`` that token was not drawn (``q`` is 1 there and 0 elsewhere).
 
-    In order, token ``x`` behind row ``i`` is accepted if ``uniforms[i] * q[x] < p[x]`` (float32 ``(rows,)`` in [0, 1)).  Behind the accepted
+    In order, token ``x`` behind row ``i`` is accepted if ``uniforms[i] * q[x] < p[x]`` (float32 ``(rows,)`` in [0, 1)), of the numbers as they are: a NaN
+    refuses, an infinite ``p[x]`` accepts (but where ``q[x]`` is infinite too), a negative ``q[x]`` accepts a ``p[x]`` of 0.  Behind the accepted
     ones comes a token drawn with ``last_uniforms[b]`` (float32 ``(batch,)``): from ``max(p - q, 0)`` of the row that refused, from ``p`` of the
     last row where none did, so that all are distributed as the target's.  It is the lowest token at which the running sum of the
-    weights passes ``last_uniforms[b]`` times their sum, in float64.  Neither ``p`` nor ``q`` need sum to one; what is not positive and finite
-    counts as 0; where no ``p - q`` is positive the token comes from ``p``, and is -1 where no ``p`` is.  A drafted token
+    weights passes ``last_uniforms[b]`` times their sum, in float64.  Neither ``p`` nor ``q`` need sum to one; in drawing that token, what of either is not
+    positive and finite counts as 0; where no ``p - q`` is positive the token comes from ``p``, and is -1 where no ``p`` is.  A drafted token
     outside the vocabulary is refused.
 
     ``new_tokens`` int32 ``(rows,)`` has a sequence's new tokens from ``starts[b]`` on and -1 behind them; ``counts`` int32 ``(batch,)`` says how many
