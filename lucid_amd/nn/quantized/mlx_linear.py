@@ -65,8 +65,9 @@ class QuantizedLinearMLX(Module):
 
 class QuantizedGatedLinearMLX(Module):
     """Both projections of a gated feed-forward block, ``act(gate(x)) * up(x)``, on group-wise int4 / int8 weights in one call
-    (``_qgemm.quantized_gated_matmul``); a ``QuantizedLinearMLX`` takes the result back.  Buffers: ``gate_packed_weight``, ``gate_scales``,
-    ``gate_biases``, ``gate_bias`` and the same of ``up``, each as ``QuantizedLinearMLX`` has it.  ``x`` is float32 or float16."""
+    (``_qgemm.quantized_gated_matmul``).  Buffers: ``gate_packed_weight``, ``gate_scales``, ``gate_biases``, ``gate_bias`` and the same of ``up``, each as
+    ``QuantizedLinearMLX`` has it.  ``x`` is float32 or float16, and the result has its type.  A ``QuantizedLinearMLX`` takes a float32 result back, as the
+    Linears of this package are float32; a float16 one goes through ``.to(float32)`` first."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, bits: int = 8, group_size: int = 64,
                  activation: str = "silu") -> None:
