@@ -463,6 +463,9 @@ typedef struct lq_wq_gated_args {
     int act, dtype;
 } lq_wq_gated_args;
 int lq_wq_gated_matmul(const lq_wq_gated_args* args, lq_stream stream);
+/* Which kernel such a call goes to, for tests and measurements: many = 1 the one of many rows, 0 those of few, and the rows and columns of a
+ * block.  (Up to four rows may have a kernel of their own, 16 columns a block.)  Needs no device. */
+int lq_wq_gated_tile(int M, int N, int K, int bits, int dtype, int* many, int* rows, int* columns);
 
 /* ------------------------------------------------- quantized key / value cache
  * No counterpart in Lucid.  Pages of page_size tokens; a page holds, per key / value head, page_size rows of head_dim codes,

@@ -301,6 +301,7 @@ class WqGatedArgs(C.Structure):
 
 WQ_GATED_ARGS = struct.Struct("@10P7i0P")  # (see RESIDUAL_NORM_ARGS)
 _SIGNATURES["lq_wq_gated_matmul"] = [_vp, _vp]
+_SIGNATURES["lq_wq_gated_tile"] = [_i] * 5 + [C.POINTER(_i)] * 3
 _SIGNATURES["lq_lstm_sequence_pays"] = [_i] * 3 + [C.POINTER(_i)]
 _SIGNATURES["lq_lstm_fused_layers"] = [_i] * 6 + [C.POINTER(_i)]
 _SIGNATURES["lq_lstm_sequence_f32"] = [C.POINTER(LstmArgs), _vp]

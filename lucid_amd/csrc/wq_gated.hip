@@ -39,9 +39,36 @@ Choice choose(const gated::Args& a) {
     return best;
 }
 
+Choice choose(const gated::Args& a, bool half, int bits) {
+    return half ? (bits == 4 ? choose<1, 4>(a) : choose<1, 8>(a)) : (bits == 4 ? choose<2, 4>(a) : choose<2, 8>(a));
+}
+
 }  // namespace
 
-extern "C" int lq_wq_gated_matmul(const lq_wq_gated_args* g, lq_stream stream) {
+extern "C" {
+
+int lq_wq_gated_tile(int M, int N, int K, int bits, int dtype, int* many, int* rows, int* columns) {
+    LQ_REQUIRE(many && rows && columns, LQ_ERR_VALUE, "wq_gated_tile: NULL pointer");
+    LQ_REQUIRE(bits == 4 || bits == 8, LQ_ERR_VALUE, "wq_gated_tile: bits must be 4 or 8 (got %d)", bits);
+    LQ_REQUIRE(dtype == LQ_F32 || dtype == LQ_F16, LQ_ERR_DTYPE, "wq_gated_tile: float32 and float16 are taken");
+    LQ_REQUIRE(M > 0 && N > 0 && K > 0, LQ_ERR_SHAPE, "wq_gated_tile: %d x %d x %d", M, N, K);
+    gated::Args a{};
+    a.M = M, a.N = N, a.K = K;
+    const bool half = dtype == LQ_F16;
+    const Choice c = choose(a, half, bits);
+    const auto of_rows = [&](const gated::RowsTile& t) { *rows = 16 * t.mt, *columns = 16 * t.cg; };
+    const auto of_many = [&](const gated::GemmTile& t) { *rows = 16 * t.mt, *columns = 64 * t.ct; };
+    *many = c.rows ? 0 : 1;
+    if (c.rows && half) of_rows(gated::kRowsTiles<1>[c.tile]);
+    else if (c.rows) of_rows(gated::kRowsTiles<2>[c.tile]);
+    else if (half && bits == 4) of_many(gated::kGemmTiles<1, 4>[c.tile]);
+    else if (half) of_many(gated::kGemmTiles<1, 8>[c.tile]);
+    else if (bits == 4) of_many(gated::kGemmTiles<2, 4>[c.tile]);
+    else of_many(gated::kGemmTiles<2, 8>[c.tile]);
+    return LQ_OK;
+}
+
+int lq_wq_gated_matmul(const lq_wq_gated_args* g, lq_stream stream) {
     LQ_REQUIRE(g, LQ_ERR_VALUE, "quantized_gated_matmul: args is NULL");
     LQ_REQUIRE(g->bits == 4 || g->bits == 8, LQ_ERR_VALUE, "quantized_gated_matmul: bits must be 4 or 8 (got %d)", g->bits);
     LQ_REQUIRE(g->group_size == 32 || g->group_size == 64 || g->group_size == 128, LQ_ERR_VALUE,
@@ -74,8 +101,10 @@ extern "C" int lq_wq_gated_matmul(const lq_wq_gated_args* g, lq_stream stream) {
     LQ_REQUIRE(sound, LQ_ERR_VALUE, "quantized_gated_matmul: the result cannot lie on x, a weight or a bias");
     const hipStream_t st = as_stream(stream);
     const bool half = g->dtype == LQ_F16;
-    const Choice c = half ? (g->bits == 4 ? choose<1, 4>(a) : choose<1, 8>(a)) : (g->bits == 4 ? choose<2, 4>(a) : choose<2, 8>(a));
+    const Choice c = choose(a, half, g->bits);
     if (c.rows) return half ? gated::launch_rows_f16(a, g->bits, c.tile, st) : gated::launch_rows_f32(a, g->bits, c.tile, st);
     if (half) return g->bits == 4 ? gated::launch_gemm_f16_4(a, c.tile, st) : gated::launch_gemm_f16_8(a, c.tile, st);
     return g->bits == 4 ? gated::launch_gemm_f32_4(a, c.tile, st) : gated::launch_gemm_f32_8(a, c.tile, st);
 }
+
+}  // extern "C"
