@@ -380,8 +380,8 @@ class LayerNorm(Module):
 
 
 class RMSNorm(Module):
-    """``functional.rms_norm`` over the last axis; float32 or float16 in, the same out.  ``residual_norm`` takes ``weight`` and ``eps`` where
-    the norm stands behind a residual connection."""
+    """``functional.rms_norm`` over the last axis; float32 or float16 in, the same out.  ``residual_norm`` takes ``weight`` (on the device: after
+    ``.to("hip")`` or a call) and ``eps`` where the norm stands behind a residual connection."""
 
     def __init__(self, normalized_shape: int, eps: float = 1e-6) -> None:
         super().__init__()
@@ -391,8 +391,9 @@ class RMSNorm(Module):
     def forward(self, x):
         from . import functional as F
 
-        weight = self.weight if self.weight.device == "hip" else self.weight.to("hip")
-        return F.rms_norm(x, self.normalized_shape, weight, self.eps)
+        if self.weight.device != "hip":  # (for good: a copy from the host ends in a wait, and none can be captured)
+            self.weight = self.weight.to("hip")
+        return F.rms_norm(x, self.normalized_shape, self.weight, self.eps)
 
 
 class GELU(Module):
