@@ -1,8 +1,9 @@
-"""Verified drafts at the numbers that are no probabilities, acceptance and drawing told apart."""
+"""Verified drafts at the numbers that are no probabilities, acceptance and drawing told apart, and of no rows."""
 
 import numpy as np
 import pytest
 
+import lucid_amd as L
 import lucid_amd.nn.functional as F
 from test_hip_verify_drafts import hip
 
@@ -26,3 +27,12 @@ def test_acceptance_compares_the_numbers_as_they_are_and_drawing_counts_them_as_
         return
     # what is left of p - q: token 4, and where q counts as nothing a p of 0.25 at token 3, which 0.75 of the sum 0.375 passes
     assert new.numpy().tolist() == [4, -1] and counts.numpy().tolist() == [1]
+
+
+def test_drafts_of_no_rows():
+    """A step in which no sequence has a token, results given or not."""
+    ids, f32 = lambda n: L.tensor(np.zeros(n, np.int32), device="hip"), lambda *s: L.tensor(np.zeros(s, np.float32), device="hip")
+    for batch in (0, 3):
+        for out in (None, (ids(0), L.tensor(np.full(batch, 9, np.int32), device="hip"))):
+            new, counts = F.verify_drafts(f32(0, 50), ids(0), ids(batch + 1), f32(0), f32(batch), out=out)
+            assert new.shape == (0,) and counts.numpy().tolist() == [0] * batch
