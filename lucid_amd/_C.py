@@ -275,7 +275,7 @@ _SIGNATURES["lq_kv_cache_compact"] = [C.POINTER(KvCache), _vp, _i, _i, _vp, _sz,
 
 
 class ResidualNormArgs(C.Structure):
-    """``lq_residual_norm_args`` of ``include/lucid_hip.h``."""
+    """``lq_residual_norm_args`` of ``include/lucid_hip.h``: for callers of the C entry; ``functional`` packs the bytes below."""
 
     _fields_ = [
         ("x", _vp), ("r", _vp), ("gate", _vp), ("scale", _vp), ("weight", _vp), ("bias", _vp), ("post_weight", _vp), ("post_bias", _vp),
@@ -291,7 +291,7 @@ _SIGNATURES["lq_verify_drafts"] = [_vp, _vp, _i, _i, _i, _vp, _vp, _i, _vp, _vp,
 
 
 class WqGatedArgs(C.Structure):
-    """``lq_wq_gated_args`` of ``include/lucid_hip.h``."""
+    """``lq_wq_gated_args`` of ``include/lucid_hip.h`` (see ResidualNormArgs)."""
 
     _fields_ = [
         ("x", _vp), ("out", _vp), ("packed", _vp * 2), ("scales", _vp * 2), ("biases", _vp * 2), ("bias", _vp * 2), ("M", _i), ("N", _i), ("K", _i),
