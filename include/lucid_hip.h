@@ -446,11 +446,11 @@ int lq_bias_act_f32(float* y, const float* bias, size_t M, int N, int relu, lq_s
 
 /* Both projections of a gated feed-forward block on such weights, with the activation and the product (no counterpart in Lucid):
  *     out[m, n] = act(x[m] . w_gate[n] + bias_gate[n]) * (x[m] . w_up[n] + bias_up[n])
- * x [M, K] and out [M, N] are both LQ_F32 or both LQ_F16; weights as lq_wq_matmul takes them; x and packed are 16-byte aligned, out lies on nothing that is read; index 0 is the gate, 1 the way up.  act: 0
- * silu v / (1 + exp(-v)), 1 gelu (erf form), 2 relu, 3 sigmoid.  Codes enter the products as whole numbers; scales and sums are float32, and
- * so are the terms of the biases, in which b + 2^(bits-1) s is rounded once: nothing else of a weight is.  A value of a float32 x is off by at most 2^-22 of
- * itself or 2^-39 of its row's largest, whichever is more; float16 results are rounded once.  A
- * non-finite x gives a non-finite row before the activation.  May take scratch of the stream. */
+ * x [M, K] and out [M, N] are both LQ_F32 or both LQ_F16; weights as lq_wq_matmul takes them, index 0 the gate's, 1 the way up's; x and packed are
+ * 16-byte aligned, out lies on nothing that is read.  act: 0 silu v / (1 + exp(-v)), 1 gelu (erf form), 2 relu, 3 sigmoid.  Codes enter the products
+ * as whole numbers; scales and sums are float32, and so are the terms of the biases, in which b + 2^(bits-1) s is rounded once: nothing else of a
+ * weight is.  A value of a float32 x enters within 2^-22 of itself or 2^-39 of its row's largest, whichever is more; float16 results are rounded
+ * once.  A non-finite x gives a non-finite row before the activation.  May take scratch of the stream. */
 typedef struct lq_wq_gated_args {
     const void* x;
     void* out;
@@ -552,14 +552,14 @@ int lq_residual_norm(const lq_residual_norm_args* args, lq_stream stream);
 /* Drafted tokens against the target's probabilities, from given random numbers.  Sequence b has the rows starts[b] .. starts[b + 1] - 1
  * (int32 [batch + 1], rising, within `rows`) of a step: its last token, and behind it the drafted ones (tokens int32 [rows]).  Row i of
  * target ([rows, vocab], LQ_F32 or LQ_F16) holds the probabilities p of the token behind row i, row i of draft (the same type) those, q,
- * that token i + 1 was drawn from; draft NULL: q = 1.  In order, x = tokens[i + 1] is accepted if uniforms[i] * q[x] < p[x] (exactly, of
- * the numbers as they are, NaN and infinities too; a token outside the vocabulary is refused).  Behind the accepted tokens comes one drawn with last[b]: from max(p - q, 0) of the row that
- * refused (draft NULL: from p without x), from p of the last row where none did, or where nothing of p - q is positive: the lowest
- * token of positive weight at which the weights' running sum passes last[b] times their sum, in float64 (the last of positive weight if
- * none does; -1 if there is none).  There, p and q that are not positive and finite count as 0.  new_tokens (int32 [rows]): in a sequence's
- * rows its new tokens, then -1; rows of no sequence stay.  counts (int32 [batch]): how many; 0 of an empty sequence.  The results lie apart
- * from each other and from all that is read.  At most
- * 65535 sequences, 2^24 tokens.  Takes scratch of the stream. */
+ * that token i + 1 was drawn from; draft NULL: q = 1.  In order, x = tokens[i + 1] is accepted if uniforms[i] * q[x] < p[x] (exactly,
+ * of the numbers as they are, NaN and infinities too; a token outside the vocabulary is refused).  Behind the accepted tokens comes one drawn
+ * with last[b]: from max(p - q, 0) of the row that refused (draft NULL: from p without x), from p of the last row where none did, or where
+ * nothing of p - q is positive: the lowest token of positive weight at which the weights' running sum passes last[b] times their sum, in
+ * float64 (the last of positive weight if none does; -1 if there is none).  There, p and q that are not positive and finite count as 0.
+ * new_tokens (int32 [rows]): in a sequence's rows its new tokens, then -1; rows of no sequence stay.  counts (int32 [batch]): how many; 0 of an
+ * empty sequence.  The results lie apart from each other and from all that is read.  At most 65535 sequences, 2^24 tokens.  Takes scratch of
+ * the stream. */
 int lq_verify_drafts(const void* target, const void* draft, int dtype, int rows, int vocab, const int32_t* tokens, const int32_t* starts,
                      int batch, const float* uniforms, const float* last, int32_t* new_tokens, int32_t* counts, lq_stream stream);
 
